@@ -81,6 +81,11 @@ def draw(rng):
         return case
 
 
+def _scale(largest):
+    """fl32(largest / 448), at least 2^-126; by a tensor, since a division by a plain number may become a product with its reciprocal"""
+    return torch.maximum(largest / torch.full_like(largest, TOP_E4M3), torch.full_like(largest, SMALLEST))
+
+
 # ---- inputs --------------------------------------------------------------------------------------------------------------
 def _rows(m, k, gen):
     """Rows as a norm leaves them: about one in size, a few channels several times as large."""
@@ -95,7 +100,7 @@ def _weight(lead, n, k, gen):
     w = torch.zeros((*lead, nb * BLOCK, kb * BLOCK), device=DEV)
     w[..., :n, :k] = 0.02 * torch.randn((*lead, n, k), generator=gen, device=DEV)
     w = w.view(*lead, nb, BLOCK, kb, BLOCK)
-    scales = (w.abs().amax(dim=(-3, -1)) / TOP_E4M3).clamp_min(SMALLEST)
+    scales = _scale(w.abs().amax(dim=(-3, -1)))
     values = (w / scales[..., :, None, :, None]).to(torch.float8_e4m3fn)
     values = values.view(torch.uint8).reshape(*lead, nb * BLOCK, kb * BLOCK)[..., :n, :k].contiguous().view(torch.float8_e4m3fn)
     return values, scales.contiguous()
@@ -143,7 +148,7 @@ def _quantised(x):
     m, k = x.shape
     kb = -(-k // BLOCK)
     pad = torch.nn.functional.pad(x, (0, kb * BLOCK - k)).view(m, kb, BLOCK)
-    s = (pad.abs().amax(dim=2, keepdim=True) / TOP_E4M3).clamp_min(SMALLEST)
+    s = _scale(pad.abs().amax(dim=2, keepdim=True))
     return ((pad / s).to(torch.float8_e4m3fn).float() * s).view(m, kb * BLOCK)[:, :k]
 
 
@@ -252,8 +257,8 @@ def _rows_64(x):
     out = torch.empty_like(x)
     for at in range(0, x.shape[1], BLOCK):
         part = x[:, at:at + BLOCK]
-        largest = part.abs().max(dim=1, keepdim=True).values.float()
-        s = torch.maximum(largest / TOP_E4M3, torch.full_like(largest, SMALLEST))
+        largest = part.abs().max(dim=1, keepdim=True).values.float().double()
+        s = torch.clamp((largest / TOP_E4M3).float(), min=SMALLEST)
         out[:, at:at + BLOCK] = _e4m3_64((part.float() / s).double()) * s.double()
     return out
 
