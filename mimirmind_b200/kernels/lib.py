@@ -112,6 +112,9 @@ _PROTOTYPES = {
     "mm_cast_rows": [P, P, I, c_longlong, P],
     "mm_scaled_sum2": [P, P, P, I, c_longlong, F, F, P, I, P],
     "mm_gemm_tcgen05_grouped": [P, P, P, I, I, I, I, I, I, I, P, P, I, P, P],
+    "mm_fp8_quant_rows": [P, I, c_longlong, P, P, I, P, I, I, P],
+    "mm_fp8_quant_weight": [P, I, P, I, P, I, I, I, P],
+    "mm_gemm_fp8_simple": [P, I, P, P, c_longlong, P, P, I, I, P, I, I, I, I, I, P, P, I, I, F, P, P, P],
 }
 
 

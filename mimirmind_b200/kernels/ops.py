@@ -1999,3 +1999,233 @@ def qk_prep(rows: torch.Tensor, q_off: int, k_off: int, v_off: int, q_norm: Opti
                                  float(eps), _ptr(rot) if rot_dims else None, int(rot_dims), int(bool(unit)), q_out.data_ptr(), _ptr(k_pages),
                                  _ptr(v_pages), dtype_code(q_out.dtype), _ptr(slots) if k_pages is not None else None, int(page_size), n,
                                  int(heads), int(kv_heads), int(key_dim), int(value_dim), _stream()), "qk_prep")
+
+
+# ---- layer weights in 8 bits (csrc/fp8.cuh has the formulas) ---------------------------------------------------------------
+FP8_BLOCK = 128           # numbers of a row, and rows and columns of a weight, that share a scale
+FP8_MAX_ROWS = 1 << 20    # of a product; sizes along a matrix fit in 32 bits well above any model's
+_E4M3 = torch.float8_e4m3fn
+
+
+def _blocks(n: int) -> int:
+    return -(-n // FP8_BLOCK)
+
+
+def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """All tensors are on the current CUDA device: the launch goes to its current stream."""
+    dev = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.device.index != dev:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
+
+
+def _need_fp8(values: torch.Tensor, scales: torch.Tensor, what: str, lead, rows: int, k: int, blocks: int) -> None:
+    if not isinstance(values, torch.Tensor) or not values.is_cuda or values.dtype != _E4M3:
+        raise KernelError(f"{what}: expected float8_e4m3fn numbers on a CUDA device")
+    if rows < 1 and lead is not None or k < 1:
+        raise KernelError(f"{what}: sizes must be positive")
+    ld = values.stride(-2) if values.shape[-2] > 1 else -(-k // 16) * 16
+    if (values.stride(-1) != 1 and k > 1) or ld % 16 or ld < k or values.data_ptr() % 16:
+        raise KernelError(f"{what}: rows must be contiguous and start on 16-byte boundaries")
+    _need(scales, what + " scales", torch.float32)
+    if tuple(scales.shape) != tuple(lead or ()) + (blocks, _blocks(k)):
+        raise KernelError(f"{what}: scales are {tuple(scales.shape)}, expected {tuple(lead or ()) + (blocks, _blocks(k))}")
+
+
+@dataclass
+class Fp8Rows:
+    """Rows in 8 bits: ``values`` e4m3 [m, K] (rows start on 16-byte boundaries) and ``scales`` fp32 [m, K / 128 rounded up];
+    a number stands for ``values * scales``."""
+
+    values: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self):
+        if self.values.dim() != 2:
+            raise KernelError("fp8 rows: expected a matrix")
+        m, k = self.values.shape
+        _need_fp8(self.values, self.scales, "fp8 rows", None, m, k, m)
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+
+@dataclass
+class Fp8Weight:
+    """A weight in 8 bits, or several stacked ones: ``values`` e4m3 [..., N, K] (rows start on 16-byte boundaries) and ``scales``
+    fp32 [..., N / 128, K / 128] (both rounded up), one for every block of 128 x 128 of a matrix; a number stands for ``values * scales``."""
+
+    values: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self):
+        if self.values.dim() < 2:
+            raise KernelError("fp8 weight: expected a matrix or stacked matrices")
+        n, k = self.values.shape[-2:]
+        lead = tuple(self.values.shape[:-2])
+        _need_fp8(self.values, self.scales, "fp8 weight", lead, n, k, _blocks(n))
+        step = n * self.ld
+        for i in reversed(range(len(lead))):
+            if lead[i] > 1 and self.values.stride(i) != step:
+                raise KernelError("fp8 weight: stacked matrices must follow one another")
+            step *= lead[i]
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    @property
+    def ld(self) -> int:
+        """The row stride in numbers."""
+        n, k = self.values.shape[-2:]
+        return self.values.stride(-2) if n > 1 else -(-k // 16) * 16
+
+    def float(self) -> torch.Tensor:
+        """The numbers that the weight stands for, in fp32."""
+        n, k = self.shape[-2:]
+        s = self.scales.repeat_interleave(FP8_BLOCK, dim=-2)[..., :n, :].repeat_interleave(FP8_BLOCK, dim=-1)[..., :k]
+        return self.values.float() * s
+
+
+def _fp8_buffer(*shape, device) -> torch.Tensor:
+    """e4m3 [..., K] whose rows start on 16-byte boundaries."""
+    k = shape[-1]
+    return torch.empty(shape[:-1] + (-(-k // 16) * 16,), dtype=torch.uint8, device=device).view(_E4M3)[..., :k]
+
+
+def quantize_fp8_rows(x: torch.Tensor, source: Optional[torch.Tensor] = None) -> Fp8Rows:
+    """Rows [m, K] (bf16 or fp32, contiguous along K) in 8 bits, per row and block of 128: ``s = max(max|x| / 448, 2^-126)``,
+    ``q = e4m3(x / s)``, quotients in fp32.  ``source`` int32 [rows]: row r is made from row ``source[r]`` (each within x).
+    A NaN or an infinity in a row makes every product with it NaN; other rows do not see it."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 2:
+        raise KernelError("fp8 rows: expected a CUDA matrix")
+    m, k = x.shape
+    if k < 1 or (x.stride(1) != 1 and k > 1) or (x.stride(0) < 0):
+        raise KernelError("fp8 rows: a row's numbers must follow one another")
+    if source is not None:
+        _need(source, "fp8 rows source", torch.int32)
+        if source.numel() and not m:
+            raise KernelError("fp8 rows: there is no row to make others from")
+        m = source.numel()
+    _here("fp8 rows", x, source)
+    out = Fp8Rows(_fp8_buffer(m, k, device=x.device), torch.empty((m, _blocks(k)), dtype=torch.float32, device=x.device))
+    check(_lib.load().mm_fp8_quant_rows(x.data_ptr(), dtype_code(x.dtype), x.stride(0), _ptr(source), out.values.data_ptr(), -(-k // 16) * 16,
+                                        out.scales.data_ptr(), m, k, _stream()), "quantize_fp8_rows")
+    return out
+
+
+def quantize_fp8_weight(w: torch.Tensor) -> Fp8Weight:
+    """A weight [..., N, K] (bf16 or fp32) in 8 bits with a scale per block of 128 x 128 of every matrix: ``s = max(max|w| / 448, 2^-126)``,
+    ``q = e4m3(w / s)``."""
+    _need(w, "fp8 weight")
+    if w.dim() < 2 or w.numel() == 0:
+        raise KernelError("fp8 weight: expected a matrix or stacked matrices")
+    _here("fp8 weight", w)
+    lead, (n, k) = tuple(w.shape[:-2]), w.shape[-2:]
+    out = Fp8Weight(_fp8_buffer(*lead, n, k, device=w.device), torch.empty(lead + (_blocks(n), _blocks(k)), dtype=torch.float32, device=w.device))
+    check(_lib.load().mm_fp8_quant_weight(w.data_ptr(), dtype_code(w.dtype), out.values.data_ptr(), -(-k // 16) * 16, out.scales.data_ptr(),
+                                          w.numel() // (n * k), n, k, _stream()), "quantize_fp8_weight")
+    return out
+
+
+def _fp8_rows_of(x, k: int, what: str) -> Fp8Rows:
+    if not isinstance(x, Fp8Rows):
+        if isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[1] != k:
+            raise KernelError(f"{what}: rows of {x.shape[1]} numbers meet a weight of {k}")
+        return quantize_fp8_rows(x)
+    if x.shape[1] != k:
+        raise KernelError(f"{what}: rows of {x.shape[1]} numbers meet a weight of {k}")
+    return x
+
+
+def _fp8_product(x: Fp8Rows, w: Fp8Weight, out: torch.Tensor, glu: bool = False, bias=None, rows: Optional["ExpertRows"] = None, act: int = 0,
+                 limit: float = 0.0, row_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    _here("gemm_fp8", x.values, x.scales, w.values, w.scales, bias, row_scale)
+    m, k = x.shape
+    n = w.shape[-2]
+    check(_lib.load().mm_gemm_fp8_simple(x.values.data_ptr(), x.values.stride(0) if m > 1 else -(-k // 16) * 16, x.scales.data_ptr(), w.values.data_ptr(),
+                                         w.ld, w.scales.data_ptr(), out.data_ptr(), dtype_code(out.dtype), out.shape[1],
+                                         _ptr(bias), dtype_code(bias.dtype) if bias is not None else F32, m, n, k, int(glu),
+                                         rows.tiles.data_ptr() if rows else None, rows.n_tiles.data_ptr() if rows else None, rows.max_tiles if rows else 0,
+                                         act, float(limit), _ptr(row_scale), rows.order.data_ptr() if rows else None, _stream()), "gemm_fp8")
+    return out
+
+
+def gemm_fp8(x, w: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """x [m, K] times a weight [N, K] in 8 bits (+ bias [N]): ``sum_b sx[m, b] sw[n / 128, b] sum_{k in b} qx[m, k] qw[n, k]``, sums in
+    fp32, rounded once to ``out_dtype`` (bf16 or fp32).  ``x``: :class:`Fp8Rows`, or bf16 or fp32 rows, which are quantised first
+    (:func:`quantize_fp8_rows`)."""
+    if not isinstance(w, Fp8Weight) or w.values.dim() != 2:
+        raise KernelError("gemm_fp8: the weight must be one matrix in 8 bits (Fp8Weight [N, K])")
+    n, k = w.shape
+    if bias is not None:
+        _need(bias, "gemm_fp8 bias")
+        dtype_code(bias.dtype)
+        if bias.shape != (n,):
+            raise KernelError("gemm_fp8: bias shape mismatch")
+    dtype_code(out_dtype)
+    _here("gemm_fp8", w.values, w.scales, bias)
+    x = _fp8_rows_of(x, k, "gemm_fp8")
+    return _fp8_product(x, w, torch.empty((x.shape[0], n), dtype=out_dtype, device=w.values.device), bias=bias)
+
+
+def _glu_code(activation: str, limit: float, what: str) -> int:
+    if activation not in GLU_ACTIVATIONS:
+        raise KernelError(f"{what}: activation '{activation}' is not one of {', '.join(sorted(GLU_ACTIVATIONS))}")
+    return GLU_ACTIVATIONS[activation]
+
+
+def glu_mlp_fp8(x, w_in: Fp8Weight, w_out: Fp8Weight, activation: str = "silu", limit: float = 0.0) -> torch.Tensor:
+    """A gated feed-forward in 8 bits: ``h = act(x Wg^T, x Wu^T)`` in fp32, quantised per row and block of 128 from its fp32 values, and
+    ``h Wd^T`` as bf16 [m, D].  ``w_in`` [2, F, K]: the gate's matrix, then the up projection's; ``w_out`` [D, F].  ``x`` as for
+    :func:`gemm_fp8`; ``activation`` and ``limit`` as for :func:`moe_gemm`."""
+    if not isinstance(w_in, Fp8Weight) or w_in.values.dim() != 3 or w_in.shape[0] != 2:
+        raise KernelError("glu_mlp_fp8: w_in must be two matrices in 8 bits (Fp8Weight [2, F, K])")
+    if not isinstance(w_out, Fp8Weight) or w_out.values.dim() != 2 or w_out.shape[1] != w_in.shape[1]:
+        raise KernelError("glu_mlp_fp8: w_out must be a matrix in 8 bits that takes the hidden rows (Fp8Weight [D, F])")
+    act = _glu_code(activation, limit, "glu_mlp_fp8")
+    _here("glu_mlp_fp8", w_in.values, w_in.scales, w_out.values, w_out.scales)
+    f, k = w_in.shape[1:]
+    x = _fp8_rows_of(x, k, "glu_mlp_fp8")
+    hidden = _fp8_product(x, w_in, torch.empty((x.shape[0], f), dtype=torch.float32, device=w_in.values.device), glu=True, act=act, limit=limit)
+    return gemm_fp8(hidden, w_out)
+
+
+def _check_experts_fp8(x: torch.Tensor, w_in: Fp8Weight, w_out: Fp8Weight, what: str) -> None:
+    if (not isinstance(w_in, Fp8Weight) or not isinstance(w_out, Fp8Weight) or w_in.values.dim() != 4 or w_in.shape[1] != 2 or w_out.values.dim() != 3
+            or w_in.shape[0] != w_out.shape[0] or w_in.shape[2] != w_out.shape[2]):
+        raise KernelError(f"{what}: w_in must be Fp8Weight [E, 2, F, D] (gate, up) and w_out Fp8Weight [E, D, F]")
+    if x.dim() != 2 or x.shape[1] != w_in.shape[3]:
+        raise KernelError(f"{what}: rows of {tuple(x.shape)} meet experts of {w_in.shape[3]}")
+
+
+def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, wts: torch.Tensor, w_in: Fp8Weight, w_out: Fp8Weight, activation: str = "silu",
+                    limit: float = 0.0, weight_on: str = "output") -> torch.Tensor:
+    """The chosen experts in 8 bits over a step's rows: ``out[t] = sum_c wts[t, c] Wd_e act(Wg_e x_t, Wu_e x_t)``, ``e = idx[t, c]``, as bf16
+    [n, D].  ``x`` bf16 or fp32 [n, D] and the hidden rows (from their fp32 values) are quantised per row and block of 128.  ``idx`` int32 and
+    ``wts`` fp32 [n, top] as :func:`moe_router` gives them (every expert's number below E); ``w_in`` [E, 2, F, D] the gates' and up projections' matrices,
+    ``w_out`` [E, D, F].  ``weight_on`` ``input``: the weight multiplies the first products instead of the result."""
+    _need(x, "moe rows")
+    _need(idx, "expert choice", torch.int32)
+    _need(wts, "moe weights", torch.float32)
+    _check_experts_fp8(x, w_in, w_out, "moe_experts_fp8")
+    if idx.dim() != 2 or idx.shape != wts.shape or idx.shape[0] != x.shape[0] or idx.shape[1] < 1:
+        raise KernelError("moe_experts_fp8: choice and weights must be [n, top]")
+    if weight_on not in ("output", "input"):
+        raise KernelError("moe_experts_fp8: weight_on is 'output' or 'input'")
+    act = _glu_code(activation, limit, "moe_experts_fp8")
+    dtype_code(x.dtype)
+    _here("moe_experts_fp8", x, idx, wts, w_in.values, w_in.scales, w_out.values, w_out.scales)
+    n, d = x.shape
+    E, _, f, _ = w_in.shape
+    top = idx.shape[1]
+    if n == 0:
+        return torch.empty((0, d), dtype=torch.bfloat16, device=x.device)
+    rows = moe_sort(idx, E, with_tiles=True)
+    sorted_x = quantize_fp8_rows(x, rows.row_token)
+    on_input = weight_on == "input"
+    hidden = _fp8_product(sorted_x, w_in, torch.empty((n * top, f), dtype=torch.float32, device=x.device), glu=True, rows=rows, act=act, limit=limit,
+                          row_scale=wts if on_input else None)
+    y = _fp8_product(quantize_fp8_rows(hidden), w_out, torch.empty((n * top, d), dtype=torch.float32, device=x.device), rows=rows)
+    return moe_combine(y, None if on_input else wts, torch.bfloat16, place=rows.place, top=top)
