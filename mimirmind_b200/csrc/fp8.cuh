@@ -31,3 +31,9 @@ __device__ __forceinline__ float fp8_to_f32(uint8_t v) {
     const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)v, __NV_E4M3);
     return __half2float(*reinterpret_cast<const __half*>(&h));
 }
+
+// glu_act, with a NaN in either half kept (the clamped form's minimum and maximum would lose it)
+__device__ __forceinline__ float fp8_glu(float g, float u, int act, float limit, float s) {
+    const float h = glu_act<false>(g, u, act, limit, s);
+    return g != g || u != u ? __uint_as_float(0x7fffffffu) : h;
+}

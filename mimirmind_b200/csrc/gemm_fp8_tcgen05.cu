@@ -1,0 +1,507 @@
+// Products of rows and weights in 8 bits on the fifth-generation tensor cores, with a scale per row and block of 128 and per weight
+// block of 128 x 128 (fp8.cuh):
+//   y[m, n] = sum over blocks b of sa[m, b] sw[n / 128, b] (sum over k in b of qa[m, k] qw[n, k])  (+ bias[n]).
+//
+// tcgen05.mma kind::f8f6f4 (128 x BN x 32, fp32 in tensor memory) makes one block's inner sums from operands that TMA brought into shared
+// memory (rows of 128 bytes, 128-byte swizzle); while it makes the next block's, eight warps read these back, multiply them by the block's
+// scales and add them to sums in registers, BN / 2 columns of one row a thread.  Two accumulators in tensor memory keep both sides busy:
+// per block of a 128 x 256 tile the products take 512 cycles and the sums 256 of each scheduler's, so the sums ride along.
+//
+// Roles: warps 0..7 sums and results, warp 8 TMA, warp 9 products.  A CTA walks over tiles, row tiles first, so that CTAs at work at
+// the same time share weight tiles in L2.  Few tiles: a cluster of S CTAs splits a tile's blocks; every CTA puts its sums into its own shared
+// memory, and after a cluster barrier each finishes every S-th row from all S in rank order (the same order on every run).
+//
+// Kinds of result: rows in bf16 or fp32 (+ bias); or, GLU, W holds pairs of matrices (the gate's and the up projection's), a tile is 128 columns of
+// both, and act(gate, up) leaves as e4m3 rows with their scales: the 128 columns are one block of the next product's rows, so its largest
+// number is known here and the hidden rows never exist in another form.
+//
+// Grouped form: row tiles of a device-made list (first row, end row, matrix), as in gemm_tcgen05.cu.
+//
+// Every wait is bounded; when one runs out, the CTA's tiles from there on become NaN, copies in flight get time to land, `err` is set.
+#include "fp8.cuh"
+#include "tcgen05.cuh"
+
+namespace {
+
+using namespace tc;
+
+constexpr int T_ROWS = 128, T_THREADS = 320, SUM_WARPS = 8;
+constexpr int HALF_BYTES = 128 * 128;              // 128 rows of 128 bytes
+enum { OUT_BF16 = 0, OUT_F32 = 1 };
+
+struct Fp8Args {
+    void* out;                  // rows, or (GLU) the hidden rows' e4m3 numbers
+    float* out_scales;          // (GLU) [M, NB]
+    const float* sa;            // [M, KB]
+    const float* sw;            // [matrices, NB, KB]
+    const void* bias;
+    const float* row_scale;     // (GLU) [.] fp32 or null: gate and up sums of row r are multiplied by row_scale[order ? order[r] : r]
+    const int32_t* order;
+    const int32_t* tiles;       // grouped: 3 ints a row tile
+    const int32_t* n_tiles;
+    int* err;
+    int out_kind, bias_dtype, act;
+    float limit;
+    int M, N, K, KB, NB, ldo, S;
+};
+
+template <int BN>
+struct Layout {
+    static constexpr int STAGE_BYTES = HALF_BYTES * (1 + BN / 128);
+    static constexpr int STAGES = BN == 256 ? 4 : 6;
+    static constexpr int PIPE_BYTES = STAGES * STAGE_BYTES;
+    static constexpr int STAGING = 4096;           // per warp: 32 rows of 128 bytes
+    static constexpr int PART_LD = BN + 4;         // floats of a row of a split tile's sums
+};
+
+struct Ctl {
+    uint64_t full[6], empty[6];
+    uint64_t sum_full[2], sum_empty[2];
+    uint64_t pair[4];                              // two warps that hold a row's halves
+    uint32_t tmem_base;
+    int abort_flag;
+};
+static_assert(128 * Layout<256>::PART_LD * 4 <= Layout<256>::PIPE_BYTES && 128 * Layout<128>::PART_LD * 4 <= Layout<128>::PIPE_BYTES, "split sums");
+
+// fp32 accumulate, e4m3 x e4m3, both K-major, M = 128
+__host__ __device__ constexpr uint32_t idesc_e4m3(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(T_ROWS >> 4) << 24); }
+
+__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
+}
+
+__device__ __forceinline__ float bias_at(const Fp8Args& g, int n) {
+    return g.bias_dtype == MM_F32 ? ((const float*)g.bias)[n] : __bfloat162float(((const __nv_bfloat16*)g.bias)[n]);
+}
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// A tile: rows lo .. hi - 1 (of one group), first column of the result, first rows of W's two boxes, the scales' rows of W.
+struct Tile {
+    int m0, hi, n0, w0, w1;
+    const float *s0, *s1;
+};
+template <int BN, bool GLU>
+__device__ __forceinline__ Tile tile_of(const Fp8Args& g, int t, int m_tiles) {
+    Tile x;
+    const int mt = t % m_tiles, nt = t / m_tiles;
+    int e = 0;
+    if (g.tiles != nullptr) {
+        x.m0 = g.tiles[3 * mt];
+        x.hi = g.tiles[3 * mt + 1];
+        e = g.tiles[3 * mt + 2];
+    } else {
+        x.m0 = mt * T_ROWS;
+        x.hi = g.M;
+    }
+    if (GLU) {
+        x.n0 = nt * 128;
+        x.w0 = 2 * e * g.N + x.n0;
+        x.w1 = x.w0 + g.N;
+        x.s0 = g.sw + ((size_t)2 * e * g.NB + nt) * g.KB;
+        x.s1 = x.s0 + (size_t)g.NB * g.KB;
+    } else {
+        x.n0 = nt * BN;
+        x.w0 = e * g.N + x.n0;
+        x.w1 = x.w0 + 128;
+        const int nb = x.n0 / FP8_BLOCK;
+        x.s0 = g.sw + ((size_t)e * g.NB + nb) * g.KB;
+        x.s1 = g.sw + ((size_t)e * g.NB + min(nb + 1, g.NB - 1)) * g.KB;      // (columns from N on are not stored)
+    }
+    return x;
+}
+
+template <int BN, bool GLU, bool SPLIT>
+__global__ void __launch_bounds__(T_THREADS, 1)
+gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Fp8Args g) {
+    static_assert(!GLU || BN == 256, "a gated tile holds 128 columns of both matrices");
+    typedef Layout<BN> L;
+    constexpr int COLS = BN / 2;                   // columns a thread sums
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* pipe = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* staging = pipe + L::PIPE_BYTES;
+    Ctl* ctl = reinterpret_cast<Ctl*>(staging + SUM_WARPS * L::STAGING);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int* abort_flag = &ctl->abort_flag;
+
+    if (threadIdx.x == 0) {
+        prefetch_tensormap(&tmA);
+        prefetch_tensormap(&tmW);
+        for (int s = 0; s < L::STAGES; ++s) {
+            mbar_init(smem_u32(&ctl->full[s]), 1);
+            mbar_init(smem_u32(&ctl->empty[s]), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(smem_u32(&ctl->sum_full[a]), 1);
+            mbar_init(smem_u32(&ctl->sum_empty[a]), SUM_WARPS);
+        }
+        for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&ctl->pair[q]), 2);
+        ctl->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)), "r"(2 * BN) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = ctl->tmem_base;
+
+    const int m_tiles = g.tiles ? *g.n_tiles : (g.M + T_ROWS - 1) / T_ROWS, n_tiles = (g.N + (GLU ? 128 : BN) - 1) / (GLU ? 128 : BN);
+    const int total = m_tiles * n_tiles;
+    const int S = SPLIT ? g.S : 1, rank = SPLIT ? (int)cluster_ctarank() : 0;
+    const int first = SPLIT ? blockIdx.x / S : blockIdx.x, step = SPLIT ? 0x40000000 : (int)gridDim.x;      // a split tile has its cluster for itself
+    const int b_lo = SPLIT ? (int)((long long)g.KB * rank / S) : 0, b_hi = SPLIT ? (int)((long long)g.KB * (rank + 1) / S) : g.KB;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int t = first; t < total && ok; t += step) {
+                const Tile x = tile_of<BN, GLU>(g, t, m_tiles);
+                for (int b = b_lo; b < b_hi; ++b, ++it) {
+                    const int s = it % L::STAGES;
+                    if (!mbar_wait(smem_u32(&ctl->empty[s]), ((it / L::STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                    const uint32_t full = smem_u32(&ctl->full[s]), dst = smem_u32(pipe + s * L::STAGE_BYTES);
+                    mbar_expect_tx(full, L::STAGE_BYTES);
+                    tma_load_2d(dst, &tmA, b * FP8_BLOCK, x.m0, full);
+                    tma_load_2d(dst + HALF_BYTES, &tmW, b * FP8_BLOCK, x.w0, full);
+                    if (BN == 256) tma_load_2d(dst + 2 * HALF_BYTES, &tmW, b * FP8_BLOCK, x.w1, full);
+                }
+            }
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int t = first; t < total && ok; t += step)
+                for (int b = b_lo; b < b_hi; ++b, ++it) {
+                    const int s = it % L::STAGES, acc = it & 1;
+                    if (!mbar_wait(smem_u32(&ctl->sum_empty[acc]), ((it >> 1) & 1) ^ 1, abort_flag) ||
+                        !mbar_wait(smem_u32(&ctl->full[s]), (it / L::STAGES) & 1, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t a_addr = smem_u32(pipe + s * L::STAGE_BYTES);
+                    const uint64_t a_desc = smem_desc_sw128(a_addr, 16, 1024), b_desc = smem_desc_sw128(a_addr + HALF_BYTES, 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)          // 32 numbers a product: 32 bytes on along the swizzled rows
+                        umma_e4m3(tmem_base + acc * BN, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc_e4m3(BN), k ? 1u : 0u);
+                    umma_commit(smem_u32(&ctl->empty[s]));
+                    umma_commit(smem_u32(&ctl->sum_full[acc]));
+                }
+        }
+    } else {
+        const int q = warp & 3, half = warp >> 2;
+        const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
+        unsigned char* wstage = staging + warp * L::STAGING;
+        uint32_t it = 0, local = 0;
+        bool ok = true;
+        for (int t = first; t < total; t += step, ++local) {
+            const Tile x = tile_of<BN, GLU>(g, t, m_tiles);
+            const int row = x.m0 + q * 32 + lane;
+            const float* sa = g.sa + (size_t)min(row, x.hi - 1) * g.KB;
+            const float* sw = GLU || BN == 128 || half == 0 ? x.s0 : x.s1;
+            float acc[COLS];
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
+            float a_next = b_lo < b_hi ? sa[b_lo] : 0.0f, w_next = b_lo < b_hi ? sw[b_lo] : 0.0f, u_next = GLU && b_lo < b_hi ? x.s1[b_lo] : 0.0f;
+#pragma unroll 1
+            for (int b = b_lo; b < b_hi && ok; ++b, ++it) {
+                const uint32_t ph = it & 1;
+                const float s0 = a_next * w_next, s1 = GLU ? a_next * u_next : 0.0f;
+                if (b + 1 < b_hi) {
+                    a_next = sa[b + 1];
+                    w_next = sw[b + 1];
+                    if (GLU) u_next = x.s1[b + 1];
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->sum_full[ph]), (it >> 1) & 1, abort_flag));
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < COLS / 32; ++c) {
+                    // GLU: the thread's first half of sums is of the gate's columns, the second of the up projection's
+                    const int col = GLU ? (c < COLS / 64 ? half * 64 + c * 32 : 128 + half * 64 + (c - COLS / 64) * 32) : half * COLS + c * 32;
+                    uint32_t r[32];
+                    tmem_ld32(taddr + ph * BN + col, r);
+                    const float s = GLU && c >= COLS / 64 ? s1 : s0;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(s, __uint_as_float(r[i]), acc[c * 32 + i]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->sum_empty[ph]));
+            }
+            if (!ok) {
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) acc[i] = __uint_as_float(0x7fffffffu);
+            }
+            if (SPLIT) {
+                // this CTA's sums into its own shared memory: the copies have all been read by products that are through
+                float* part = reinterpret_cast<float*>(pipe) + (q * 32 + lane) * L::PART_LD;
+                if (row < x.hi) {
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        const int col = GLU ? (c < COLS / 64 ? half * 64 + c * 32 : 128 + half * 64 + (c - COLS / 64) * 32) : half * COLS + c * 32;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<float4*>(part + col + i) = make_float4(acc[c * 32 + i], acc[c * 32 + i + 1], acc[c * 32 + i + 2], acc[c * 32 + i + 3]);
+                    }
+                }
+            } else if (GLU) {
+                const float rs = g.row_scale && row < x.hi ? g.row_scale[g.order ? g.order[row] : row] : 1.0f;
+                uint32_t largest = 0;
+#pragma unroll
+                for (int i = 0; i < COLS / 2; ++i) {
+                    const float h = fp8_glu(acc[i], acc[COLS / 2 + i], g.act, g.limit, rs);
+                    acc[i] = x.n0 + half * 64 + i < g.N ? h : 0.0f;
+                    largest = max(largest, fp8_size_bits(acc[i]));
+                }
+                // the other half of the row's block is the warp's with the same rows
+                volatile uint32_t* sizes = reinterpret_cast<volatile uint32_t*>(staging);      // [tile parity][rows' quarter][half][row]
+                const int par = local & 1;
+                sizes[((par * 4 + q) * 2 + half) * 32 + lane] = largest;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->pair[q]));
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(smem_u32(&ctl->pair[q]), par, abort_flag));
+                const float s = ok ? fp8_scale_of(max(largest, sizes[((par * 4 + q) * 2 + (half ^ 1)) * 32 + lane])) : __uint_as_float(0x7fffffffu);
+                if (row < x.hi) {
+                    if (half == 0) g.out_scales[(size_t)row * g.NB + x.n0 / 128] = s;
+                    uint8_t* dst = (uint8_t*)g.out + (size_t)row * g.ldo + x.n0 + half * 64;
+#pragma unroll
+                    for (int i = 0; i < COLS / 2; i += 16) {
+                        uint32_t p[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            p[j] = fp8_pack4(__fdiv_rn(acc[i + 4 * j], s), __fdiv_rn(acc[i + 4 * j + 1], s), __fdiv_rn(acc[i + 4 * j + 2], s), __fdiv_rn(acc[i + 4 * j + 3], s));
+                        if (x.n0 + half * 64 + i < g.ldo) *reinterpret_cast<uint4*>(dst + i) = make_uint4(p[0], p[1], p[2], p[3]);
+                    }
+                }
+            } else {
+                // 128 bytes of 32 rows at a time through shared memory (16-byte unit u of row r at u ^ (r & 7)), so that stores are of whole rows
+                const bool f32 = g.out_kind == OUT_F32;
+                const int esz = f32 ? 4 : 2, per = 128 / esz, col_base = x.n0 + half * COLS;
+                const bool aligned = (((uintptr_t)g.out | ((size_t)g.ldo * esz)) & 15) == 0;
+#pragma unroll
+                for (int c = 0; c < COLS / 32; ++c) {
+                    const int col0 = col_base + c * 32;
+                    if (g.bias != nullptr) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (col0 + i < g.N) acc[c * 32 + i] += bias_at(g, col0 + i);
+                    }
+                    unsigned char* srow = wstage + lane * 128;
+                    if (f32) {
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            *reinterpret_cast<float4*>(srow + ((u ^ (lane & 7)) << 4)) =
+                                make_float4(acc[c * 32 + u * 4], acc[c * 32 + u * 4 + 1], acc[c * 32 + u * 4 + 2], acc[c * 32 + u * 4 + 3]);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            uint32_t p[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const __nv_bfloat162 v = __floats2bfloat162_rn(acc[c * 32 + u * 8 + 2 * j], acc[c * 32 + u * 8 + 2 * j + 1]);
+                                p[j] = *reinterpret_cast<const uint32_t*>(&v);
+                            }
+                            *reinterpret_cast<uint4*>(srow + ((((c & 1) * 4 + u) ^ (lane & 7)) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
+                        }
+                        if ((c & 1) == 0) continue;          // (COLS / 32 is even)
+                    }
+                    __syncwarp();
+                    const int cbase = f32 ? col0 : col0 - 32;          // the `per` columns that stand in the staging rows
+                    unsigned char* out = (unsigned char*)g.out;
+#pragma unroll 1
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = i * 4 + (lane >> 3), u = lane & 7, grow = x.m0 + q * 32 + r, gcol = cbase + u * (16 / esz);
+                        if (grow >= x.hi || gcol >= g.N) continue;
+                        const unsigned char* src = wstage + r * 128 + ((u ^ (r & 7)) << 4);
+                        unsigned char* dst = out + ((size_t)grow * g.ldo + gcol) * esz;
+                        if (aligned && gcol + 16 / esz <= g.N) {
+                            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+                        } else {
+                            const int n = min(16 / esz, g.N - gcol);
+                            for (int j = 0; j < n; ++j) {
+                                if (f32) reinterpret_cast<float*>(dst)[j] = reinterpret_cast<const float*>(src)[j];
+                                else reinterpret_cast<uint16_t*>(dst)[j] = reinterpret_cast<const uint16_t*>(src)[j];
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    (void)per;
+                }
+            }
+        }
+    }
+
+    if (SPLIT) {
+        __syncwarp();
+        pair_sync();               // every CTA's sums stand in its shared memory
+        if (warp < SUM_WARPS && first < total) {
+            const Tile x = tile_of<BN, GLU>(g, first, m_tiles);
+            const uint32_t base = smem_u32(pipe);
+            const int rows = min(T_ROWS, x.hi - x.m0);
+            for (int r = rank + S * warp; r < rows; r += S * SUM_WARPS) {
+                const int row = x.m0 + r;
+                const float rs = GLU && g.row_scale ? g.row_scale[g.order ? g.order[row] : row] : 1.0f;
+                float4 v[BN / 128];
+#pragma unroll
+                for (int j = 0; j < BN / 128; ++j) {
+                    const uint32_t at = base + (uint32_t)((r * L::PART_LD + j * 128 + lane * 4) * 4);
+                    v[j] = ld_cluster_f4(map_to_rank(at, 0));
+                    for (int p = 1; p < S; ++p) {
+                        const float4 o = ld_cluster_f4(map_to_rank(at, p));
+                        v[j].x += o.x; v[j].y += o.y; v[j].z += o.z; v[j].w += o.w;
+                    }
+                }
+                if (GLU) {
+                    const float4 ga = v[0], up = v[BN / 128 - 1];
+                    const int n = x.n0 + lane * 4;
+                    float h[4] = {fp8_glu(ga.x, up.x, g.act, g.limit, rs), fp8_glu(ga.y, up.y, g.act, g.limit, rs),
+                                  fp8_glu(ga.z, up.z, g.act, g.limit, rs), fp8_glu(ga.w, up.w, g.act, g.limit, rs)};
+                    uint32_t largest = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (n + i >= g.N) h[i] = 0.0f;
+                        largest = max(largest, fp8_size_bits(h[i]));
+                    }
+                    const float s = fp8_scale_of(__reduce_max_sync(0xffffffffu, largest));
+                    if (lane == 0) g.out_scales[(size_t)row * g.NB + x.n0 / 128] = s;
+                    if (n < g.ldo)
+                        *reinterpret_cast<uint32_t*>((uint8_t*)g.out + (size_t)row * g.ldo + n) =
+                            fp8_pack4(__fdiv_rn(h[0], s), __fdiv_rn(h[1], s), __fdiv_rn(h[2], s), __fdiv_rn(h[3], s));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < BN / 128; ++j) {
+                        const int n = x.n0 + j * 128 + lane * 4;
+                        const float y[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (n + i >= g.N) continue;
+                            const float z = g.bias ? y[i] + bias_at(g, n + i) : y[i];
+                            if (g.out_kind == OUT_F32) ((float*)g.out)[(size_t)row * g.ldo + n + i] = z;
+                            else ((__nv_bfloat16*)g.out)[(size_t)row * g.ldo + n + i] = __float2bfloat16_rn(z);
+                        }
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    }
+
+    if (*abort_flag) {
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (SPLIT) pair_sync();        // nobody leaves while another may read its shared memory
+    tc_fence_after();
+    if (threadIdx.x == 0 && ctl->abort_flag && g.err != nullptr) atomicExch(g.err, 1);
+    if (warp == 9) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN) : "memory");
+    }
+}
+
+template <int BN, bool GLU, bool SPLIT>
+int launch(const CUtensorMap& a, const CUtensorMap& w, const Fp8Args& g, int grid, cudaStream_t s) {
+    typedef Layout<BN> L;
+    constexpr size_t smem = (size_t)L::PIPE_BYTES + SUM_WARPS * L::STAGING + 1024 + sizeof(Ctl);
+    static_assert(smem <= 227 * 1024, "shared memory");
+    if (!mm_allow_smem<gemm_fp8_tcgen05_kernel<BN, GLU, SPLIT>>(smem)) {
+        mm_set_last_error("gemm_fp8: cannot reserve shared memory");
+        return MM_ERR_LAUNCH;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(T_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = SPLIT ? g.S : 1;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = SPLIT ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, gemm_fp8_tcgen05_kernel<BN, GLU, SPLIT>, a, w, g);
+    MM_CHECK_LAUNCH();
+    return MM_OK;
+}
+
+// rows x cols bytes, row stride ld; boxes of 128 x 128, 128-byte swizzle, noughts outside
+bool make_map_bytes(CUtensorMap* map, const void* base, long long rows, int cols, long long ld) {
+    EncodeTiledFn enc = get_encode();
+    if (enc == nullptr) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {128u, 128u};
+    cuuint32_t estr[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+// A e4m3 [M, lda], sa fp32 [M, KB]; W e4m3 [matrices * N, ldw], sw fp32 [matrices, NB, KB] (GLU: pairs of matrices, gate and up).
+// glu 0: out [M, ldo] bf16 or fp32 (+ bias [N]); glu 1: out e4m3 [M, ldo] (ldo = N rounded up to 16) and out_scales fp32 [M, NB].
+// tiles, n_tiles, max_tiles: the grouped form's row tiles.  wide: 256 columns a tile instead of 128 (GLU: always).  splits: CTAs that share a tile's
+// blocks (1, 2, 4 or 8; only without a list).
+MM_EXPORT int mm_gemm_fp8_tcgen05(const void* A, long long lda, const void* sa, const void* W, long long ldw, const void* sw, int matrices, void* out,
+                                  int out_dtype, void* out_scales, int ldo, const void* bias, int bias_dtype, int M, int N, int K, int glu, int act, float limit,
+                                  const void* row_scale, const void* order, const void* tiles, const void* n_tiles, int max_tiles, int wide, int splits,
+                                  void* err, void* stream) {
+    MM_REQUIRE(M > 0 && N > 0 && K > 0 && matrices > 0 && lda >= K && ldw >= K && ldo >= N, "gemm_fp8: bad sizes");
+    MM_REQUIRE(lda % 16 == 0 && ldw % 16 == 0 && (((uintptr_t)A | (uintptr_t)W) & 15) == 0, "gemm_fp8: rows must start on 16-byte boundaries");
+    MM_REQUIRE((long long)matrices * N + 256 < 0x7fffffffLL, "gemm_fp8: too many weight rows");
+    MM_REQUIRE(out_dtype == MM_F32 || out_dtype == MM_BF16, "gemm_fp8: the result is bf16 or fp32");
+    MM_REQUIRE(!glu || (matrices % 2 == 0 && act >= 0 && act <= MM_GLU_GELU_TANH && ldo % 16 == 0 && ((uintptr_t)out & 15) == 0 && out_scales && !bias),
+               "gemm_fp8: bad gated product");
+    MM_REQUIRE(splits == 1 || splits == 2 || splits == 4 || splits == 8, "gemm_fp8: 1, 2, 4 or 8 splits");
+    MM_REQUIRE(tiles == nullptr || (n_tiles && max_tiles > 0 && splits == 1), "gemm_fp8: a grouped product has a list and no splits");
+    CUtensorMap ta, tw;
+    if (!make_map_bytes(&ta, A, M, K, lda) || !make_map_bytes(&tw, W, (long long)matrices * N, K, ldw)) {
+        mm_set_last_error("gemm_fp8: cuTensorMapEncodeTiled failed or is not available");
+        return MM_ERR_DRIVER;
+    }
+    Fp8Args g = {};
+    g.out = out;
+    g.out_scales = (float*)out_scales;
+    g.sa = (const float*)sa;
+    g.sw = (const float*)sw;
+    g.bias = bias;
+    g.row_scale = (const float*)row_scale;
+    g.order = (const int32_t*)order;
+    g.tiles = (const int32_t*)tiles;
+    g.n_tiles = (const int32_t*)n_tiles;
+    g.err = (int*)err;
+    g.out_kind = out_dtype == MM_F32 ? OUT_F32 : OUT_BF16;
+    g.bias_dtype = bias_dtype;
+    g.act = act;
+    g.limit = limit;
+    g.M = M;
+    g.N = N;
+    g.K = K;
+    g.KB = ceil_div(K, FP8_BLOCK);
+    g.NB = ceil_div(N, FP8_BLOCK);
+    g.ldo = ldo;
+    g.S = splits;
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int bn = glu ? 128 : (wide ? 256 : 128);
+    const long long total = (long long)(tiles ? max_tiles : ceil_div(M, T_ROWS)) * ceil_div(N, bn);
+    MM_REQUIRE(total < 0x40000000LL, "gemm_fp8: too many tiles");
+    cudaStream_t s = (cudaStream_t)stream;
+    const int grid = splits > 1 ? (int)total * splits : (int)(total < sms ? total : sms);
+    if (glu) return splits > 1 ? launch<256, true, true>(ta, tw, g, grid, s) : launch<256, true, false>(ta, tw, g, grid, s);
+    if (wide) return splits > 1 ? launch<256, false, true>(ta, tw, g, grid, s) : launch<256, false, false>(ta, tw, g, grid, s);
+    return splits > 1 ? launch<128, false, true>(ta, tw, g, grid, s) : launch<128, false, false>(ta, tw, g, grid, s);
+}

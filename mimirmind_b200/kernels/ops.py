@@ -2139,16 +2139,51 @@ def _fp8_rows_of(x, k: int, what: str) -> Fp8Rows:
     return x
 
 
-def _fp8_product(x: Fp8Rows, w: Fp8Weight, out: torch.Tensor, glu: bool = False, bias=None, rows: Optional["ExpertRows"] = None, act: int = 0,
-                 limit: float = 0.0, row_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+FP8_SMS = 148
+
+
+def _fp8_plan(m: int, n: int, k: int, glu: bool):
+    """(256 columns a tile, CTAs that share a tile's blocks)"""
+    m_tiles, blocks = -(-m // 128), _blocks(k)
+    if not glu and m_tiles * -(-n // 256) >= FP8_SMS:
+        return True, 1
+    tiles = m_tiles * -(-n // 128)
+    splits = 1
+    while splits < 8 and tiles * splits * 2 <= FP8_SMS and blocks >= splits * 4:
+        splits *= 2
+    return glu, splits
+
+
+def _fp8_gemm(x: Fp8Rows, w: Fp8Weight, out: torch.Tensor, out_scales: Optional[torch.Tensor], bias, rows: Optional["ExpertRows"], act: int,
+              limit: float, row_scale: Optional[torch.Tensor]) -> None:
     _here("gemm_fp8", x.values, x.scales, w.values, w.scales, bias, row_scale)
     m, k = x.shape
     n = w.shape[-2]
-    check(_lib.load().mm_gemm_fp8_simple(x.values.data_ptr(), x.values.stride(0) if m > 1 else -(-k // 16) * 16, x.scales.data_ptr(), w.values.data_ptr(),
-                                         w.ld, w.scales.data_ptr(), out.data_ptr(), dtype_code(out.dtype), out.shape[1],
-                                         _ptr(bias), dtype_code(bias.dtype) if bias is not None else F32, m, n, k, int(glu),
-                                         rows.tiles.data_ptr() if rows else None, rows.n_tiles.data_ptr() if rows else None, rows.max_tiles if rows else 0,
-                                         act, float(limit), _ptr(row_scale), rows.order.data_ptr() if rows else None, _stream()), "gemm_fp8")
+    glu = out_scales is not None
+    wide, splits = (True, 1) if rows is not None else _fp8_plan(m, n, k, glu)
+    ldo = out.stride(0) if m > 1 else (-(-n // 16) * 16 if glu else n)
+    check(_lib.load().mm_gemm_fp8_tcgen05(x.values.data_ptr(), x.values.stride(0) if m > 1 else -(-k // 16) * 16, x.scales.data_ptr(), w.values.data_ptr(),
+                                          w.ld, w.scales.data_ptr(), w.values.numel() // (n * k), out.data_ptr(), F32 if out.dtype == torch.float32 else BF16,
+                                          _ptr(out_scales), ldo, _ptr(bias), dtype_code(bias.dtype) if bias is not None else F32, m, n, k, int(glu),
+                                          act, float(limit), _ptr(row_scale), rows.order.data_ptr() if rows else None,
+                                          rows.tiles.data_ptr() if rows else None, rows.n_tiles.data_ptr() if rows else None, rows.max_tiles if rows else 0,
+                                          int(wide), splits, tcgen05_error_flag(w.values.device).data_ptr(), _stream()), "gemm_fp8")
+
+
+def _fp8_product(x: Fp8Rows, w: Fp8Weight, out_dtype: torch.dtype, bias=None, rows: Optional["ExpertRows"] = None) -> torch.Tensor:
+    out = torch.empty((x.shape[0], w.shape[-2]), dtype=out_dtype, device=w.values.device)
+    if x.shape[0]:
+        _fp8_gemm(x, w, out, None, bias, rows, 0, 0.0, None)
+    return out
+
+
+def _fp8_hidden(x: Fp8Rows, w_in: Fp8Weight, act: int, limit: float, rows: Optional["ExpertRows"] = None, row_scale=None) -> Fp8Rows:
+    """act(gate, up) of pairs of matrices [..., 2, F, K], quantised from its fp32 values."""
+    m, f = x.shape[0], w_in.shape[-2]
+    dev = w_in.values.device
+    out = Fp8Rows(_fp8_buffer(m, f, device=dev), torch.empty((m, _blocks(f)), dtype=torch.float32, device=dev))
+    if m:
+        _fp8_gemm(x, w_in, out.values, out.scales, None, rows, act, limit, row_scale)
     return out
 
 
@@ -2167,7 +2202,7 @@ def gemm_fp8(x, w: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: to
     dtype_code(out_dtype)
     _here("gemm_fp8", w.values, w.scales, bias)
     x = _fp8_rows_of(x, k, "gemm_fp8")
-    return _fp8_product(x, w, torch.empty((x.shape[0], n), dtype=out_dtype, device=w.values.device), bias=bias)
+    return _fp8_product(x, w, out_dtype, bias)
 
 
 def _glu_code(activation: str, limit: float, what: str) -> int:
@@ -2188,8 +2223,7 @@ def glu_mlp_fp8(x, w_in: Fp8Weight, w_out: Fp8Weight, activation: str = "silu", 
     _here("glu_mlp_fp8", w_in.values, w_in.scales, w_out.values, w_out.scales)
     f, k = w_in.shape[1:]
     x = _fp8_rows_of(x, k, "glu_mlp_fp8")
-    hidden = _fp8_product(x, w_in, torch.empty((x.shape[0], f), dtype=torch.float32, device=w_in.values.device), glu=True, act=act, limit=limit)
-    return gemm_fp8(hidden, w_out)
+    return _fp8_product(_fp8_hidden(x, w_in, act, limit), w_out, torch.bfloat16)
 
 
 def _check_experts_fp8(x: torch.Tensor, w_in: Fp8Weight, w_out: Fp8Weight, what: str) -> None:
@@ -2225,7 +2259,6 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, wts: torch.Tensor, w_in:
     rows = moe_sort(idx, E, with_tiles=True)
     sorted_x = quantize_fp8_rows(x, rows.row_token)
     on_input = weight_on == "input"
-    hidden = _fp8_product(sorted_x, w_in, torch.empty((n * top, f), dtype=torch.float32, device=x.device), glu=True, rows=rows, act=act, limit=limit,
-                          row_scale=wts if on_input else None)
-    y = _fp8_product(quantize_fp8_rows(hidden), w_out, torch.empty((n * top, d), dtype=torch.float32, device=x.device), rows=rows)
+    hidden = _fp8_hidden(sorted_x, w_in, act, limit, rows, wts if on_input else None)
+    y = _fp8_product(hidden, w_out, torch.float32, rows=rows)
     return moe_combine(y, None if on_input else wts, torch.bfloat16, place=rows.place, top=top)
