@@ -25,7 +25,11 @@ namespace {
 
 using namespace tc;
 
-constexpr int T_ROWS = 128, T_THREADS = 320, SUM_WARPS = 8;
+constexpr int T_ROWS = 128, T_THREADS = 384, SUM_WARPS = 8;      // (two warps of the last warpgroup have no role)
+// A summing thread of a 256-column tile holds 128 sums and two pieces of 32 on their way: registers move from the last warpgroup to the others.
+// 256 x 224 + 128 x 56 = 384 x 168, what the block starts with (the launch checks that).
+constexpr int START_REGS = 168, SUM_REGS = 224, OTHER_REGS = 56;
+static_assert(256 * SUM_REGS + 128 * OTHER_REGS <= 384 * START_REGS, "registers");
 constexpr int HALF_BYTES = 128 * 128;              // 128 rows of 128 bytes
 enum { OUT_BF16 = 0, OUT_F32 = 1 };
 
@@ -72,6 +76,37 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
+}
+
+// a tensor-memory load on its way, and the wait for it (all earlier ones of the warp): the values may only be used behind it
+__device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait32(uint32_t* r) {
+    asm volatile(
+        "tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+          "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+          "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+          "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+        :: "memory");
+}
+// two sums in one instruction: a += s x, b += s y
+__device__ __forceinline__ void fma_pair(float& a, float& b, float s, uint32_t x, uint32_t y) {
+    asm("{\n\t.reg .b64 p, q, r;\n\t"
+        "mov.b64 p, {%2, %3};\n\t"
+        "mov.b64 q, {%4, %4};\n\t"
+        "mov.b64 r, {%0, %1};\n\t"
+        "fma.rn.f32x2 r, p, q, r;\n\t"
+        "mov.b64 {%0, %1}, r;\n\t}"
+        : "+f"(a), "+f"(b) : "r"(x), "r"(y), "f"(s));
 }
 
 __device__ __forceinline__ float bias_at(const Fp8Args& g, int n) {
@@ -131,6 +166,8 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     Ctl* ctl = reinterpret_cast<Ctl*>(staging + SUM_WARPS * L::STAGING);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &ctl->abort_flag;
+    // the tile's column of a thread's piece c.  GLU: the first half of its sums is of the gate's columns, the second of the up projection's
+    auto column = [](int c, int half) { return GLU ? (c < COLS / 64 ? half * 64 + c * 32 : 128 + half * 64 + (c - COLS / 64) * 32) : half * COLS + c * 32; };
 
     if (threadIdx.x == 0) {
         prefetch_tensormap(&tmA);
@@ -163,43 +200,51 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     const int first = SPLIT ? blockIdx.x / S : blockIdx.x, step = SPLIT ? 0x40000000 : (int)gridDim.x;      // a split tile has its cluster for itself
     const int b_lo = SPLIT ? (int)((long long)g.KB * rank / S) : 0, b_hi = SPLIT ? (int)((long long)g.KB * (rank + 1) / S) : g.KB;
 
-    if (warp == 8) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (int t = first; t < total && ok; t += step) {
-                const Tile x = tile_of<BN, GLU>(g, t, m_tiles);
-                for (int b = b_lo; b < b_hi; ++b, ++it) {
-                    const int s = it % L::STAGES;
-                    if (!mbar_wait(smem_u32(&ctl->empty[s]), ((it / L::STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                    const uint32_t full = smem_u32(&ctl->full[s]), dst = smem_u32(pipe + s * L::STAGE_BYTES);
-                    mbar_expect_tx(full, L::STAGE_BYTES);
-                    tma_load_2d(dst, &tmA, b * FP8_BLOCK, x.m0, full);
-                    tma_load_2d(dst + HALF_BYTES, &tmW, b * FP8_BLOCK, x.w0, full);
-                    if (BN == 256) tma_load_2d(dst + 2 * HALF_BYTES, &tmW, b * FP8_BLOCK, x.w1, full);
+    if (warp >= SUM_WARPS) {
+        if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+        if (warp == 8) {
+            if (lane == 0) {
+                uint32_t it = 0;
+                bool ok = true;
+                for (int t = first; t < total && ok; t += step) {
+                    const Tile x = tile_of<BN, GLU>(g, t, m_tiles);
+                    for (int b = b_lo; b < b_hi; ++b, ++it) {
+                        const int s = it % L::STAGES;
+                        if (!mbar_wait(smem_u32(&ctl->empty[s]), ((it / L::STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                        const uint32_t full = smem_u32(&ctl->full[s]), dst = smem_u32(pipe + s * L::STAGE_BYTES);
+                        mbar_expect_tx(full, L::STAGE_BYTES);
+                        tma_load_2d(dst, &tmA, b * FP8_BLOCK, x.m0, full);
+                        tma_load_2d(dst + HALF_BYTES, &tmW, b * FP8_BLOCK, x.w0, full);
+                        if (BN == 256) tma_load_2d(dst + 2 * HALF_BYTES, &tmW, b * FP8_BLOCK, x.w1, full);
+                    }
                 }
             }
-        }
-    } else if (warp == 9) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (int t = first; t < total && ok; t += step)
-                for (int b = b_lo; b < b_hi; ++b, ++it) {
-                    const int s = it % L::STAGES, acc = it & 1;
-                    if (!mbar_wait(smem_u32(&ctl->sum_empty[acc]), ((it >> 1) & 1) ^ 1, abort_flag) ||
-                        !mbar_wait(smem_u32(&ctl->full[s]), (it / L::STAGES) & 1, abort_flag)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t a_addr = smem_u32(pipe + s * L::STAGE_BYTES);
-                    const uint64_t a_desc = smem_desc_sw128(a_addr, 16, 1024), b_desc = smem_desc_sw128(a_addr + HALF_BYTES, 16, 1024);
+        } else if (warp == 9) {
+            if (lane == 0) {
+                uint32_t it = 0;
+                bool ok = true;
+                for (int t = first; t < total && ok; t += step)
+                    for (int b = b_lo; b < b_hi; ++b, ++it) {
+                        const int s = it % L::STAGES, acc = it & 1;
+                        if (!mbar_wait(smem_u32(&ctl->sum_empty[acc]), ((it >> 1) & 1) ^ 1, abort_flag) ||
+                            !mbar_wait(smem_u32(&ctl->full[s]), (it / L::STAGES) & 1, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t a_addr = smem_u32(pipe + s * L::STAGE_BYTES);
+                        const uint64_t a_desc = smem_desc_sw128(a_addr, 16, 1024), b_desc = smem_desc_sw128(a_addr + HALF_BYTES, 16, 1024);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)          // 32 numbers a product: 32 bytes on along the swizzled rows
-                        umma_e4m3(tmem_base + acc * BN, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc_e4m3(BN), k ? 1u : 0u);
-                    umma_commit(smem_u32(&ctl->empty[s]));
-                    umma_commit(smem_u32(&ctl->sum_full[acc]));
-                }
+                        for (int k = 0; k < 4; ++k)          // 32 numbers a product: 32 bytes on along the swizzled rows
+                            umma_e4m3(tmem_base + acc * BN, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc_e4m3(BN), k ? 1u : 0u);
+                        umma_commit(smem_u32(&ctl->empty[s]));
+                        umma_commit(smem_u32(&ctl->sum_full[acc]));
+                    }
+            }
+        }
+        if (SPLIT) {
+            __syncwarp();
+            pair_sync();
         }
     } else {
+        if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SUM_REGS));
         const int q = warp & 3, half = warp >> 2;
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
         unsigned char* wstage = staging + warp * L::STAGING;
@@ -226,19 +271,23 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->sum_full[ph]), (it >> 1) & 1, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
+                // a piece of 32 columns is multiplied while the next is on its way; the accumulator is free once the last has arrived
+                uint32_t r[2][32];
+                tmem_ld32_issue(taddr + ph * BN + column(0, half), r[0]);
 #pragma unroll
                 for (int c = 0; c < COLS / 32; ++c) {
-                    // GLU: the thread's first half of sums is of the gate's columns, the second of the up projection's
-                    const int col = GLU ? (c < COLS / 64 ? half * 64 + c * 32 : 128 + half * 64 + (c - COLS / 64) * 32) : half * COLS + c * 32;
-                    uint32_t r[32];
-                    tmem_ld32(taddr + ph * BN + col, r);
+                    tmem_wait32(r[c & 1]);
+                    if (c + 1 < COLS / 32) {
+                        tmem_ld32_issue(taddr + ph * BN + column(c + 1, half), r[(c + 1) & 1]);
+                    } else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&ctl->sum_empty[ph]));
+                    }
                     const float s = GLU && c >= COLS / 64 ? s1 : s0;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(s, __uint_as_float(r[i]), acc[c * 32 + i]);
+                    for (int i = 0; i < 32; i += 2) fma_pair(acc[c * 32 + i], acc[c * 32 + i + 1], s, r[c & 1][i], r[c & 1][i + 1]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&ctl->sum_empty[ph]));
             }
             if (!ok) {
 #pragma unroll
@@ -250,7 +299,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 if (row < x.hi) {
 #pragma unroll
                     for (int c = 0; c < COLS / 32; ++c) {
-                        const int col = GLU ? (c < COLS / 64 ? half * 64 + c * 32 : 128 + half * 64 + (c - COLS / 64) * 32) : half * COLS + c * 32;
+                        const int col = column(c, half);
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
                             *reinterpret_cast<float4*>(part + col + i) = make_float4(acc[c * 32 + i], acc[c * 32 + i + 1], acc[c * 32 + i + 2], acc[c * 32 + i + 3]);
@@ -341,61 +390,60 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 }
             }
         }
-    }
-
-    if (SPLIT) {
-        __syncwarp();
-        pair_sync();               // every CTA's sums stand in its shared memory
-        if (warp < SUM_WARPS && first < total) {
-            const Tile x = tile_of<BN, GLU>(g, first, m_tiles);
-            const uint32_t base = smem_u32(pipe);
-            const int rows = min(T_ROWS, x.hi - x.m0);
-            for (int r = rank + S * warp; r < rows; r += S * SUM_WARPS) {
-                const int row = x.m0 + r;
-                const float rs = GLU && g.row_scale ? g.row_scale[g.order ? g.order[row] : row] : 1.0f;
-                float4 v[BN / 128];
-#pragma unroll
-                for (int j = 0; j < BN / 128; ++j) {
-                    const uint32_t at = base + (uint32_t)((r * L::PART_LD + j * 128 + lane * 4) * 4);
-                    v[j] = ld_cluster_f4(map_to_rank(at, 0));
-                    for (int p = 1; p < S; ++p) {
-                        const float4 o = ld_cluster_f4(map_to_rank(at, p));
-                        v[j].x += o.x; v[j].y += o.y; v[j].z += o.z; v[j].w += o.w;
-                    }
-                }
-                if (GLU) {
-                    const float4 ga = v[0], up = v[BN / 128 - 1];
-                    const int n = x.n0 + lane * 4;
-                    float h[4] = {fp8_glu(ga.x, up.x, g.act, g.limit, rs), fp8_glu(ga.y, up.y, g.act, g.limit, rs),
-                                  fp8_glu(ga.z, up.z, g.act, g.limit, rs), fp8_glu(ga.w, up.w, g.act, g.limit, rs)};
-                    uint32_t largest = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (n + i >= g.N) h[i] = 0.0f;
-                        largest = max(largest, fp8_size_bits(h[i]));
-                    }
-                    const float s = fp8_scale_of(__reduce_max_sync(0xffffffffu, largest));
-                    if (lane == 0) g.out_scales[(size_t)row * g.NB + x.n0 / 128] = s;
-                    if (n < g.ldo)
-                        *reinterpret_cast<uint32_t*>((uint8_t*)g.out + (size_t)row * g.ldo + n) =
-                            fp8_pack4(__fdiv_rn(h[0], s), __fdiv_rn(h[1], s), __fdiv_rn(h[2], s), __fdiv_rn(h[3], s));
-                } else {
+        if (SPLIT) {
+            __syncwarp();
+            pair_sync();               // every CTA's sums stand in its shared memory
+            if (first < total) {
+                const Tile x = tile_of<BN, GLU>(g, first, m_tiles);
+                const uint32_t base = smem_u32(pipe);
+                const int rows = min(T_ROWS, x.hi - x.m0);
+                for (int r = rank + S * warp; r < rows; r += S * SUM_WARPS) {
+                    const int row = x.m0 + r;
+                    const float rs = GLU && g.row_scale ? g.row_scale[g.order ? g.order[row] : row] : 1.0f;
+                    float4 v[BN / 128];
 #pragma unroll
                     for (int j = 0; j < BN / 128; ++j) {
-                        const int n = x.n0 + j * 128 + lane * 4;
-                        const float y[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+                        const uint32_t at = base + (uint32_t)((r * L::PART_LD + j * 128 + lane * 4) * 4);
+                        v[j] = ld_cluster_f4(map_to_rank(at, 0));
+                        for (int p = 1; p < S; ++p) {
+                            const float4 o = ld_cluster_f4(map_to_rank(at, p));
+                            v[j].x += o.x; v[j].y += o.y; v[j].z += o.z; v[j].w += o.w;
+                        }
+                    }
+                    if (GLU) {
+                        const float4 ga = v[0], up = v[BN / 128 - 1];
+                        const int n = x.n0 + lane * 4;
+                        float h[4] = {fp8_glu(ga.x, up.x, g.act, g.limit, rs), fp8_glu(ga.y, up.y, g.act, g.limit, rs),
+                                      fp8_glu(ga.z, up.z, g.act, g.limit, rs), fp8_glu(ga.w, up.w, g.act, g.limit, rs)};
+                        uint32_t largest = 0;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            if (n + i >= g.N) continue;
-                            const float z = g.bias ? y[i] + bias_at(g, n + i) : y[i];
-                            if (g.out_kind == OUT_F32) ((float*)g.out)[(size_t)row * g.ldo + n + i] = z;
-                            else ((__nv_bfloat16*)g.out)[(size_t)row * g.ldo + n + i] = __float2bfloat16_rn(z);
+                            if (n + i >= g.N) h[i] = 0.0f;
+                            largest = max(largest, fp8_size_bits(h[i]));
+                        }
+                        const float s = fp8_scale_of(__reduce_max_sync(0xffffffffu, largest));
+                        if (lane == 0) g.out_scales[(size_t)row * g.NB + x.n0 / 128] = s;
+                        if (n < g.ldo)
+                            *reinterpret_cast<uint32_t*>((uint8_t*)g.out + (size_t)row * g.ldo + n) =
+                                fp8_pack4(__fdiv_rn(h[0], s), __fdiv_rn(h[1], s), __fdiv_rn(h[2], s), __fdiv_rn(h[3], s));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < BN / 128; ++j) {
+                            const int n = x.n0 + j * 128 + lane * 4;
+                            const float y[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if (n + i >= g.N) continue;
+                                const float z = g.bias ? y[i] + bias_at(g, n + i) : y[i];
+                                if (g.out_kind == OUT_F32) ((float*)g.out)[(size_t)row * g.ldo + n + i] = z;
+                                else ((__nv_bfloat16*)g.out)[(size_t)row * g.ldo + n + i] = __float2bfloat16_rn(z);
+                            }
                         }
                     }
                 }
             }
+            __syncwarp();
         }
-        __syncwarp();
     }
 
     if (*abort_flag) {
@@ -419,6 +467,18 @@ int launch(const CUtensorMap& a, const CUtensorMap& w, const Fp8Args& g, int gri
     if (!mm_allow_smem<gemm_fp8_tcgen05_kernel<BN, GLU, SPLIT>>(smem)) {
         mm_set_last_error("gemm_fp8: cannot reserve shared memory");
         return MM_ERR_LAUNCH;
+    }
+    if (BN == 256) {
+        static std::atomic<int> regs{0};          // a register split above what the block starts with would never be granted
+        if (regs.load(std::memory_order_relaxed) == 0) {
+            cudaFuncAttributes at;
+            if (cudaFuncGetAttributes(&at, gemm_fp8_tcgen05_kernel<BN, GLU, SPLIT>) != cudaSuccess) {
+                mm_set_last_error("gemm_fp8: cannot read the kernel's attributes");
+                return MM_ERR_LAUNCH;
+            }
+            regs.store(at.numRegs, std::memory_order_relaxed);
+        }
+        MM_REQUIRE(regs.load(std::memory_order_relaxed) == START_REGS, "gemm_fp8: built with another number of registers than the split wants");
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
