@@ -26,10 +26,12 @@ namespace {
 using namespace tc;
 
 constexpr int T_ROWS = 128, T_THREADS = 384, SUM_WARPS = 8;      // (two warps of the last warpgroup have no role)
-// A summing thread of a 256-column tile holds 128 sums and two pieces of 32 on their way: registers move from the last warpgroup to the others.
-// 256 x 224 + 128 x 56 = 384 x 168, what the block starts with (the launch checks that).
+constexpr int PIECE = 32;                                        // columns that a summing warp has on their way from tensor memory
+// A summing thread of a 256-column tile holds 128 sums and two pieces: registers move from the last warpgroup to the others.
+// 256 x 224 + 128 x 56 = 384 x 168, what the block starts with (the launch checks that).  Sixteen summing warps of half the columns, which 112
+// registers each allow, were slower (2,048 x 4,736 x 13,824: 218 us against 178).
 constexpr int START_REGS = 168, SUM_REGS = 224, OTHER_REGS = 56;
-static_assert(256 * SUM_REGS + 128 * OTHER_REGS <= 384 * START_REGS, "registers");
+static_assert(SUM_WARPS * 32 * SUM_REGS + 128 * OTHER_REGS <= T_THREADS * START_REGS, "registers");
 constexpr int HALF_BYTES = 128 * 128;              // 128 rows of 128 bytes
 enum { OUT_BF16 = 0, OUT_F32 = 1 };
 
@@ -54,14 +56,14 @@ struct Layout {
     static constexpr int STAGE_BYTES = HALF_BYTES * (1 + BN / 128);
     static constexpr int STAGES = BN == 256 ? 4 : 6;
     static constexpr int PIPE_BYTES = STAGES * STAGE_BYTES;
-    static constexpr int STAGING = 4096;           // per warp: 32 rows of 128 bytes
+    static constexpr int STAGING = 2048;           // per warp: 32 rows of 64 bytes
     static constexpr int PART_LD = BN + 4;         // floats of a row of a split tile's sums
 };
 
 struct Ctl {
     uint64_t full[6], empty[6];
     uint64_t sum_full[2], sum_empty[2];
-    uint64_t pair[4];                              // two warps that hold a row's halves
+    uint64_t row_known[4];                         // the two warps that hold a row's parts (GLU)
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -78,36 +80,28 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
 }
 
-// a tensor-memory load on its way, and the wait for it (all earlier ones of the warp): the values may only be used behind it
+// a tensor-memory load on its way, and the wait for it (and all earlier ones of the warp): the values may only be used behind it
 __device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_wait32(uint32_t* r) {
-    asm volatile(
-        "tcgen05.wait::ld.sync.aligned;"
-        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-          "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
-          "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
-          "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-        :: "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :: "memory");
 }
-// two sums in one instruction: a += s x, b += s y
-__device__ __forceinline__ void fma_pair(float& a, float& b, float s, uint32_t x, uint32_t y) {
-    asm("{\n\t.reg .b64 p, q, r;\n\t"
-        "mov.b64 p, {%2, %3};\n\t"
-        "mov.b64 q, {%4, %4};\n\t"
-        "mov.b64 r, {%0, %1};\n\t"
-        "fma.rn.f32x2 r, p, q, r;\n\t"
-        "mov.b64 {%0, %1}, r;\n\t}"
-        : "+f"(a), "+f"(b) : "r"(x), "r"(y), "f"(s));
+// two sums in one instruction: (a, b) += s (x, y), s = (s, s)
+__device__ __forceinline__ void fma_pair(uint64_t& ab, uint64_t s, uint32_t x, uint32_t y) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(ab) : "l"(((uint64_t)y << 32) | x), "l"(s));
 }
+__device__ __forceinline__ uint64_t twice(float s) { return ((uint64_t)__float_as_uint(s) << 32) | __float_as_uint(s); }
 
 __device__ __forceinline__ float bias_at(const Fp8Args& g, int n) {
     return g.bias_dtype == MM_F32 ? ((const float*)g.bias)[n] : __bfloat162float(((const __nv_bfloat16*)g.bias)[n]);
@@ -154,20 +148,43 @@ __device__ __forceinline__ Tile tile_of(const Fp8Args& g, int t, int m_tiles) {
     return x;
 }
 
+// 64 bytes of 32 rows on their way to memory: 16-byte unit u of row r at u ^ (r / 2 & 3), so that neither side meets bank conflicts
+__device__ __forceinline__ unsigned char* staged(unsigned char* base, int r, int u) { return base + r * 64 + ((u ^ ((r >> 1) & 3)) << 4); }
+
+template <typename T>
+__device__ __forceinline__ void store_staged(unsigned char* base, int lane, T* out, int ldo, int row0, int hi, int col0, int N) {
+    constexpr int PER = 64 / sizeof(T), UNIT = 16 / sizeof(T);
+    __syncwarp();
+    if ((((uintptr_t)out | ((size_t)ldo * sizeof(T))) & 15) == 0 && col0 + PER <= N) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2), u = lane & 3;
+            if (row0 + r < hi) *reinterpret_cast<uint4*>(out + (size_t)(row0 + r) * ldo + col0 + u * UNIT) = *reinterpret_cast<const uint4*>(staged(base, r, u));
+        }
+    } else {          // rows that start anywhere, or columns that end here: number by number, neighbours side by side
+#pragma unroll 4
+        for (int i = lane; i < 32 * PER; i += 32) {
+            const int r = i / PER, c = i % PER;
+            if (row0 + r < hi && col0 + c < N) out[(size_t)(row0 + r) * ldo + col0 + c] = reinterpret_cast<const T*>(staged(base, r, c / UNIT))[c % UNIT];
+        }
+    }
+    __syncwarp();
+}
+
 template <int BN, bool GLU, bool SPLIT>
 __global__ void __launch_bounds__(T_THREADS, 1)
 gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Fp8Args g) {
     static_assert(!GLU || BN == 256, "a gated tile holds 128 columns of both matrices");
     typedef Layout<BN> L;
-    constexpr int COLS = BN / 2;                   // columns a thread sums
+    constexpr int COLS = BN / 2, PIECES = COLS / PIECE;      // columns a thread sums
     extern __shared__ unsigned char smem_raw[];
     unsigned char* pipe = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* staging = pipe + L::PIPE_BYTES;
     Ctl* ctl = reinterpret_cast<Ctl*>(staging + SUM_WARPS * L::STAGING);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &ctl->abort_flag;
-    // the tile's column of a thread's piece c.  GLU: the first half of its sums is of the gate's columns, the second of the up projection's
-    auto column = [](int c, int half) { return GLU ? (c < COLS / 64 ? half * 64 + c * 32 : 128 + half * 64 + (c - COLS / 64) * 32) : half * COLS + c * 32; };
+    // the tile's column of a thread's piece.  GLU: the first half of its sums is of the gate's columns, the second of the up projection's
+    auto column = [](int c, int part) { return GLU ? (c < PIECES / 2 ? part * (COLS / 2) + c * PIECE : 128 + part * (COLS / 2) + (c - PIECES / 2) * PIECE) : part * COLS + c * PIECE; };
 
     if (threadIdx.x == 0) {
         prefetch_tensormap(&tmA);
@@ -180,12 +197,12 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             mbar_init(smem_u32(&ctl->sum_full[a]), 1);
             mbar_init(smem_u32(&ctl->sum_empty[a]), SUM_WARPS);
         }
-        for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&ctl->pair[q]), 2);
+        for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&ctl->row_known[q]), 2);
         ctl->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == SUM_WARPS + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)), "r"(2 * BN) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -202,7 +219,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
 
     if (warp >= SUM_WARPS) {
         if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-        if (warp == 8) {
+        if (warp == SUM_WARPS) {
             if (lane == 0) {
                 uint32_t it = 0;
                 bool ok = true;
@@ -219,7 +236,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                     }
                 }
             }
-        } else if (warp == 9) {
+        } else if (warp == SUM_WARPS + 1) {
             if (lane == 0) {
                 uint32_t it = 0;
                 bool ok = true;
@@ -234,7 +251,6 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
 #pragma unroll
                         for (int k = 0; k < 4; ++k)          // 32 numbers a product: 32 bytes on along the swizzled rows
                             umma_e4m3(tmem_base + acc * BN, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc_e4m3(BN), k ? 1u : 0u);
-                        umma_commit(smem_u32(&ctl->empty[s]));
                         umma_commit(smem_u32(&ctl->sum_full[acc]));
                     }
             }
@@ -245,7 +261,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         }
     } else {
         if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SUM_REGS));
-        const int q = warp & 3, half = warp >> 2;
+        const int q = warp & 3, part = warp >> 2;
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
         unsigned char* wstage = staging + warp * L::STAGING;
         uint32_t it = 0, local = 0;
@@ -254,15 +270,15 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             const Tile x = tile_of<BN, GLU>(g, t, m_tiles);
             const int row = x.m0 + q * 32 + lane;
             const float* sa = g.sa + (size_t)min(row, x.hi - 1) * g.KB;
-            const float* sw = GLU || BN == 128 || half == 0 ? x.s0 : x.s1;
-            float acc[COLS];
+            const float* sw = GLU || BN == 128 || part == 0 ? x.s0 : x.s1;
+            uint64_t sums[COLS / 2];
 #pragma unroll
-            for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
+            for (int i = 0; i < COLS / 2; ++i) sums[i] = 0;
             float a_next = b_lo < b_hi ? sa[b_lo] : 0.0f, w_next = b_lo < b_hi ? sw[b_lo] : 0.0f, u_next = GLU && b_lo < b_hi ? x.s1[b_lo] : 0.0f;
 #pragma unroll 1
             for (int b = b_lo; b < b_hi && ok; ++b, ++it) {
                 const uint32_t ph = it & 1;
-                const float s0 = a_next * w_next, s1 = GLU ? a_next * u_next : 0.0f;
+                const uint64_t s0 = twice(a_next * w_next), s1 = GLU ? twice(a_next * u_next) : 0;
                 if (b + 1 < b_hi) {
                     a_next = sa[b + 1];
                     w_next = sw[b + 1];
@@ -271,23 +287,29 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->sum_full[ph]), (it >> 1) & 1, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
-                // a piece of 32 columns is multiplied while the next is on its way; the accumulator is free once the last has arrived
-                uint32_t r[2][32];
-                tmem_ld32_issue(taddr + ph * BN + column(0, half), r[0]);
+                if (threadIdx.x == 0) mbar_arrive(smem_u32(&ctl->empty[it % L::STAGES]));      // the block's products are through: so are its copies
+                // a piece is multiplied while the next is on its way; the accumulator is free once the last has arrived
+                uint32_t r[2][PIECE];
+                tmem_ld32_issue(taddr + ph * BN + column(0, part), r[0]);
 #pragma unroll
-                for (int c = 0; c < COLS / 32; ++c) {
+                for (int c = 0; c < PIECES; ++c) {
                     tmem_wait32(r[c & 1]);
-                    if (c + 1 < COLS / 32) {
-                        tmem_ld32_issue(taddr + ph * BN + column(c + 1, half), r[(c + 1) & 1]);
+                    if (c + 1 < PIECES) {
+                        tmem_ld32_issue(taddr + ph * BN + column(c + 1, part), r[(c + 1) & 1]);
                     } else {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(smem_u32(&ctl->sum_empty[ph]));
                     }
-                    const float s = GLU && c >= COLS / 64 ? s1 : s0;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) fma_pair(acc[c * 32 + i], acc[c * 32 + i + 1], s, r[c & 1][i], r[c & 1][i + 1]);
+                    for (int i = 0; i < PIECE; i += 2) fma_pair(sums[(c * PIECE + i) / 2], GLU && c >= PIECES / 2 ? s1 : s0, r[c & 1][i], r[c & 1][i + 1]);
                 }
+            }
+            float acc[COLS];
+#pragma unroll
+            for (int i = 0; i < COLS / 2; ++i) {
+                acc[2 * i] = __uint_as_float((uint32_t)sums[i]);
+                acc[2 * i + 1] = __uint_as_float((uint32_t)(sums[i] >> 32));
             }
             if (!ok) {
 #pragma unroll
@@ -295,98 +317,70 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             }
             if (SPLIT) {
                 // this CTA's sums into its own shared memory: the copies have all been read by products that are through
-                float* part = reinterpret_cast<float*>(pipe) + (q * 32 + lane) * L::PART_LD;
+                float* mine = reinterpret_cast<float*>(pipe) + (q * 32 + lane) * L::PART_LD;
                 if (row < x.hi) {
 #pragma unroll
-                    for (int c = 0; c < COLS / 32; ++c) {
-                        const int col = column(c, half);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<float4*>(part + col + i) = make_float4(acc[c * 32 + i], acc[c * 32 + i + 1], acc[c * 32 + i + 2], acc[c * 32 + i + 3]);
-                    }
+                    for (int i = 0; i < COLS; i += 4)
+                        *reinterpret_cast<float4*>(mine + column(i / PIECE, part) + i % PIECE) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
                 }
             } else if (GLU) {
                 const float rs = g.row_scale && row < x.hi ? g.row_scale[g.order ? g.order[row] : row] : 1.0f;
+                const int n0 = x.n0 + part * (COLS / 2);
                 uint32_t largest = 0;
 #pragma unroll
                 for (int i = 0; i < COLS / 2; ++i) {
                     const float h = fp8_glu(acc[i], acc[COLS / 2 + i], g.act, g.limit, rs);
-                    acc[i] = x.n0 + half * 64 + i < g.N ? h : 0.0f;
+                    acc[i] = n0 + i < g.N ? h : 0.0f;
                     largest = max(largest, fp8_size_bits(acc[i]));
                 }
-                // the other half of the row's block is the warp's with the same rows
-                volatile uint32_t* sizes = reinterpret_cast<volatile uint32_t*>(staging);      // [tile parity][rows' quarter][half][row]
-                const int par = local & 1;
-                sizes[((par * 4 + q) * 2 + half) * 32 + lane] = largest;
+                // the other parts of the row's block are the warps' with the same rows
+                volatile uint32_t* sizes = reinterpret_cast<volatile uint32_t*>(staging) + ((local & 1) * 4 + q) * 64 + lane;      // [tile parity][rows' quarter][part][row]
+                sizes[part * 32] = largest;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&ctl->pair[q]));
-                ok = __all_sync(0xffffffffu, ok && mbar_wait(smem_u32(&ctl->pair[q]), par, abort_flag));
-                const float s = ok ? fp8_scale_of(max(largest, sizes[((par * 4 + q) * 2 + (half ^ 1)) * 32 + lane])) : __uint_as_float(0x7fffffffu);
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->row_known[q]));
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(smem_u32(&ctl->row_known[q]), local & 1, abort_flag));
+                const float s = ok ? fp8_scale_of(max(sizes[0], sizes[32])) : __uint_as_float(0x7fffffffu);
+                const float inv = __fdiv_rn(1.0f, s);      // the sums are no closer to their exact values than a product with this to the quotient
                 if (row < x.hi) {
-                    if (half == 0) g.out_scales[(size_t)row * g.NB + x.n0 / 128] = s;
-                    uint8_t* dst = (uint8_t*)g.out + (size_t)row * g.ldo + x.n0 + half * 64;
+                    if (part == 0) g.out_scales[(size_t)row * g.NB + x.n0 / 128] = s;
+                    uint8_t* dst = (uint8_t*)g.out + (size_t)row * g.ldo + n0;
 #pragma unroll
                     for (int i = 0; i < COLS / 2; i += 16) {
                         uint32_t p[4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            p[j] = fp8_pack4(__fdiv_rn(acc[i + 4 * j], s), __fdiv_rn(acc[i + 4 * j + 1], s), __fdiv_rn(acc[i + 4 * j + 2], s), __fdiv_rn(acc[i + 4 * j + 3], s));
-                        if (x.n0 + half * 64 + i < g.ldo) *reinterpret_cast<uint4*>(dst + i) = make_uint4(p[0], p[1], p[2], p[3]);
+                        for (int j = 0; j < 4; ++j) p[j] = fp8_pack4(acc[i + 4 * j] * inv, acc[i + 4 * j + 1] * inv, acc[i + 4 * j + 2] * inv, acc[i + 4 * j + 3] * inv);
+                        if (n0 + i < g.ldo) *reinterpret_cast<uint4*>(dst + i) = make_uint4(p[0], p[1], p[2], p[3]);
                     }
                 }
             } else {
-                // 128 bytes of 32 rows at a time through shared memory (16-byte unit u of row r at u ^ (r & 7)), so that stores are of whole rows
-                const bool f32 = g.out_kind == OUT_F32;
-                const int esz = f32 ? 4 : 2, per = 128 / esz, col_base = x.n0 + half * COLS;
-                const bool aligned = (((uintptr_t)g.out | ((size_t)g.ldo * esz)) & 15) == 0;
+                if (g.bias != nullptr) {
 #pragma unroll
-                for (int c = 0; c < COLS / 32; ++c) {
-                    const int col0 = col_base + c * 32;
-                    if (g.bias != nullptr) {
+                    for (int i = 0; i < COLS; ++i)
+                        if (x.n0 + part * COLS + i < g.N) acc[i] += bias_at(g, x.n0 + part * COLS + i);
+                }
+                if (g.out_kind == OUT_F32) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (col0 + i < g.N) acc[c * 32 + i] += bias_at(g, col0 + i);
+                    for (int c = 0; c < COLS; c += 16) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            *reinterpret_cast<float4*>(staged(wstage, lane, u)) = make_float4(acc[c + u * 4], acc[c + u * 4 + 1], acc[c + u * 4 + 2], acc[c + u * 4 + 3]);
+                        store_staged<float>(wstage, lane, (float*)g.out, g.ldo, x.m0 + q * 32, x.hi, x.n0 + part * COLS + c, g.N);
                     }
-                    unsigned char* srow = wstage + lane * 128;
-                    if (f32) {
+                } else {
 #pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            *reinterpret_cast<float4*>(srow + ((u ^ (lane & 7)) << 4)) =
-                                make_float4(acc[c * 32 + u * 4], acc[c * 32 + u * 4 + 1], acc[c * 32 + u * 4 + 2], acc[c * 32 + u * 4 + 3]);
-                    } else {
+                    for (int c = 0; c < COLS; c += 32) {
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
                             uint32_t p[4];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                const __nv_bfloat162 v = __floats2bfloat162_rn(acc[c * 32 + u * 8 + 2 * j], acc[c * 32 + u * 8 + 2 * j + 1]);
+                                const __nv_bfloat162 v = __floats2bfloat162_rn(acc[c + u * 8 + 2 * j], acc[c + u * 8 + 2 * j + 1]);
                                 p[j] = *reinterpret_cast<const uint32_t*>(&v);
                             }
-                            *reinterpret_cast<uint4*>(srow + ((((c & 1) * 4 + u) ^ (lane & 7)) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
+                            *reinterpret_cast<uint4*>(staged(wstage, lane, u)) = make_uint4(p[0], p[1], p[2], p[3]);
                         }
-                        if ((c & 1) == 0) continue;          // (COLS / 32 is even)
+                        store_staged<__nv_bfloat16>(wstage, lane, (__nv_bfloat16*)g.out, g.ldo, x.m0 + q * 32, x.hi, x.n0 + part * COLS + c, g.N);
                     }
-                    __syncwarp();
-                    const int cbase = f32 ? col0 : col0 - 32;          // the `per` columns that stand in the staging rows
-                    unsigned char* out = (unsigned char*)g.out;
-#pragma unroll 1
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = i * 4 + (lane >> 3), u = lane & 7, grow = x.m0 + q * 32 + r, gcol = cbase + u * (16 / esz);
-                        if (grow >= x.hi || gcol >= g.N) continue;
-                        const unsigned char* src = wstage + r * 128 + ((u ^ (r & 7)) << 4);
-                        unsigned char* dst = out + ((size_t)grow * g.ldo + gcol) * esz;
-                        if (aligned && gcol + 16 / esz <= g.N) {
-                            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-                        } else {
-                            const int n = min(16 / esz, g.N - gcol);
-                            for (int j = 0; j < n; ++j) {
-                                if (f32) reinterpret_cast<float*>(dst)[j] = reinterpret_cast<const float*>(src)[j];
-                                else reinterpret_cast<uint16_t*>(dst)[j] = reinterpret_cast<const uint16_t*>(src)[j];
-                            }
-                        }
-                    }
-                    __syncwarp();
-                    (void)per;
                 }
             }
         }
@@ -421,11 +415,11 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                             if (n + i >= g.N) h[i] = 0.0f;
                             largest = max(largest, fp8_size_bits(h[i]));
                         }
-                        const float s = fp8_scale_of(__reduce_max_sync(0xffffffffu, largest));
+                        const float s = fp8_scale_of(__reduce_max_sync(0xffffffffu, largest)), inv = __fdiv_rn(1.0f, s);
                         if (lane == 0) g.out_scales[(size_t)row * g.NB + x.n0 / 128] = s;
                         if (n < g.ldo)
                             *reinterpret_cast<uint32_t*>((uint8_t*)g.out + (size_t)row * g.ldo + n) =
-                                fp8_pack4(__fdiv_rn(h[0], s), __fdiv_rn(h[1], s), __fdiv_rn(h[2], s), __fdiv_rn(h[3], s));
+                                fp8_pack4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
                     } else {
 #pragma unroll
                         for (int j = 0; j < BN / 128; ++j) {
@@ -454,7 +448,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     if (SPLIT) pair_sync();        // nobody leaves while another may read its shared memory
     tc_fence_after();
     if (threadIdx.x == 0 && ctl->abort_flag && g.err != nullptr) atomicExch(g.err, 1);
-    if (warp == 9) {
+    if (warp == SUM_WARPS + 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN) : "memory");
     }
 }
