@@ -28,10 +28,13 @@ using namespace tc;
 constexpr int T_ROWS = 128, T_THREADS = 384, SUM_WARPS = 8;      // (two warps of the last warpgroup have no role)
 constexpr int PIECE = 32;                                        // columns that a summing warp has on their way from tensor memory
 // A summing thread of a 256-column tile holds 128 sums and two pieces: registers move from the last warpgroup to the others.
-// 256 x 224 + 128 x 56 = 384 x 168, what the block starts with (the launch checks that).  Sixteen summing warps of half the columns, which 112
+// 256 x 224 + 128 x 56 = 256 x 232 + 128 x 40 = 384 x 168, what the block starts with (the launch checks that).  Sixteen summing warps of half the columns, which 112
 // registers each allow, were slower (2,048 x 4,736 x 13,824: 218 us against 178).
-constexpr int START_REGS = 168, SUM_REGS = 224, OTHER_REGS = 56;
-static_assert(SUM_WARPS * 32 * SUM_REGS + 128 * OTHER_REGS <= T_THREADS * START_REGS, "registers");
+constexpr int START_REGS = 168;
+__host__ __device__ constexpr int sum_regs(bool glu) { return glu ? 232 : 224; }
+__host__ __device__ constexpr int other_regs(bool glu) { return glu ? 40 : 56; }
+static_assert(SUM_WARPS * 32 * sum_regs(false) + 128 * other_regs(false) <= T_THREADS * START_REGS &&
+              SUM_WARPS * 32 * sum_regs(true) + 128 * other_regs(true) <= T_THREADS * START_REGS, "registers");
 constexpr int HALF_BYTES = 128 * 128;              // 128 rows of 128 bytes
 enum { OUT_BF16 = 0, OUT_F32 = 1 };
 
@@ -218,7 +221,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     const int b_lo = SPLIT ? (int)((long long)g.KB * rank / S) : 0, b_hi = SPLIT ? (int)((long long)g.KB * (rank + 1) / S) : g.KB;
 
     if (warp >= SUM_WARPS) {
-        if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+        if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(other_regs(GLU)));
         if (warp == SUM_WARPS) {
             if (lane == 0) {
                 uint32_t it = 0;
@@ -260,7 +263,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             pair_sync();
         }
     } else {
-        if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SUM_REGS));
+        if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(sum_regs(GLU)));
         const int q = warp & 3, part = warp >> 2;
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
         unsigned char* wstage = staging + warp * L::STAGING;
