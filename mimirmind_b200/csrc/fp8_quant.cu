@@ -1,7 +1,10 @@
 // Rows and weights as e4m3 numbers with a scale per block (fp8.cuh has the formula).
 #include "fp8.cuh"
+#include "fp8_launch.h"
 
 namespace {
+
+constexpr int UNITS = 3;
 
 template <typename T>
 __device__ __forceinline__ void load_wide8(const T* p, float* v);
@@ -21,34 +24,48 @@ __device__ __forceinline__ void load_wide8<__nv_bfloat16>(const __nv_bfloat16* p
     }
 }
 
-// Two blocks of a row per warp, eight numbers a lane; where rows start on 16-byte boundaries the loads are wide ones.
+// Two blocks of a row per warp and unit, eight numbers a lane, three units' loads on their way at once; where rows start on 16-byte boundaries the loads are wide ones.
 // Bound by memory (3 bytes a number): 4,096 rows of 3,584 bf16 (44 MB) with a division a number 19.7 us, with fp8_quotient PLACEHOLDER us.
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const T* __restrict__ x, long long ldx, const int32_t* __restrict__ source,
                                                              uint8_t* __restrict__ q, int ldq, float* __restrict__ scales, uint32_t units, int K,
                                                              uint32_t pairs, int blocks, int wide) {
     const int lane = threadIdx.x & 31;
-    for (uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += gridDim.x * 8) {
-        const uint32_t row = u / pairs;
-        const int b = (int)(u - row * pairs) * 2 + (lane >> 4), k = b * FP8_BLOCK + (lane & 15) * 8;
-        const T* src = x + (source ? source[row] : (int)row) * ldx + k;
-        float v[8];
-        if (wide && k + 8 <= K) {
-            load_wide8<T>(src, v);
-        } else {
+    pdl_trigger();        // a product launched behind this may fetch its first weights meanwhile
+    const uint32_t step = gridDim.x * 8;
+    for (uint32_t u0 = blockIdx.x * 8 + (threadIdx.x >> 5); u0 < units; u0 += UNITS * step) {
+        float v[UNITS][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f32<T>(src[i]) : 0.0f;
+        for (int n = 0; n < UNITS; ++n) {
+            const uint32_t u = u0 + n * step;
+            if (u >= units) break;
+            const uint32_t row = u / pairs;
+            const int k = ((int)(u - row * pairs) * 2 + (lane >> 4)) * FP8_BLOCK + (lane & 15) * 8;
+            const T* src = x + (source ? source[row] : (int)row) * ldx + k;
+            if (wide && k + 8 <= K) {
+                load_wide8<T>(src, v[n]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[n][i] = k + i < K ? to_f32<T>(src[i]) : 0.0f;
+            }
         }
-        uint32_t largest = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) largest = max(largest, fp8_size_bits(v[i]));
+        for (int n = 0; n < UNITS; ++n) {
+            const uint32_t u = u0 + n * step;
+            if (u >= units) break;
+            const uint32_t row = u / pairs;
+            const int b = (int)(u - row * pairs) * 2 + (lane >> 4), k = b * FP8_BLOCK + (lane & 15) * 8;
+            uint32_t largest = 0;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-        const float s = fp8_scale_of(largest);
-        if ((lane & 15) == 0 && b < blocks) scales[(size_t)row * blocks + b] = s;
-        fp8_quotients<8>(v, s);
-        if (k + 8 <= ldq)      // ldq is a multiple of 16: the row's padding gets noughts
-            *reinterpret_cast<uint2*>(q + (size_t)row * ldq + k) = make_uint2(fp8_pack4(v[0], v[1], v[2], v[3]), fp8_pack4(v[4], v[5], v[6], v[7]));
+            for (int i = 0; i < 8; ++i) largest = max(largest, fp8_size_bits(v[n][i]));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+            const float s = fp8_scale_of(largest);
+            if ((lane & 15) == 0 && b < blocks) scales[(size_t)row * blocks + b] = s;
+            fp8_quotients<8>(v[n], s);
+            if (k + 8 <= ldq)      // ldq is a multiple of 16: the row's padding gets noughts
+                *reinterpret_cast<uint2*>(q + (size_t)row * ldq + k) = make_uint2(fp8_pack4(v[n][0], v[n][1], v[n][2], v[n][3]), fp8_pack4(v[n][4], v[n][5], v[n][6], v[n][7]));
+        }
     }
 }
 
@@ -82,9 +99,7 @@ __global__ void __launch_bounds__(256) fp8_quant_weight_kernel(const T* __restri
 
 }  // namespace
 
-// x [rows, ldx] (K leading columns) -> q [rows, ldq] e4m3 (ldq = K rounded up to 16, the rest noughts), scales fp32 [rows, K / 128 rounded up].
-// source [rows] int32 or null: row r is made from row source[r] of x.
-MM_EXPORT int mm_fp8_quant_rows(const void* x, int x_dtype, long long ldx, const void* source, void* q, int ldq, void* scales, int rows, int K, void* stream) {
+int fp8_quant_rows(const void* x, int x_dtype, long long ldx, const int32_t* source, void* q, int ldq, float* scales, int rows, int K, cudaStream_t s) {
     MM_REQUIRE(rows >= 0 && K > 0 && ldx >= 0 && ldq >= K && ldq % 16 == 0 && ldq < K + 16, "fp8 rows: bad sizes");
     MM_REQUIRE(((uintptr_t)q & 15) == 0, "fp8 rows: the numbers must start on a 16-byte boundary");
     if (rows == 0) return MM_OK;
@@ -93,18 +108,23 @@ MM_EXPORT int mm_fp8_quant_rows(const void* x, int x_dtype, long long ldx, const
     const long long units = (long long)rows * pairs;
     MM_REQUIRE(units < 0x7fffffffLL, "fp8 rows: too many rows");
     const int grid = (int)((units + 7) / 8 < 148 * 8 ? (units + 7) / 8 : 148 * 8);
-    cudaStream_t s = (cudaStream_t)stream;
     const int wide = ldx % (x_dtype == MM_BF16 ? 8 : 4) == 0 && ((uintptr_t)x & 15) == 0;
     if (x_dtype == MM_BF16)
-        mm_launch(fp8_quant_rows_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, (const __nv_bfloat16*)x, ldx, (const int32_t*)source, (uint8_t*)q, ldq,
-                  (float*)scales, (uint32_t)units, K, (uint32_t)pairs, blocks, wide);
+        mm_launch(fp8_quant_rows_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, (const __nv_bfloat16*)x, ldx, source, (uint8_t*)q, ldq,
+                  scales, (uint32_t)units, K, (uint32_t)pairs, blocks, wide);
     else if (x_dtype == MM_F32)
-        mm_launch(fp8_quant_rows_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)x, ldx, (const int32_t*)source, (uint8_t*)q, ldq, (float*)scales,
+        mm_launch(fp8_quant_rows_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)x, ldx, source, (uint8_t*)q, ldq, scales,
                   (uint32_t)units, K, (uint32_t)pairs, blocks, wide);
     else
         MM_REQUIRE(false, "fp8 rows: dtype must be float32 or bfloat16");
     MM_CHECK_LAUNCH();
     return MM_OK;
+}
+
+// x [rows, ldx] (K leading columns) -> q [rows, ldq] e4m3 (ldq = K rounded up to 16, the rest noughts), scales fp32 [rows, K / 128 rounded up].
+// source [rows] int32 or null: row r is made from row source[r] of x.
+MM_EXPORT int mm_fp8_quant_rows(const void* x, int x_dtype, long long ldx, const void* source, void* q, int ldq, void* scales, int rows, int K, void* stream) {
+    return fp8_quant_rows(x, x_dtype, ldx, (const int32_t*)source, q, ldq, (float*)scales, rows, K, (cudaStream_t)stream);
 }
 
 // w [matrices, N, K] -> q [matrices, N, ldq] e4m3, scales fp32 [matrices, N / 128, K / 128] (both rounded up)

@@ -19,6 +19,7 @@
 //
 // Every wait is bounded; when one runs out, the CTA's tiles from there on become NaN, copies in flight get time to land, `err` is set.
 #include "fp8.cuh"
+#include "fp8_launch.h"
 #include "tcgen05.cuh"
 
 namespace {
@@ -561,4 +562,15 @@ MM_EXPORT int mm_gemm_fp8_tcgen05(const void* A, long long lda, const void* sa, 
     if (glu) return splits > 1 ? launch<256, true, true>(ta, tw, g, grid, s) : launch<256, true, false>(ta, tw, g, grid, s);
     if (wide) return splits > 1 ? launch<256, false, true>(ta, tw, g, grid, s) : launch<256, false, false>(ta, tw, g, grid, s);
     return splits > 1 ? launch<128, false, true>(ta, tw, g, grid, s) : launch<128, false, false>(ta, tw, g, grid, s);
+}
+
+// Tiles of 256 columns where they fill the SMs, else of 128, and as many CTAs to a tile as find room.
+int fp8_gemm(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, int* err, cudaStream_t s) {
+    const long long m_tiles = ceil_div(x.rows, 128), blocks = ceil_div(w.K, FP8_BLOCK);
+    int splits = 1;
+    const bool fills = m_tiles * ceil_div(w.N, 256) >= FP8_SM_COUNT;
+    if (!fills)
+        while (splits < 8 && m_tiles * ceil_div(w.N, 128) * splits * 2 <= FP8_SM_COUNT && blocks >= splits * 4) splits *= 2;
+    return mm_gemm_fp8_tcgen05(x.data, x.ld, x.scales, w.values, w.ld, w.scales, w.matrices, out.data, out.dtype, out.scales, out.ld, out.bias, out.bias_dtype,
+                               x.rows, w.N, w.K, glu, out.act, out.limit, nullptr, nullptr, nullptr, nullptr, 0, glu || fills, splits, err, s);
 }

@@ -2003,7 +2003,6 @@ def qk_prep(rows: torch.Tensor, q_off: int, k_off: int, v_off: int, q_norm: Opti
 
 # ---- layer weights in 8 bits (csrc/fp8.cuh has the formulas) ---------------------------------------------------------------
 FP8_BLOCK = 128           # numbers of a row, and rows and columns of a weight, that share a scale
-FP8_MAX_ROWS = 1 << 20    # of a product; sizes along a matrix fit in 32 bits well above any model's
 _E4M3 = torch.float8_e4m3fn
 
 
@@ -2019,67 +2018,61 @@ def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
 
 
-def _need_fp8(values: torch.Tensor, scales: torch.Tensor, what: str, lead, rows: int, k: int, blocks: int) -> None:
-    if not isinstance(values, torch.Tensor) or not values.is_cuda or values.dtype != _E4M3:
+def _fp8_layout(values, scales, what: str) -> int:
+    """The row stride of e4m3 numbers [..., rows, K] in numbers, once the tensors are what a kernel reads."""
+    if not isinstance(values, torch.Tensor) or not isinstance(scales, torch.Tensor) or values.dtype is not _E4M3 or not values.is_cuda:
         raise KernelError(f"{what}: expected float8_e4m3fn numbers on a CUDA device")
-    if rows < 1 and lead is not None or k < 1:
-        raise KernelError(f"{what}: sizes must be positive")
-    ld = values.stride(-2) if values.shape[-2] > 1 else -(-k // 16) * 16
-    if (values.stride(-1) != 1 and k > 1) or ld % 16 or ld < k or values.data_ptr() % 16:
+    if scales.dtype is not torch.float32 or scales.device != values.device or not scales.is_contiguous():
+        raise KernelError(f"{what} scales: expected contiguous float32 on the numbers' device")
+    shape, stride = values.shape, values.stride()
+    if len(shape) < 2 or shape[-1] < 1:
+        raise KernelError(f"{what}: expected a matrix or stacked matrices")
+    k = shape[-1]
+    ld = stride[-2] if shape[-2] > 1 else (k + 15) // 16 * 16
+    if (stride[-1] != 1 and k > 1) or ld % 16 or ld < k or values.data_ptr() % 16:
         raise KernelError(f"{what}: rows must be contiguous and start on 16-byte boundaries")
-    _need(scales, what + " scales", torch.float32)
-    if tuple(scales.shape) != tuple(lead or ()) + (blocks, _blocks(k)):
-        raise KernelError(f"{what}: scales are {tuple(scales.shape)}, expected {tuple(lead or ()) + (blocks, _blocks(k))}")
+    return ld
 
 
-@dataclass
 class Fp8Rows:
     """Rows in 8 bits: ``values`` e4m3 [m, K] (rows start on 16-byte boundaries) and ``scales`` fp32 [m, K / 128 rounded up];
     a number stands for ``values * scales``."""
 
-    values: torch.Tensor
-    scales: torch.Tensor
+    __slots__ = ("values", "scales", "ld", "shape")
 
-    def __post_init__(self):
-        if self.values.dim() != 2:
-            raise KernelError("fp8 rows: expected a matrix")
-        m, k = self.values.shape
-        _need_fp8(self.values, self.scales, "fp8 rows", None, m, k, m)
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        self.ld = _fp8_layout(values, scales, "fp8 rows")
+        self.values, self.scales, self.shape = values, scales, values.shape
+        if len(self.shape) != 2 or tuple(scales.shape) != (self.shape[0], _blocks(self.shape[1])):
+            raise KernelError(f"fp8 rows: numbers {tuple(self.shape)} and scales {tuple(scales.shape)} do not fit together")
 
-    @property
-    def shape(self):
-        return self.values.shape
+    def float(self) -> torch.Tensor:
+        """The numbers that the rows stand for, in fp32."""
+        return self.values.float() * self.scales.repeat_interleave(FP8_BLOCK, dim=1)[:, :self.shape[1]]
 
 
-@dataclass
 class Fp8Weight:
     """A weight in 8 bits, or several stacked ones: ``values`` e4m3 [..., N, K] (rows start on 16-byte boundaries) and ``scales``
     fp32 [..., N / 128, K / 128] (both rounded up), one for every block of 128 x 128 of a matrix; a number stands for ``values * scales``."""
 
-    values: torch.Tensor
-    scales: torch.Tensor
+    __slots__ = ("values", "scales", "ld", "shape", "matrices")
 
-    def __post_init__(self):
-        if self.values.dim() < 2:
-            raise KernelError("fp8 weight: expected a matrix or stacked matrices")
-        n, k = self.values.shape[-2:]
-        lead = tuple(self.values.shape[:-2])
-        _need_fp8(self.values, self.scales, "fp8 weight", lead, n, k, _blocks(n))
-        step = n * self.ld
-        for i in reversed(range(len(lead))):
-            if lead[i] > 1 and self.values.stride(i) != step:
-                raise KernelError("fp8 weight: stacked matrices must follow one another")
-            step *= lead[i]
-
-    @property
-    def shape(self):
-        return self.values.shape
-
-    @property
-    def ld(self) -> int:
-        """The row stride in numbers."""
-        n, k = self.values.shape[-2:]
-        return self.values.stride(-2) if n > 1 else -(-k // 16) * 16
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        self.ld = _fp8_layout(values, scales, "fp8 weight")
+        self.values, self.scales, self.shape = values, scales, values.shape
+        n, k = self.shape[-2:]
+        if n < 1 or tuple(scales.shape) != tuple(self.shape[:-2]) + (_blocks(n), _blocks(k)):
+            raise KernelError(f"fp8 weight: numbers {tuple(self.shape)} and scales {tuple(scales.shape)} do not fit together")
+        self.matrices = 1
+        if len(self.shape) > 2:
+            step, stride = n * self.ld, values.stride()
+            for i in range(len(self.shape) - 3, -1, -1):
+                if self.shape[i] != 1 and stride[i] != step:
+                    raise KernelError("fp8 weight: stacked matrices must follow one another")
+                step *= self.shape[i]
+                self.matrices *= self.shape[i]
+            if self.matrices < 1:
+                raise KernelError("fp8 weight: there is no matrix")
 
     def float(self) -> torch.Tensor:
         """The numbers that the weight stands for, in fp32."""
@@ -2129,80 +2122,64 @@ def quantize_fp8_weight(w: torch.Tensor) -> Fp8Weight:
     return out
 
 
-def _fp8_rows_of(x, k: int, what: str) -> Fp8Rows:
-    if not isinstance(x, Fp8Rows):
-        if isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[1] != k:
-            raise KernelError(f"{what}: rows of {x.shape[1]} numbers meet a weight of {k}")
-        return quantize_fp8_rows(x)
-    if x.shape[1] != k:
-        raise KernelError(f"{what}: rows of {x.shape[1]} numbers meet a weight of {k}")
-    return x
+def _fp8_input(x, k: int, what: str):
+    """(pointer, dtype code, row stride, scales' pointer, rows) of what an 8-bit product takes: Fp8Rows, or bf16 or fp32 rows."""
+    if isinstance(x, Fp8Rows):
+        _here(what, x.values)
+        m, kx = x.shape
+        found = (x.values.data_ptr(), _FP8_QUANTISED, x.ld, x.scales.data_ptr(), m)
+    else:
+        if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 2:
+            raise KernelError(f"{what}: expected Fp8Rows or a CUDA matrix")
+        _here(what, x)
+        (m, kx), (ld, one) = x.shape, x.stride()
+        if (one != 1 and kx > 1) or ld < 0:
+            raise KernelError(f"{what}: a row's numbers must follow one another")
+        found = (x.data_ptr(), dtype_code(x.dtype), ld, None, m)
+    if kx != k:
+        raise KernelError(f"{what}: rows of {kx} numbers meet a weight of {k}")
+    return found
 
 
-FP8_SMS = 148
+_FP8_QUANTISED = 2
 
 
-def _fp8_plan(m: int, n: int, k: int, glu: bool):
-    """(256 columns a tile, CTAs that share a tile's blocks)"""
-    m_tiles, blocks = -(-m // 128), _blocks(k)
-    if not glu and m_tiles * -(-n // 256) >= FP8_SMS:
-        return True, 1
-    tiles = m_tiles * -(-n // 128)
-    splits = 1
-    while splits < 8 and tiles * splits * 2 <= FP8_SMS and blocks >= splits * 4:
-        splits *= 2
-    return glu, splits
-
-
-def _fp8_gemm(x: Fp8Rows, w: Fp8Weight, out: torch.Tensor, out_scales: Optional[torch.Tensor], bias, rows: Optional["ExpertRows"], act: int,
-              limit: float, row_scale: Optional[torch.Tensor]) -> None:
-    _here("gemm_fp8", x.values, x.scales, w.values, w.scales, bias, row_scale)
-    m, k = x.shape
-    n = w.shape[-2]
-    glu = out_scales is not None
-    wide, splits = (True, 1) if rows is not None else _fp8_plan(m, n, k, glu)
-    ldo = out.stride(0) if m > 1 else (-(-n // 16) * 16 if glu else n)
-    check(_lib.load().mm_gemm_fp8_tcgen05(x.values.data_ptr(), x.values.stride(0) if m > 1 else -(-k // 16) * 16, x.scales.data_ptr(), w.values.data_ptr(),
-                                          w.ld, w.scales.data_ptr(), w.values.numel() // (n * k), out.data_ptr(), F32 if out.dtype == torch.float32 else BF16,
-                                          _ptr(out_scales), ldo, _ptr(bias), dtype_code(bias.dtype) if bias is not None else F32, m, n, k, int(glu),
-                                          act, float(limit), _ptr(row_scale), rows.order.data_ptr() if rows else None,
-                                          rows.tiles.data_ptr() if rows else None, rows.n_tiles.data_ptr() if rows else None, rows.max_tiles if rows else 0,
-                                          int(wide), splits, tcgen05_error_flag(w.values.device).data_ptr(), _stream()), "gemm_fp8")
-
-
-def _fp8_product(x: Fp8Rows, w: Fp8Weight, out_dtype: torch.dtype, bias=None, rows: Optional["ExpertRows"] = None) -> torch.Tensor:
-    out = torch.empty((x.shape[0], w.shape[-2]), dtype=out_dtype, device=w.values.device)
-    if x.shape[0]:
-        _fp8_gemm(x, w, out, None, bias, rows, 0, 0.0, None)
-    return out
-
-
-def _fp8_hidden(x: Fp8Rows, w_in: Fp8Weight, act: int, limit: float, rows: Optional["ExpertRows"] = None, row_scale=None) -> Fp8Rows:
-    """act(gate, up) of pairs of matrices [..., 2, F, K], quantised from its fp32 values."""
-    m, f = x.shape[0], w_in.shape[-2]
-    dev = w_in.values.device
-    out = Fp8Rows(_fp8_buffer(m, f, device=dev), torch.empty((m, _blocks(f)), dtype=torch.float32, device=dev))
-    if m:
-        _fp8_gemm(x, w_in, out.values, out.scales, None, rows, act, limit, row_scale)
-    return out
+def _fp8_scratch(m: int, k: int) -> int:
+    """Bytes of m rows of k quantised numbers and their scales, as the library lays them out."""
+    return m * ((k + 15) // 16 * 16) + (4 * m * _blocks(k) + 15) // 16 * 16
 
 
 def gemm_fp8(x, w: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """x [m, K] times a weight [N, K] in 8 bits (+ bias [N]): ``sum_b sx[m, b] sw[n / 128, b] sum_{k in b} qx[m, k] qw[n, k]``, sums in
     fp32, rounded once to ``out_dtype`` (bf16 or fp32).  ``x``: :class:`Fp8Rows`, or bf16 or fp32 rows, which are quantised first
     (:func:`quantize_fp8_rows`)."""
-    if not isinstance(w, Fp8Weight) or w.values.dim() != 2:
+    if not isinstance(w, Fp8Weight) or len(w.shape) != 2:
         raise KernelError("gemm_fp8: the weight must be one matrix in 8 bits (Fp8Weight [N, K])")
     n, k = w.shape
+    _here("gemm_fp8", w.values, bias)
     if bias is not None:
         _need(bias, "gemm_fp8 bias")
-        dtype_code(bias.dtype)
         if bias.shape != (n,):
             raise KernelError("gemm_fp8: bias shape mismatch")
-    dtype_code(out_dtype)
-    _here("gemm_fp8", w.values, w.scales, bias)
-    x = _fp8_rows_of(x, k, "gemm_fp8")
-    return _fp8_product(x, w, out_dtype, bias)
+    ptr, code, ld, scales, m = _fp8_input(x, k, "gemm_fp8")
+    dev = w.values.device
+    out_code = dtype_code(out_dtype)
+    out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    scratch = None if code == _FP8_QUANTISED else torch.empty(_fp8_scratch(m, k), dtype=torch.uint8, device=dev)
+    check(_lib.load().mm_fp8_linear(ptr, code, ld, scales, m, w.values.data_ptr(), w.ld, w.scales.data_ptr(), n, k, _ptr(bias),
+                                    F32 if bias is None else dtype_code(bias.dtype), out.data_ptr(), out_code, _ptr(scratch),
+                                    tcgen05_error_flag(dev).data_ptr(), _stream()), "gemm_fp8")
+    return out
+
+
+def _fp8_grouped(x: Fp8Rows, w: Fp8Weight, rows: "ExpertRows", out: torch.Tensor, out_scales: Optional[torch.Tensor], act: int = 0, limit: float = 0.0,
+                 row_scale: Optional[torch.Tensor] = None) -> None:
+    """Row tiles of ``rows.tiles`` times their expert's matrix; with ``out_scales`` its pair of matrices, act(gate, up) quantised."""
+    n, k = w.shape[-2:]
+    check(_lib.load().mm_gemm_fp8_tcgen05(x.values.data_ptr(), x.ld, x.scales.data_ptr(), w.values.data_ptr(), w.ld, w.scales.data_ptr(), w.matrices,
+                                          out.data_ptr(), F32 if out.dtype == torch.float32 else BF16, _ptr(out_scales), out.stride(0), None, F32, x.shape[0], n, k,
+                                          int(out_scales is not None), act, float(limit), _ptr(row_scale), rows.order.data_ptr(), rows.tiles.data_ptr(),
+                                          rows.n_tiles.data_ptr(), rows.max_tiles, 1, 1, tcgen05_error_flag(w.values.device).data_ptr(), _stream()), "gemm_fp8")
 
 
 def _glu_code(activation: str, limit: float, what: str) -> int:
@@ -2215,19 +2192,25 @@ def glu_mlp_fp8(x, w_in: Fp8Weight, w_out: Fp8Weight, activation: str = "silu", 
     """A gated feed-forward in 8 bits: ``h = act(x Wg^T, x Wu^T)`` in fp32, quantised per row and block of 128 from its fp32 values, and
     ``h Wd^T`` as bf16 [m, D].  ``w_in`` [2, F, K]: the gate's matrix, then the up projection's; ``w_out`` [D, F].  ``x`` as for
     :func:`gemm_fp8`; ``activation`` and ``limit`` as for :func:`moe_gemm`."""
-    if not isinstance(w_in, Fp8Weight) or w_in.values.dim() != 3 or w_in.shape[0] != 2:
+    if not isinstance(w_in, Fp8Weight) or len(w_in.shape) != 3 or w_in.shape[0] != 2:
         raise KernelError("glu_mlp_fp8: w_in must be two matrices in 8 bits (Fp8Weight [2, F, K])")
-    if not isinstance(w_out, Fp8Weight) or w_out.values.dim() != 2 or w_out.shape[1] != w_in.shape[1]:
+    _, f, k = w_in.shape
+    if not isinstance(w_out, Fp8Weight) or len(w_out.shape) != 2 or w_out.shape[1] != f:
         raise KernelError("glu_mlp_fp8: w_out must be a matrix in 8 bits that takes the hidden rows (Fp8Weight [D, F])")
     act = _glu_code(activation, limit, "glu_mlp_fp8")
-    _here("glu_mlp_fp8", w_in.values, w_in.scales, w_out.values, w_out.scales)
-    f, k = w_in.shape[1:]
-    x = _fp8_rows_of(x, k, "glu_mlp_fp8")
-    return _fp8_product(_fp8_hidden(x, w_in, act, limit), w_out, torch.bfloat16)
+    _here("glu_mlp_fp8", w_in.values, w_out.values)
+    ptr, code, ld, scales, m = _fp8_input(x, k, "glu_mlp_fp8")
+    d, dev = w_out.shape[0], w_in.values.device
+    out = torch.empty((m, d), dtype=torch.bfloat16, device=dev)
+    scratch = torch.empty(_fp8_scratch(m, k) + _fp8_scratch(m, f), dtype=torch.uint8, device=dev)
+    check(_lib.load().mm_fp8_glu_mlp(ptr, code, ld, scales, m, w_in.values.data_ptr(), w_in.ld, w_in.scales.data_ptr(), f, k, w_out.values.data_ptr(), w_out.ld,
+                                     w_out.scales.data_ptr(), d, act, float(limit), out.data_ptr(), scratch.data_ptr(),
+                                     tcgen05_error_flag(dev).data_ptr(), _stream()), "glu_mlp_fp8")
+    return out
 
 
 def _check_experts_fp8(x: torch.Tensor, w_in: Fp8Weight, w_out: Fp8Weight, what: str) -> None:
-    if (not isinstance(w_in, Fp8Weight) or not isinstance(w_out, Fp8Weight) or w_in.values.dim() != 4 or w_in.shape[1] != 2 or w_out.values.dim() != 3
+    if (not isinstance(w_in, Fp8Weight) or not isinstance(w_out, Fp8Weight) or len(w_in.shape) != 4 or w_in.shape[1] != 2 or len(w_out.shape) != 3
             or w_in.shape[0] != w_out.shape[0] or w_in.shape[2] != w_out.shape[2]):
         raise KernelError(f"{what}: w_in must be Fp8Weight [E, 2, F, D] (gate, up) and w_out Fp8Weight [E, D, F]")
     if x.dim() != 2 or x.shape[1] != w_in.shape[3]:
@@ -2259,6 +2242,8 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, wts: torch.Tensor, w_in:
     rows = moe_sort(idx, E, with_tiles=True)
     sorted_x = quantize_fp8_rows(x, rows.row_token)
     on_input = weight_on == "input"
-    hidden = _fp8_hidden(sorted_x, w_in, act, limit, rows, wts if on_input else None)
-    y = _fp8_product(hidden, w_out, torch.float32, rows=rows)
+    hidden = Fp8Rows(_fp8_buffer(n * top, f, device=x.device), torch.empty((n * top, _blocks(f)), dtype=torch.float32, device=x.device))
+    _fp8_grouped(sorted_x, w_in, rows, hidden.values, hidden.scales, act, limit, wts if on_input else None)
+    y = torch.empty((n * top, d), dtype=torch.float32, device=x.device)
+    _fp8_grouped(hidden, w_out, rows, y, None)
     return moe_combine(y, None if on_input else wts, torch.bfloat16, place=rows.place, top=top)
