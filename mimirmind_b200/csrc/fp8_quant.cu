@@ -4,7 +4,7 @@
 
 namespace {
 
-constexpr int UNITS = 3;
+constexpr int UNITS = 1;
 
 template <typename T>
 __device__ __forceinline__ void load_wide8(const T* p, float* v);
@@ -107,7 +107,7 @@ int fp8_quant_rows(const void* x, int x_dtype, long long ldx, const int32_t* sou
     const int pairs = (blocks + 1) / 2;
     const long long units = (long long)rows * pairs;
     MM_REQUIRE(units < 0x7fffffffLL, "fp8 rows: too many rows");
-    const int grid = (int)((units + 7) / 8 < 148 * 8 ? (units + 7) / 8 : 148 * 8);
+    const int grid = (int)((units + 7) / 8);
     const int wide = ldx % (x_dtype == MM_BF16 ? 8 : 4) == 0 && ((uintptr_t)x & 15) == 0;
     if (x_dtype == MM_BF16)
         mm_launch(fp8_quant_rows_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, (const __nv_bfloat16*)x, ldx, source, (uint8_t*)q, ldq,

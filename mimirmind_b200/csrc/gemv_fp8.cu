@@ -38,9 +38,12 @@ struct GemvArgs {
 };
 
 // 16 bytes of a row of K from k on, noughts behind its end (nothing there is read): on their way to shared memory, or into registers
-__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* row, int k, int K) {
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, int k, int K) {      // src = row + k
     const int n = min(max(K - k, 0), 16);
-    const uint8_t* src = n > 0 ? row + k : row;
+    if (n == 0) src -= k;
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ uint4 load16(const uint8_t* row, int k, int K) {
@@ -51,23 +54,18 @@ __device__ __forceinline__ uint4 load16(const uint8_t* row, int k, int K) {
         if (k + i < K) w[i >> 2] |= (uint32_t)row[k + i] << (8 * (i & 3));
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void copy4(uint32_t dst, const float* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-
 __device__ __forceinline__ void mma_e4m3(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A slot of a warp's ring: a block of its tile's 16 rows (a lane's four pieces: bytes t * 16 .. + 15 and 64 on of rows g and g + 8), the
-// block's scales once per lane.
-__host__ __device__ constexpr int slot_bytes(bool glu) { return 2048 + (glu ? 256 : 128); }
+// A slot of a warp's ring: a block of its tile's 16 rows (a lane's four pieces: bytes t * 16 .. + 15 and 64 on of rows g and g + 8).
+constexpr int SLOT = 2048;
 __host__ __device__ inline int q_stride(int KB) { return KB * FP8_BLOCK + 64; }      // 64: rows of neighbouring lanes in different banks
 
 template <int G, bool GLU, bool QUANT>
 __global__ void __launch_bounds__(GV_THREADS, 2) gemv_fp8_kernel(const __grid_constant__ GemvArgs g) {
-    constexpr int TOK = 8 * G, SLOT = slot_bytes(GLU);
+    constexpr int TOK = 8 * G;
     extern __shared__ __align__(16) unsigned char gv_smem[];
     float* part = reinterpret_cast<float*>(gv_smem + GV_WARPS * RING * SLOT);              // [2][8 warps][16 rows][TOK]
     float* hidden = part + 2 * GV_WARPS * 16 * TOK;                                        // GLU: [TOK][128 / S]
@@ -83,36 +81,58 @@ __global__ void __launch_bounds__(GV_THREADS, 2) gemv_fp8_kernel(const __grid_co
     unsigned char* ring = gv_smem + warp * RING * SLOT;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
 
-    // the weights of the run's next block into slot `slot`
+    // the cursor of loading: the run's next block, over the steps
     const int total = nb * steps;
+    const bool whole = g.K % FP8_BLOCK == 0;
     int load_step = 0, load_b = lo;
+    const uint8_t *pa, *pb;
+    auto first_row = [&](int step) {
+        return GLU ? first * 128 + (rank * (16 / g.S) + step * g.RT + rt) * 8 : ((first + step * (int)gridDim.x) * g.RT + rt) * 16;
+    };
+    auto point = [&]() {
+        const int n0 = first_row(load_step), ra = min(n0 + gr, g.N - 1), rb = GLU ? g.N + ra : min(n0 + gr + 8, g.N - 1);
+        const int k = lo * FP8_BLOCK + t4 * 16;
+        pa = g.W + (size_t)ra * g.ldw + k;
+        pb = g.W + (size_t)rb * g.ldw + k;
+    };
+    point();
     auto load_weights = [&](int slot) {
-        const int n0 = GLU ? first * 128 + (rank * (16 / g.S) + load_step * g.RT + rt) * 8 : ((first + load_step * (int)gridDim.x) * g.RT + rt) * 16;
-        const int ra = min(n0 + gr, g.N - 1), rb = GLU ? g.N + ra : min(n0 + gr + 8, g.N - 1);
-        const uint8_t *pa = g.W + (size_t)ra * g.ldw, *pb = g.W + (size_t)rb * g.ldw;
-        const int k = load_b * FP8_BLOCK + t4 * 16, block = min(n0, g.N - 1) / FP8_BLOCK;
         const uint32_t dst = ring_at + slot * SLOT;
-        copy16(dst, pa, k, g.K);
-        copy16(dst + 512, pb, k, g.K);
-        copy16(dst + 1024, pa, k + 64, g.K);
-        copy16(dst + 1536, pb, k + 64, g.K);
-        const uint32_t sc = ring_at - lane * 12 + slot * SLOT + 2048;
-        copy4(sc, g.sw + (size_t)block * g.KB + load_b);
-        if (GLU) copy4(sc + 128, g.sw + ((size_t)g.NB + block) * g.KB + load_b);
+        if (whole) {
+            copy16(dst, pa);
+            copy16(dst + 512, pb);
+            copy16(dst + 1024, pa + 64);
+            copy16(dst + 1536, pb + 64);
+        } else {
+            const int k = load_b * FP8_BLOCK + t4 * 16;
+            copy16(dst, pa, k, g.K);
+            copy16(dst + 512, pb, k, g.K);
+            copy16(dst + 1024, pa + 64, k + 64, g.K);
+            copy16(dst + 1536, pb + 64, k + 64, g.K);
+        }
+        pa += FP8_BLOCK;
+        pb += FP8_BLOCK;
         if (++load_b == hi) {
             load_b = lo;
             ++load_step;
+            point();
         }
     };
     // the same block of x, a block ahead in registers (a warp's block takes longer than a load from L2)
     uint4 next[G][2];
+    const uint8_t* rows[G];
+#pragma unroll
+    for (int j = 0; j < G; ++j) rows[j] = QUANT ? q_rows + (size_t)min(j * 8 + gr, g.m - 1) * q_stride(g.KB) : g.q + (size_t)min(j * 8 + gr, g.m - 1) * g.ldq;
     auto load_rows = [&](int b) {
 #pragma unroll
         for (int j = 0; j < G; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int tok = j * 8 + gr;
-                next[j][h] = tok < g.m ? load16(g.q + (size_t)tok * g.ldq, b * FP8_BLOCK + t4 * 16 + 64 * h, g.K) : make_uint4(0, 0, 0, 0);
+                const int k = b * FP8_BLOCK + t4 * 16 + 64 * h;
+                if (tok >= g.m) next[j][h] = make_uint4(0, 0, 0, 0);
+                else if (whole) next[j][h] = *reinterpret_cast<const uint4*>(rows[j] + k);
+                else next[j][h] = load16(rows[j], k, g.K);
             }
     };
 #pragma unroll 1
@@ -160,7 +180,16 @@ __global__ void __launch_bounds__(GV_THREADS, 2) gemv_fp8_kernel(const __grid_co
         for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
 
     int done = 0, slot = 0;
+    const float *xa[G], *xb[G];
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+        xa[j] = x_scales + min(j * 8 + t4 * 2, g.m - 1) * g.KB;
+        xb[j] = x_scales + min(j * 8 + t4 * 2 + 1, g.m - 1) * g.KB;
+    }
     for (int step = 0; step < steps; ++step) {
+        const float* sw = g.sw + (size_t)(min(first_row(step), g.N - 1) / FP8_BLOCK) * g.KB;      // (read a block ahead)
+        const float* su = sw + (size_t)g.NB * g.KB;
+        float s0_next = sw[lo], s1_next = GLU ? su[lo] : 0.0f;
 #pragma unroll 1
         for (int b = lo; b < hi; ++b) {
             uint4 now[G][2];
@@ -179,13 +208,16 @@ __global__ void __launch_bounds__(GV_THREADS, 2) gemv_fp8_kernel(const __grid_co
             wh[0] = *reinterpret_cast<const uint4*>(at + 512);
             wl[1] = *reinterpret_cast<const uint4*>(at + 1024);
             wh[1] = *reinterpret_cast<const uint4*>(at + 1536);
-            const float* sc = reinterpret_cast<const float*>(ring + slot * SLOT + 2048) + lane;
-            const float s0 = sc[0], s1 = GLU ? sc[32] : s0;
+            const float s0 = s0_next, s1 = GLU ? s1_next : s0;
+            if (b + 1 < hi) {
+                s0_next = sw[b + 1];
+                if (GLU) s1_next = su[b + 1];
+            }
 #pragma unroll
             for (int j = 0; j < G; ++j) {
                 uint4 x[2];
                 if (QUANT) {
-                    const uint8_t* row = q_rows + (size_t)min(j * 8 + gr, g.m - 1) * q_stride(g.KB) + b * FP8_BLOCK + t4 * 16;
+                    const uint8_t* row = rows[j] + b * FP8_BLOCK + t4 * 16;
                     x[0] = *reinterpret_cast<const uint4*>(row);
                     x[1] = *reinterpret_cast<const uint4*>(row + 64);
                 } else {
@@ -198,11 +230,11 @@ __global__ void __launch_bounds__(GV_THREADS, 2) gemv_fp8_kernel(const __grid_co
                     mma_e4m3(c, wl[h].x, wh[h].x, wl[h].y, wh[h].y, x[h].x, x[h].y);
                     mma_e4m3(c, wl[h].z, wh[h].z, wl[h].w, wh[h].w, x[h].z, x[h].w);
                 }
-                const float xa = x_scales[min(j * 8 + t4 * 2, g.m - 1) * g.KB + b], xb = x_scales[min(j * 8 + t4 * 2 + 1, g.m - 1) * g.KB + b];
-                acc[j][0] = fmaf(xa * s0, c[0], acc[j][0]);
-                acc[j][1] = fmaf(xb * s0, c[1], acc[j][1]);
-                acc[j][2] = fmaf(xa * s1, c[2], acc[j][2]);
-                acc[j][3] = fmaf(xb * s1, c[3], acc[j][3]);
+                const float sa = xa[j][b], sb = xb[j][b];
+                acc[j][0] = fmaf(sa * s0, c[0], acc[j][0]);
+                acc[j][1] = fmaf(sb * s0, c[1], acc[j][1]);
+                acc[j][2] = fmaf(sa * s1, c[2], acc[j][2]);
+                acc[j][3] = fmaf(sb * s1, c[3], acc[j][3]);
             }
             // the slot's numbers have been multiplied: the run's next block but three goes there
             if (done + RING < total) load_weights(slot);
@@ -313,7 +345,7 @@ int launch(const GemvArgs& g, int grid, size_t smem, bool dependent, cudaStream_
 
 static size_t gemv_smem(int m, int KB, bool glu, bool quant) {
     const int tok = m <= 8 ? 8 : 16;
-    return (size_t)GV_WARPS * RING * slot_bytes(glu) + (size_t)2 * GV_WARPS * 16 * tok * 4 + (glu ? (size_t)tok * 128 * 4 + tok * 4 : 0) +
+    return (size_t)GV_WARPS * RING * SLOT + (size_t)2 * GV_WARPS * 16 * tok * 4 + (glu ? (size_t)tok * 128 * 4 + tok * 4 : 0) +
            (size_t)((m * KB + 3) & ~3) * 4 + (quant ? (size_t)m * q_stride(KB) : 0);
 }
 
@@ -346,20 +378,27 @@ int fp8_gemv(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, bool 
     g.K = w.K;
     g.KB = ceil_div(w.K, FP8_BLOCK);
     g.NB = ceil_div(w.N, FP8_BLOCK);
-    // as many runs of blocks as there are warps, or blocks
-    g.KS = GV_WARPS;
-    while (g.KS > g.KB) g.KS /= 2;
-    g.RT = GV_WARPS / g.KS;
     g.tiles = ceil_div(w.N, 16);
+    // Tiles side by side in a CTA (8, 4, 2, 1) as long as there are one and a half CTAs an SM: the runs of blocks are longer and the
+    // warps meet less often.  No more runs than blocks.
     int grid;
     if (glu) {
-        g.S = 1;      // two CTAs an SM, a tile of every row of warps at the least
-        while (g.S < 8 && g.NB * g.S * 2 <= 2 * FP8_SM_COUNT && 16 / (g.S * 2) >= g.RT) g.S *= 2;
+        g.S = 1;
+        while (g.S < 8 && g.NB * g.S * 2 <= 2 * FP8_SM_COUNT) g.S *= 2;
+        g.RT = g.S == 1 ? GV_WARPS : 16 / g.S;
+        while (GV_WARPS / g.RT > g.KB) {
+            if (16 / g.S < g.RT * 2) g.S /= 2;
+            g.RT *= 2;
+        }
         grid = g.NB * g.S;
     } else {
+        g.RT = GV_WARPS;
+        while (g.RT > 1 && ceil_div(g.tiles, g.RT) < FP8_SM_COUNT * 3 / 2) g.RT /= 2;
+        while (GV_WARPS / g.RT > g.KB) g.RT *= 2;
         const int groups = ceil_div(g.tiles, g.RT);
         grid = groups < 2 * FP8_SM_COUNT ? groups : 2 * FP8_SM_COUNT;
     }
+    g.KS = GV_WARPS / g.RT;
     const int G = g.m <= 8 ? 1 : 2;
     const size_t smem = gemv_smem(g.m, g.KB, glu, quant);
     MM_REQUIRE(smem <= GV_MAX_SMEM, "gemv_fp8: rows too long for the kernel's shared memory");
