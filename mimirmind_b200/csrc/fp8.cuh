@@ -50,6 +50,25 @@ __device__ __forceinline__ float fp8_to_f32(uint8_t v) {
     return __half2float(*reinterpret_cast<const __half*>(&h));
 }
 
+// eight numbers from a 16-byte boundary
+template <typename T>
+__device__ __forceinline__ void fp8_load8(const T* p, float* v);
+template <>
+__device__ __forceinline__ void fp8_load8<float>(const float* p, float* v) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void fp8_load8<__nv_bfloat16>(const __nv_bfloat16* p, float* v) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
 // The gated activations of glu_act for values that are quantised or rounded to 16 bits next: exponentials and quotients of about 2^-20
 // instead of 2^-23 (a tile's 128 x 128 activations in front of nothing else to do took 7 us with the exact ones, 1 us so).  A NaN in either half is
 // kept, also where the clamped form's minimum and maximum would lose it.

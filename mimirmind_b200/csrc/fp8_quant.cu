@@ -6,24 +6,6 @@ namespace {
 
 constexpr int UNITS = 1;
 
-template <typename T>
-__device__ __forceinline__ void load_wide8(const T* p, float* v);
-template <>
-__device__ __forceinline__ void load_wide8<float>(const float* p, float* v) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <>
-__device__ __forceinline__ void load_wide8<__nv_bfloat16>(const __nv_bfloat16* p, float* v) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
-
 // Two blocks of a row per warp and unit, eight numbers a lane, three units' loads on their way at once; where rows start on 16-byte boundaries the loads are wide ones.
 // Bound by memory (3 bytes a number): 4,096 rows of 3,584 bf16 (44 MB) with a division a number 19.7 us, with fp8_quotient PLACEHOLDER us.
 template <typename T>
@@ -43,7 +25,7 @@ __global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const T* __restrict
             const int k = ((int)(u - row * pairs) * 2 + (lane >> 4)) * FP8_BLOCK + (lane & 15) * 8;
             const T* src = x + (source ? source[row] : (int)row) * ldx + k;
             if (wide && k + 8 <= K) {
-                load_wide8<T>(src, v[n]);
+                fp8_load8<T>(src, v[n]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[n][i] = k + i < K ? to_f32<T>(src[i]) : 0.0f;

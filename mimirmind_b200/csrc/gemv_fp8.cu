@@ -144,29 +144,33 @@ __global__ void __launch_bounds__(GV_THREADS, 2) gemv_fp8_kernel(const __grid_co
     if (!QUANT) load_rows(lo);
 
     if (QUANT) {
-        // half a warp per (row, block of the warp's run): eight numbers a lane
-        if (rt == 0 && nb > 0) {
-            const int hl = lane & 15;
-            for (int u = lane >> 4; u < (nb * g.m + 1) / 2 * 2; u += 2) {
-                const int row = u / nb, b = lo + u % nb, k = b * FP8_BLOCK + hl * 8;
-                const bool on = row < g.m;
-                float v[8];
+        // half a warp per (row, block), eight numbers a lane
+        const bool wide = g.K % 8 == 0 && g.ldx % 8 == 0 && ((uintptr_t)g.x & 15) == 0;
+        const int hl = lane & 15, units = g.m * g.KB;
+        for (int u0 = warp * 2; u0 < units; u0 += 2 * GV_WARPS) {
+            const int u = u0 + (lane >> 4), row = u / g.KB, b = u - row * g.KB, k = b * FP8_BLOCK + hl * 8;
+            const bool on = u < units;
+            float v[8];
+            if (on && wide && k + 8 <= g.K) {
+                if (g.x_dtype == MM_F32) fp8_load8<float>((const float*)g.x + (size_t)row * g.ldx + k, v);
+                else fp8_load8<__nv_bfloat16>((const __nv_bfloat16*)g.x + (size_t)row * g.ldx + k, v);
+            } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     v[i] = !on || k + i >= g.K ? 0.0f
                            : g.x_dtype == MM_F32 ? ((const float*)g.x)[(size_t)row * g.ldx + k + i]
                                                  : __bfloat162float(((const __nv_bfloat16*)g.x)[(size_t)row * g.ldx + k + i]);
-                uint32_t big = 0;
+            }
+            uint32_t big = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) big = max(big, fp8_size_bits(v[i]));
+            for (int i = 0; i < 8; ++i) big = max(big, fp8_size_bits(v[i]));
 #pragma unroll
-                for (int o = 8; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-                const float s = fp8_scale_of(big);
-                fp8_quotients<8>(v, s);
-                if (on) {
-                    if (hl == 0) x_scales[row * g.KB + b] = s;
-                    *reinterpret_cast<uint2*>(q_rows + (size_t)row * q_stride(g.KB) + k) = make_uint2(fp8_pack4(v[0], v[1], v[2], v[3]), fp8_pack4(v[4], v[5], v[6], v[7]));
-                }
+            for (int o = 8; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+            const float s = fp8_scale_of(big);
+            fp8_quotients<8>(v, s);
+            if (on) {
+                if (hl == 0) x_scales[row * g.KB + b] = s;
+                *reinterpret_cast<uint2*>(q_rows + (size_t)row * q_stride(g.KB) + k) = make_uint2(fp8_pack4(v[0], v[1], v[2], v[3]), fp8_pack4(v[4], v[5], v[6], v[7]));
             }
         }
     } else {
