@@ -7,7 +7,7 @@
 
 namespace {
 
-constexpr int INSIDE_NUMBERS = 16384;
+constexpr int INSIDE_NUMBERS = 4096;
 
 long long row_bytes(int K) { return (long long)(K + 15) / 16 * 16; }
 // e4m3 rows and their scales behind them

@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int GV_THREADS = 256, GV_WARPS = 8, RING = 4;
+constexpr int GV_THREADS = 256, GV_WARPS = 8, RING = 3;
 constexpr int GV_MAX_SMEM = 113 * 1024;       // two CTAs an SM
 
 struct GemvArgs {
@@ -39,12 +39,12 @@ struct GemvArgs {
 
 // 16 bytes of a row of K from k on, noughts behind its end (nothing there is read): on their way to shared memory, or into registers
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, int k, int K) {      // src = row + k
     const int n = min(max(K - k, 0), 16);
     if (n == 0) src -= k;
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ uint4 load16(const uint8_t* row, int k, int K) {
     if (k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
