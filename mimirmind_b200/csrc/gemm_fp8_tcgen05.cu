@@ -564,13 +564,56 @@ MM_EXPORT int mm_gemm_fp8_tcgen05(const void* A, long long lda, const void* sa, 
     return splits > 1 ? launch<128, false, true>(ta, tw, g, grid, s) : launch<128, false, false>(ta, tw, g, grid, s);
 }
 
-// Tiles of 256 columns where they fill the SMs, else of 128, and as many CTAs to a tile as find room.
+namespace {
+
+// How many clusters of S CTAs are resident at once (37 of 4 would be 148 CTAs, but a cluster stays within one part of the chip).
+template <int BN, bool GLU>
+int resident_clusters(int S) {
+    static std::atomic<int> known[9];
+    int n = known[S].load(std::memory_order_relaxed);
+    if (n > 0) return n;
+    typedef Layout<BN> L;
+    constexpr size_t smem = (size_t)L::PIPE_BYTES + SUM_WARPS * L::STAGING + 1024 + sizeof(Ctl);
+    n = FP8_SM_COUNT / S;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(FP8_SM_COUNT / S * S);
+    cfg.blockDim = dim3(T_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = S;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int found = 0;
+    if (mm_allow_smem<gemm_fp8_tcgen05_kernel<BN, GLU, true>>(smem) &&
+        cudaOccupancyMaxActiveClusters(&found, gemm_fp8_tcgen05_kernel<BN, GLU, true>, &cfg) == cudaSuccess && found > 0) n = found;
+    else (void)cudaGetLastError();
+    known[S].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+}  // namespace
+
+// The tile's width and the number of CTAs to a tile with the least estimated time: rounds of tiles x (a start and an end + blocks x 0.5 us, 0.58 of
+// 256 columns), as measured with 4 to 100 rows.  Us estimated and measured: 16 x 3,584 x 18,944 in 128 columns and 4 CTAs 22 and 23, in 2 CTAs 40
+// and 39, in 8 (two rounds) 26 and 29; 16 x 18,944 x 3,584 in 256 columns and 2 CTAs 12 and 19 (the weights' way from memory is 10), in 128 columns and one 16 and 22.
 int fp8_gemm(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, int* err, cudaStream_t s) {
-    const long long m_tiles = ceil_div(x.rows, 128), blocks = ceil_div(w.K, FP8_BLOCK);
-    int splits = 1;
-    const bool fills = m_tiles * ceil_div(w.N, 256) >= FP8_SM_COUNT;
-    if (!fills)
-        while (splits < 8 && m_tiles * ceil_div(w.N, 128) * splits * 2 <= FP8_SM_COUNT && blocks >= splits * 4) splits *= 2;
+    const long long m_tiles = ceil_div(x.rows, T_ROWS), blocks = ceil_div(w.K, FP8_BLOCK);
+    const float rows = x.rows < T_ROWS ? (float)x.rows / T_ROWS : 1.0f;       // of a tile: what the CTAs of a cluster hand one another
+    int best_wide = 1, best_splits = 1;
+    float best = 1e30f;
+    for (int wide = glu ? 1 : 0; wide < 2; ++wide)
+        for (int splits = 1; splits <= 8 && splits <= blocks; splits *= 2) {
+            const long long tiles = m_tiles * ceil_div(w.N, glu || !wide ? 128 : 256);
+            const int fit = splits == 1 ? FP8_SM_COUNT : glu ? resident_clusters<256, true>(splits) : wide ? resident_clusters<256, false>(splits) : resident_clusters<128, false>(splits);
+            const float us = (float)((tiles + fit - 1) / fit) * ((splits > 1 ? (wide ? 4.0f + 4.0f * rows : 3.0f + 2.0f * rows) : 2.0f) + (float)((blocks + splits - 1) / splits) * (wide ? 0.58f : 0.5f));
+            if (us < best) {
+                best = us;
+                best_wide = wide;
+                best_splits = splits;
+            }
+        }
     return mm_gemm_fp8_tcgen05(x.data, x.ld, x.scales, w.values, w.ld, w.scales, w.matrices, out.data, out.dtype, out.scales, out.ld, out.bias, out.bias_dtype,
-                               x.rows, w.N, w.K, glu, out.act, out.limit, nullptr, nullptr, nullptr, nullptr, 0, glu || fills, splits, err, s);
+                               x.rows, w.N, w.K, glu, out.act, out.limit, nullptr, nullptr, nullptr, nullptr, 0, best_wide, best_splits, err, s);
 }
