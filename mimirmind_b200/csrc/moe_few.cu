@@ -1,0 +1,698 @@
+// A whole routed-experts layer for up to 16 tokens in two launches.
+//
+//   z = x W_router^T;  the choice of `top` experts and their weights (moe_route.cuh)
+//   h[t, c] = act(W_gate[e] x_t, W_up[e] x_t),   out[t] = sum over the choices c in order of wts[t, c] W_down[e] h[t, c],   e = idx[t, c].
+//
+// A few tokens are bound by the chosen experts' matrices: each is read once, by mma.sync with 16 weight rows as the 16-row operand and the expert's
+// rows of x, found by their places, as its 8 (or twice 8) columns.  Nothing is sorted or copied.
+//
+// First launch, clusters of eight CTAs: every cluster makes all logits (an eighth of the router's rows each, handed round over distributed
+// shared memory), every CTA makes the choice and the list of experts with their tokens; then its share of the units of 8 gate and 8 up rows.
+// That costs a read of the router per cluster from L2 and saves a launch and its wait for another.
+// Second launch: 16 output columns a CTA; its warps share out the experts' runs of hidden columns, whose sums are kept apart per (token, choice) and added
+// in the order of the choice.  A token's output does not depend on the others: every sum is cut by the layer's sizes alone.
+//
+// The router's weights are fp32: each is three bf16 parts (hi, mid, lo, 24 bits together), x is bf16, the sums are fp32.
+// Experts in bf16: x as it is, the fp32 hidden rows as two bf16 parts (2^-17 of a number is lost).  Experts in e4m3 with a scale per block of 128 x 128: weights
+// become fp16 exactly; the rows of x and the hidden rows become fp16 after a power of two that brings their largest number to 2^14 .. 2^15
+// (x loses nothing above 2^-29 of its largest, hidden rows keep 11 bits: rounding them to bf16 would cost as much again as rounding the result).
+//
+// Bound by memory: PLACEHOLDER
+#include <cuda_fp16.h>
+
+#include "fp8.cuh"
+#include "fp8_launch.h"
+#include "moe_route.cuh"
+
+namespace {
+
+constexpr int FEW_THREADS = 512, FEW_WARPS = 16, FEW_RING = 3, FEW_SLOT = 2048, FEW_CLUSTER = 8;
+constexpr int FEW_TOKENS = 16, FEW_MAX_EXPERTS = 512, FEW_MAX_TOP = 32;
+constexpr int FEW_SPLIT_BYTES = 64 * 1024;       // of the second launch's sums per (token, choice)
+
+struct FewArgs {
+    const __nv_bfloat16* x;
+    const float* w_router;
+    const float* correction;
+    const uint8_t *w_in, *w_out;          // rows of ld_in, ld_out bytes
+    const float *s_in, *s_out;            // e4m3: scales
+    float* hidden;                        // [pairs][F]
+    uint32_t* largest;                    // [pairs][F / 8]: bits of the units' largest sizes
+    int32_t* lists;                       // entries' number, entries (expert, first place, rows) 3 each, places' pairs
+    float* weights;                       // [pairs]
+    __nv_bfloat16* out;
+    long long ldx, ld_in, ld_out;
+    int n, D, E, top, groups, keep, scoring, renorm, pair_sum, F, act, on_input, interleaved;
+    float wscale, limit;
+    int KS, RT, splits;
+};
+
+__device__ __forceinline__ void few_copy16(uint32_t dst, const uint8_t* row, int at, int bytes) {      // 16 bytes of a row, noughts behind its end
+    const int n = min(max(bytes - at, 0), 16);
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(n > 0 ? row + at : row), "r"(n) : "memory");
+}
+__device__ __forceinline__ void few_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+__device__ __forceinline__ void mma_bf16_f32(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_f32(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pair_f16(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float low_of(uint32_t bf16_pair) { return __uint_as_float(bf16_pair << 16); }
+__device__ __forceinline__ float high_of(uint32_t bf16_pair) { return __uint_as_float(bf16_pair & 0xffff0000u); }
+// four e4m3 numbers as two fp16 pairs
+__device__ __forceinline__ void f16_of(uint32_t w, uint32_t& a, uint32_t& b) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(a), "=r"(b) : "r"(w));
+}
+
+// The power of two that brings a size to 2^14 .. 2^15 (sizes below 2^-112: 2^126), and its inverse; an infinity or a NaN stays one under it.
+__device__ __forceinline__ float f16_scale(uint32_t size_bits) {
+    const int e = min(max((int)(size_bits >> 23), 15), 254);
+    return __uint_as_float((uint32_t)(268 - e) << 23);
+}
+__device__ __forceinline__ float f16_unscale(uint32_t size_bits) {
+    const int e = min(max((int)(size_bits >> 23), 15), 254);
+    return __uint_as_float((uint32_t)(e - 14) << 23);
+}
+
+// A slot of a warp's ring: 128 bytes of 16 weight rows (a lane's four pieces: bytes t * 16 .. + 15 and 64 on of rows g and g + 8), 128 e4m3 or 64
+// bf16 numbers a row.  The order of k inside it is free as long as both operands agree: a lane's pieces are multiplied as they lie.
+
+// ---------------------------------------------------------------------------------------------------------------
+// first launch: router, choice, gate and up products, activation
+// ---------------------------------------------------------------------------------------------------------------
+template <bool FP8, int G>
+__global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_constant__ FewArgs g) {
+    constexpr int TOK = 8 * G;
+    extern __shared__ __align__(16) unsigned char few_smem[];
+    unsigned char* rings = few_smem;                                                            // later also the choice's scratch
+    float* part = reinterpret_cast<float*>(few_smem + FEW_WARPS * FEW_RING * FEW_SLOT);         // [2][16 warps][16][TOK]
+    float* logits = part + 2 * FEW_WARPS * 16 * TOK;                                            // [n][E]
+    const int pairs = g.n * g.top;
+    float* wts = logits + g.n * g.E;                                                            // [pairs]
+    int32_t* idx = reinterpret_cast<int32_t*>(wts + pairs);                                     // [pairs]
+    int32_t* places = idx + pairs;                                                              // [pairs]: the pair at every place, by expert
+    int32_t* entries = places + pairs;                                                          // [pairs][3]
+    int32_t* sums = entries + 3 * pairs;                                                        // [2][16 warps], [2] totals
+    uint32_t* x_largest = reinterpret_cast<uint32_t*>(sums + 2 * FEW_WARPS + 2);                // [16]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t4 = lane & 3;
+    uint32_t rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    pdl_trigger();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // waited for in front of the first store to another CTA: by then it runs
+
+    if (FP8) {
+        if (threadIdx.x < FEW_TOKENS) x_largest[threadIdx.x] = 0;
+        __syncthreads();
+        for (int t = 0; t < g.n; ++t) {
+            uint32_t big = 0;
+            for (int d = threadIdx.x * 8; d < g.D; d += FEW_THREADS * 8) {
+                const uint4 v = *reinterpret_cast<const uint4*>(g.x + (size_t)t * g.ldx + d);       // (D is a multiple of 8)
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) big = max(big, max((w[i] & 0x7fffu) << 16, w[i] & 0x7fff0000u));
+            }
+            big = __reduce_max_sync(0xffffffffu, big);
+            if (lane == 0) atomicMax(x_largest + t, big);
+        }
+    }
+    // ---- logits: 16 experts a tile, a sixteenth of the depth a warp ----
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    {
+        const int steps = (g.D + 15) / 16, lo = steps * warp / FEW_WARPS, hi = steps * (warp + 1) / FEW_WARPS;
+        for (int tile = rank; tile * 16 < g.E; tile += FEW_CLUSTER) {
+            const float *wa = g.w_router + (size_t)min(tile * 16 + gr, g.E - 1) * g.D, *wb = g.w_router + (size_t)min(tile * 16 + gr + 8, g.E - 1) * g.D;
+            float acc[G][4];
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
+#pragma unroll 4
+            for (int s = lo; s < hi; ++s) {
+                const int k = s * 16 + t4 * 4;
+                const bool on = k < g.D;
+                const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float4 a = on ? *reinterpret_cast<const float4*>(wa + k) : zero, b = on ? *reinterpret_cast<const float4*>(wb + k) : zero;
+                uint2 xv[G];
+#pragma unroll
+                for (int j = 0; j < G; ++j)
+                    xv[j] = on && j * 8 + gr < g.n ? *reinterpret_cast<const uint2*>(g.x + (size_t)(j * 8 + gr) * g.ldx + k) : make_uint2(0, 0);
+                float r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {       // hi, mid, lo
+                    const uint32_t a0 = pair_bf16(r[0], r[1]), a2 = pair_bf16(r[2], r[3]), a1 = pair_bf16(r[4], r[5]), a3 = pair_bf16(r[6], r[7]);
+                    if (p < 2) {
+                        r[0] -= low_of(a0); r[1] -= high_of(a0); r[2] -= low_of(a2); r[3] -= high_of(a2);
+                        r[4] -= low_of(a1); r[5] -= high_of(a1); r[6] -= low_of(a3); r[7] -= high_of(a3);
+                    }
+#pragma unroll
+                    for (int j = 0; j < G; ++j) mma_bf16_f32(acc[j], a0, a1, a2, a3, xv[j].x, xv[j].y);
+                }
+            }
+            float* mine = part + (warp * 16 + gr) * TOK + t4 * 2;
+            __syncthreads();        // the tile before has been read
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                *reinterpret_cast<float2*>(mine + j * 8) = make_float2(acc[j][0], acc[j][1]);
+                *reinterpret_cast<float2*>(mine + 8 * TOK + j * 8) = make_float2(acc[j][2], acc[j][3]);
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < 16 * g.n; i += FEW_THREADS) {
+                const int row = i & 15, tok = i >> 4, e = tile * 16 + row;
+                float z = 0.0f;
+#pragma unroll
+                for (int w = 0; w < FEW_WARPS; ++w) z += part[(w * 16 + row) * TOK + tok];
+                if (e < g.E) {
+                    const uint32_t at = (uint32_t)__cvta_generic_to_shared(logits + tok * g.E + e);
+#pragma unroll
+                    for (int r = 0; r < FEW_CLUSTER; ++r) {
+                        uint32_t there;
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(r));
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(z) : "memory");
+                    }
+                }
+            }
+        }
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (no CTA has more logits to hand out behind this: one barrier does)
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+
+    // ---- the choice: a warp per token ----
+    if (warp < g.n)
+        moe_route_warp(logits + warp * g.E, reinterpret_cast<float*>(rings) + (size_t)warp * 2 * (g.E + g.groups), lane, g.E, g.top, g.groups, g.keep, idx, wts,
+                       (size_t)warp, g.scoring, g.correction, g.pair_sum, g.renorm, g.wscale);
+    __syncthreads();
+    // ---- the experts that someone chose, in order, with their pairs (token * top + choice): a thread per expert ----
+    {
+        const int e = threadIdx.x;
+        int count = 0;
+        if (e < g.E)
+            for (int p = 0; p < pairs; ++p) count += idx[p] == e;
+        const int parts = (count + TOK - 1) / TOK;
+        int upto = count, parts_upto = parts;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int a = __shfl_up_sync(0xffffffffu, upto, o), b = __shfl_up_sync(0xffffffffu, parts_upto, o);
+            if (lane >= o) {
+                upto += a;
+                parts_upto += b;
+            }
+        }
+        if (lane == 31) {
+            sums[warp] = upto;
+            sums[FEW_WARPS + warp] = parts_upto;
+        }
+        __syncthreads();
+        int first = upto - count, entry = parts_upto - parts;
+        for (int w = 0; w < warp; ++w) {
+            first += sums[w];
+            entry += sums[FEW_WARPS + w];
+        }
+        if (threadIdx.x == FEW_THREADS - 1) sums[2 * FEW_WARPS] = entry + parts;
+        if (count > 0) {
+            int at = first;
+            for (int p = 0; p < pairs; ++p)
+                if (idx[p] == e) places[at++] = p;
+            for (int i = 0; i < parts; ++i) {
+                entries[3 * (entry + i)] = e;
+                entries[3 * (entry + i) + 1] = first + i * TOK;
+                entries[3 * (entry + i) + 2] = min(TOK, count - i * TOK);
+            }
+        }
+        __syncthreads();
+    }
+    const int n_entries = sums[2 * FEW_WARPS];
+    if (blockIdx.x == 0) {
+        if (threadIdx.x == 0) g.lists[0] = n_entries;
+        for (int i = threadIdx.x; i < 3 * n_entries; i += FEW_THREADS) g.lists[1 + i] = entries[i];
+        for (int i = threadIdx.x; i < pairs; i += FEW_THREADS) {
+            g.lists[1 + 3 * pairs + i] = places[i];
+            g.weights[i] = g.on_input ? 1.0f : wts[i];
+        }
+    }
+
+    // ---- units of 8 gate and 8 up rows: RT side by side, KS runs of slots each ----
+    constexpr int PER = FP8 ? 128 : 64;                  // numbers in a slot's row
+    const int bytes = FP8 ? g.D : 2 * g.D, blocks = (bytes + 127) / 128, uf = g.F / 8, units = n_entries * uf;
+    const int ks = warp % g.KS, rt = warp / g.KS, lo = blocks * ks / g.KS, hi = blocks * (ks + 1) / g.KS, nb = hi - lo;
+    const int groups = (units + g.RT - 1) / g.RT, steps = ((int)blockIdx.x < groups) ? (groups - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+    unsigned char* ring = rings + warp * FEW_RING * FEW_SLOT;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+    const int kb = (g.D + 127) / 128, fb = (g.F + 127) / 128;
+    auto unit_of = [&](int step) { return min(((int)blockIdx.x + step * (int)gridDim.x) * g.RT + rt, units - 1); };      // (a unit behind the last: the last once more, not stored)
+    const uint8_t *pa = nullptr, *pb = nullptr;
+    int load_step = 0, load_b = lo;
+    auto point = [&]() {
+        const int u = unit_of(load_step), e = entries[3 * (u / uf)], f = (u % uf) * 8 + gr;
+        size_t ra, rb;
+        if (FP8) {
+            ra = (size_t)2 * e * g.F + f;
+            rb = ra + g.F;
+        } else if (g.interleaved) {
+            ra = (size_t)2 * e * g.F + 2 * (f - gr) + gr;
+            rb = ra + 8;
+        } else {
+            ra = (size_t)2 * e * g.F + f;
+            rb = ra + g.F;
+        }
+        pa = g.w_in + ra * g.ld_in;
+        pb = g.w_in + rb * g.ld_in;
+    };
+    const int total = nb * steps;
+    auto load = [&](int slot) {
+        const uint32_t dst = ring_at + slot * FEW_SLOT;
+        const int at = load_b * 128 + t4 * 16;
+        few_copy16(dst, pa, at, bytes);
+        few_copy16(dst + 512, pb, at, bytes);
+        few_copy16(dst + 1024, pa, at + 64, bytes);
+        few_copy16(dst + 1536, pb, at + 64, bytes);
+        if (++load_b == hi) {
+            load_b = lo;
+            if (++load_step < steps) point();
+        }
+    };
+    if (total > 0) point();
+#pragma unroll 1
+    for (int i = 0; i < FEW_RING; ++i) {
+        if (i < total) load(i);
+        few_commit();
+    }
+    int done = 0, slot = 0;
+    for (int step = 0; step < steps; ++step) {
+        const int u = unit_of(step), entry = u / uf, f0 = (u % uf) * 8, first = entries[3 * entry + 1], count = entries[3 * entry + 2], e = entries[3 * entry];
+        const __nv_bfloat16* rows[G];
+        float scale[G];
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            const int t = places[first + min(j * 8 + gr, count - 1)] / g.top;
+            rows[j] = g.x + (size_t)t * g.ldx;
+            scale[j] = FP8 ? f16_scale(x_largest[t]) : 1.0f;
+        }
+        const float *sg = nullptr, *su = nullptr;
+        if (FP8) {
+            sg = g.s_in + ((size_t)2 * e * fb + f0 / 128) * kb;
+            su = sg + (size_t)fb * kb;
+        }
+        float acc[G][4];
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
+#pragma unroll 1
+        for (int b = lo; b < hi; ++b) {
+            // the rows of x first: they come while the weights are waited for
+            constexpr int XW = FP8 ? 2 : 1;              // 16-byte pieces of x beside 16 bytes of a weight row
+            uint4 xv[G][2][XW];
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < XW; ++i) {
+                        const int k = b * PER + h * (PER / 2) + t4 * (PER / 8) + i * 8;
+                        xv[j][h][i] = j * 8 + gr < count && k < g.D ? *reinterpret_cast<const uint4*>(rows[j] + k) : make_uint4(0, 0, 0, 0);      // (D is a multiple of 8)
+                    }
+            const float s0 = FP8 ? sg[b] : 1.0f, s1 = FP8 ? su[b] : 1.0f;
+            asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
+            const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
+            uint4 wl[2], wh[2];
+            wl[0] = *reinterpret_cast<const uint4*>(at);
+            wh[0] = *reinterpret_cast<const uint4*>(at + 512);
+            wl[1] = *reinterpret_cast<const uint4*>(at + 1024);
+            wh[1] = *reinterpret_cast<const uint4*>(at + 1536);
+            if (FP8) {
+                float c[G][4];
+#pragma unroll
+                for (int j = 0; j < G; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) c[j][i] = 0.0f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t lw[4] = {wl[h].x, wl[h].y, wl[h].z, wl[h].w}, hw[4] = {wh[h].x, wh[h].y, wh[h].z, wh[h].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t a0, a1, a2, a3;
+                        f16_of(lw[i], a0, a2);
+                        f16_of(hw[i], a1, a3);
+#pragma unroll
+                        for (int j = 0; j < G; ++j) {
+                            if (j > 0 && count <= 8 * j) break;
+                            const uint4 v = xv[j][h][(i >> 1) * (XW - 1)];
+                            const uint32_t p0 = (i & 1) ? v.z : v.x, p1 = (i & 1) ? v.w : v.y;
+                            mma_f16_f32(c[j], a0, a1, a2, a3, pair_f16(low_of(p0) * scale[j], high_of(p0) * scale[j]), pair_f16(low_of(p1) * scale[j], high_of(p1) * scale[j]));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                    acc[j][0] = fmaf(s0, c[j][0], acc[j][0]);
+                    acc[j][1] = fmaf(s0, c[j][1], acc[j][1]);
+                    acc[j][2] = fmaf(s1, c[j][2], acc[j][2]);
+                    acc[j][3] = fmaf(s1, c[j][3], acc[j][3]);
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < G; ++j) {
+                        if (j > 0 && count <= 8 * j) break;
+                        mma_bf16_f32(acc[j], wl[h].x, wh[h].x, wl[h].y, wh[h].y, xv[j][h][0].x, xv[j][h][0].y);
+                        mma_bf16_f32(acc[j], wl[h].z, wh[h].z, wl[h].w, wh[h].w, xv[j][h][0].z, xv[j][h][0].w);
+                    }
+            }
+            if (done + FEW_RING < total) load(slot);
+            few_commit();
+            ++done;
+            slot = slot + 1 == FEW_RING ? 0 : slot + 1;
+        }
+        float* mine = part + (((step & 1) * FEW_WARPS + warp) * 16 + gr) * TOK + t4 * 2;
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            *reinterpret_cast<float2*>(mine + j * 8) = make_float2(acc[j][0], acc[j][1]);
+            *reinterpret_cast<float2*>(mine + 8 * TOK + j * 8) = make_float2(acc[j][2], acc[j][3]);
+        }
+        __syncthreads();
+        // eight columns of a pair by eight neighbouring threads
+        const float* all = part + (step & 1) * FEW_WARPS * 16 * TOK;
+        for (int i = threadIdx.x; i < g.RT * TOK * 8; i += FEW_THREADS) {      // (a multiple of 32)
+            const int f = i & 7, j = (i >> 3) % TOK, tile = (i >> 3) / TOK, unit = ((int)blockIdx.x + step * (int)gridDim.x) * g.RT + tile;
+            const int mine_e = min(unit, units - 1) / uf, cnt = entries[3 * mine_e + 2];
+            const bool on = unit < units && j < cnt;
+            float h = 0.0f;
+            int pair = 0;
+            const int fu = unit % uf;
+            if (on) {
+                pair = places[entries[3 * mine_e + 1] + j];
+                const float* p = all + (tile * g.KS * 16 + f) * TOK + j;
+                float y = 0.0f, v = 0.0f;
+                for (int s = 0; s < g.KS; ++s) {
+                    y += p[s * 16 * TOK];
+                    v += p[s * 16 * TOK + 8 * TOK];
+                }
+                if (FP8) {
+                    const float back = f16_unscale(x_largest[pair / g.top]);
+                    y *= back;
+                    v *= back;
+                }
+                h = fp8_glu(y, v, g.act, g.limit, g.on_input ? wts[pair] : 1.0f);
+                g.hidden[(size_t)pair * g.F + fu * 8 + f] = h;
+            }
+            if (FP8) {
+                uint32_t big = fp8_size_bits(h);
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+                if (on && f == 0) g.largest[(size_t)pair * uf + fu] = big;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// second launch: down products and the weighted sum
+// ---------------------------------------------------------------------------------------------------------------
+template <bool FP8, int G>
+__global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_constant__ FewArgs g) {
+    extern __shared__ __align__(16) unsigned char few_smem[];
+    const int pairs = g.n * g.top;
+    float* sums = reinterpret_cast<float*>(few_smem + FEW_WARPS * FEW_RING * FEW_SLOT);         // [splits][pairs][16]
+    float* wts = sums + (size_t)g.splits * pairs * 16;                                          // [pairs]
+    uint32_t* largest = reinterpret_cast<uint32_t*>(wts + pairs);                               // [pairs]
+    int32_t* places = reinterpret_cast<int32_t*>(largest + pairs);                              // [pairs]
+    int32_t* entries = places + pairs;                                                          // [pairs][3]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t4 = lane & 3;
+    pdl_wait();
+    const int n_entries = g.lists[0];
+    for (int i = threadIdx.x; i < 3 * n_entries; i += FEW_THREADS) entries[i] = g.lists[1 + i];
+    for (int i = threadIdx.x; i < pairs; i += FEW_THREADS) {
+        places[i] = g.lists[1 + 3 * pairs + i];
+        wts[i] = g.weights[i];
+    }
+    __syncthreads();
+    constexpr int PER = FP8 ? 128 : 64;
+    const int bytes = FP8 ? g.F : 2 * g.F, blocks = (bytes + 127) / 128, items = n_entries * g.splits, n0 = blockIdx.x * 16;
+    const int fb = (g.F + 127) / 128, db = (g.D + 127) / 128;
+    unsigned char* ring = few_smem + warp * FEW_RING * FEW_SLOT;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+    const int ra = min(n0 + gr, g.D - 1), rb = min(n0 + gr + 8, g.D - 1);
+    auto run_lo = [&](int split) { return blocks * split / g.splits; };
+    // the cursor of loading: this warp's items (entry, run of hidden columns) one after the other, slot by slot
+    int load_item = warp, load_b = 0, load_hi = 0;
+    const uint8_t *pa = nullptr, *pb = nullptr;
+    auto point = [&]() {
+        if (load_item >= items) return;
+        const int e = entries[3 * (load_item / g.splits)], split = load_item % g.splits;
+        load_b = run_lo(split);
+        load_hi = run_lo(split + 1);
+        pa = g.w_out + ((size_t)e * g.D + ra) * g.ld_out;
+        pb = g.w_out + ((size_t)e * g.D + rb) * g.ld_out;
+    };
+    auto load = [&](int slot) {
+        if (load_item >= items) return;
+        const uint32_t dst = ring_at + slot * FEW_SLOT;
+        const int at = load_b * 128 + t4 * 16;
+        few_copy16(dst, pa, at, bytes);
+        few_copy16(dst + 512, pb, at, bytes);
+        few_copy16(dst + 1024, pa, at + 64, bytes);
+        few_copy16(dst + 1536, pb, at + 64, bytes);
+        if (++load_b == load_hi) {
+            load_item += FEW_WARPS;
+            point();
+        }
+    };
+    point();
+#pragma unroll 1
+    for (int i = 0; i < FEW_RING; ++i) {
+        load(i);
+        few_commit();
+    }
+    if (FP8) {
+        const int uf = g.F / 8;
+        for (int p = warp; p < pairs; p += FEW_WARPS) {
+            uint32_t big = 0;
+            for (int i = lane; i < uf; i += 32) big = max(big, g.largest[(size_t)p * uf + i]);
+            big = __reduce_max_sync(0xffffffffu, big);
+            if (lane == 0) largest[p] = big;
+        }
+        __syncthreads();
+    }
+    int slot = 0;
+    for (int item = warp; item < items; item += FEW_WARPS) {
+        const int entry = item / g.splits, split = item % g.splits, e = entries[3 * entry], first = entries[3 * entry + 1], count = entries[3 * entry + 2];
+        const float* rows[G];
+        float scale[G];
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            const int pair = places[first + min(j * 8 + gr, count - 1)];
+            rows[j] = g.hidden + (size_t)pair * g.F;
+            scale[j] = FP8 ? f16_scale(largest[pair]) : 1.0f;
+        }
+        const float* sw = FP8 ? g.s_out + ((size_t)e * db + min(n0, g.D - 1) / 128) * fb : nullptr;
+        float acc[G][4];
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
+        const int hi = run_lo(split + 1);
+#pragma unroll 1
+        for (int b = run_lo(split); b < hi; ++b) {
+            const float s0 = FP8 ? sw[b] : 1.0f;
+            asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
+            const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
+            float c[G][4];
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) c[j][i] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint4 wl = *reinterpret_cast<const uint4*>(at + 1024 * h), wh = *reinterpret_cast<const uint4*>(at + 512 + 1024 * h);
+                const uint32_t lw[4] = {wl.x, wl.y, wl.z, wl.w}, hw[4] = {wh.x, wh.y, wh.z, wh.w};
+#pragma unroll
+                for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
+                    uint32_t a0, a1, a2, a3;
+                    if (FP8) {
+                        f16_of(lw[i], a0, a2);
+                        f16_of(hw[i], a1, a3);
+                    } else {
+                        a0 = lw[2 * i];
+                        a2 = lw[2 * i + 1];
+                        a1 = hw[2 * i];
+                        a3 = hw[2 * i + 1];
+                    }
+                    const int k = b * PER + h * (PER / 2) + t4 * (PER / 8) + i * 4;
+#pragma unroll
+                    for (int j = 0; j < G; ++j) {
+                        if (j > 0 && count <= 8 * j) break;
+                        const float4 v = j * 8 + gr < count && k < g.F ? *reinterpret_cast<const float4*>(rows[j] + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);      // (F is a multiple of 8)
+                        if (FP8) {
+                            mma_f16_f32(c[j], a0, a1, a2, a3, pair_f16(v.x * scale[j], v.y * scale[j]), pair_f16(v.z * scale[j], v.w * scale[j]));
+                        } else {
+                            const uint32_t p0 = pair_bf16(v.x, v.y), p1 = pair_bf16(v.z, v.w);
+                            mma_bf16_f32(acc[j], a0, a1, a2, a3, p0, p1);
+                            mma_bf16_f32(acc[j], a0, a1, a2, a3, pair_bf16(v.x - low_of(p0), v.y - high_of(p0)), pair_bf16(v.z - low_of(p1), v.w - high_of(p1)));
+                        }
+                    }
+                }
+            }
+            if (FP8) {
+#pragma unroll
+                for (int j = 0; j < G; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(s0, c[j][i], acc[j][i]);
+            }
+            load(slot);
+            few_commit();
+            slot = slot + 1 == FEW_RING ? 0 : slot + 1;
+        }
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int col = j * 8 + t4 * 2 + c;
+                if (col >= count) continue;
+                const int pair = places[first + col];
+                const float back = FP8 ? f16_unscale(largest[pair]) : 1.0f;
+                float* at = sums + ((size_t)split * pairs + pair) * 16 + gr;
+                at[0] = acc[j][c] * back;
+                at[8] = acc[j][2 + c] * back;
+            }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * g.n; i += FEW_THREADS) {
+        const int row = i & 15, t = i >> 4;
+        if (n0 + row >= g.D) continue;
+        float total = 0.0f;
+        for (int c = 0; c < g.top; ++c) {
+            float y = 0.0f;
+            for (int s = 0; s < g.splits; ++s) y += sums[((size_t)s * pairs + t * g.top + c) * 16 + row];
+            total = fmaf(wts[t * g.top + c], y, total);
+        }
+        g.out[(size_t)t * g.D + n0 + row] = __float2bfloat16_rn(total);
+    }
+}
+
+size_t in_smem(const FewArgs& g) {
+    const int tok = g.n <= 8 ? 8 : 16, pairs = g.n * g.top;
+    return (size_t)FEW_WARPS * FEW_RING * FEW_SLOT + 4 * ((size_t)2 * FEW_WARPS * 16 * tok + g.n * g.E + 6 * pairs + 2 * FEW_WARPS + 2 + FEW_TOKENS);
+}
+size_t out_smem(const FewArgs& g) {
+    const int pairs = g.n * g.top;
+    return (size_t)FEW_WARPS * FEW_RING * FEW_SLOT + 4 * ((size_t)g.splits * pairs * 16 + 6 * pairs);
+}
+
+template <bool FP8, int G>
+int launch(FewArgs& g, cudaStream_t s) {
+    constexpr size_t most = 227 * 1024;
+    const size_t smem_in = in_smem(g), smem_out = out_smem(g);
+    MM_REQUIRE(smem_in <= most && smem_out <= most, "moe few: too many experts or choices for the kernels' shared memory");
+    if (!mm_allow_smem<few_in_kernel<FP8, G>>(most) || !mm_allow_smem<few_out_kernel<FP8, G>>(most)) {
+        mm_set_last_error("moe few: cannot reserve shared memory");
+        return MM_ERR_LAUNCH;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(FEW_THREADS);
+    cfg.dynamicSmemBytes = smem_in;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = FEW_CLUSTER;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    // as many clusters as are resident at once, or as there are units for
+    static std::atomic<int> resident{0};
+    int fit = resident.load(std::memory_order_relaxed);
+    if (fit == 0) {
+        cfg.gridDim = dim3(FP8_SM_COUNT / FEW_CLUSTER * FEW_CLUSTER);
+        if (cudaOccupancyMaxActiveClusters(&fit, few_in_kernel<FP8, G>, &cfg) != cudaSuccess || fit < 1) {
+            (void)cudaGetLastError();
+            fit = FP8_SM_COUNT / FEW_CLUSTER;
+        }
+        resident.store(fit, std::memory_order_relaxed);
+    }
+    const int most_experts = g.E < g.n * g.top ? g.E : g.n * g.top;
+    const long long groups = ((long long)most_experts * (g.F / 8) + g.RT - 1) / g.RT, clusters = (groups + FEW_CLUSTER - 1) / FEW_CLUSTER;
+    cfg.gridDim = dim3((unsigned)(clusters < fit ? clusters : fit) * FEW_CLUSTER);
+    cudaLaunchKernelEx(&cfg, few_in_kernel<FP8, G>, g);
+    MM_CHECK_LAUNCH();
+    mm_launch_dependent(g_mm_pdl != 0, few_out_kernel<FP8, G>, dim3(ceil_div(g.D, 16)), dim3(FEW_THREADS), smem_out, s, g);
+    MM_CHECK_LAUNCH();
+    return MM_OK;
+}
+
+}  // namespace
+
+// x bf16 [n, ldx]; w_router fp32 [E, D]; experts bf16 (s_in, s_out null): w_in [E, 2 F, D] (gate rows then up rows, or with `interleaved` alternating in
+// blocks of 8), w_out [E, D, F]; or e4m3 with scales: w_in [E, 2, F, ld_in], w_out [E, D, ld_out].  ld_in, ld_out: bytes of a row.
+// out bf16 [n, D].  scratch: pairs * (4 F + F / 2 + 24) + 16 bytes, pairs = n * top.
+MM_EXPORT int mm_moe_few(const void* x, long long ldx, int n, int D, const void* w_router, int E, int top, int groups, int keep, int scoring, const void* correction,
+                         int pair_sum, int renorm, float wscale, const void* w_in, const void* s_in, long long ld_in, const void* w_out, const void* s_out, long long ld_out,
+                         int F, int act, float limit, int on_input, int interleaved, void* out, void* scratch, void* stream) {
+    MM_REQUIRE(n >= 0 && n <= FEW_TOKENS, "moe few: at most 16 tokens");
+    MM_REQUIRE(E > 0 && E <= FEW_MAX_EXPERTS && top > 0 && top <= FEW_MAX_TOP, "moe few: at most 512 experts and 32 choices");
+    MM_REQUIRE(groups > 0 && E % groups == 0 && keep > 0 && keep <= groups && top <= keep * (E / groups),
+               "moe few: experts must split into equal runs, 0 < keep <= runs, and top fits into the kept runs");
+    MM_REQUIRE(scoring == 0 || scoring == 1, "moe few: the scoring is 0 (softmax) or 1 (sigmoid)");
+    MM_REQUIRE(act >= 0 && act <= MM_GLU_GELU_TANH, "moe few: unknown activation");
+    const bool fp8 = s_in != nullptr;
+    MM_REQUIRE(fp8 == (s_out != nullptr) && !(fp8 && interleaved), "moe few: both matrices are in bf16 or both in 8 bits");
+    MM_REQUIRE(D > 0 && F > 0 && D % 8 == 0 && F % 8 == 0 && ldx % 8 == 0 && ldx >= 0, "moe few: widths and row strides must be multiples of 8");
+    MM_REQUIRE(ld_in % 16 == 0 && ld_out % 16 == 0 && ld_in >= (fp8 ? D : 2 * (long long)D) && ld_out >= (fp8 ? F : 2 * (long long)F), "moe few: weight rows must start on 16-byte boundaries");
+    MM_REQUIRE((((uintptr_t)x | (uintptr_t)w_router | (uintptr_t)w_in | (uintptr_t)w_out | (uintptr_t)scratch) & 15) == 0, "moe few: tensors must start on 16-byte boundaries");
+    MM_REQUIRE((long long)E * (F / 8) < 0x3fffffff && D < (1 << 28) && F < (1 << 28), "moe few: too large");
+    if (n == 0) return MM_OK;
+    FewArgs g = {};
+    const size_t pairs = (size_t)n * top;
+    g.x = (const __nv_bfloat16*)x;
+    g.ldx = ldx;
+    g.w_router = (const float*)w_router;
+    g.correction = (const float*)correction;
+    g.w_in = (const uint8_t*)w_in;
+    g.w_out = (const uint8_t*)w_out;
+    g.s_in = (const float*)s_in;
+    g.s_out = (const float*)s_out;
+    g.ld_in = ld_in;
+    g.ld_out = ld_out;
+    g.hidden = (float*)scratch;
+    g.largest = (uint32_t*)(g.hidden + pairs * F);
+    g.weights = (float*)(g.largest + pairs * (F / 8));
+    g.lists = (int32_t*)(g.weights + pairs);
+    g.out = (__nv_bfloat16*)out;
+    g.n = n;
+    g.D = D;
+    g.E = E;
+    g.top = top;
+    g.groups = groups;
+    g.keep = keep;
+    g.scoring = scoring;
+    g.renorm = renorm;
+    g.pair_sum = pair_sum;
+    g.wscale = wscale;
+    g.F = F;
+    g.act = act;
+    g.limit = limit;
+    g.on_input = on_input;
+    g.interleaved = interleaved;
+    const int in_blocks = (int)(((fp8 ? 1LL : 2LL) * D + 127) / 128), out_blocks = (int)(((fp8 ? 1LL : 2LL) * F + 127) / 128);
+    g.KS = 8;
+    while (g.KS > in_blocks) g.KS /= 2;
+    g.RT = FEW_WARPS / g.KS;
+    g.splits = FEW_SPLIT_BYTES / (FEW_TOKENS * top * 64);
+    if (g.splits < 1) g.splits = 1;
+    if (g.splits > out_blocks) g.splits = out_blocks;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (fp8) return n <= 8 ? launch<true, 1>(g, s) : launch<true, 2>(g, s);
+    return n <= 8 ? launch<false, 1>(g, s) : launch<false, 2>(g, s);
+}

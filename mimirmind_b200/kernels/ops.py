@@ -2247,3 +2247,63 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, wts: torch.Tensor, w_in:
     y = torch.empty((n * top, d), dtype=torch.float32, device=x.device)
     _fp8_grouped(hidden, w_out, rows, y, None)
     return moe_combine(y, None if on_input else wts, torch.bfloat16, place=rows.place, top=top)
+
+
+MOE_FEW_TOKENS = 16         # rows of a step that a routed-experts layer takes in two launches
+
+
+def moe_few_supported(n: int, experts: int, top: int, d: int, f: int) -> bool:
+    """True if :func:`moe_few` takes a layer of these sizes."""
+    return 0 <= n <= MOE_FEW_TOKENS and 1 <= experts <= 512 and 1 <= top <= min(32, experts) and d % 8 == 0 and f % 8 == 0 and d > 0 and f > 0
+
+
+def moe_few(x: torch.Tensor, w_router: torch.Tensor, w_in, w_out, top: int, groups: int = 1, keep: int = 1, *, scoring: str = "softmax",
+            renorm: Optional[bool] = None, scale: float = 1.0, correction: Optional[torch.Tensor] = None, group_score: str = "max",
+            activation: str = "silu", limit: float = 0.0, weight_on: str = "output", interleaved: bool = False) -> torch.Tensor:
+    """A whole routed-experts layer for up to 16 rows ``x`` bf16 [n, D] in two launches: the router's product and choice (as
+    :func:`moe_router`: ``top``, ``groups``, ``keep``, ``scoring``, ``renorm``, ``scale``, ``correction``, ``group_score``; ``w_router`` fp32 [E, D]) and
+    ``out[t] = sum_c wts[t, c] Wd_e act(Wg_e x_t, Wu_e x_t)``, ``e`` the token's c-th choice, as bf16 [n, D].  Experts in bf16: ``w_in`` [E, 2F, D], the gate's rows then the
+    up rows of every expert (``interleaved``: alternating in blocks of 8), ``w_out`` [E, D, F]; or in 8 bits: :class:`Fp8Weight` [E, 2, F, D] and [E, D, F]
+    (the rows are not quantised: they become fp16 after a power of two).  ``activation``, ``limit``: as for :func:`moe_gemm`; ``weight_on`` ``input``: the weight
+    multiplies the first products.  D and F are multiples of 8; a row of x starts on a 16-byte boundary."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() != 2:
+        raise KernelError("moe_few: expected bfloat16 rows on a CUDA device")
+    _need(w_router, "moe_few router", torch.float32)
+    n, d = x.shape
+    fp8 = isinstance(w_in, Fp8Weight)
+    if fp8:
+        _check_experts_fp8(x, w_in, w_out, "moe_few")
+        E, _, f, _ = w_in.shape
+        tensors = (w_in.values, w_in.scales, w_out.values, w_out.scales)
+        ld_in, ld_out = w_in.ld, w_out.ld
+    else:
+        _need(w_in, "moe_few w_in", torch.bfloat16)
+        _need(w_out, "moe_few w_out", torch.bfloat16)
+        if w_in.dim() != 3 or w_out.dim() != 3 or w_in.shape[1] % 2 or w_in.shape[2] != d or tuple(w_out.shape) != (w_in.shape[0], d, w_in.shape[1] // 2):
+            raise KernelError("moe_few: w_in must be [E, 2F, D] and w_out [E, D, F]")
+        E, f = w_in.shape[0], w_in.shape[1] // 2
+        tensors = (w_in, None, w_out, None)
+        ld_in, ld_out = 2 * d, 2 * f
+    if tuple(w_router.shape) != (E, d):
+        raise KernelError("moe_few: the router's matrix must be [E, D]")
+    if not moe_few_supported(n, E, top, d, f):
+        raise KernelError(f"moe_few: {n} rows, {E} experts, {top} choices, widths {d} and {f} are not supported")
+    if n and (x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < 0 or x.data_ptr() % 16):
+        raise KernelError("moe_few: rows must be contiguous and start on 16-byte boundaries")
+    if scoring not in ROUTER_SCORINGS or group_score not in GROUP_SCORES or weight_on not in ("output", "input"):
+        raise KernelError("moe_few: scoring is 'softmax' or 'sigmoid', group_score 'max' or 'top2_sum', weight_on 'output' or 'input'")
+    if interleaved and fp8:
+        raise KernelError("moe_few: experts in 8 bits are not interleaved")
+    if correction is not None:
+        _need(correction, "moe_few correction", torch.float32)
+        if correction.numel() != E:
+            raise KernelError("moe_few: one correction per expert is needed")
+    act = _glu_code(activation, limit, "moe_few")
+    _here("moe_few", x, w_router, correction, *tensors)
+    out = torch.empty((n, d), dtype=torch.bfloat16, device=x.device)
+    scratch = torch.empty(n * top * (4 * f + f // 2 + 24) + 16, dtype=torch.uint8, device=x.device)
+    check(_lib.load().mm_moe_few(x.data_ptr(), x.stride(0), n, d, w_router.data_ptr(), E, int(top), int(groups), int(keep), ROUTER_SCORINGS[scoring], _ptr(correction),
+                                 GROUP_SCORES[group_score], int(scoring == "softmax" if renorm is None else renorm), float(scale), tensors[0].data_ptr(), _ptr(tensors[1]),
+                                 ld_in, tensors[2].data_ptr(), _ptr(tensors[3]), ld_out, f, act, float(limit), int(weight_on == "input"), int(bool(interleaved)),
+                                 out.data_ptr(), scratch.data_ptr(), _stream()), "moe_few")
+    return out
