@@ -28,7 +28,7 @@ namespace {
 
 constexpr int FEW_THREADS = 512, FEW_WARPS = 16, FEW_RING = 3, FEW_SLOT = 2048, FEW_CLUSTER = 8;
 constexpr int FEW_TOKENS = 16, FEW_MAX_EXPERTS = 512, FEW_MAX_TOP = 32;
-constexpr int FEW_SPLIT_BYTES = 64 * 1024;       // of the second launch's sums per (token, choice)
+constexpr int FEW_CLUSTERS = FP8_SM_COUNT / FEW_CLUSTER;      // at the most
 
 struct FewArgs {
     const __nv_bfloat16* x;
@@ -40,16 +40,20 @@ struct FewArgs {
     uint32_t* largest;                    // [pairs][F / 8]: bits of the units' largest sizes
     int32_t* lists;                       // entries' number, entries (expert, first place, rows) 3 each, places' pairs
     float* weights;                       // [pairs]
+    uint16_t* x_half;                     // e4m3 experts: [clusters][n][D] fp16
     __nv_bfloat16* out;
     long long ldx, ld_in, ld_out;
     int n, D, E, top, groups, keep, scoring, renorm, pair_sum, F, act, on_input, interleaved;
     float wscale, limit;
-    int KS, RT, splits;
+    int KS, splits;
 };
 
 __device__ __forceinline__ void few_copy16(uint32_t dst, const uint8_t* row, int at, int bytes) {      // 16 bytes of a row, noughts behind its end
     const int n = min(max(bytes - at, 0), 16);
     asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(n > 0 ? row + at : row), "r"(n) : "memory");
+}
+__device__ __forceinline__ void few_copy16(uint32_t dst, const uint8_t* src) {
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void few_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
@@ -106,6 +110,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
     int32_t* entries = places + pairs;                                                          // [pairs][3]
     int32_t* sums = entries + 3 * pairs;                                                        // [2][16 warps], [2] totals
     uint32_t* x_largest = reinterpret_cast<uint32_t*>(sums + 2 * FEW_WARPS + 2);                // [16]
+    uint16_t* x_half = FP8 ? g.x_half + (size_t)(blockIdx.x / FEW_CLUSTER) * g.n * g.D : nullptr;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t4 = lane & 3;
     uint32_t rank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -125,6 +130,18 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
             }
             big = __reduce_max_sync(0xffffffffu, big);
             if (lane == 0) atomicMax(x_largest + t, big);
+        }
+        __syncthreads();
+        // the cluster's own copy of x in fp16, an eighth by every CTA (read behind the cluster's barrier)
+        for (int i = rank * FEW_THREADS + threadIdx.x; i < g.n * (g.D / 8); i += FEW_CLUSTER * FEW_THREADS) {
+            const int t = i / (g.D / 8), d = (i - t * (g.D / 8)) * 8;
+            const uint4 v = *reinterpret_cast<const uint4*>(g.x + (size_t)t * g.ldx + d);
+            const float s = f16_scale(x_largest[t]);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = pair_f16(low_of(w[k]) * s, high_of(w[k]) * s);
+            *reinterpret_cast<uint4*>(x_half + (size_t)t * g.D + d) = make_uint4(o[0], o[1], o[2], o[3]);
         }
     }
     // ---- logits: 16 experts a tile, a sixteenth of the depth a warp ----
@@ -243,24 +260,45 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
         }
     }
 
-    // ---- units of 8 gate and 8 up rows: RT side by side, KS runs of slots each ----
+    // ---- units of 8 gate and 8 up rows, a unit's depth in KS runs: a warp per run and the runs' sums added over shared memory, or, where there are many
+    // units, a warp per unit that goes through the runs itself.  The sums are the same to the bit.  The cheaper one by rounds of slots (a meeting of the
+    // warps costs about two)  ----
     constexpr int PER = FP8 ? 128 : 64;                  // numbers in a slot's row
     const int bytes = FP8 ? g.D : 2 * g.D, blocks = (bytes + 127) / 128, uf = g.F / 8, units = n_entries * uf;
-    const int ks = warp % g.KS, rt = warp / g.KS, lo = blocks * ks / g.KS, hi = blocks * (ks + 1) / g.KS, nb = hi - lo;
-    const int groups = (units + g.RT - 1) / g.RT, steps = ((int)blockIdx.x < groups) ? (groups - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+    const int side = FEW_WARPS / g.KS;
+    const bool alone = (units + (int)gridDim.x * FEW_WARPS - 1) / ((int)gridDim.x * FEW_WARPS) * blocks <=
+                       (units + (int)gridDim.x * side - 1) / ((int)gridDim.x * side) * (blocks / g.KS + 2);
+    const int RT = alone ? FEW_WARPS : side, rt = alone ? warp : warp / g.KS, run_lo = alone ? 0 : warp % g.KS, run_hi = alone ? g.KS : run_lo + 1;
+    const int lo = blocks * run_lo / g.KS, hi = blocks * run_hi / g.KS, nb = hi - lo;
+    const int groups = (units + RT - 1) / RT, steps = (int)blockIdx.x < groups ? (groups - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+    const int stride = (int)gridDim.x * RT, unit0 = (int)blockIdx.x * RT + rt;
+    const int my_steps = alone ? (unit0 < units ? (units - 1 - unit0) / stride + 1 : 0) : steps;
     unsigned char* ring = rings + warp * FEW_RING * FEW_SLOT;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
     const int kb = (g.D + 127) / 128, fb = (g.F + 127) / 128;
-    auto unit_of = [&](int step) { return min(((int)blockIdx.x + step * (int)gridDim.x) * g.RT + rt, units - 1); };      // (a unit behind the last: the last once more, not stored)
+    // a place in the units: (entry, unit of 8 columns), carried along; behind the last unit it stays on it (not stored)
+    struct Cursor {
+        int entry, fu;
+    };
+    auto cursor_at = [&](int u) {
+        u = min(u, units - 1);
+        return Cursor{u / uf, u % uf};
+    };
+    auto advance = [&](Cursor& c) {
+        c.fu += stride;
+        while (c.fu >= uf && c.entry < n_entries) {
+            c.fu -= uf;
+            ++c.entry;
+        }
+        if (c.entry >= n_entries) c = {n_entries - 1, uf - 1};
+    };
     const uint8_t *pa = nullptr, *pb = nullptr;
-    int load_step = 0, load_b = lo;
+    Cursor ahead = cursor_at(unit0), here = ahead;
+    int load_b = lo;
     auto point = [&]() {
-        const int u = unit_of(load_step), e = entries[3 * (u / uf)], f = (u % uf) * 8 + gr;
+        const int e = entries[3 * ahead.entry], f = ahead.fu * 8 + gr;
         size_t ra, rb;
-        if (FP8) {
-            ra = (size_t)2 * e * g.F + f;
-            rb = ra + g.F;
-        } else if (g.interleaved) {
+        if (!FP8 && g.interleaved) {
             ra = (size_t)2 * e * g.F + 2 * (f - gr) + gr;
             rb = ra + 8;
         } else {
@@ -270,17 +308,26 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
         pa = g.w_in + ra * g.ld_in;
         pb = g.w_in + rb * g.ld_in;
     };
-    const int total = nb * steps;
+    const int total = nb * my_steps;
+    const bool whole = bytes % 128 == 0;
     auto load = [&](int slot) {
         const uint32_t dst = ring_at + slot * FEW_SLOT;
         const int at = load_b * 128 + t4 * 16;
-        few_copy16(dst, pa, at, bytes);
-        few_copy16(dst + 512, pb, at, bytes);
-        few_copy16(dst + 1024, pa, at + 64, bytes);
-        few_copy16(dst + 1536, pb, at + 64, bytes);
+        if (whole) {
+            few_copy16(dst, pa + at);
+            few_copy16(dst + 512, pb + at);
+            few_copy16(dst + 1024, pa + at + 64);
+            few_copy16(dst + 1536, pb + at + 64);
+        } else {
+            few_copy16(dst, pa, at, bytes);
+            few_copy16(dst + 512, pb, at, bytes);
+            few_copy16(dst + 1024, pa, at + 64, bytes);
+            few_copy16(dst + 1536, pb, at + 64, bytes);
+        }
         if (++load_b == hi) {
             load_b = lo;
-            if (++load_step < steps) point();
+            advance(ahead);
+            point();
         }
     };
     if (total > 0) point();
@@ -290,49 +337,50 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
         few_commit();
     }
     int done = 0, slot = 0;
-    for (int step = 0; step < steps; ++step) {
-        const int u = unit_of(step), entry = u / uf, f0 = (u % uf) * 8, first = entries[3 * entry + 1], count = entries[3 * entry + 2], e = entries[3 * entry];
-        const __nv_bfloat16* rows[G];
-        float scale[G];
+#pragma unroll 1
+    for (int step = 0; step < my_steps; ++step) {
+        const int first = entries[3 * here.entry + 1], count = entries[3 * here.entry + 2], f0 = here.fu * 8;
+        const uint16_t* rows[G];
 #pragma unroll
         for (int j = 0; j < G; ++j) {
             const int t = places[first + min(j * 8 + gr, count - 1)] / g.top;
-            rows[j] = g.x + (size_t)t * g.ldx;
-            scale[j] = FP8 ? f16_scale(x_largest[t]) : 1.0f;
+            rows[j] = (FP8 ? x_half + (size_t)t * g.D : reinterpret_cast<const uint16_t*>(g.x) + (size_t)t * g.ldx) + t4 * (PER / 8);
         }
         const float *sg = nullptr, *su = nullptr;
         if (FP8) {
-            sg = g.s_in + ((size_t)2 * e * fb + f0 / 128) * kb;
+            sg = g.s_in + ((size_t)2 * entries[3 * here.entry] * fb + f0 / 128) * kb;
             su = sg + (size_t)fb * kb;
         }
-        float acc[G][4];
+        float sum[G][4];
 #pragma unroll
         for (int j = 0; j < G; ++j)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
+            for (int c = 0; c < 4; ++c) sum[j][c] = 0.0f;
 #pragma unroll 1
-        for (int b = lo; b < hi; ++b) {
-            // the rows of x first: they come while the weights are waited for
-            constexpr int XW = FP8 ? 2 : 1;              // 16-byte pieces of x beside 16 bytes of a weight row
-            uint4 xv[G][2][XW];
+        for (int run = run_lo; run < run_hi; ++run) {
+            float acc[G][4];
 #pragma unroll
             for (int j = 0; j < G; ++j)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
+            const int end = blocks * (run + 1) / g.KS;
+#pragma unroll 1
+            for (int b = blocks * run / g.KS; b < end; ++b) {
+                // the rows of x first: they come while the weights are waited for
+                constexpr int XW = FP8 ? 2 : 1;              // 16-byte pieces of x beside 16 bytes of a weight row
+                uint4 xv[G][2][XW];
 #pragma unroll
-                    for (int i = 0; i < XW; ++i) {
-                        const int k = b * PER + h * (PER / 2) + t4 * (PER / 8) + i * 8;
-                        xv[j][h][i] = j * 8 + gr < count && k < g.D ? *reinterpret_cast<const uint4*>(rows[j] + k) : make_uint4(0, 0, 0, 0);      // (D is a multiple of 8)
-                    }
-            const float s0 = FP8 ? sg[b] : 1.0f, s1 = FP8 ? su[b] : 1.0f;
-            asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
-            const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
-            uint4 wl[2], wh[2];
-            wl[0] = *reinterpret_cast<const uint4*>(at);
-            wh[0] = *reinterpret_cast<const uint4*>(at + 512);
-            wl[1] = *reinterpret_cast<const uint4*>(at + 1024);
-            wh[1] = *reinterpret_cast<const uint4*>(at + 1536);
-            if (FP8) {
+                for (int j = 0; j < G; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < XW; ++i) {
+                            const int k = b * PER + h * (PER / 2) + i * 8;
+                            xv[j][h][i] = j * 8 + gr < count && (whole || k + t4 * (PER / 8) < g.D) ? *reinterpret_cast<const uint4*>(rows[j] + k) : make_uint4(0, 0, 0, 0);      // (D is a multiple of 8)
+                        }
+                const float s0 = FP8 ? sg[b] : 1.0f, s1 = FP8 ? su[b] : 1.0f;
+                asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
+                const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
                 float c[G][4];
 #pragma unroll
                 for (int j = 0; j < G; ++j)
@@ -340,82 +388,115 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
                     for (int i = 0; i < 4; ++i) c[j][i] = 0.0f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t lw[4] = {wl[h].x, wl[h].y, wl[h].z, wl[h].w}, hw[4] = {wh[h].x, wh[h].y, wh[h].z, wh[h].w};
+                    const uint4 wl = *reinterpret_cast<const uint4*>(at + 1024 * h), wh = *reinterpret_cast<const uint4*>(at + 512 + 1024 * h);
+                    const uint32_t lw[4] = {wl.x, wl.y, wl.z, wl.w}, hw[4] = {wh.x, wh.y, wh.z, wh.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
                         uint32_t a0, a1, a2, a3;
-                        f16_of(lw[i], a0, a2);
-                        f16_of(hw[i], a1, a3);
+                        if (FP8) {
+                            f16_of(lw[i], a0, a2);
+                            f16_of(hw[i], a1, a3);
+                        } else {
+                            a0 = lw[2 * i];
+                            a2 = lw[2 * i + 1];
+                            a1 = hw[2 * i];
+                            a3 = hw[2 * i + 1];
+                        }
 #pragma unroll
                         for (int j = 0; j < G; ++j) {
                             if (j > 0 && count <= 8 * j) break;
-                            const uint4 v = xv[j][h][(i >> 1) * (XW - 1)];
+                            const uint4 v = xv[j][h][FP8 ? i >> 1 : 0];
                             const uint32_t p0 = (i & 1) ? v.z : v.x, p1 = (i & 1) ? v.w : v.y;
-                            mma_f16_f32(c[j], a0, a1, a2, a3, pair_f16(low_of(p0) * scale[j], high_of(p0) * scale[j]), pair_f16(low_of(p1) * scale[j], high_of(p1) * scale[j]));
+                            if (FP8) mma_f16_f32(c[j], a0, a1, a2, a3, p0, p1);
+                            else mma_bf16_f32(acc[j], a0, a1, a2, a3, p0, p1);
                         }
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    acc[j][0] = fmaf(s0, c[j][0], acc[j][0]);
-                    acc[j][1] = fmaf(s0, c[j][1], acc[j][1]);
-                    acc[j][2] = fmaf(s1, c[j][2], acc[j][2]);
-                    acc[j][3] = fmaf(s1, c[j][3], acc[j][3]);
-                }
-            } else {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
+                if (FP8) {
 #pragma unroll
                     for (int j = 0; j < G; ++j) {
-                        if (j > 0 && count <= 8 * j) break;
-                        mma_bf16_f32(acc[j], wl[h].x, wh[h].x, wl[h].y, wh[h].y, xv[j][h][0].x, xv[j][h][0].y);
-                        mma_bf16_f32(acc[j], wl[h].z, wh[h].z, wl[h].w, wh[h].w, xv[j][h][0].z, xv[j][h][0].w);
+                        acc[j][0] = fmaf(s0, c[j][0], acc[j][0]);
+                        acc[j][1] = fmaf(s0, c[j][1], acc[j][1]);
+                        acc[j][2] = fmaf(s1, c[j][2], acc[j][2]);
+                        acc[j][3] = fmaf(s1, c[j][3], acc[j][3]);
                     }
+                }
+                if (done + FEW_RING < total) load(slot);
+                few_commit();
+                ++done;
+                slot = slot + 1 == FEW_RING ? 0 : slot + 1;
             }
-            if (done + FEW_RING < total) load(slot);
-            few_commit();
-            ++done;
-            slot = slot + 1 == FEW_RING ? 0 : slot + 1;
-        }
-        float* mine = part + (((step & 1) * FEW_WARPS + warp) * 16 + gr) * TOK + t4 * 2;
 #pragma unroll
-        for (int j = 0; j < G; ++j) {
-            *reinterpret_cast<float2*>(mine + j * 8) = make_float2(acc[j][0], acc[j][1]);
-            *reinterpret_cast<float2*>(mine + 8 * TOK + j * 8) = make_float2(acc[j][2], acc[j][3]);
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sum[j][c] += acc[j][c];
         }
-        __syncthreads();
-        // eight columns of a pair by eight neighbouring threads
-        const float* all = part + (step & 1) * FEW_WARPS * 16 * TOK;
-        for (int i = threadIdx.x; i < g.RT * TOK * 8; i += FEW_THREADS) {      // (a multiple of 32)
-            const int f = i & 7, j = (i >> 3) % TOK, tile = (i >> 3) / TOK, unit = ((int)blockIdx.x + step * (int)gridDim.x) * g.RT + tile;
-            const int mine_e = min(unit, units - 1) / uf, cnt = entries[3 * mine_e + 2];
-            const bool on = unit < units && j < cnt;
-            float h = 0.0f;
-            int pair = 0;
-            const int fu = unit % uf;
-            if (on) {
-                pair = places[entries[3 * mine_e + 1] + j];
-                const float* p = all + (tile * g.KS * 16 + f) * TOK + j;
-                float y = 0.0f, v = 0.0f;
-                for (int s = 0; s < g.KS; ++s) {
-                    y += p[s * 16 * TOK];
-                    v += p[s * 16 * TOK + 8 * TOK];
+        if (alone) {
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                if (j > 0 && count <= 8 * j) break;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int col = j * 8 + t4 * 2 + c;
+                    const bool on = col < count;
+                    const int pair = on ? places[first + col] : 0;
+                    float y = sum[j][c], v = sum[j][2 + c];
+                    if (FP8) {
+                        const float back = f16_unscale(x_largest[pair / g.top]);
+                        y *= back;
+                        v *= back;
+                    }
+                    const float h = fp8_glu(y, v, g.act, g.limit, g.on_input ? wts[pair] : 1.0f);
+                    if (on) g.hidden[(size_t)pair * g.F + f0 + gr] = h;
+                    if (FP8) {
+                        uint32_t big = fp8_size_bits(h);
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+                        if (on && gr == 0) g.largest[(size_t)pair * uf + f0 / 8] = big;
+                    }
+                }
+            }
+        } else {
+            float* mine = part + (((step & 1) * FEW_WARPS + warp) * 16 + gr) * TOK + t4 * 2;
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                *reinterpret_cast<float2*>(mine + j * 8) = make_float2(sum[j][0], sum[j][1]);
+                *reinterpret_cast<float2*>(mine + 8 * TOK + j * 8) = make_float2(sum[j][2], sum[j][3]);
+            }
+            __syncthreads();
+            // eight columns of a pair by eight neighbouring threads; other warps every time
+            const float* all = part + (step & 1) * FEW_WARPS * 16 * TOK;
+            for (int i = (threadIdx.x + step * 128) & (FEW_THREADS - 1); i < RT * TOK * 8; i += FEW_THREADS) {      // (a multiple of 32)
+                const int f = i & 7, j = (i >> 3) % TOK, tile = (i >> 3) / TOK, unit = (int)blockIdx.x * RT + step * stride + tile;
+                const Cursor at = cursor_at(unit);
+                const bool on = unit < units && j < entries[3 * at.entry + 2];
+                float h = 0.0f;
+                int pair = 0;
+                if (on) {
+                    pair = places[entries[3 * at.entry + 1] + j];
+                    const float* p = all + (tile * g.KS * 16 + f) * TOK + j;
+                    float y = 0.0f, v = 0.0f;
+                    for (int s = 0; s < g.KS; ++s) {
+                        y += p[s * 16 * TOK];
+                        v += p[s * 16 * TOK + 8 * TOK];
+                    }
+                    if (FP8) {
+                        const float back = f16_unscale(x_largest[pair / g.top]);
+                        y *= back;
+                        v *= back;
+                    }
+                    h = fp8_glu(y, v, g.act, g.limit, g.on_input ? wts[pair] : 1.0f);
+                    g.hidden[(size_t)pair * g.F + at.fu * 8 + f] = h;
                 }
                 if (FP8) {
-                    const float back = f16_unscale(x_largest[pair / g.top]);
-                    y *= back;
-                    v *= back;
-                }
-                h = fp8_glu(y, v, g.act, g.limit, g.on_input ? wts[pair] : 1.0f);
-                g.hidden[(size_t)pair * g.F + fu * 8 + f] = h;
-            }
-            if (FP8) {
-                uint32_t big = fp8_size_bits(h);
+                    uint32_t big = fp8_size_bits(h);
 #pragma unroll
-                for (int o = 4; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-                if (on && f == 0) g.largest[(size_t)pair * uf + fu] = big;
+                    for (int o = 4; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+                    if (on && f == 0) g.largest[(size_t)pair * uf + at.fu] = big;
+                }
             }
         }
+        advance(here);
     }
 }
 
@@ -507,6 +588,18 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
         const int hi = run_lo(split + 1);
 #pragma unroll 1
         for (int b = run_lo(split); b < hi; ++b) {
+            // the hidden rows first: they come while the weights are waited for
+            constexpr int HW = FP8 ? 4 : 2;              // groups of four numbers beside 16 bytes of a weight row
+            float4 hv[G][2][HW];
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < HW; ++i) {
+                        const int k = b * PER + h * (PER / 2) + t4 * (PER / 8) + i * 4;
+                        hv[j][h][i] = j * 8 + gr < count && k < g.F ? *reinterpret_cast<const float4*>(rows[j] + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);      // (F is a multiple of 8)
+                    }
             const float s0 = FP8 ? sw[b] : 1.0f;
             asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
             const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
@@ -520,7 +613,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
                 const uint4 wl = *reinterpret_cast<const uint4*>(at + 1024 * h), wh = *reinterpret_cast<const uint4*>(at + 512 + 1024 * h);
                 const uint32_t lw[4] = {wl.x, wl.y, wl.z, wl.w}, hw[4] = {wh.x, wh.y, wh.z, wh.w};
 #pragma unroll
-                for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
+                for (int i = 0; i < HW; ++i) {
                     uint32_t a0, a1, a2, a3;
                     if (FP8) {
                         f16_of(lw[i], a0, a2);
@@ -531,11 +624,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
                         a1 = hw[2 * i];
                         a3 = hw[2 * i + 1];
                     }
-                    const int k = b * PER + h * (PER / 2) + t4 * (PER / 8) + i * 4;
 #pragma unroll
                     for (int j = 0; j < G; ++j) {
                         if (j > 0 && count <= 8 * j) break;
-                        const float4 v = j * 8 + gr < count && k < g.F ? *reinterpret_cast<const float4*>(rows[j] + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);      // (F is a multiple of 8)
+                        const float4 v = hv[j][h][i];
                         if (FP8) {
                             mma_f16_f32(c[j], a0, a1, a2, a3, pair_f16(v.x * scale[j], v.y * scale[j]), pair_f16(v.z * scale[j], v.w * scale[j]));
                         } else {
@@ -618,12 +710,13 @@ int launch(FewArgs& g, cudaStream_t s) {
         cfg.gridDim = dim3(FP8_SM_COUNT / FEW_CLUSTER * FEW_CLUSTER);
         if (cudaOccupancyMaxActiveClusters(&fit, few_in_kernel<FP8, G>, &cfg) != cudaSuccess || fit < 1) {
             (void)cudaGetLastError();
-            fit = FP8_SM_COUNT / FEW_CLUSTER;
+            fit = FEW_CLUSTERS;
         }
+        if (fit > FEW_CLUSTERS) fit = FEW_CLUSTERS;
         resident.store(fit, std::memory_order_relaxed);
     }
     const int most_experts = g.E < g.n * g.top ? g.E : g.n * g.top;
-    const long long groups = ((long long)most_experts * (g.F / 8) + g.RT - 1) / g.RT, clusters = (groups + FEW_CLUSTER - 1) / FEW_CLUSTER;
+    const long long groups = ((long long)most_experts * (g.F / 8) * g.KS + FEW_WARPS - 1) / FEW_WARPS, clusters = (groups + FEW_CLUSTER - 1) / FEW_CLUSTER;
     cfg.gridDim = dim3((unsigned)(clusters < fit ? clusters : fit) * FEW_CLUSTER);
     cudaLaunchKernelEx(&cfg, few_in_kernel<FP8, G>, g);
     MM_CHECK_LAUNCH();
@@ -636,7 +729,7 @@ int launch(FewArgs& g, cudaStream_t s) {
 
 // x bf16 [n, ldx]; w_router fp32 [E, D]; experts bf16 (s_in, s_out null): w_in [E, 2 F, D] (gate rows then up rows, or with `interleaved` alternating in
 // blocks of 8), w_out [E, D, F]; or e4m3 with scales: w_in [E, 2, F, ld_in], w_out [E, D, ld_out].  ld_in, ld_out: bytes of a row.
-// out bf16 [n, D].  scratch: pairs * (4 F + F / 2 + 24) + 16 bytes, pairs = n * top.
+// out bf16 [n, D].  scratch: pairs * (4 F + F / 2 + 24) + 32 bytes, pairs = n * top, and with e4m3 experts 36 n D more.
 MM_EXPORT int mm_moe_few(const void* x, long long ldx, int n, int D, const void* w_router, int E, int top, int groups, int keep, int scoring, const void* correction,
                          int pair_sum, int renorm, float wscale, const void* w_in, const void* s_in, long long ld_in, const void* w_out, const void* s_out, long long ld_out,
                          int F, int act, float limit, int on_input, int interleaved, void* out, void* scratch, void* stream) {
@@ -669,6 +762,7 @@ MM_EXPORT int mm_moe_few(const void* x, long long ldx, int n, int D, const void*
     g.largest = (uint32_t*)(g.hidden + pairs * F);
     g.weights = (float*)(g.largest + pairs * (F / 8));
     g.lists = (int32_t*)(g.weights + pairs);
+    g.x_half = (uint16_t*)(((uintptr_t)(g.lists + 1 + 4 * pairs) + 15) & ~(uintptr_t)15);
     g.out = (__nv_bfloat16*)out;
     g.n = n;
     g.D = D;
@@ -688,9 +782,7 @@ MM_EXPORT int mm_moe_few(const void* x, long long ldx, int n, int D, const void*
     const int in_blocks = (int)(((fp8 ? 1LL : 2LL) * D + 127) / 128), out_blocks = (int)(((fp8 ? 1LL : 2LL) * F + 127) / 128);
     g.KS = 8;
     while (g.KS > in_blocks) g.KS /= 2;
-    g.RT = FEW_WARPS / g.KS;
-    g.splits = FEW_SPLIT_BYTES / (FEW_TOKENS * top * 64);
-    if (g.splits < 1) g.splits = 1;
+    g.splits = (FEW_WARPS + top - 1) / top;          // a run for every warp when there is one token
     if (g.splits > out_blocks) g.splits = out_blocks;
     cudaStream_t s = (cudaStream_t)stream;
     if (fp8) return n <= 8 ? launch<true, 1>(g, s) : launch<true, 2>(g, s);
