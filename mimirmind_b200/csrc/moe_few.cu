@@ -90,13 +90,83 @@ __device__ __forceinline__ float f16_unscale(uint32_t size_bits) {
     return __uint_as_float((uint32_t)(e - 14) << 23);
 }
 
+// moe_route_warp's choice where every run of experts is kept, with the scores' order in registers: a choice is two reductions over the warp (128
+// experts, 8 choices: 7,600 cycles there, 1,500 here).  s: E floats of the warp's own.
+__device__ __forceinline__ void few_choose(const float* __restrict__ z, float* s, int lane, int E, int top, int scoring, const float* __restrict__ correction, int renorm,
+                                           float wscale, int32_t* idx, float* wts) {
+    constexpr int HELD = FEW_MAX_EXPERTS / 32;
+    uint32_t key[HELD];          // orders as the scores do; 0: not to be chosen (a NaN, minus infinity, chosen already)
+    float m = -INFINITY, sum = 0.0f;
+    if (scoring == 0) {
+        for (int e = lane; e < E; e += 32) m = fmaxf(m, z[e]);
+        m = warp_max(m);
+        for (int e = lane; e < E; e += 32) {
+            const float p = expf(z[e] - m);
+            s[e] = p;
+            sum += p;
+        }
+        sum = warp_sum(sum);
+    }
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        key[i] = 0;
+        if (i * 32 >= E) continue;
+        const int e = i * 32 + lane;
+        if (e >= E) continue;
+        const float v = scoring == 1 ? 1.0f / (1.0f + expf(-z[e])) : s[e] * inv;
+        s[e] = v;
+        const float c = correction ? v + correction[e] : v;
+        const uint32_t u = __float_as_uint(c);
+        key[i] = c != c || c == -INFINITY ? 0u : (u >> 31) ? ~u : u | 0x80000000u;
+    }
+    __syncwarp();
+    float total = 0.0f, mine_w = 0.0f;
+    int mine_e = 0;
+    for (int k = 0; k < top; ++k) {
+        uint32_t best = 0;
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (i * 32 < E && key[i] > best) {
+                best = key[i];
+                at = i * 32 + lane;
+            }
+        const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+        int e = (int)__reduce_min_sync(0xffffffffu, best == most && most != 0 ? (uint32_t)at : 0x7fffffffu);      // the lowest number among equals
+        float weight = 0.0f;
+        if (e == 0x7fffffff) {
+            e = 0;               // fewer to choose from than `top`: the rest of the choice carries no weight
+        } else {
+            weight = s[e];
+#pragma unroll
+            for (int i = 0; i < HELD; ++i)
+                if (i * 32 + lane == e) key[i] = 0;
+        }
+        total += weight;
+        if (lane == k) {
+            mine_e = e;
+            mine_w = weight;
+        }
+    }
+    if (lane < top) {
+        idx[lane] = mine_e;
+        wts[lane] = renorm || wscale != 1.0f ? mine_w / (renorm ? total + 1e-20f : 1.0f) * wscale : mine_w;
+    }
+}
+
 // A slot of a warp's ring: 128 bytes of 16 weight rows (a lane's four pieces: bytes t * 16 .. + 15 and 64 on of rows g and g + 8), 128 e4m3 or 64
 // bf16 numbers a row.  The order of k inside it is free as long as both operands agree: a lane's pieces are multiplied as they lie.
+
+// numbers of a row of x in shared memory: rows of neighbouring columns lie in different banks (a lane takes 32 bytes beside e4m3 weights, 16 beside bf16)
+__host__ __device__ inline int few_x_stride(int D, bool fp8) { return (D + 63) / 64 * 64 + (fp8 ? 8 : 32); }
+// 4-byte words in front of the rows that make them start on 16 bytes
+__host__ __device__ inline int few_pad(int n, int E, int pairs) { return (-(((n * E + 3) & ~3) + 6 * pairs + 2 * FEW_WARPS + 2 + FEW_TOKENS)) & 3; }
 
 // ---------------------------------------------------------------------------------------------------------------
 // first launch: router, choice, gate and up products, activation
 // ---------------------------------------------------------------------------------------------------------------
-template <bool FP8, int G>
+template <bool FP8, int G, bool XS>
 __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_constant__ FewArgs g) {
     constexpr int TOK = 8 * G;
     extern __shared__ __align__(16) unsigned char few_smem[];
@@ -104,13 +174,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
     float* part = reinterpret_cast<float*>(few_smem + FEW_WARPS * FEW_RING * FEW_SLOT);         // [2][16 warps][16][TOK]
     float* logits = part + 2 * FEW_WARPS * 16 * TOK;                                            // [n][E]
     const int pairs = g.n * g.top;
-    float* wts = logits + g.n * g.E;                                                            // [pairs]
-    int32_t* idx = reinterpret_cast<int32_t*>(wts + pairs);                                     // [pairs]
-    int32_t* places = idx + pairs;                                                              // [pairs]: the pair at every place, by expert
+    int32_t* idx = reinterpret_cast<int32_t*>(logits + ((g.n * g.E + 3) & ~3));                // [pairs]
+    float* wts = reinterpret_cast<float*>(idx + pairs);                                         // [pairs]
+    int32_t* places = reinterpret_cast<int32_t*>(wts + pairs);                                  // [pairs]: the pair at every place, by expert
     int32_t* entries = places + pairs;                                                          // [pairs][3]
     int32_t* sums = entries + 3 * pairs;                                                        // [2][16 warps], [2] totals
     uint32_t* x_largest = reinterpret_cast<uint32_t*>(sums + 2 * FEW_WARPS + 2);                // [16]
-    uint16_t* x_half = FP8 ? g.x_half + (size_t)(blockIdx.x / FEW_CLUSTER) * g.n * g.D : nullptr;
+    uint16_t* x_rows = reinterpret_cast<uint16_t*>(x_largest + FEW_TOKENS + few_pad(g.n, g.E, pairs));      // XS: [n][x_stride]
+    const int x_stride = few_x_stride(g.D, FP8);
+    uint16_t* x_half = FP8 && !XS ? g.x_half + (size_t)(blockIdx.x / FEW_CLUSTER) * g.n * g.D : nullptr;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t4 = lane & 3;
     uint32_t rank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -118,30 +190,34 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // waited for in front of the first store to another CTA: by then it runs
 
     if (FP8) {
-        if (threadIdx.x < FEW_TOKENS) x_largest[threadIdx.x] = 0;
-        __syncthreads();
-        for (int t = 0; t < g.n; ++t) {
+        if (warp < g.n) {            // a warp per token
             uint32_t big = 0;
-            for (int d = threadIdx.x * 8; d < g.D; d += FEW_THREADS * 8) {
-                const uint4 v = *reinterpret_cast<const uint4*>(g.x + (size_t)t * g.ldx + d);       // (D is a multiple of 8)
+#pragma unroll 4
+            for (int d = lane * 8; d < g.D; d += 256) {       // (D is a multiple of 8)
+                const uint4 v = *reinterpret_cast<const uint4*>(g.x + (size_t)warp * g.ldx + d);
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) big = max(big, max((w[i] & 0x7fffu) << 16, w[i] & 0x7fff0000u));
             }
             big = __reduce_max_sync(0xffffffffu, big);
-            if (lane == 0) atomicMax(x_largest + t, big);
+            if (lane == 0) x_largest[warp] = big;
         }
         __syncthreads();
-        // the cluster's own copy of x in fp16, an eighth by every CTA (read behind the cluster's barrier)
-        for (int i = rank * FEW_THREADS + threadIdx.x; i < g.n * (g.D / 8); i += FEW_CLUSTER * FEW_THREADS) {
-            const int t = i / (g.D / 8), d = (i - t * (g.D / 8)) * 8;
-            const uint4 v = *reinterpret_cast<const uint4*>(g.x + (size_t)t * g.ldx + d);
-            const float s = f16_scale(x_largest[t]);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            uint32_t o[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[k] = pair_f16(low_of(w[k]) * s, high_of(w[k]) * s);
-            *reinterpret_cast<uint4*>(x_half + (size_t)t * g.D + d) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    // x as the products read it: into shared memory, or (rows too long for that; e4m3 experts) the cluster's own copy in memory, an eighth by every CTA
+    // (read behind the cluster's barrier)
+    if (XS || FP8) {
+        const int chunks = g.D / 8, first = XS ? threadIdx.x : rank * FEW_THREADS + threadIdx.x, step = XS ? FEW_THREADS : FEW_CLUSTER * FEW_THREADS;
+#pragma unroll 4
+        for (int i = first; i < g.n * chunks; i += step) {
+            const int t = i / chunks, d = (i - t * chunks) * 8;
+            uint4 v = *reinterpret_cast<const uint4*>(g.x + (size_t)t * g.ldx + d);
+            if (FP8) {
+                const float s = f16_scale(x_largest[t]);
+                v = make_uint4(pair_f16(low_of(v.x) * s, high_of(v.x) * s), pair_f16(low_of(v.y) * s, high_of(v.y) * s), pair_f16(low_of(v.z) * s, high_of(v.z) * s),
+                               pair_f16(low_of(v.w) * s, high_of(v.w) * s));
+            }
+            *reinterpret_cast<uint4*>(XS ? x_rows + (size_t)t * x_stride + d : x_half + (size_t)t * g.D + d) = v;
         }
     }
     // ---- logits: 16 experts a tile, a sixteenth of the depth a warp ----
@@ -155,7 +231,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
             for (int j = 0; j < G; ++j)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
             for (int s = lo; s < hi; ++s) {
                 const int k = s * 16 + t4 * 4;
                 const bool on = k < g.D;
@@ -207,7 +283,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
     // ---- the choice: a warp per token ----
-    if (warp < g.n)
+    if (warp < g.n && g.keep == g.groups)
+        few_choose(logits + warp * g.E, reinterpret_cast<float*>(rings) + (size_t)warp * g.E, lane, g.E, g.top, g.scoring, g.correction, g.renorm, g.wscale,
+                   idx + warp * g.top, wts + warp * g.top);
+    else if (warp < g.n)
         moe_route_warp(logits + warp * g.E, reinterpret_cast<float*>(rings) + (size_t)warp * 2 * (g.E + g.groups), lane, g.E, g.top, g.groups, g.keep, idx, wts,
                        (size_t)warp, g.scoring, g.correction, g.pair_sum, g.renorm, g.wscale);
     __syncthreads();
@@ -215,8 +294,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
     {
         const int e = threadIdx.x;
         int count = 0;
-        if (e < g.E)
-            for (int p = 0; p < pairs; ++p) count += idx[p] == e;
+        if (e < g.E) {
+            int p = 0;
+            for (; p + 4 <= pairs; p += 4) {
+                const int4 v = *reinterpret_cast<const int4*>(idx + p);
+                count += (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
+            }
+            for (; p < pairs; ++p) count += idx[p] == e;
+        }
         const int parts = (count + TOK - 1) / TOK;
         int upto = count, parts_upto = parts;
 #pragma unroll
@@ -344,13 +429,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
 #pragma unroll
         for (int j = 0; j < G; ++j) {
             const int t = places[first + min(j * 8 + gr, count - 1)] / g.top;
-            rows[j] = (FP8 ? x_half + (size_t)t * g.D : reinterpret_cast<const uint16_t*>(g.x) + (size_t)t * g.ldx) + t4 * (PER / 8);
+            rows[j] = (XS ? x_rows + t * x_stride : FP8 ? x_half + (size_t)t * g.D : reinterpret_cast<const uint16_t*>(g.x) + (size_t)t * g.ldx) + t4 * (PER / 8);
         }
         const float *sg = nullptr, *su = nullptr;
         if (FP8) {
             sg = g.s_in + ((size_t)2 * entries[3 * here.entry] * fb + f0 / 128) * kb;
             su = sg + (size_t)fb * kb;
         }
+        float s0_next = FP8 ? sg[lo] : 1.0f, s1_next = FP8 ? su[lo] : 1.0f;
         float sum[G][4];
 #pragma unroll
         for (int j = 0; j < G; ++j)
@@ -378,7 +464,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
                             const int k = b * PER + h * (PER / 2) + i * 8;
                             xv[j][h][i] = j * 8 + gr < count && (whole || k + t4 * (PER / 8) < g.D) ? *reinterpret_cast<const uint4*>(rows[j] + k) : make_uint4(0, 0, 0, 0);      // (D is a multiple of 8)
                         }
-                const float s0 = FP8 ? sg[b] : 1.0f, s1 = FP8 ? su[b] : 1.0f;
+                const float s0 = s0_next, s1 = s1_next;
+                if (FP8 && b + 1 < hi) {
+                    s0_next = sg[b + 1];
+                    s1_next = su[b + 1];
+                }
                 asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
                 const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
                 float c[G][4];
@@ -560,11 +650,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
     }
     if (FP8) {
         const int uf = g.F / 8;
-        for (int p = warp; p < pairs; p += FEW_WARPS) {
+        for (int p0 = warp * 8; p0 < pairs; p0 += FEW_WARPS * 8) {       // four lanes a pair
+            const int p = min(p0 + gr, pairs - 1);
             uint32_t big = 0;
-            for (int i = lane; i < uf; i += 32) big = max(big, g.largest[(size_t)p * uf + i]);
-            big = __reduce_max_sync(0xffffffffu, big);
-            if (lane == 0) largest[p] = big;
+#pragma unroll 8
+            for (int i = t4; i < uf; i += 4) big = max(big, g.largest[(size_t)p * uf + i]);
+            big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            if (t4 == 0) largest[p] = big;
         }
         __syncthreads();
     }
@@ -576,7 +669,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
 #pragma unroll
         for (int j = 0; j < G; ++j) {
             const int pair = places[first + min(j * 8 + gr, count - 1)];
-            rows[j] = g.hidden + (size_t)pair * g.F;
+            rows[j] = g.hidden + (size_t)pair * g.F + t4 * (PER / 8);
             scale[j] = FP8 ? f16_scale(largest[pair]) : 1.0f;
         }
         const float* sw = FP8 ? g.s_out + ((size_t)e * db + min(n0, g.D - 1) / 128) * fb : nullptr;
@@ -585,22 +678,43 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
         for (int j = 0; j < G; ++j)
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
-        const int hi = run_lo(split + 1);
-#pragma unroll 1
-        for (int b = run_lo(split); b < hi; ++b) {
-            // the hidden rows first: they come while the weights are waited for
-            constexpr int HW = FP8 ? 4 : 2;              // groups of four numbers beside 16 bytes of a weight row
-            float4 hv[G][2][HW];
+        // the first eight columns' hidden numbers of a block (more columns are rare and read when they are multiplied), a block ahead
+        constexpr int HW = FP8 ? 4 : 2;                  // groups of four numbers beside 16 bytes of a weight row
+        float4 next[2][HW];
+        auto fetch = [&](int j, int b, int h, int i) {
+            const int k = b * PER + h * (PER / 2) + i * 4;
+            return j * 8 + gr < count && k + t4 * (PER / 8) < g.F ? *reinterpret_cast<const float4*>(rows[j] + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);      // (F is a multiple of 8)
+        };
+        const int lo = run_lo(split), hi = run_lo(split + 1);
 #pragma unroll
-            for (int j = 0; j < G; ++j)
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < HW; ++i) next[h][i] = fetch(0, lo, h, i);
+        float s_next = FP8 ? sw[lo] : 1.0f;
+#pragma unroll 1
+        for (int b = lo; b < hi; ++b) {
+            // the operand's pairs: fp16, or two bf16 parts
+            uint2 high[2][HW], low[2][FP8 ? 1 : HW];
+            auto split_up = [&](float4 v, float sc, uint2& p, uint2& r) {
+                if (FP8) {
+                    p = make_uint2(pair_f16(v.x * sc, v.y * sc), pair_f16(v.z * sc, v.w * sc));
+                } else {
+                    p = make_uint2(pair_bf16(v.x, v.y), pair_bf16(v.z, v.w));
+                    r = make_uint2(pair_bf16(v.x - low_of(p.x), v.y - high_of(p.x)), pair_bf16(v.z - low_of(p.y), v.w - high_of(p.y)));
+                }
+            };
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < HW; ++i) split_up(next[h][i], scale[0], high[h][i], low[h][FP8 ? 0 : i]);
+            const float s0 = s_next;
+            if (b + 1 < hi) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < HW; ++i) {
-                        const int k = b * PER + h * (PER / 2) + t4 * (PER / 8) + i * 4;
-                        hv[j][h][i] = j * 8 + gr < count && k < g.F ? *reinterpret_cast<const float4*>(rows[j] + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);      // (F is a multiple of 8)
-                    }
-            const float s0 = FP8 ? sw[b] : 1.0f;
+                    for (int i = 0; i < HW; ++i) next[h][i] = fetch(0, b + 1, h, i);
+                if (FP8) s_next = sw[b + 1];
+            }
             asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
             const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
             float c[G][4];
@@ -627,13 +741,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
 #pragma unroll
                     for (int j = 0; j < G; ++j) {
                         if (j > 0 && count <= 8 * j) break;
-                        const float4 v = hv[j][h][i];
+                        uint2 p = high[h][i], r = low[h][FP8 ? 0 : i];
+                        if (j > 0) split_up(fetch(j, b, h, i), scale[j], p, r);
                         if (FP8) {
-                            mma_f16_f32(c[j], a0, a1, a2, a3, pair_f16(v.x * scale[j], v.y * scale[j]), pair_f16(v.z * scale[j], v.w * scale[j]));
+                            mma_f16_f32(c[j], a0, a1, a2, a3, p.x, p.y);
                         } else {
-                            const uint32_t p0 = pair_bf16(v.x, v.y), p1 = pair_bf16(v.z, v.w);
-                            mma_bf16_f32(acc[j], a0, a1, a2, a3, p0, p1);
-                            mma_bf16_f32(acc[j], a0, a1, a2, a3, pair_bf16(v.x - low_of(p0), v.y - high_of(p0)), pair_bf16(v.z - low_of(p1), v.w - high_of(p1)));
+                            mma_bf16_f32(acc[j], a0, a1, a2, a3, p.x, p.y);
+                            mma_bf16_f32(acc[j], a0, a1, a2, a3, r.x, r.y);
                         }
                     }
                 }
@@ -677,19 +791,22 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
 
 size_t in_smem(const FewArgs& g) {
     const int tok = g.n <= 8 ? 8 : 16, pairs = g.n * g.top;
-    return (size_t)FEW_WARPS * FEW_RING * FEW_SLOT + 4 * ((size_t)2 * FEW_WARPS * 16 * tok + g.n * g.E + 6 * pairs + 2 * FEW_WARPS + 2 + FEW_TOKENS);
+    return (size_t)FEW_WARPS * FEW_RING * FEW_SLOT + 4 * ((size_t)2 * FEW_WARPS * 16 * tok + ((g.n * g.E + 3) & ~3) + 6 * pairs + 2 * FEW_WARPS + 2 + FEW_TOKENS);
 }
+size_t in_x_bytes(const FewArgs& g, bool fp8) { return 4 * (size_t)few_pad(g.n, g.E, g.n * g.top) + 2 * (size_t)g.n * few_x_stride(g.D, fp8); }
 size_t out_smem(const FewArgs& g) {
     const int pairs = g.n * g.top;
     return (size_t)FEW_WARPS * FEW_RING * FEW_SLOT + 4 * ((size_t)g.splits * pairs * 16 + 6 * pairs);
 }
 
-template <bool FP8, int G>
+constexpr size_t FEW_SMEM = 227 * 1024;
+
+template <bool FP8, int G, bool XS>
 int launch(FewArgs& g, cudaStream_t s) {
-    constexpr size_t most = 227 * 1024;
-    const size_t smem_in = in_smem(g), smem_out = out_smem(g);
+    constexpr size_t most = FEW_SMEM;
+    const size_t smem_in = in_smem(g) + (XS ? in_x_bytes(g, FP8) : 0), smem_out = out_smem(g);
     MM_REQUIRE(smem_in <= most && smem_out <= most, "moe few: too many experts or choices for the kernels' shared memory");
-    if (!mm_allow_smem<few_in_kernel<FP8, G>>(most) || !mm_allow_smem<few_out_kernel<FP8, G>>(most)) {
+    if (!mm_allow_smem<few_in_kernel<FP8, G, XS>>(most) || !mm_allow_smem<few_out_kernel<FP8, G>>(most)) {
         mm_set_last_error("moe few: cannot reserve shared memory");
         return MM_ERR_LAUNCH;
     }
@@ -708,7 +825,7 @@ int launch(FewArgs& g, cudaStream_t s) {
     int fit = resident.load(std::memory_order_relaxed);
     if (fit == 0) {
         cfg.gridDim = dim3(FP8_SM_COUNT / FEW_CLUSTER * FEW_CLUSTER);
-        if (cudaOccupancyMaxActiveClusters(&fit, few_in_kernel<FP8, G>, &cfg) != cudaSuccess || fit < 1) {
+        if (cudaOccupancyMaxActiveClusters(&fit, few_in_kernel<FP8, G, XS>, &cfg) != cudaSuccess || fit < 1) {
             (void)cudaGetLastError();
             fit = FEW_CLUSTERS;
         }
@@ -718,7 +835,7 @@ int launch(FewArgs& g, cudaStream_t s) {
     const int most_experts = g.E < g.n * g.top ? g.E : g.n * g.top;
     const long long groups = ((long long)most_experts * (g.F / 8) * g.KS + FEW_WARPS - 1) / FEW_WARPS, clusters = (groups + FEW_CLUSTER - 1) / FEW_CLUSTER;
     cfg.gridDim = dim3((unsigned)(clusters < fit ? clusters : fit) * FEW_CLUSTER);
-    cudaLaunchKernelEx(&cfg, few_in_kernel<FP8, G>, g);
+    cudaLaunchKernelEx(&cfg, few_in_kernel<FP8, G, XS>, g);
     MM_CHECK_LAUNCH();
     mm_launch_dependent(g_mm_pdl != 0, few_out_kernel<FP8, G>, dim3(ceil_div(g.D, 16)), dim3(FEW_THREADS), smem_out, s, g);
     MM_CHECK_LAUNCH();
@@ -785,6 +902,11 @@ MM_EXPORT int mm_moe_few(const void* x, long long ldx, int n, int D, const void*
     g.splits = (FEW_WARPS + top - 1) / top;          // a run for every warp when there is one token
     if (g.splits > out_blocks) g.splits = out_blocks;
     cudaStream_t s = (cudaStream_t)stream;
-    if (fp8) return n <= 8 ? launch<true, 1>(g, s) : launch<true, 2>(g, s);
-    return n <= 8 ? launch<false, 1>(g, s) : launch<false, 2>(g, s);
+    const bool xs = in_smem(g) + in_x_bytes(g, fp8) <= FEW_SMEM;
+    if (fp8) {
+        if (xs) return n <= 8 ? launch<true, 1, true>(g, s) : launch<true, 2, true>(g, s);
+        return n <= 8 ? launch<true, 1, false>(g, s) : launch<true, 2, false>(g, s);
+    }
+    if (xs) return n <= 8 ? launch<false, 1, true>(g, s) : launch<false, 2, true>(g, s);
+    return n <= 8 ? launch<false, 1, false>(g, s) : launch<false, 2, false>(g, s);
 }
