@@ -90,48 +90,50 @@ __device__ __forceinline__ float f16_unscale(uint32_t size_bits) {
     return __uint_as_float((uint32_t)(e - 14) << 23);
 }
 
-// moe_route_warp's choice where every run of experts is kept, with the scores' order in registers: a choice is two reductions over the warp (128
-// experts, 8 choices: 7,600 cycles there, 1,500 here).  s: E floats of the warp's own.
+// moe_route_warp's choice where every run of experts is kept: a choice is two reductions over the warp.  Code that runs once in a launch is
+// fetched from L2 as it goes: kept short, it takes 2,000 cycles for 8 of 128 experts instead of 7,600.
+// s: 2 E words of the warp's own: the scores, and their order (0: not to be chosen, a NaN, minus infinity or chosen already).
 __device__ __forceinline__ void few_choose(const float* __restrict__ z, float* s, int lane, int E, int top, int scoring, const float* __restrict__ correction, int renorm,
                                            float wscale, int32_t* idx, float* wts) {
-    constexpr int HELD = FEW_MAX_EXPERTS / 32;
-    uint32_t key[HELD];          // orders as the scores do; 0: not to be chosen (a NaN, minus infinity, chosen already)
-    float m = -INFINITY, sum = 0.0f;
+    uint32_t* key = reinterpret_cast<uint32_t*>(s + E);
+    float m = 0.0f, inv = 1.0f;
     if (scoring == 0) {
+        m = -INFINITY;
+#pragma unroll 1
         for (int e = lane; e < E; e += 32) m = fmaxf(m, z[e]);
         m = warp_max(m);
+        float sum = 0.0f;
+#pragma unroll 1
         for (int e = lane; e < E; e += 32) {
             const float p = expf(z[e] - m);
             s[e] = p;
             sum += p;
         }
-        sum = warp_sum(sum);
+        inv = 1.0f / warp_sum(sum);
     }
-    const float inv = 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        key[i] = 0;
-        if (i * 32 >= E) continue;
-        const int e = i * 32 + lane;
-        if (e >= E) continue;
+#pragma unroll 1
+    for (int e = lane; e < E; e += 32) {
         const float v = scoring == 1 ? 1.0f / (1.0f + expf(-z[e])) : s[e] * inv;
         s[e] = v;
         const float c = correction ? v + correction[e] : v;
         const uint32_t u = __float_as_uint(c);
-        key[i] = c != c || c == -INFINITY ? 0u : (u >> 31) ? ~u : u | 0x80000000u;
+        key[e] = c != c || c == -INFINITY ? 0u : (u >> 31) ? ~u : u | 0x80000000u;
     }
     __syncwarp();
     float total = 0.0f, mine_w = 0.0f;
     int mine_e = 0;
+#pragma unroll 1
     for (int k = 0; k < top; ++k) {
         uint32_t best = 0;
         int at = 0x7fffffff;
-#pragma unroll
-        for (int i = 0; i < HELD; ++i)
-            if (i * 32 < E && key[i] > best) {
-                best = key[i];
-                at = i * 32 + lane;
+#pragma unroll 1
+        for (int e = lane; e < E; e += 32) {
+            const uint32_t v = key[e];
+            if (v > best) {
+                best = v;
+                at = e;
             }
+        }
         const uint32_t most = __reduce_max_sync(0xffffffffu, best);
         int e = (int)__reduce_min_sync(0xffffffffu, best == most && most != 0 ? (uint32_t)at : 0x7fffffffu);      // the lowest number among equals
         float weight = 0.0f;
@@ -139,10 +141,9 @@ __device__ __forceinline__ void few_choose(const float* __restrict__ z, float* s
             e = 0;               // fewer to choose from than `top`: the rest of the choice carries no weight
         } else {
             weight = s[e];
-#pragma unroll
-            for (int i = 0; i < HELD; ++i)
-                if (i * 32 + lane == e) key[i] = 0;
+            if ((e & 31) == lane) key[e] = 0;
         }
+        __syncwarp();
         total += weight;
         if (lane == k) {
             mine_e = e;
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
             for (int j = 0; j < G; ++j)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
-#pragma unroll 8
+#pragma unroll (G == 1 ? 4 : 2)
             for (int s = lo; s < hi; ++s) {
                 const int k = s * 16 + t4 * 4;
                 const bool on = k < g.D;
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
 
     // ---- the choice: a warp per token ----
     if (warp < g.n && g.keep == g.groups)
-        few_choose(logits + warp * g.E, reinterpret_cast<float*>(rings) + (size_t)warp * g.E, lane, g.E, g.top, g.scoring, g.correction, g.renorm, g.wscale,
+        few_choose(logits + warp * g.E, reinterpret_cast<float*>(rings) + (size_t)warp * 2 * g.E, lane, g.E, g.top, g.scoring, g.correction, g.renorm, g.wscale,
                    idx + warp * g.top, wts + warp * g.top);
     else if (warp < g.n)
         moe_route_warp(logits + warp * g.E, reinterpret_cast<float*>(rings) + (size_t)warp * 2 * (g.E + g.groups), lane, g.E, g.top, g.groups, g.keep, idx, wts,
@@ -356,7 +357,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
     const int RT = alone ? FEW_WARPS : side, rt = alone ? warp : warp / g.KS, run_lo = alone ? 0 : warp % g.KS, run_hi = alone ? g.KS : run_lo + 1;
     const int lo = blocks * run_lo / g.KS, hi = blocks * run_hi / g.KS, nb = hi - lo;
     const int groups = (units + RT - 1) / RT, steps = (int)blockIdx.x < groups ? (groups - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
-    const int stride = (int)gridDim.x * RT, unit0 = (int)blockIdx.x * RT + rt;
+    // (warps that are alone take every grid's-width unit, so that few units are spread over all CTAs)
+    const int stride = (int)gridDim.x * RT, unit0 = alone ? (int)blockIdx.x + rt * (int)gridDim.x : (int)blockIdx.x * RT + rt;
     const int my_steps = alone ? (unit0 < units ? (units - 1 - unit0) / stride + 1 : 0) : steps;
     unsigned char* ring = rings + warp * FEW_RING * FEW_SLOT;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
@@ -471,11 +473,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
                 }
                 asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
                 const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
-                float c[G][4];
+                float c[G][2][4];            // two chains of products: one's results are 23 cycles away
 #pragma unroll
                 for (int j = 0; j < G; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) c[j][i] = 0.0f;
+                    for (int i = 0; i < 8; ++i) c[j][i >> 2][i & 3] = 0.0f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint4 wl = *reinterpret_cast<const uint4*>(at + 1024 * h), wh = *reinterpret_cast<const uint4*>(at + 512 + 1024 * h);
@@ -497,20 +499,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
                             if (j > 0 && count <= 8 * j) break;
                             const uint4 v = xv[j][h][FP8 ? i >> 1 : 0];
                             const uint32_t p0 = (i & 1) ? v.z : v.x, p1 = (i & 1) ? v.w : v.y;
-                            if (FP8) mma_f16_f32(c[j], a0, a1, a2, a3, p0, p1);
-                            else mma_bf16_f32(acc[j], a0, a1, a2, a3, p0, p1);
+                            if (FP8) mma_f16_f32(c[j][h], a0, a1, a2, a3, p0, p1);
+                            else mma_bf16_f32(h ? c[j][1] : acc[j], a0, a1, a2, a3, p0, p1);
                         }
                     }
                 }
-                if (FP8) {
 #pragma unroll
-                    for (int j = 0; j < G; ++j) {
-                        acc[j][0] = fmaf(s0, c[j][0], acc[j][0]);
-                        acc[j][1] = fmaf(s0, c[j][1], acc[j][1]);
-                        acc[j][2] = fmaf(s1, c[j][2], acc[j][2]);
-                        acc[j][3] = fmaf(s1, c[j][3], acc[j][3]);
-                    }
-                }
+                for (int j = 0; j < G; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[j][i] = FP8 ? fmaf(i < 2 ? s0 : s1, c[j][0][i] + c[j][1][i], acc[j][i]) : acc[j][i] + c[j][1][i];
                 if (done + FEW_RING < total) load(slot);
                 few_commit();
                 ++done;
@@ -605,7 +602,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t4 = lane & 3;
     pdl_wait();
     const int n_entries = g.lists[0];
-    for (int i = threadIdx.x; i < 3 * n_entries; i += FEW_THREADS) entries[i] = g.lists[1 + i];
+    for (int i = threadIdx.x; i < 3 * pairs; i += FEW_THREADS) entries[i] = g.lists[1 + i];       // (behind the entries: not read)
     for (int i = threadIdx.x; i < pairs; i += FEW_THREADS) {
         places[i] = g.lists[1 + 3 * pairs + i];
         wts[i] = g.weights[i];
@@ -717,11 +714,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
             }
             asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
             const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
-            float c[G][4];
+            float c[G][2][4];
 #pragma unroll
             for (int j = 0; j < G; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) c[j][i] = 0.0f;
+                for (int i = 0; i < 8; ++i) c[j][i >> 2][i & 3] = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint4 wl = *reinterpret_cast<const uint4*>(at + 1024 * h), wh = *reinterpret_cast<const uint4*>(at + 512 + 1024 * h);
@@ -744,20 +741,18 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
                         uint2 p = high[h][i], r = low[h][FP8 ? 0 : i];
                         if (j > 0) split_up(fetch(j, b, h, i), scale[j], p, r);
                         if (FP8) {
-                            mma_f16_f32(c[j], a0, a1, a2, a3, p.x, p.y);
+                            mma_f16_f32(c[j][h], a0, a1, a2, a3, p.x, p.y);
                         } else {
                             mma_bf16_f32(acc[j], a0, a1, a2, a3, p.x, p.y);
-                            mma_bf16_f32(acc[j], a0, a1, a2, a3, r.x, r.y);
+                            mma_bf16_f32(c[j][1], a0, a1, a2, a3, r.x, r.y);
                         }
                     }
                 }
             }
-            if (FP8) {
 #pragma unroll
-                for (int j = 0; j < G; ++j)
+            for (int j = 0; j < G; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(s0, c[j][i], acc[j][i]);
-            }
+                for (int i = 0; i < 4; ++i) acc[j][i] = FP8 ? fmaf(s0, c[j][0][i] + c[j][1][i], acc[j][i]) : acc[j][i] + c[j][1][i];
             load(slot);
             few_commit();
             slot = slot + 1 == FEW_RING ? 0 : slot + 1;
