@@ -13,9 +13,11 @@
 // in the order of the choice.  A token's output does not depend on the others: every sum is cut by the layer's sizes alone.
 //
 // The router's weights are fp32: each is three bf16 parts (hi, mid, lo, 24 bits together), x is bf16, the sums are fp32.
-// Experts in bf16: x as it is, the fp32 hidden rows as two bf16 parts (2^-17 of a number is lost).  Experts in e4m3 with a scale per block of 128 x 128: weights
-// become fp16 exactly; the rows of x and the hidden rows become fp16 after a power of two that brings their largest number to 2^14 .. 2^15
-// (x loses nothing above 2^-29 of its largest, hidden rows keep 11 bits: rounding them to bf16 would cost as much again as rounding the result).
+// Experts in bf16: x as it is, the fp32 hidden rows as two bf16 parts (2^-17 of a number is lost).
+// Experts in e4m3 with a scale per block of 128 x 128: a row of x, after a power of two that brings its largest number to 2^7 .. 2^8, is two e4m3 parts, hi and
+// 16 lo: together bf16's eight bits (a number below 2^-13 of the row's largest loses what is below 2^-21 of it).  Four tokens' parts are the eight
+// columns, so the weights are multiplied as they lie.  The hidden rows become fp16 (11 bits; rounding them to bf16 would cost as much again as rounding
+// the result) after a power of two that brings their largest number to 2^14 .. 2^15, and the weights beside them fp16, exactly.
 //
 // Bound by memory: PLACEHOLDER
 #include <cuda_fp16.h>
@@ -28,6 +30,7 @@ namespace {
 
 constexpr int FEW_THREADS = 512, FEW_WARPS = 16, FEW_RING = 3, FEW_SLOT = 2048, FEW_CLUSTER = 8;
 constexpr int FEW_TOKENS = 16, FEW_MAX_EXPERTS = 512, FEW_MAX_TOP = 32;
+constexpr int FEW_ROWS = 8;              // (token, choice) rows of an entry; an expert with more has several
 constexpr int FEW_CLUSTERS = FP8_SM_COUNT / FEW_CLUSTER;      // at the most
 
 struct FewArgs {
@@ -40,7 +43,7 @@ struct FewArgs {
     uint32_t* largest;                    // [pairs][F / 8]: bits of the units' largest sizes
     int32_t* lists;                       // entries' number, entries (expert, first place, rows) 3 each, places' pairs
     float* weights;                       // [pairs]
-    uint16_t* x_half;                     // e4m3 experts: [clusters][n][D] fp16
+    uint8_t* x_copy;                      // [clusters][n][few_x_bytes]: x as the products read it, where it does not fit into shared memory
     __nv_bfloat16* out;
     long long ldx, ld_in, ld_out;
     int n, D, E, top, groups, keep, scoring, renorm, pair_sum, F, act, on_input, interleaved;
@@ -48,9 +51,9 @@ struct FewArgs {
     int KS, splits;
 };
 
-__device__ __forceinline__ void few_copy16(uint32_t dst, const uint8_t* row, int at, int bytes) {      // 16 bytes of a row, noughts behind its end
-    const int n = min(max(bytes - at, 0), 16);
-    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(n > 0 ? row + at : row), "r"(n) : "memory");
+__device__ __forceinline__ void few_copy16(uint32_t dst, const uint8_t* src, int left) {      // the first `left` of 16 bytes, noughts behind them
+    const int n = min(max(left, 0), 16);
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(n > 0 ? src : src - (16 - left + 15) / 16 * 16), "r"(n) : "memory");
 }
 __device__ __forceinline__ void few_copy16(uint32_t dst, const uint8_t* src) {
     asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -75,20 +78,21 @@ __device__ __forceinline__ uint32_t pair_f16(float lo, float hi) {
 }
 __device__ __forceinline__ float low_of(uint32_t bf16_pair) { return __uint_as_float(bf16_pair << 16); }
 __device__ __forceinline__ float high_of(uint32_t bf16_pair) { return __uint_as_float(bf16_pair & 0xffff0000u); }
+__device__ __forceinline__ void mma_e4m3_f32(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 // four e4m3 numbers as two fp16 pairs
 __device__ __forceinline__ void f16_of(uint32_t w, uint32_t& a, uint32_t& b) {
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(a), "=r"(b) : "r"(w));
 }
 
-// The power of two that brings a size to 2^14 .. 2^15 (sizes below 2^-112: 2^126), and its inverse; an infinity or a NaN stays one under it.
-__device__ __forceinline__ float f16_scale(uint32_t size_bits) {
-    const int e = min(max((int)(size_bits >> 23), 15), 254);
-    return __uint_as_float((uint32_t)(268 - e) << 23);
-}
-__device__ __forceinline__ float f16_unscale(uint32_t size_bits) {
-    const int e = min(max((int)(size_bits >> 23), 15), 254);
-    return __uint_as_float((uint32_t)(e - 14) << 23);
-}
+// The power of two that brings a size to 2^to .. 2^(to + 1) (sizes next to the smallest normal number: as far as it goes), and its inverse; an infinity or
+// a NaN stays one under it.
+__device__ __forceinline__ int few_exponent(uint32_t size_bits) { return min(max((int)(size_bits >> 23), 16), 254); }
+__device__ __forceinline__ float few_scale(uint32_t size_bits, int to) { return __uint_as_float((uint32_t)(254 + to - few_exponent(size_bits)) << 23); }
+__device__ __forceinline__ float few_unscale(uint32_t size_bits, int to) { return __uint_as_float((uint32_t)(few_exponent(size_bits) - to) << 23); }
+constexpr int X_TO = 7, HIDDEN_TO = 14;
 
 // moe_route_warp's choice where every run of experts is kept: a choice is two reductions over the warp.  Code that runs once in a launch is
 // fetched from L2 as it goes: kept short, it takes 2,000 cycles for 8 of 128 experts instead of 7,600.
@@ -122,6 +126,37 @@ __device__ __forceinline__ void few_choose(const float* __restrict__ z, float* s
     __syncwarp();
     float total = 0.0f, mine_w = 0.0f;
     int mine_e = 0;
+    if (E <= 128) {
+        // every lane counts the scores ahead of its own four: no choice waits for another
+        uint32_t own[4];
+        int ahead[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            own[j] = j * 32 + lane < E ? key[j * 32 + lane] : 0u;
+            ahead[j] = 0;
+        }
+#pragma unroll 1
+        for (int e = 0; e < E; ++e) {
+            const uint32_t v = key[e];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ahead[j] += v > own[j] || (v == own[j] && e < j * 32 + lane);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (own[j] != 0u && ahead[j] < top) key[ahead[j]] = (uint32_t)(j * 32 + lane);      // (the order is in registers now)
+        __syncwarp();
+        // how many there were to choose from
+        int found = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) found += __popc(__ballot_sync(0xffffffffu, own[j] != 0u));
+        if (lane < top && lane < found) {
+            mine_e = (int)key[lane];
+            mine_w = s[mine_e];
+        }
+#pragma unroll 1
+        for (int k = 0; k < top; ++k) total += __shfl_sync(0xffffffffu, mine_w, k);
+    } else {
 #pragma unroll 1
     for (int k = 0; k < top; ++k) {
         uint32_t best = 0;
@@ -150,6 +185,7 @@ __device__ __forceinline__ void few_choose(const float* __restrict__ z, float* s
             mine_w = weight;
         }
     }
+    }
     if (lane < top) {
         idx[lane] = mine_e;
         wts[lane] = renorm || wscale != 1.0f ? mine_w / (renorm ? total + 1e-20f : 1.0f) * wscale : mine_w;
@@ -159,31 +195,31 @@ __device__ __forceinline__ void few_choose(const float* __restrict__ z, float* s
 // A slot of a warp's ring: 128 bytes of 16 weight rows (a lane's four pieces: bytes t * 16 .. + 15 and 64 on of rows g and g + 8), 128 e4m3 or 64
 // bf16 numbers a row.  The order of k inside it is free as long as both operands agree: a lane's pieces are multiplied as they lie.
 
-// numbers of a row of x in shared memory: rows of neighbouring columns lie in different banks (a lane takes 32 bytes beside e4m3 weights, 16 beside bf16)
-__host__ __device__ inline int few_x_stride(int D, bool fp8) { return (D + 63) / 64 * 64 + (fp8 ? 8 : 32); }
-// 4-byte words in front of the rows that make them start on 16 bytes
-__host__ __device__ inline int few_pad(int n, int E, int pairs) { return (-(((n * E + 3) & ~3) + 6 * pairs + 2 * FEW_WARPS + 2 + FEW_TOKENS)) & 3; }
+// Bytes of a row of x as the products read it, noughts behind its end, rows of neighbouring columns in different banks.  e4m3: hi numbers, then lo.
+__host__ __device__ inline int few_part_bytes(int D) { return (D + 127) / 128 * 128 + 32; }
+__host__ __device__ inline int few_x_bytes(int D, bool fp8) { return fp8 ? 2 * few_part_bytes(D) : (D + 63) / 64 * 128 + 64; }
+// 4-byte words of the first launch's lists, whole 16 bytes
+__host__ __device__ inline int few_list_words(int n, int E, int pairs) { return (((n * E + 3) & ~3) + 6 * pairs + 2 * FEW_WARPS + 2 + FEW_TOKENS + 3) & ~3; }
 
 // ---------------------------------------------------------------------------------------------------------------
 // first launch: router, choice, gate and up products, activation
 // ---------------------------------------------------------------------------------------------------------------
-template <bool FP8, int G, bool XS>
+template <bool FP8, bool XS>
 __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_constant__ FewArgs g) {
-    constexpr int TOK = 8 * G;
+    constexpr int NG = FP8 ? 2 : 1, COLS = 8 * NG;                                              // columns of a unit: groups of eight
     extern __shared__ __align__(16) unsigned char few_smem[];
-    unsigned char* rings = few_smem;                                                            // later also the choice's scratch
-    float* part = reinterpret_cast<float*>(few_smem + FEW_WARPS * FEW_RING * FEW_SLOT);         // [2][16 warps][16][TOK]
-    float* logits = part + 2 * FEW_WARPS * 16 * TOK;                                            // [n][E]
+    unsigned char* rings = few_smem;                                                            // until they start: the choice's scratch
+    float* part = reinterpret_cast<float*>(few_smem + FEW_WARPS * FEW_RING * FEW_SLOT);         // [2][16 warps][16][COLS]; the router's: [16 warps][16][16]
+    float* logits = part + (FP8 ? 2 : 1) * FEW_WARPS * 16 * 16;                                 // [n][E]
     const int pairs = g.n * g.top;
-    int32_t* idx = reinterpret_cast<int32_t*>(logits + ((g.n * g.E + 3) & ~3));                // [pairs]
+    int32_t* idx = reinterpret_cast<int32_t*>(logits + ((g.n * g.E + 3) & ~3));                 // [pairs]
     float* wts = reinterpret_cast<float*>(idx + pairs);                                         // [pairs]
     int32_t* places = reinterpret_cast<int32_t*>(wts + pairs);                                  // [pairs]: the pair at every place, by expert
     int32_t* entries = places + pairs;                                                          // [pairs][3]
     int32_t* sums = entries + 3 * pairs;                                                        // [2][16 warps], [2] totals
     uint32_t* x_largest = reinterpret_cast<uint32_t*>(sums + 2 * FEW_WARPS + 2);                // [16]
-    uint16_t* x_rows = reinterpret_cast<uint16_t*>(x_largest + FEW_TOKENS + few_pad(g.n, g.E, pairs));      // XS: [n][x_stride]
-    const int x_stride = few_x_stride(g.D, FP8);
-    uint16_t* x_half = FP8 && !XS ? g.x_half + (size_t)(blockIdx.x / FEW_CLUSTER) * g.n * g.D : nullptr;
+    const int x_bytes = few_x_bytes(g.D, FP8);
+    uint8_t* x_rows = XS ? reinterpret_cast<uint8_t*>(logits + few_list_words(g.n, g.E, pairs)) : g.x_copy + (size_t)(blockIdx.x / FEW_CLUSTER) * g.n * x_bytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t4 = lane & 3;
     uint32_t rank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -203,45 +239,25 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
             big = __reduce_max_sync(0xffffffffu, big);
             if (lane == 0) x_largest[warp] = big;
         }
-        __syncthreads();
-    }
-    // x as the products read it: into shared memory, or (rows too long for that; e4m3 experts) the cluster's own copy in memory, an eighth by every CTA
-    // (read behind the cluster's barrier)
-    if (XS || FP8) {
-        const int chunks = g.D / 8, first = XS ? threadIdx.x : rank * FEW_THREADS + threadIdx.x, step = XS ? FEW_THREADS : FEW_CLUSTER * FEW_THREADS;
-#pragma unroll 4
-        for (int i = first; i < g.n * chunks; i += step) {
-            const int t = i / chunks, d = (i - t * chunks) * 8;
-            uint4 v = *reinterpret_cast<const uint4*>(g.x + (size_t)t * g.ldx + d);
-            if (FP8) {
-                const float s = f16_scale(x_largest[t]);
-                v = make_uint4(pair_f16(low_of(v.x) * s, high_of(v.x) * s), pair_f16(low_of(v.y) * s, high_of(v.y) * s), pair_f16(low_of(v.z) * s, high_of(v.z) * s),
-                               pair_f16(low_of(v.w) * s, high_of(v.w) * s));
-            }
-            *reinterpret_cast<uint4*>(XS ? x_rows + (size_t)t * x_stride + d : x_half + (size_t)t * g.D + d) = v;
-        }
     }
     // ---- logits: 16 experts a tile, a sixteenth of the depth a warp ----
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     {
         const int steps = (g.D + 15) / 16, lo = steps * warp / FEW_WARPS, hi = steps * (warp + 1) / FEW_WARPS;
+#pragma unroll 1
         for (int tile = rank; tile * 16 < g.E; tile += FEW_CLUSTER) {
             const float *wa = g.w_router + (size_t)min(tile * 16 + gr, g.E - 1) * g.D, *wb = g.w_router + (size_t)min(tile * 16 + gr + 8, g.E - 1) * g.D;
-            float acc[G][4];
+            const __nv_bfloat16 *xa = g.x + (size_t)min(gr, g.n - 1) * g.ldx, *xb = g.x + (size_t)min(gr + 8, g.n - 1) * g.ldx;      // (columns without a token: not looked at)
+            float acc[2][4];
 #pragma unroll
-            for (int j = 0; j < G; ++j)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
-#pragma unroll (G == 1 ? 4 : 2)
+            for (int c = 0; c < 4; ++c) acc[0][c] = acc[1][c] = 0.0f;
+#pragma unroll 4
             for (int s = lo; s < hi; ++s) {
                 const int k = s * 16 + t4 * 4;
                 const bool on = k < g.D;
                 const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 const float4 a = on ? *reinterpret_cast<const float4*>(wa + k) : zero, b = on ? *reinterpret_cast<const float4*>(wb + k) : zero;
-                uint2 xv[G];
-#pragma unroll
-                for (int j = 0; j < G; ++j)
-                    xv[j] = on && j * 8 + gr < g.n ? *reinterpret_cast<const uint2*>(g.x + (size_t)(j * 8 + gr) * g.ldx + k) : make_uint2(0, 0);
+                const uint2 x0 = on ? *reinterpret_cast<const uint2*>(xa + k) : make_uint2(0, 0), x1 = on && g.n > 8 ? *reinterpret_cast<const uint2*>(xb + k) : make_uint2(0, 0);
                 float r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
                 for (int p = 0; p < 3; ++p) {       // hi, mid, lo
@@ -250,23 +266,23 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
                         r[0] -= low_of(a0); r[1] -= high_of(a0); r[2] -= low_of(a2); r[3] -= high_of(a2);
                         r[4] -= low_of(a1); r[5] -= high_of(a1); r[6] -= low_of(a3); r[7] -= high_of(a3);
                     }
-#pragma unroll
-                    for (int j = 0; j < G; ++j) mma_bf16_f32(acc[j], a0, a1, a2, a3, xv[j].x, xv[j].y);
+                    mma_bf16_f32(acc[0], a0, a1, a2, a3, x0.x, x0.y);
+                    if (g.n > 8) mma_bf16_f32(acc[1], a0, a1, a2, a3, x1.x, x1.y);
                 }
             }
-            float* mine = part + (warp * 16 + gr) * TOK + t4 * 2;
+            float* mine = part + (warp * 16 + gr) * 16 + t4 * 2;
             __syncthreads();        // the tile before has been read
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 *reinterpret_cast<float2*>(mine + j * 8) = make_float2(acc[j][0], acc[j][1]);
-                *reinterpret_cast<float2*>(mine + 8 * TOK + j * 8) = make_float2(acc[j][2], acc[j][3]);
+                *reinterpret_cast<float2*>(mine + 128 + j * 8) = make_float2(acc[j][2], acc[j][3]);
             }
             __syncthreads();
-            for (int i = threadIdx.x; i < 16 * g.n; i += FEW_THREADS) {
-                const int row = i & 15, tok = i >> 4, e = tile * 16 + row;
+            if (threadIdx.x < 16 * g.n) {
+                const int row = threadIdx.x & 15, tok = threadIdx.x >> 4, e = tile * 16 + row;
                 float z = 0.0f;
 #pragma unroll
-                for (int w = 0; w < FEW_WARPS; ++w) z += part[(w * 16 + row) * TOK + tok];
+                for (int w = 0; w < FEW_WARPS; ++w) z += part[(w * 16 + row) * 16 + tok];
                 if (e < g.E) {
                     const uint32_t at = (uint32_t)__cvta_generic_to_shared(logits + tok * g.E + e);
 #pragma unroll
@@ -279,8 +295,40 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
             }
         }
     }
+    // ---- x as the products read it: into shared memory, or (rows too long for that) the cluster's own copy in memory, an eighth by every CTA ----
+    __syncthreads();        // (x_largest)
+    {
+        const int chunks = FP8 ? few_part_bytes(g.D) / 8 - 4 : (g.D + 63) / 64 * 8, step = XS ? FEW_THREADS : FEW_CLUSTER * FEW_THREADS;
+#pragma unroll 2
+        for (int i = XS ? threadIdx.x : rank * FEW_THREADS + threadIdx.x; i < g.n * chunks; i += step) {
+            const int t = i / chunks, d = (i - t * chunks) * 8;
+            const uint4 v = d < g.D ? *reinterpret_cast<const uint4*>(g.x + (size_t)t * g.ldx + d) : make_uint4(0, 0, 0, 0);
+            uint8_t* row = x_rows + (size_t)t * x_bytes;
+            if (FP8) {
+                const float s = few_scale(x_largest[t], X_TO);
+                const bool number = x_largest[t] < 0x7f800000u;      // else the row is NaN: a conversion would make a number of an infinity
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                uint32_t hi[2] = {0x7f7f7f7fu, 0x7f7f7f7fu}, lo[2] = {0x7f7f7f7fu, 0x7f7f7f7fu};
+                if (number) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float f[4] = {low_of(w[2 * j]) * s, high_of(w[2 * j]) * s, low_of(w[2 * j + 1]) * s, high_of(w[2 * j + 1]) * s};
+                        hi[j] = fp8_pack4(f[0], f[1], f[2], f[3]);
+                        uint32_t p, q;
+                        f16_of(hi[j], p, q);
+                        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&p)), b = __half22float2(*reinterpret_cast<const __half2*>(&q));
+                        lo[j] = fp8_pack4((f[0] - a.x) * 16.0f, (f[1] - a.y) * 16.0f, (f[2] - b.x) * 16.0f, (f[3] - b.y) * 16.0f);
+                    }
+                }
+                *reinterpret_cast<uint2*>(row + d) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(row + few_part_bytes(g.D) + d) = make_uint2(lo[0], lo[1]);
+            } else {
+                *reinterpret_cast<uint4*>(row + 2 * d) = v;
+            }
+        }
+    }
     __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (no CTA has more logits to hand out behind this: one barrier does)
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (no CTA has more to hand out behind this: one barrier does)
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
     // ---- the choice: a warp per token ----
@@ -297,13 +345,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
         int count = 0;
         if (e < g.E) {
             int p = 0;
+#pragma unroll 2
             for (; p + 4 <= pairs; p += 4) {
                 const int4 v = *reinterpret_cast<const int4*>(idx + p);
                 count += (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
             }
             for (; p < pairs; ++p) count += idx[p] == e;
         }
-        const int parts = (count + TOK - 1) / TOK;
+        const int parts = (count + FEW_ROWS - 1) / FEW_ROWS;
         int upto = count, parts_upto = parts;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -319,20 +368,25 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
         }
         __syncthreads();
         int first = upto - count, entry = parts_upto - parts;
+#pragma unroll 1
         for (int w = 0; w < warp; ++w) {
             first += sums[w];
             entry += sums[FEW_WARPS + w];
         }
         if (threadIdx.x == FEW_THREADS - 1) sums[2 * FEW_WARPS] = entry + parts;
         if (count > 0) {
-            int at = first;
-            for (int p = 0; p < pairs; ++p)
-                if (idx[p] == e) places[at++] = p;
             for (int i = 0; i < parts; ++i) {
                 entries[3 * (entry + i)] = e;
-                entries[3 * (entry + i) + 1] = first + i * TOK;
-                entries[3 * (entry + i) + 2] = min(TOK, count - i * TOK);
+                entries[3 * (entry + i) + 1] = first + i * FEW_ROWS;
+                entries[3 * (entry + i) + 2] = min(FEW_ROWS, count - i * FEW_ROWS);
             }
+            int left = count;
+#pragma unroll 1
+            for (int p = 0; left > 0; ++p)
+                if (idx[p] == e) {
+                    places[first++] = p;
+                    --left;
+                }
         }
         __syncthreads();
     }
@@ -348,18 +402,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
 
     // ---- units of 8 gate and 8 up rows, a unit's depth in KS runs: a warp per run and the runs' sums added over shared memory, or, where there are many
     // units, a warp per unit that goes through the runs itself.  The sums are the same to the bit.  The cheaper one by rounds of slots (a meeting of the
-    // warps costs about two)  ----
-    constexpr int PER = FP8 ? 128 : 64;                  // numbers in a slot's row
+    // warps costs about three)  ----
     const int bytes = FP8 ? g.D : 2 * g.D, blocks = (bytes + 127) / 128, uf = g.F / 8, units = n_entries * uf;
-    const int side = FEW_WARPS / g.KS;
-    const bool alone = (units + (int)gridDim.x * FEW_WARPS - 1) / ((int)gridDim.x * FEW_WARPS) * blocks <=
-                       (units + (int)gridDim.x * side - 1) / ((int)gridDim.x * side) * (blocks / g.KS + 2);
+    const int side = FEW_WARPS / g.KS, grid = (int)gridDim.x;
+    const bool alone = g.KS == 1 || (units + grid * FEW_WARPS - 1) / (grid * FEW_WARPS) * blocks <= (units + grid * side - 1) / (grid * side) * (blocks / g.KS + 3);
     const int RT = alone ? FEW_WARPS : side, rt = alone ? warp : warp / g.KS, run_lo = alone ? 0 : warp % g.KS, run_hi = alone ? g.KS : run_lo + 1;
     const int lo = blocks * run_lo / g.KS, hi = blocks * run_hi / g.KS, nb = hi - lo;
-    const int groups = (units + RT - 1) / RT, steps = (int)blockIdx.x < groups ? (groups - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
     // (warps that are alone take every grid's-width unit, so that few units are spread over all CTAs)
-    const int stride = (int)gridDim.x * RT, unit0 = alone ? (int)blockIdx.x + rt * (int)gridDim.x : (int)blockIdx.x * RT + rt;
-    const int my_steps = alone ? (unit0 < units ? (units - 1 - unit0) / stride + 1 : 0) : steps;
+    const int stride = grid * RT, unit0 = alone ? (int)blockIdx.x + rt * grid : (int)blockIdx.x * RT + rt;
+    const int begin = alone ? unit0 : (int)blockIdx.x * RT, my_steps = begin < units ? (units - 1 - begin) / stride + 1 : 0;
     unsigned char* ring = rings + warp * FEW_RING * FEW_SLOT;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
     const int kb = (g.D + 127) / 128, fb = (g.F + 127) / 128;
@@ -369,7 +420,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
     };
     auto cursor_at = [&](int u) {
         u = min(u, units - 1);
-        return Cursor{u / uf, u % uf};
+        const int e = u / uf;
+        return Cursor{e, u - e * uf};
     };
     auto advance = [&](Cursor& c) {
         c.fu += stride;
@@ -384,33 +436,32 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
     int load_b = lo;
     auto point = [&]() {
         const int e = entries[3 * ahead.entry], f = ahead.fu * 8 + gr;
-        size_t ra, rb;
+        size_t ra = (size_t)2 * e * g.F + f, rb = ra + g.F;
         if (!FP8 && g.interleaved) {
-            ra = (size_t)2 * e * g.F + 2 * (f - gr) + gr;
+            ra += f - gr;
             rb = ra + 8;
-        } else {
-            ra = (size_t)2 * e * g.F + f;
-            rb = ra + g.F;
         }
-        pa = g.w_in + ra * g.ld_in;
-        pb = g.w_in + rb * g.ld_in;
+        pa = g.w_in + ra * g.ld_in + lo * 128 + t4 * 16;
+        pb = g.w_in + rb * g.ld_in + lo * 128 + t4 * 16;
     };
     const int total = nb * my_steps;
     const bool whole = bytes % 128 == 0;
     auto load = [&](int slot) {
         const uint32_t dst = ring_at + slot * FEW_SLOT;
-        const int at = load_b * 128 + t4 * 16;
         if (whole) {
-            few_copy16(dst, pa + at);
-            few_copy16(dst + 512, pb + at);
-            few_copy16(dst + 1024, pa + at + 64);
-            few_copy16(dst + 1536, pb + at + 64);
+            few_copy16(dst, pa);
+            few_copy16(dst + 512, pb);
+            few_copy16(dst + 1024, pa + 64);
+            few_copy16(dst + 1536, pb + 64);
         } else {
-            few_copy16(dst, pa, at, bytes);
-            few_copy16(dst + 512, pb, at, bytes);
-            few_copy16(dst + 1024, pa, at + 64, bytes);
-            few_copy16(dst + 1536, pb, at + 64, bytes);
+            const int left = bytes - load_b * 128 - t4 * 16;
+            few_copy16(dst, pa, left);
+            few_copy16(dst + 512, pb, left);
+            few_copy16(dst + 1024, pa + 64, left - 64);
+            few_copy16(dst + 1536, pb + 64, left - 64);
         }
+        pa += 128;
+        pb += 128;
         if (++load_b == hi) {
             load_b = lo;
             advance(ahead);
@@ -427,45 +478,37 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
 #pragma unroll 1
     for (int step = 0; step < my_steps; ++step) {
         const int first = entries[3 * here.entry + 1], count = entries[3 * here.entry + 2], f0 = here.fu * 8;
-        const uint16_t* rows[G];
+        // e4m3: column c of group j is hi of row 4 j + c, column 4 + c its lo.  (Columns without a row: another's numbers, not stored.)
+        const uint8_t* rows[NG];
 #pragma unroll
-        for (int j = 0; j < G; ++j) {
-            const int t = places[first + min(j * 8 + gr, count - 1)] / g.top;
-            rows[j] = (XS ? x_rows + t * x_stride : FP8 ? x_half + (size_t)t * g.D : reinterpret_cast<const uint16_t*>(g.x) + (size_t)t * g.ldx) + t4 * (PER / 8);
+        for (int j = 0; j < NG; ++j) {
+            const int t = places[first + min(FP8 ? j * 4 + (gr & 3) : gr, count - 1)] / g.top;
+            rows[j] = x_rows + (size_t)t * x_bytes + (FP8 && gr >= 4 ? few_part_bytes(g.D) : 0) + t4 * 16 + lo * 128;
         }
         const float *sg = nullptr, *su = nullptr;
+        float s0_next = 1.0f, s1_next = 1.0f;
         if (FP8) {
             sg = g.s_in + ((size_t)2 * entries[3 * here.entry] * fb + f0 / 128) * kb;
             su = sg + (size_t)fb * kb;
+            s0_next = sg[lo];
+            s1_next = su[lo];
         }
-        float s0_next = FP8 ? sg[lo] : 1.0f, s1_next = FP8 ? su[lo] : 1.0f;
-        float sum[G][4];
+        float sum[NG][4];
 #pragma unroll
-        for (int j = 0; j < G; ++j)
+        for (int j = 0; j < NG; ++j)
 #pragma unroll
             for (int c = 0; c < 4; ++c) sum[j][c] = 0.0f;
+        int b = lo;
 #pragma unroll 1
         for (int run = run_lo; run < run_hi; ++run) {
-            float acc[G][4];
+            float acc[NG][4];
 #pragma unroll
-            for (int j = 0; j < G; ++j)
+            for (int j = 0; j < NG; ++j)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
             const int end = blocks * (run + 1) / g.KS;
 #pragma unroll 1
-            for (int b = blocks * run / g.KS; b < end; ++b) {
-                // the rows of x first: they come while the weights are waited for
-                constexpr int XW = FP8 ? 2 : 1;              // 16-byte pieces of x beside 16 bytes of a weight row
-                uint4 xv[G][2][XW];
-#pragma unroll
-                for (int j = 0; j < G; ++j)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < XW; ++i) {
-                            const int k = b * PER + h * (PER / 2) + i * 8;
-                            xv[j][h][i] = j * 8 + gr < count && (whole || k + t4 * (PER / 8) < g.D) ? *reinterpret_cast<const uint4*>(rows[j] + k) : make_uint4(0, 0, 0, 0);      // (D is a multiple of 8)
-                        }
+            for (; b < end; ++b) {
                 const float s0 = s0_next, s1 = s1_next;
                 if (FP8 && b + 1 < hi) {
                     s0_next = sg[b + 1];
@@ -473,63 +516,55 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
                 }
                 asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
                 const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
-                float c[G][2][4];            // two chains of products: one's results are 23 cycles away
+                const uint4 l0 = *reinterpret_cast<const uint4*>(at), h0 = *reinterpret_cast<const uint4*>(at + 512);
+                const uint4 l1 = *reinterpret_cast<const uint4*>(at + 1024), h1 = *reinterpret_cast<const uint4*>(at + 1536);
 #pragma unroll
-                for (int j = 0; j < G; ++j)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) c[j][i >> 2][i & 3] = 0.0f;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint4 wl = *reinterpret_cast<const uint4*>(at + 1024 * h), wh = *reinterpret_cast<const uint4*>(at + 512 + 1024 * h);
-                    const uint32_t lw[4] = {wl.x, wl.y, wl.z, wl.w}, hw[4] = {wh.x, wh.y, wh.z, wh.w};
-#pragma unroll
-                    for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
-                        uint32_t a0, a1, a2, a3;
-                        if (FP8) {
-                            f16_of(lw[i], a0, a2);
-                            f16_of(hw[i], a1, a3);
-                        } else {
-                            a0 = lw[2 * i];
-                            a2 = lw[2 * i + 1];
-                            a1 = hw[2 * i];
-                            a3 = hw[2 * i + 1];
-                        }
-#pragma unroll
-                        for (int j = 0; j < G; ++j) {
-                            if (j > 0 && count <= 8 * j) break;
-                            const uint4 v = xv[j][h][FP8 ? i >> 1 : 0];
-                            const uint32_t p0 = (i & 1) ? v.z : v.x, p1 = (i & 1) ? v.w : v.y;
-                            if (FP8) mma_f16_f32(c[j][h], a0, a1, a2, a3, p0, p1);
-                            else mma_bf16_f32(h ? c[j][1] : acc[j], a0, a1, a2, a3, p0, p1);
-                        }
+                for (int j = 0; j < NG; ++j) {
+                    if (j > 0 && count <= 4) break;
+                    const uint4 x0 = *reinterpret_cast<const uint4*>(rows[j]), x1 = *reinterpret_cast<const uint4*>(rows[j] + 64);
+                    float c0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, c1[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // two chains: a product's results are 26 cycles away
+                    if (FP8) {
+                        mma_e4m3_f32(c0, l0.x, h0.x, l0.y, h0.y, x0.x, x0.y);
+                        mma_e4m3_f32(c1, l1.x, h1.x, l1.y, h1.y, x1.x, x1.y);
+                        mma_e4m3_f32(c0, l0.z, h0.z, l0.w, h0.w, x0.z, x0.w);
+                        mma_e4m3_f32(c1, l1.z, h1.z, l1.w, h1.w, x1.z, x1.w);
+                    } else {
+                        mma_bf16_f32(c0, l0.x, h0.x, l0.y, h0.y, x0.x, x0.y);
+                        mma_bf16_f32(c1, l1.x, h1.x, l1.y, h1.y, x1.x, x1.y);
+                        mma_bf16_f32(c0, l0.z, h0.z, l0.w, h0.w, x0.z, x0.w);
+                        mma_bf16_f32(c1, l1.z, h1.z, l1.w, h1.w, x1.z, x1.w);
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[j][i] = FP8 ? fmaf(i < 2 ? s0 : s1, c0[i] + c1[i], acc[j][i]) : acc[j][i] + (c0[i] + c1[i]);
                 }
 #pragma unroll
-                for (int j = 0; j < G; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[j][i] = FP8 ? fmaf(i < 2 ? s0 : s1, c[j][0][i] + c[j][1][i], acc[j][i]) : acc[j][i] + c[j][1][i];
+                for (int j = 0; j < NG; ++j) rows[j] += 128;
                 if (done + FEW_RING < total) load(slot);
                 few_commit();
                 ++done;
                 slot = slot + 1 == FEW_RING ? 0 : slot + 1;
             }
 #pragma unroll
-            for (int j = 0; j < G; ++j)
+            for (int j = 0; j < NG; ++j)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) sum[j][c] += acc[j][c];
         }
         if (alone) {
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
-                if (j > 0 && count <= 8 * j) break;
+            for (int j = 0; j < NG; ++j) {
+                if (j > 0 && count <= 4) break;
+                if (FP8) {       // hi + lo
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) sum[j][c] = fmaf(__shfl_xor_sync(0xffffffffu, sum[j][c], 2), 0.0625f, sum[j][c]);
+                }
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const int col = j * 8 + t4 * 2 + c;
-                    const bool on = col < count;
+                    const int col = (FP8 ? j * 4 : 0) + t4 * 2 + c;
+                    const bool on = col < count && (!FP8 || t4 < 2);
                     const int pair = on ? places[first + col] : 0;
                     float y = sum[j][c], v = sum[j][2 + c];
                     if (FP8) {
-                        const float back = f16_unscale(x_largest[pair / g.top]);
+                        const float back = few_unscale(x_largest[pair / g.top], X_TO);
                         y *= back;
                         v *= back;
                     }
@@ -544,33 +579,38 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
                 }
             }
         } else {
-            float* mine = part + (((step & 1) * FEW_WARPS + warp) * 16 + gr) * TOK + t4 * 2;
+            float* mine = part + (((step & 1) * FEW_WARPS + warp) * 16 + gr) * COLS + t4 * 2;
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
+            for (int j = 0; j < NG; ++j) {
                 *reinterpret_cast<float2*>(mine + j * 8) = make_float2(sum[j][0], sum[j][1]);
-                *reinterpret_cast<float2*>(mine + 8 * TOK + j * 8) = make_float2(sum[j][2], sum[j][3]);
+                *reinterpret_cast<float2*>(mine + 8 * COLS + j * 8) = make_float2(sum[j][2], sum[j][3]);
             }
             __syncthreads();
             // eight columns of a pair by eight neighbouring threads; other warps every time
-            const float* all = part + (step & 1) * FEW_WARPS * 16 * TOK;
-            for (int i = (threadIdx.x + step * 128) & (FEW_THREADS - 1); i < RT * TOK * 8; i += FEW_THREADS) {      // (a multiple of 32)
-                const int f = i & 7, j = (i >> 3) % TOK, tile = (i >> 3) / TOK, unit = (int)blockIdx.x * RT + step * stride + tile;
+            const float* all = part + (step & 1) * FEW_WARPS * 16 * COLS;
+#pragma unroll 1
+            for (int i = (threadIdx.x + step * 128) & (FEW_THREADS - 1); i < RT * FEW_ROWS * 8; i += FEW_THREADS) {      // (a multiple of 32)
+                const int f = i & 7, j = (i >> 3) % FEW_ROWS, tile = (i >> 3) / FEW_ROWS, unit = (int)blockIdx.x * RT + step * stride + tile;
                 const Cursor at = cursor_at(unit);
                 const bool on = unit < units && j < entries[3 * at.entry + 2];
                 float h = 0.0f;
                 int pair = 0;
                 if (on) {
                     pair = places[entries[3 * at.entry + 1] + j];
-                    const float* p = all + (tile * g.KS * 16 + f) * TOK + j;
-                    float y = 0.0f, v = 0.0f;
+                    const float* p = all + (tile * g.KS * 16 + f) * COLS + (FP8 ? (j >> 2) * 8 + (j & 3) : j);
+                    float y = 0.0f, v = 0.0f, yl = 0.0f, vl = 0.0f;
                     for (int s = 0; s < g.KS; ++s) {
-                        y += p[s * 16 * TOK];
-                        v += p[s * 16 * TOK + 8 * TOK];
+                        y += p[s * 16 * COLS];
+                        v += p[s * 16 * COLS + 8 * COLS];
+                        if (FP8) {
+                            yl += p[s * 16 * COLS + 4];
+                            vl += p[s * 16 * COLS + 8 * COLS + 4];
+                        }
                     }
                     if (FP8) {
-                        const float back = f16_unscale(x_largest[pair / g.top]);
-                        y *= back;
-                        v *= back;
+                        const float back = few_unscale(x_largest[pair / g.top], X_TO);
+                        y = fmaf(yl, 0.0625f, y) * back;
+                        v = fmaf(vl, 0.0625f, v) * back;
                     }
                     h = fp8_glu(y, v, g.act, g.limit, g.on_input ? wts[pair] : 1.0f);
                     g.hidden[(size_t)pair * g.F + at.fu * 8 + f] = h;
@@ -590,7 +630,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
 // ---------------------------------------------------------------------------------------------------------------
 // second launch: down products and the weighted sum
 // ---------------------------------------------------------------------------------------------------------------
-template <bool FP8, int G>
+template <bool FP8>
 __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_constant__ FewArgs g) {
     extern __shared__ __align__(16) unsigned char few_smem[];
     const int pairs = g.n * g.top;
@@ -608,32 +648,41 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
         wts[i] = g.weights[i];
     }
     __syncthreads();
-    constexpr int PER = FP8 ? 128 : 64;
+    constexpr int PER = FP8 ? 128 : 64, HW = FP8 ? 4 : 2;      // numbers in a slot's row; groups of four numbers beside 16 bytes of a weight row
     const int bytes = FP8 ? g.F : 2 * g.F, blocks = (bytes + 127) / 128, items = n_entries * g.splits, n0 = blockIdx.x * 16;
     const int fb = (g.F + 127) / 128, db = (g.D + 127) / 128;
+    const bool whole = bytes % 128 == 0;
     unsigned char* ring = few_smem + warp * FEW_RING * FEW_SLOT;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
     const int ra = min(n0 + gr, g.D - 1), rb = min(n0 + gr + 8, g.D - 1);
-    auto run_lo = [&](int split) { return blocks * split / g.splits; };
     // the cursor of loading: this warp's items (entry, run of hidden columns) one after the other, slot by slot
     int load_item = warp, load_b = 0, load_hi = 0;
     const uint8_t *pa = nullptr, *pb = nullptr;
     auto point = [&]() {
         if (load_item >= items) return;
-        const int e = entries[3 * (load_item / g.splits)], split = load_item % g.splits;
-        load_b = run_lo(split);
-        load_hi = run_lo(split + 1);
-        pa = g.w_out + ((size_t)e * g.D + ra) * g.ld_out;
-        pb = g.w_out + ((size_t)e * g.D + rb) * g.ld_out;
+        const int entry = load_item / g.splits, split = load_item - entry * g.splits, e = entries[3 * entry];
+        load_b = blocks * split / g.splits;
+        load_hi = blocks * (split + 1) / g.splits;
+        pa = g.w_out + ((size_t)e * g.D + ra) * g.ld_out + load_b * 128 + t4 * 16;
+        pb = g.w_out + ((size_t)e * g.D + rb) * g.ld_out + load_b * 128 + t4 * 16;
     };
     auto load = [&](int slot) {
         if (load_item >= items) return;
         const uint32_t dst = ring_at + slot * FEW_SLOT;
-        const int at = load_b * 128 + t4 * 16;
-        few_copy16(dst, pa, at, bytes);
-        few_copy16(dst + 512, pb, at, bytes);
-        few_copy16(dst + 1024, pa, at + 64, bytes);
-        few_copy16(dst + 1536, pb, at + 64, bytes);
+        if (whole) {
+            few_copy16(dst, pa);
+            few_copy16(dst + 512, pb);
+            few_copy16(dst + 1024, pa + 64);
+            few_copy16(dst + 1536, pb + 64);
+        } else {
+            const int left = bytes - load_b * 128 - t4 * 16;
+            few_copy16(dst, pa, left);
+            few_copy16(dst + 512, pb, left);
+            few_copy16(dst + 1024, pa + 64, left - 64);
+            few_copy16(dst + 1536, pb + 64, left - 64);
+        }
+        pa += 128;
+        pb += 128;
         if (++load_b == load_hi) {
             load_item += FEW_WARPS;
             point();
@@ -647,128 +696,135 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
     }
     if (FP8) {
         const int uf = g.F / 8;
-        for (int p0 = warp * 8; p0 < pairs; p0 += FEW_WARPS * 8) {       // four lanes a pair
-            const int p = min(p0 + gr, pairs - 1);
-            uint32_t big = 0;
+        if (pairs <= 2 * FEW_WARPS) {
+            for (int p = warp; p < pairs; p += FEW_WARPS) {
+                uint32_t big = 0;
+#pragma unroll 4
+                for (int i = lane; i < uf; i += 32) big = max(big, g.largest[(size_t)p * uf + i]);
+                big = __reduce_max_sync(0xffffffffu, big);
+                if (lane == 0) largest[p] = big;
+            }
+        } else {
+            for (int p0 = warp * 8; p0 < pairs; p0 += FEW_WARPS * 8) {       // four lanes a pair
+                const int p = min(p0 + gr, pairs - 1);
+                uint32_t big = 0;
 #pragma unroll 8
-            for (int i = t4; i < uf; i += 4) big = max(big, g.largest[(size_t)p * uf + i]);
-            big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-            big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            if (t4 == 0) largest[p] = big;
+                for (int i = t4; i < uf; i += 4) big = max(big, g.largest[(size_t)p * uf + i]);
+                big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                if (t4 == 0) largest[p] = big;
+            }
         }
         __syncthreads();
     }
-    int slot = 0;
-    for (int item = warp; item < items; item += FEW_WARPS) {
-        const int entry = item / g.splits, split = item % g.splits, e = entries[3 * entry], first = entries[3 * entry + 1], count = entries[3 * entry + 2];
-        const float* rows[G];
-        float scale[G];
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-            const int pair = places[first + min(j * 8 + gr, count - 1)];
-            rows[j] = g.hidden + (size_t)pair * g.F + t4 * (PER / 8);
-            scale[j] = FP8 ? f16_scale(largest[pair]) : 1.0f;
-        }
-        const float* sw = FP8 ? g.s_out + ((size_t)e * db + min(n0, g.D - 1) / 128) * fb : nullptr;
-        float acc[G][4];
-#pragma unroll
-        for (int j = 0; j < G; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
-        // the first eight columns' hidden numbers of a block (more columns are rare and read when they are multiplied), a block ahead
-        constexpr int HW = FP8 ? 4 : 2;                  // groups of four numbers beside 16 bytes of a weight row
-        float4 next[2][HW];
-        auto fetch = [&](int j, int b, int h, int i) {
-            const int k = b * PER + h * (PER / 2) + i * 4;
-            return j * 8 + gr < count && k + t4 * (PER / 8) < g.F ? *reinterpret_cast<const float4*>(rows[j] + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);      // (F is a multiple of 8)
-        };
-        const int lo = run_lo(split), hi = run_lo(split + 1);
+    // an item under way; the hidden numbers of its next block, or of the next item's first, are fetched a block ahead
+    struct Item {
+        const float* row;        // of the lane's column, null without one
+        const float* sw;
+        float scale;
+        int first, count, split, b, hi;
+    };
+    auto start = [&](int item) {
+        Item it;
+        const int entry = item / g.splits;
+        it.split = item - entry * g.splits;
+        it.first = entries[3 * entry + 1];
+        it.count = entries[3 * entry + 2];
+        it.b = blocks * it.split / g.splits;
+        it.hi = blocks * (it.split + 1) / g.splits;
+        const int pair = places[it.first + min(gr, it.count - 1)];
+        it.row = gr < it.count ? g.hidden + (size_t)pair * g.F + t4 * (PER / 8) : nullptr;
+        it.scale = FP8 ? few_scale(largest[pair], HIDDEN_TO) : 1.0f;
+        it.sw = FP8 ? g.s_out + ((size_t)entries[3 * entry] * db + min(n0, g.D - 1) / 128) * fb : nullptr;
+        return it;
+    };
+    float4 next[2][HW];
+    float s_next = 1.0f;
+    auto fetch = [&](const Item& it, int b) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < HW; ++i) next[h][i] = fetch(0, lo, h, i);
-        float s_next = FP8 ? sw[lo] : 1.0f;
+            for (int i = 0; i < HW; ++i) {
+                const int k = b * PER + h * (PER / 2) + i * 4;
+                next[h][i] = it.row != nullptr && (whole || k + t4 * (PER / 8) < g.F) ? *reinterpret_cast<const float4*>(it.row + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);      // (F is a multiple of 8)
+            }
+        if (FP8) s_next = it.sw[b];
+    };
+    int item = warp, slot = 0;
+    Item here, after;
+    if (item < items) {
+        here = start(item);
+        fetch(here, here.b);
+    }
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-        for (int b = lo; b < hi; ++b) {
-            // the operand's pairs: fp16, or two bf16 parts
-            uint2 high[2][HW], low[2][FP8 ? 1 : HW];
-            auto split_up = [&](float4 v, float sc, uint2& p, uint2& r) {
+    while (item < items) {
+        // the operand's pairs: fp16, or two bf16 parts
+        uint2 high[2][HW], low[2][FP8 ? 1 : HW];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < HW; ++i) {
+                const float4 v = next[h][i];
                 if (FP8) {
-                    p = make_uint2(pair_f16(v.x * sc, v.y * sc), pair_f16(v.z * sc, v.w * sc));
+                    high[h][i] = make_uint2(pair_f16(v.x * here.scale, v.y * here.scale), pair_f16(v.z * here.scale, v.w * here.scale));
                 } else {
-                    p = make_uint2(pair_bf16(v.x, v.y), pair_bf16(v.z, v.w));
-                    r = make_uint2(pair_bf16(v.x - low_of(p.x), v.y - high_of(p.x)), pair_bf16(v.z - low_of(p.y), v.w - high_of(p.y)));
+                    const uint2 p = make_uint2(pair_bf16(v.x, v.y), pair_bf16(v.z, v.w));
+                    high[h][i] = p;
+                    low[h][FP8 ? 0 : i] = make_uint2(pair_bf16(v.x - low_of(p.x), v.y - high_of(p.x)), pair_bf16(v.z - low_of(p.y), v.w - high_of(p.y)));
                 }
-            };
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < HW; ++i) split_up(next[h][i], scale[0], high[h][i], low[h][FP8 ? 0 : i]);
-            const float s0 = s_next;
-            if (b + 1 < hi) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < HW; ++i) next[h][i] = fetch(0, b + 1, h, i);
-                if (FP8) s_next = sw[b + 1];
             }
-            asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
-            const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
-            float c[G][2][4];
+        const float s0 = s_next;
+        const bool last = here.b + 1 == here.hi;
+        if (!last) {
+            fetch(here, here.b + 1);
+        } else if (item + FEW_WARPS < items) {
+            after = start(item + FEW_WARPS);
+            fetch(after, after.b);
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(FEW_RING - 1) : "memory");
+        const unsigned char* at = ring + slot * FEW_SLOT + lane * 16;
+        float c[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-            for (int j = 0; j < G; ++j)
+        for (int h = 0; h < 2; ++h) {
+            const uint4 wl = *reinterpret_cast<const uint4*>(at + 1024 * h), wh = *reinterpret_cast<const uint4*>(at + 512 + 1024 * h);
+            const uint32_t lw[4] = {wl.x, wl.y, wl.z, wl.w}, hw[4] = {wh.x, wh.y, wh.z, wh.w};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) c[j][i >> 2][i & 3] = 0.0f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint4 wl = *reinterpret_cast<const uint4*>(at + 1024 * h), wh = *reinterpret_cast<const uint4*>(at + 512 + 1024 * h);
-                const uint32_t lw[4] = {wl.x, wl.y, wl.z, wl.w}, hw[4] = {wh.x, wh.y, wh.z, wh.w};
-#pragma unroll
-                for (int i = 0; i < HW; ++i) {
+            for (int i = 0; i < HW; ++i) {
+                if (FP8) {
                     uint32_t a0, a1, a2, a3;
-                    if (FP8) {
-                        f16_of(lw[i], a0, a2);
-                        f16_of(hw[i], a1, a3);
-                    } else {
-                        a0 = lw[2 * i];
-                        a2 = lw[2 * i + 1];
-                        a1 = hw[2 * i];
-                        a3 = hw[2 * i + 1];
-                    }
-#pragma unroll
-                    for (int j = 0; j < G; ++j) {
-                        if (j > 0 && count <= 8 * j) break;
-                        uint2 p = high[h][i], r = low[h][FP8 ? 0 : i];
-                        if (j > 0) split_up(fetch(j, b, h, i), scale[j], p, r);
-                        if (FP8) {
-                            mma_f16_f32(c[j][h], a0, a1, a2, a3, p.x, p.y);
-                        } else {
-                            mma_bf16_f32(acc[j], a0, a1, a2, a3, p.x, p.y);
-                            mma_bf16_f32(c[j][1], a0, a1, a2, a3, r.x, r.y);
-                        }
-                    }
+                    f16_of(lw[i], a0, a2);
+                    f16_of(hw[i], a1, a3);
+                    mma_f16_f32(c[h], a0, a1, a2, a3, high[h][i].x, high[h][i].y);
+                } else {
+                    mma_bf16_f32(c[0], lw[2 * i], hw[2 * i], lw[2 * i + 1], hw[2 * i + 1], high[h][i].x, high[h][i].y);
+                    mma_bf16_f32(c[1], lw[2 * i], hw[2 * i], lw[2 * i + 1], hw[2 * i + 1], low[h][FP8 ? 0 : i].x, low[h][FP8 ? 0 : i].y);
                 }
             }
-#pragma unroll
-            for (int j = 0; j < G; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[j][i] = FP8 ? fmaf(s0, c[j][0][i] + c[j][1][i], acc[j][i]) : acc[j][i] + c[j][1][i];
-            load(slot);
-            few_commit();
-            slot = slot + 1 == FEW_RING ? 0 : slot + 1;
         }
 #pragma unroll
-        for (int j = 0; j < G; ++j)
+        for (int i = 0; i < 4; ++i) acc[i] = FP8 ? fmaf(s0, c[0][i] + c[1][i], acc[i]) : acc[i] + (c[0][i] + c[1][i]);
+        load(slot);
+        few_commit();
+        slot = slot + 1 == FEW_RING ? 0 : slot + 1;
+        if (last) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int col = j * 8 + t4 * 2 + c;
-                if (col >= count) continue;
-                const int pair = places[first + col];
-                const float back = FP8 ? f16_unscale(largest[pair]) : 1.0f;
-                float* at = sums + ((size_t)split * pairs + pair) * 16 + gr;
-                at[0] = acc[j][c] * back;
-                at[8] = acc[j][2 + c] * back;
+            for (int j = 0; j < 2; ++j) {
+                const int col = t4 * 2 + j;
+                if (col < here.count) {
+                    const int pair = places[here.first + col];
+                    const float back = FP8 ? few_unscale(largest[pair], HIDDEN_TO) : 1.0f;
+                    float* to = sums + ((size_t)here.split * pairs + pair) * 16 + gr;
+                    to[0] = acc[j] * back;
+                    to[8] = acc[2 + j] * back;
+                }
+                acc[j] = acc[2 + j] = 0.0f;
             }
+            here = after;
+            item += FEW_WARPS;
+        } else {
+            ++here.b;
+        }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * g.n; i += FEW_THREADS) {
@@ -785,10 +841,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
 }
 
 size_t in_smem(const FewArgs& g) {
-    const int tok = g.n <= 8 ? 8 : 16, pairs = g.n * g.top;
-    return (size_t)FEW_WARPS * FEW_RING * FEW_SLOT + 4 * ((size_t)2 * FEW_WARPS * 16 * tok + ((g.n * g.E + 3) & ~3) + 6 * pairs + 2 * FEW_WARPS + 2 + FEW_TOKENS);
+    return (size_t)FEW_WARPS * FEW_RING * FEW_SLOT + 4 * ((size_t)(g.s_in ? 2 : 1) * FEW_WARPS * 16 * 16 + few_list_words(g.n, g.E, g.n * g.top));
 }
-size_t in_x_bytes(const FewArgs& g, bool fp8) { return 4 * (size_t)few_pad(g.n, g.E, g.n * g.top) + 2 * (size_t)g.n * few_x_stride(g.D, fp8); }
 size_t out_smem(const FewArgs& g) {
     const int pairs = g.n * g.top;
     return (size_t)FEW_WARPS * FEW_RING * FEW_SLOT + 4 * ((size_t)g.splits * pairs * 16 + 6 * pairs);
@@ -796,12 +850,12 @@ size_t out_smem(const FewArgs& g) {
 
 constexpr size_t FEW_SMEM = 227 * 1024;
 
-template <bool FP8, int G, bool XS>
+template <bool FP8, bool XS>
 int launch(FewArgs& g, cudaStream_t s) {
     constexpr size_t most = FEW_SMEM;
-    const size_t smem_in = in_smem(g) + (XS ? in_x_bytes(g, FP8) : 0), smem_out = out_smem(g);
+    const size_t smem_in = in_smem(g) + (XS ? (size_t)g.n * few_x_bytes(g.D, FP8) : 0), smem_out = out_smem(g);
     MM_REQUIRE(smem_in <= most && smem_out <= most, "moe few: too many experts or choices for the kernels' shared memory");
-    if (!mm_allow_smem<few_in_kernel<FP8, G, XS>>(most) || !mm_allow_smem<few_out_kernel<FP8, G>>(most)) {
+    if (!mm_allow_smem<few_in_kernel<FP8, XS>>(most) || !mm_allow_smem<few_out_kernel<FP8>>(most)) {
         mm_set_last_error("moe few: cannot reserve shared memory");
         return MM_ERR_LAUNCH;
     }
@@ -820,7 +874,7 @@ int launch(FewArgs& g, cudaStream_t s) {
     int fit = resident.load(std::memory_order_relaxed);
     if (fit == 0) {
         cfg.gridDim = dim3(FP8_SM_COUNT / FEW_CLUSTER * FEW_CLUSTER);
-        if (cudaOccupancyMaxActiveClusters(&fit, few_in_kernel<FP8, G, XS>, &cfg) != cudaSuccess || fit < 1) {
+        if (cudaOccupancyMaxActiveClusters(&fit, few_in_kernel<FP8, XS>, &cfg) != cudaSuccess || fit < 1) {
             (void)cudaGetLastError();
             fit = FEW_CLUSTERS;
         }
@@ -830,9 +884,9 @@ int launch(FewArgs& g, cudaStream_t s) {
     const int most_experts = g.E < g.n * g.top ? g.E : g.n * g.top;
     const long long groups = ((long long)most_experts * (g.F / 8) * g.KS + FEW_WARPS - 1) / FEW_WARPS, clusters = (groups + FEW_CLUSTER - 1) / FEW_CLUSTER;
     cfg.gridDim = dim3((unsigned)(clusters < fit ? clusters : fit) * FEW_CLUSTER);
-    cudaLaunchKernelEx(&cfg, few_in_kernel<FP8, G, XS>, g);
+    cudaLaunchKernelEx(&cfg, few_in_kernel<FP8, XS>, g);
     MM_CHECK_LAUNCH();
-    mm_launch_dependent(g_mm_pdl != 0, few_out_kernel<FP8, G>, dim3(ceil_div(g.D, 16)), dim3(FEW_THREADS), smem_out, s, g);
+    mm_launch_dependent(g_mm_pdl != 0, few_out_kernel<FP8>, dim3(ceil_div(g.D, 16)), dim3(FEW_THREADS), smem_out, s, g);
     MM_CHECK_LAUNCH();
     return MM_OK;
 }
@@ -841,7 +895,7 @@ int launch(FewArgs& g, cudaStream_t s) {
 
 // x bf16 [n, ldx]; w_router fp32 [E, D]; experts bf16 (s_in, s_out null): w_in [E, 2 F, D] (gate rows then up rows, or with `interleaved` alternating in
 // blocks of 8), w_out [E, D, F]; or e4m3 with scales: w_in [E, 2, F, ld_in], w_out [E, D, ld_out].  ld_in, ld_out: bytes of a row.
-// out bf16 [n, D].  scratch: pairs * (4 F + F / 2 + 24) + 32 bytes, pairs = n * top, and with e4m3 experts 36 n D more.
+// out bf16 [n, D].  scratch: pairs * (4 F + F / 2 + 24) + 32 + 36 n (D + 160) bytes, pairs = n * top.
 MM_EXPORT int mm_moe_few(const void* x, long long ldx, int n, int D, const void* w_router, int E, int top, int groups, int keep, int scoring, const void* correction,
                          int pair_sum, int renorm, float wscale, const void* w_in, const void* s_in, long long ld_in, const void* w_out, const void* s_out, long long ld_out,
                          int F, int act, float limit, int on_input, int interleaved, void* out, void* scratch, void* stream) {
@@ -850,6 +904,8 @@ MM_EXPORT int mm_moe_few(const void* x, long long ldx, int n, int D, const void*
     MM_REQUIRE(groups > 0 && E % groups == 0 && keep > 0 && keep <= groups && top <= keep * (E / groups),
                "moe few: experts must split into equal runs, 0 < keep <= runs, and top fits into the kept runs");
     MM_REQUIRE(scoring == 0 || scoring == 1, "moe few: the scoring is 0 (softmax) or 1 (sigmoid)");
+    // (the choice's scratch is what the rings and the sums take up later)
+    MM_REQUIRE((size_t)n * 8 * (E + groups) <= (size_t)FEW_WARPS * FEW_RING * FEW_SLOT + 4 * FEW_WARPS * 16 * 16, "moe few: too many experts and runs of them");
     MM_REQUIRE(act >= 0 && act <= MM_GLU_GELU_TANH, "moe few: unknown activation");
     const bool fp8 = s_in != nullptr;
     MM_REQUIRE(fp8 == (s_out != nullptr) && !(fp8 && interleaved), "moe few: both matrices are in bf16 or both in 8 bits");
@@ -874,7 +930,7 @@ MM_EXPORT int mm_moe_few(const void* x, long long ldx, int n, int D, const void*
     g.largest = (uint32_t*)(g.hidden + pairs * F);
     g.weights = (float*)(g.largest + pairs * (F / 8));
     g.lists = (int32_t*)(g.weights + pairs);
-    g.x_half = (uint16_t*)(((uintptr_t)(g.lists + 1 + 4 * pairs) + 15) & ~(uintptr_t)15);
+    g.x_copy = (uint8_t*)(((uintptr_t)(g.lists + 1 + 4 * pairs) + 15) & ~(uintptr_t)15);
     g.out = (__nv_bfloat16*)out;
     g.n = n;
     g.D = D;
@@ -897,11 +953,7 @@ MM_EXPORT int mm_moe_few(const void* x, long long ldx, int n, int D, const void*
     g.splits = (FEW_WARPS + top - 1) / top;          // a run for every warp when there is one token
     if (g.splits > out_blocks) g.splits = out_blocks;
     cudaStream_t s = (cudaStream_t)stream;
-    const bool xs = in_smem(g) + in_x_bytes(g, fp8) <= FEW_SMEM;
-    if (fp8) {
-        if (xs) return n <= 8 ? launch<true, 1, true>(g, s) : launch<true, 2, true>(g, s);
-        return n <= 8 ? launch<true, 1, false>(g, s) : launch<true, 2, false>(g, s);
-    }
-    if (xs) return n <= 8 ? launch<false, 1, true>(g, s) : launch<false, 2, true>(g, s);
-    return n <= 8 ? launch<false, 1, false>(g, s) : launch<false, 2, false>(g, s);
+    const bool xs = in_smem(g) + (size_t)n * few_x_bytes(D, fp8) <= FEW_SMEM;
+    if (fp8) return xs ? launch<true, true>(g, s) : launch<true, false>(g, s);
+    return xs ? launch<false, true>(g, s) : launch<false, false>(g, s);
 }

@@ -2301,7 +2301,7 @@ def moe_few(x: torch.Tensor, w_router: torch.Tensor, w_in, w_out, top: int, grou
     act = _glu_code(activation, limit, "moe_few")
     _here("moe_few", x, w_router, correction, *tensors)
     out = torch.empty((n, d), dtype=torch.bfloat16, device=x.device)
-    scratch = torch.empty(n * top * (4 * f + f // 2 + 24) + 32 + (36 * n * d if fp8 else 0), dtype=torch.uint8, device=x.device)
+    scratch = torch.empty(n * top * (4 * f + f // 2 + 24) + 32 + 36 * n * (d + 160), dtype=torch.uint8, device=x.device)
     check(_lib.load().mm_moe_few(x.data_ptr(), x.stride(0), n, d, w_router.data_ptr(), E, int(top), int(groups), int(keep), ROUTER_SCORINGS[scoring], _ptr(correction),
                                  GROUP_SCORES[group_score], int(scoring == "softmax" if renorm is None else renorm), float(scale), tensors[0].data_ptr(), _ptr(tensors[1]),
                                  ld_in, tensors[2].data_ptr(), _ptr(tensors[3]), ld_out, f, act, float(limit), int(weight_on == "input"), int(bool(interleaved)),

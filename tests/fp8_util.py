@@ -76,10 +76,10 @@ def act64(g, u, name, limit):
     return g * torch.sigmoid(g) * u
 
 
-def hidden64(x, gate, up, name, limit, scale=None):
+def hidden64(x, gate, up, name, limit, scale=None, off=None):
     """act(x gate^T, x up^T) in 64 bits and what fp32 sums and an fp32 activation may put it off by: the sums' errors through slopes of
-    at most 1.2 |u| + 0.2 (g) and 1.2 |g| + 1.2 (u), and 2^-18 of its size for the activation's own arithmetic."""
-    (g, ge), (u, ue) = product(x, gate), product(x, up)
+    at most 1.2 |u| + 0.2 (g) and 1.2 |g| + 1.2 (u), and 2^-18 of its size for the activation's own arithmetic.  ``off``: as for ``product``."""
+    (g, ge), (u, ue) = product(x, gate, off=off), product(x, up, off=off)
     if scale is not None:
         g, ge, u, ue = g * scale, ge * scale.abs(), u * scale, ue * scale.abs()
     h = act64(g, u, name, limit)

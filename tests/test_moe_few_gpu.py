@@ -47,8 +47,9 @@ def _choice64(x, router, top, groups=1, keep=1, scoring="softmax", renorm=True, 
 
 
 def _layer64(x, idx, wts, w_in, w_out, f, act, limit, on_input, fp8):
-    """The result and what it may be off by: the sums' errors (f8.sum_error; its 128 a block covers the products' own order), hidden rows in two
-    bf16 parts (2^-16) or fp16 (2^-11 of a number is a step; 2^-39 of the row's largest below), weights and score in fp32 (2^-20 with the router's sums)."""
+    """The result and what it may be off by: the sums' errors (f8.sum_error; its 128 a block covers the products' own order), x in two e4m3 parts (2^-21
+    of its largest), hidden rows in two bf16 parts (2^-17) or fp16 (half a step is 2^-12 of a number; 2^-38 of the row's largest below), weights and score in fp32
+    (2^-18 with the router's sums)."""
     y = torch.zeros(x.shape, dtype=torch.float64, device=DEV)
     err = torch.zeros_like(y)
     wide_in, wide_out = _wide(w_in).view(-1, 2, f, x.shape[1]), _wide(w_out)
@@ -56,7 +57,8 @@ def _layer64(x, idx, wts, w_in, w_out, f, act, limit, on_input, fp8):
         for c in range(idx.shape[1]):
             e, w = idx[t, c], wts[t, c]
             row = x[t:t + 1].double()
-            h, off = f8.hidden64(row, wide_in[e][0], wide_in[e][1], act, limit, w.view(1, 1) if on_input else None)
+            h, off = f8.hidden64(row, wide_in[e][0], wide_in[e][1], act, limit, w.view(1, 1) if on_input else None,
+                                off=torch.full_like(row, row.abs().max().item() * 2.0 ** -21) if fp8 else None)
             off = off + (h.abs() * 2.0 ** -12 + h.abs().amax() * 2.0 ** -38 if fp8 else h.abs() * 2.0 ** -17) + (h.abs() + off) * (2.0 ** -18 if on_input else 0.0)
             part, part_err = f8.product(h, wide_out[e], off=off)
             if not on_input:
@@ -160,7 +162,7 @@ def test_a_token_does_not_depend_on_its_neighbours(n, fp8):
 
 @pytest.mark.parametrize("size", [1e-30, 1e-4, 1e4, 1e18])
 def test_rows_of_any_size_in_8_bit_experts(size):
-    """the power of two in front of fp16 follows the rows: scaling x and the router's rows against one another changes nothing but the scale of a linear layer"""
+    """the powers of two in front of the parts follow the rows: scaling x and the router's rows against one another changes nothing but the scale of a linear layer"""
     from mimirmind_b200.kernels import ops
     n, d, f, experts = 5, 128, 64, 4
     x, router, w_in, w_out = _layer(n, d, f, experts, _gen(11), True)
