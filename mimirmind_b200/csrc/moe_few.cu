@@ -30,6 +30,7 @@ namespace {
 
 constexpr int FEW_THREADS = 512, FEW_WARPS = 16, FEW_RING = 3, FEW_SLOT = 2048, FEW_CLUSTER = 8;
 constexpr int FEW_TOKENS = 16, FEW_MAX_EXPERTS = 512, FEW_MAX_TOP = 32;
+constexpr int FEW_RANK_EXPERTS = 192;    // up to here a token's scores are ranked all at once, beyond by searches
 constexpr int FEW_ROWS = 8;              // (token, choice) rows of an entry; an expert with more has several
 constexpr int FEW_CLUSTERS = FP8_SM_COUNT / FEW_CLUSTER;      // at the most
 
@@ -94,20 +95,17 @@ __device__ __forceinline__ float few_scale(uint32_t size_bits, int to) { return 
 __device__ __forceinline__ float few_unscale(uint32_t size_bits, int to) { return __uint_as_float((uint32_t)(few_exponent(size_bits) - to) << 23); }
 constexpr int X_TO = 7, HIDDEN_TO = 14;
 
-// moe_route_warp's choice where every run of experts is kept: a choice is two reductions over the warp.  Code that runs once in a launch is
-// fetched from L2 as it goes: kept short, it takes 2,000 cycles for 8 of 128 experts instead of 7,600.
-// s: 2 E words of the warp's own: the scores, and their order (0: not to be chosen, a NaN, minus infinity or chosen already).
-__device__ __forceinline__ void few_choose(const float* __restrict__ z, float* s, int lane, int E, int top, int scoring, const float* __restrict__ correction, int renorm,
-                                           float wscale, int32_t* idx, float* wts) {
-    uint32_t* key = reinterpret_cast<uint32_t*>(s + E);
+// moe_route_warp's scores (the same formula), and their order as numbers: 0 is not to be chosen (a NaN, minus infinity).  A warp; s, key: E words each.
+// (Code that runs once in a launch is fetched from L2 as it goes: short loops beat unrolled ones here.)
+__device__ __forceinline__ void few_scores(const float* __restrict__ z, float* s, uint32_t* key, int lane, int E, int scoring, const float* __restrict__ correction) {
     float m = 0.0f, inv = 1.0f;
     if (scoring == 0) {
         m = -INFINITY;
-#pragma unroll 1
+#pragma unroll 2
         for (int e = lane; e < E; e += 32) m = fmaxf(m, z[e]);
         m = warp_max(m);
         float sum = 0.0f;
-#pragma unroll 1
+#pragma unroll 2
         for (int e = lane; e < E; e += 32) {
             const float p = expf(z[e] - m);
             s[e] = p;
@@ -115,7 +113,7 @@ __device__ __forceinline__ void few_choose(const float* __restrict__ z, float* s
         }
         inv = 1.0f / warp_sum(sum);
     }
-#pragma unroll 1
+#pragma unroll 2
     for (int e = lane; e < E; e += 32) {
         const float v = scoring == 1 ? 1.0f / (1.0f + expf(-z[e])) : s[e] * inv;
         s[e] = v;
@@ -123,45 +121,16 @@ __device__ __forceinline__ void few_choose(const float* __restrict__ z, float* s
         const uint32_t u = __float_as_uint(c);
         key[e] = c != c || c == -INFINITY ? 0u : (u >> 31) ? ~u : u | 0x80000000u;
     }
-    __syncwarp();
-    float total = 0.0f, mine_w = 0.0f;
-    int mine_e = 0;
-    if (E <= 128) {
-        // every lane counts the scores ahead of its own four: no choice waits for another
-        uint32_t own[4];
-        int ahead[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            own[j] = j * 32 + lane < E ? key[j * 32 + lane] : 0u;
-            ahead[j] = 0;
-        }
-#pragma unroll 1
-        for (int e = 0; e < E; ++e) {
-            const uint32_t v = key[e];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) ahead[j] += v > own[j] || (v == own[j] && e < j * 32 + lane);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (own[j] != 0u && ahead[j] < top) key[ahead[j]] = (uint32_t)(j * 32 + lane);      // (the order is in registers now)
-        __syncwarp();
-        // how many there were to choose from
-        int found = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) found += __popc(__ballot_sync(0xffffffffu, own[j] != 0u));
-        if (lane < top && lane < found) {
-            mine_e = (int)key[lane];
-            mine_w = s[mine_e];
-        }
-#pragma unroll 1
-        for (int k = 0; k < top; ++k) total += __shfl_sync(0xffffffffu, mine_w, k);
-    } else {
+    for (int e = E + lane; e < (E + 3) / 4 * 4; e += 32) key[e] = 0;
+}
+
+// A warp: the choice by `top` searches for the largest number, the lowest expert among equals; chosen[k] = expert, or -1 where fewer can be chosen.
+__device__ __forceinline__ void few_search(uint32_t* key, int lane, int E, int top, int32_t* chosen) {
 #pragma unroll 1
     for (int k = 0; k < top; ++k) {
         uint32_t best = 0;
         int at = 0x7fffffff;
-#pragma unroll 1
+#pragma unroll 4
         for (int e = lane; e < E; e += 32) {
             const uint32_t v = key[e];
             if (v > best) {
@@ -170,25 +139,10 @@ __device__ __forceinline__ void few_choose(const float* __restrict__ z, float* s
             }
         }
         const uint32_t most = __reduce_max_sync(0xffffffffu, best);
-        int e = (int)__reduce_min_sync(0xffffffffu, best == most && most != 0 ? (uint32_t)at : 0x7fffffffu);      // the lowest number among equals
-        float weight = 0.0f;
-        if (e == 0x7fffffff) {
-            e = 0;               // fewer to choose from than `top`: the rest of the choice carries no weight
-        } else {
-            weight = s[e];
-            if ((e & 31) == lane) key[e] = 0;
-        }
+        const int e = (int)__reduce_min_sync(0xffffffffu, best == most && most != 0 ? (uint32_t)at : 0x7fffffffu);
+        if (lane == 0) chosen[k] = e == 0x7fffffff ? -1 : e;
+        if (e != 0x7fffffff && (e & 31) == lane) key[e] = 0;
         __syncwarp();
-        total += weight;
-        if (lane == k) {
-            mine_e = e;
-            mine_w = weight;
-        }
-    }
-    }
-    if (lane < top) {
-        idx[lane] = mine_e;
-        wts[lane] = renorm || wscale != 1.0f ? mine_w / (renorm ? total + 1e-20f : 1.0f) * wscale : mine_w;
     }
 }
 
@@ -226,48 +180,57 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
     pdl_trigger();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // waited for in front of the first store to another CTA: by then it runs
 
-    if (FP8) {
-        if (warp < g.n) {            // a warp per token
-            uint32_t big = 0;
-#pragma unroll 4
-            for (int d = lane * 8; d < g.D; d += 256) {       // (D is a multiple of 8)
-                const uint4 v = *reinterpret_cast<const uint4*>(g.x + (size_t)warp * g.ldx + d);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) big = max(big, max((w[i] & 0x7fffu) << 16, w[i] & 0x7fff0000u));
-            }
-            big = __reduce_max_sync(0xffffffffu, big);
-            if (lane == 0) x_largest[warp] = big;
-        }
-    }
-    // ---- logits: 16 experts a tile, a sixteenth of the depth a warp ----
+    if (FP8 && threadIdx.x < FEW_TOKENS) x_largest[threadIdx.x] = 0;
+    // ---- logits: 16 experts a tile, a sixteenth of the depth a warp; and the rows' largest sizes ----
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    __syncthreads();
     {
+        constexpr int BATCH = 4, STEP_BYTES = 32 * 48;          // steps of 16 that are on their way together: what a lane multiplies of them, in its own places
+        static_assert(BATCH * STEP_BYTES <= FEW_RING * FEW_SLOT, "a warp's share of the rings");
         const int steps = (g.D + 15) / 16, lo = steps * warp / FEW_WARPS, hi = steps * (warp + 1) / FEW_WARPS;
+        unsigned char* mine_at = rings + warp * FEW_RING * FEW_SLOT + lane * 16;
+        const uint32_t stage = (uint32_t)__cvta_generic_to_shared(mine_at);
+        const __nv_bfloat16 *xa = g.x + (size_t)min(gr, g.n - 1) * g.ldx, *xb = g.x + (size_t)min(gr + 8, g.n - 1) * g.ldx;      // (columns without a token: not looked at)
+        uint32_t big0 = 0, big1 = 0;
 #pragma unroll 1
-        for (int tile = rank; tile * 16 < g.E; tile += FEW_CLUSTER) {
+        for (int tile = rank; tile * 16 < g.E || (FP8 && tile == (int)rank); tile += FEW_CLUSTER) {      // (a CTA without a tile still looks at x)
             const float *wa = g.w_router + (size_t)min(tile * 16 + gr, g.E - 1) * g.D, *wb = g.w_router + (size_t)min(tile * 16 + gr + 8, g.E - 1) * g.D;
-            const __nv_bfloat16 *xa = g.x + (size_t)min(gr, g.n - 1) * g.ldx, *xb = g.x + (size_t)min(gr + 8, g.n - 1) * g.ldx;      // (columns without a token: not looked at)
             float acc[2][4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[0][c] = acc[1][c] = 0.0f;
-#pragma unroll 4
-            for (int s = lo; s < hi; ++s) {
-                const int k = s * 16 + t4 * 4;
-                const bool on = k < g.D;
-                const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                const float4 a = on ? *reinterpret_cast<const float4*>(wa + k) : zero, b = on ? *reinterpret_cast<const float4*>(wb + k) : zero;
-                const uint2 x0 = on ? *reinterpret_cast<const uint2*>(xa + k) : make_uint2(0, 0), x1 = on && g.n > 8 ? *reinterpret_cast<const uint2*>(xb + k) : make_uint2(0, 0);
-                float r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll 1
+            for (int s0 = lo; s0 < hi; s0 += BATCH) {
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {       // hi, mid, lo
-                    const uint32_t a0 = pair_bf16(r[0], r[1]), a2 = pair_bf16(r[2], r[3]), a1 = pair_bf16(r[4], r[5]), a3 = pair_bf16(r[6], r[7]);
-                    if (p < 2) {
-                        r[0] -= low_of(a0); r[1] -= high_of(a0); r[2] -= low_of(a2); r[3] -= high_of(a2);
-                        r[4] -= low_of(a1); r[5] -= high_of(a1); r[6] -= low_of(a3); r[7] -= high_of(a3);
+                for (int i = 0; i < BATCH; ++i) {
+                    const int k = (s0 + i) * 16 + t4 * 4, on = s0 + i < hi && k < g.D ? 1 : 0;       // (D is a multiple of 8)
+                    const uint32_t dst = stage + i * STEP_BYTES;
+                    const float *pa = wa + (on ? k : 0), *pb = wb + (on ? k : 0);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(pa), "r"(on * 16) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 512), "l"(pb), "r"(on * 16) : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + 1024), "l"(xa + (on ? k : 0)), "r"(on * 8) : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + 1032), "l"(xb + (on ? k : 0)), "r"(on * 8) : "memory");
+                }
+                asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+#pragma unroll 1
+                for (int i = 0; i < BATCH; ++i) {
+                    const unsigned char* at = mine_at + i * STEP_BYTES;
+                    const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + 512);
+                    const uint4 xv = *reinterpret_cast<const uint4*>(at + 1024);
+                    float r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) {       // hi, mid, lo
+                        const uint32_t a0 = pair_bf16(r[0], r[1]), a2 = pair_bf16(r[2], r[3]), a1 = pair_bf16(r[4], r[5]), a3 = pair_bf16(r[6], r[7]);
+                        if (p < 2) {
+                            r[0] -= low_of(a0); r[1] -= high_of(a0); r[2] -= low_of(a2); r[3] -= high_of(a2);
+                            r[4] -= low_of(a1); r[5] -= high_of(a1); r[6] -= low_of(a3); r[7] -= high_of(a3);
+                        }
+                        mma_bf16_f32(acc[0], a0, a1, a2, a3, xv.x, xv.y);
+                        if (g.n > 8) mma_bf16_f32(acc[1], a0, a1, a2, a3, xv.z, xv.w);
                     }
-                    mma_bf16_f32(acc[0], a0, a1, a2, a3, x0.x, x0.y);
-                    if (g.n > 8) mma_bf16_f32(acc[1], a0, a1, a2, a3, x1.x, x1.y);
+                    if (FP8) {
+                        big0 = max(big0, max(max((xv.x & 0x7fffu) << 16, xv.x & 0x7fff0000u), max((xv.y & 0x7fffu) << 16, xv.y & 0x7fff0000u)));
+                        big1 = max(big1, max(max((xv.z & 0x7fffu) << 16, xv.z & 0x7fff0000u), max((xv.w & 0x7fffu) << 16, xv.w & 0x7fff0000u)));
+                    }
                 }
             }
             float* mine = part + (warp * 16 + gr) * 16 + t4 * 2;
@@ -294,9 +257,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
                 }
             }
         }
+        if (FP8) {
+            if (gr < g.n) atomicMax(x_largest + gr, big0);
+            if (gr + 8 < g.n) atomicMax(x_largest + gr + 8, big1);
+        }
     }
     // ---- x as the products read it: into shared memory, or (rows too long for that) the cluster's own copy in memory, an eighth by every CTA ----
-    __syncthreads();        // (x_largest)
+    __syncthreads();        // (x_largest; the rings' bytes)
     {
         const int chunks = FP8 ? few_part_bytes(g.D) / 8 - 4 : (g.D + 63) / 64 * 8, step = XS ? FEW_THREADS : FEW_CLUSTER * FEW_THREADS;
 #pragma unroll 2
@@ -331,27 +298,67 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (no CTA has more to hand out behind this: one barrier does)
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
-    // ---- the choice: a warp per token ----
-    if (warp < g.n && g.keep == g.groups)
-        few_choose(logits + warp * g.E, reinterpret_cast<float*>(rings) + (size_t)warp * 2 * g.E, lane, g.E, g.top, g.scoring, g.correction, g.renorm, g.wscale,
-                   idx + warp * g.top, wts + warp * g.top);
-    else if (warp < g.n)
+    // ---- the choice ----
+    if (g.keep == g.groups) {
+        const int Ew = (g.E + 3) & ~3;
+        float* scores = reinterpret_cast<float*>(rings);                                        // [n][Ew]
+        uint32_t* keys = reinterpret_cast<uint32_t*>(scores + g.n * Ew);                        // [n][Ew]
+        if (warp < g.n) few_scores(logits + warp * g.E, scores + warp * Ew, keys + warp * Ew, lane, g.E, g.scoring, g.correction);
+        if (threadIdx.x < pairs) idx[threadIdx.x] = -1;
+        __syncthreads();
+        if (g.E <= FEW_RANK_EXPERTS) {
+            // a thread per token and expert counts the scores ahead of its own
+#pragma unroll 1
+            for (int i = threadIdx.x; i < g.n * Ew; i += FEW_THREADS) {
+                const int t = i / Ew, e = i - t * Ew;
+                const uint32_t* key = keys + t * Ew;
+                const uint32_t own = key[e];
+                int ahead = 0;
+#pragma unroll 2
+                for (int o = 0; o < Ew; o += 4) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(key + o);
+                    ahead += (v.x > own || (v.x == own && o < e)) + (v.y > own || (v.y == own && o + 1 < e)) + (v.z > own || (v.z == own && o + 2 < e)) +
+                             (v.w > own || (v.w == own && o + 3 < e));
+                }
+                if (own != 0 && ahead < g.top) idx[t * g.top + ahead] = e;
+            }
+        } else if (warp < g.n) {
+            few_search(keys + warp * Ew, lane, g.E, g.top, idx + warp * g.top);
+        }
+        __syncthreads();
+        if (warp < g.n) {
+            // the weights, summed in the order of the choice; fewer to choose from than `top`: the rest is expert 0 without a weight
+            const int e = lane < g.top ? idx[warp * g.top + lane] : -1;
+            const float w = e >= 0 ? scores[warp * Ew + e] : 0.0f;
+            float total = 0.0f;
+#pragma unroll 2
+            for (int k = 0; k < g.top; ++k) total += __shfl_sync(0xffffffffu, w, k);
+            if (lane < g.top) {
+                idx[warp * g.top + lane] = max(e, 0);
+                wts[warp * g.top + lane] = g.renorm || g.wscale != 1.0f ? w / (g.renorm ? total + 1e-20f : 1.0f) * g.wscale : w;
+            }
+        }
+    } else if (warp < g.n) {
         moe_route_warp(logits + warp * g.E, reinterpret_cast<float*>(rings) + (size_t)warp * 2 * (g.E + g.groups), lane, g.E, g.top, g.groups, g.keep, idx, wts,
                        (size_t)warp, g.scoring, g.correction, g.pair_sum, g.renorm, g.wscale);
+    }
     __syncthreads();
-    // ---- the experts that someone chose, in order, with their pairs (token * top + choice): a thread per expert ----
+    // ---- the experts that someone chose, in order, with their pairs (token * top + choice): a thread per expert counts, a thread per pair finds its place ----
     {
-        const int e = threadIdx.x;
-        int count = 0;
-        if (e < g.E) {
-            int p = 0;
+        const int e = threadIdx.x, mine = threadIdx.x < pairs ? idx[threadIdx.x] : -1;
+        int count = 0, before = 0;
 #pragma unroll 2
-            for (; p + 4 <= pairs; p += 4) {
-                const int4 v = *reinterpret_cast<const int4*>(idx + p);
-                count += (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
-            }
-            for (; p < pairs; ++p) count += idx[p] == e;
+        for (int p = 0; p + 4 <= pairs; p += 4) {
+            const int4 v = *reinterpret_cast<const int4*>(idx + p);
+            count += (v.x == e) + (v.y == e) + (v.z == e) + (v.w == e);
+            before += (v.x == mine && p < e) + (v.y == mine && p + 1 < e) + (v.z == mine && p + 2 < e) + (v.w == mine && p + 3 < e);
         }
+        for (int p = pairs & ~3; p < pairs; ++p) {
+            const int v = idx[p];
+            count += v == e;
+            before += v == mine && p < e;
+        }
+        if (e >= g.E) count = 0;
         const int parts = (count + FEW_ROWS - 1) / FEW_ROWS;
         int upto = count, parts_upto = parts;
 #pragma unroll
@@ -368,26 +375,21 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
         }
         __syncthreads();
         int first = upto - count, entry = parts_upto - parts;
-#pragma unroll 1
+#pragma unroll 4
         for (int w = 0; w < warp; ++w) {
             first += sums[w];
             entry += sums[FEW_WARPS + w];
         }
         if (threadIdx.x == FEW_THREADS - 1) sums[2 * FEW_WARPS] = entry + parts;
-        if (count > 0) {
-            for (int i = 0; i < parts; ++i) {
-                entries[3 * (entry + i)] = e;
-                entries[3 * (entry + i) + 1] = first + i * FEW_ROWS;
-                entries[3 * (entry + i) + 2] = min(FEW_ROWS, count - i * FEW_ROWS);
-            }
-            int left = count;
-#pragma unroll 1
-            for (int p = 0; left > 0; ++p)
-                if (idx[p] == e) {
-                    places[first++] = p;
-                    --left;
-                }
+        int32_t* firsts = reinterpret_cast<int32_t*>(rings) + 2 * FEW_TOKENS * FEW_MAX_EXPERTS;      // [E], behind the scores
+        if (e < g.E) firsts[e] = first;
+        for (int i = 0; i < parts; ++i) {
+            entries[3 * (entry + i)] = e;
+            entries[3 * (entry + i) + 1] = first + i * FEW_ROWS;
+            entries[3 * (entry + i) + 2] = min(FEW_ROWS, count - i * FEW_ROWS);
         }
+        __syncthreads();
+        if (mine >= 0) places[firsts[mine] + before] = threadIdx.x;
         __syncthreads();
     }
     const int n_entries = sums[2 * FEW_WARPS];
@@ -905,6 +907,7 @@ MM_EXPORT int mm_moe_few(const void* x, long long ldx, int n, int D, const void*
                "moe few: experts must split into equal runs, 0 < keep <= runs, and top fits into the kept runs");
     MM_REQUIRE(scoring == 0 || scoring == 1, "moe few: the scoring is 0 (softmax) or 1 (sigmoid)");
     // (the choice's scratch is what the rings and the sums take up later)
+    static_assert(4 * (2 * FEW_TOKENS * FEW_MAX_EXPERTS + FEW_MAX_EXPERTS) <= FEW_WARPS * FEW_RING * FEW_SLOT, "scores, their order and the experts' first places");
     MM_REQUIRE((size_t)n * 8 * (E + groups) <= (size_t)FEW_WARPS * FEW_RING * FEW_SLOT + 4 * FEW_WARPS * 16 * 16, "moe few: too many experts and runs of them");
     MM_REQUIRE(act >= 0 && act <= MM_GLU_GELU_TANH, "moe few: unknown activation");
     const bool fp8 = s_in != nullptr;
