@@ -6,8 +6,8 @@
 // A few tokens are bound by the chosen experts' matrices: each is read once, by mma.sync with 16 weight rows as the 16-row operand and the expert's
 // rows of x, found by their places, as its 8 (or twice 8) columns.  Nothing is sorted or copied.
 //
-// First launch, clusters of eight CTAs: every cluster makes all logits (an eighth of the router's rows each, handed round over distributed
-// shared memory), every CTA makes the choice and the list of experts with their tokens; then its share of the units of 8 gate and 8 up rows.
+// First launch, clusters of eight CTAs: every cluster makes all logits (an eighth of the router's rows each) and the choice (every eighth token each), handed
+// round over distributed shared memory; every CTA makes the list of experts with their tokens, then its share of the units of 8 gate and 8 up rows.
 // That costs a read of the router per cluster from L2 and saves a launch and its wait for another.
 // Second launch: 16 output columns a CTA; its warps share out the experts' runs of hidden columns, whose sums are kept apart per (token, choice) and added
 // in the order of the choice.  A token's output does not depend on the others: every sum is cut by the layer's sizes alone.
@@ -88,12 +88,27 @@ __device__ __forceinline__ void f16_of(uint32_t w, uint32_t& a, uint32_t& b) {
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(a), "=r"(b) : "r"(w));
 }
 
+// a word into the same place of a CTA of the cluster
+__device__ __forceinline__ void st_cluster(void* at, uint32_t cta, uint32_t v) {
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(cta));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_barrier() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // The power of two that brings a size to 2^to .. 2^(to + 1) (sizes next to the smallest normal number: as far as it goes), and its inverse; an infinity or
 // a NaN stays one under it.
 __device__ __forceinline__ int few_exponent(uint32_t size_bits) { return min(max((int)(size_bits >> 23), 16), 254); }
 __device__ __forceinline__ float few_scale(uint32_t size_bits, int to) { return __uint_as_float((uint32_t)(254 + to - few_exponent(size_bits)) << 23); }
 __device__ __forceinline__ float few_unscale(uint32_t size_bits, int to) { return __uint_as_float((uint32_t)(few_exponent(size_bits) - to) << 23); }
 constexpr int X_TO = 7, HIDDEN_TO = 14;
+
+static_assert(4 * (4 * (FEW_MAX_EXPERTS + FEW_MAX_TOP) + FEW_MAX_EXPERTS) <= FEW_WARPS * FEW_RING * FEW_SLOT && 2 * 8 * 2 * FEW_MAX_EXPERTS <= FEW_WARPS * FEW_RING * FEW_SLOT,
+              "the choice's scratch and the experts' first places stand where the rings start later");
 
 // moe_route_warp's scores (the same formula), and their order as numbers: 0 is not to be chosen (a NaN, minus infinity).  A warp; s, key: E words each.
 // (Code that runs once in a launch is fetched from L2 as it goes: short loops beat unrolled ones here.)
@@ -246,15 +261,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
                 float z = 0.0f;
 #pragma unroll
                 for (int w = 0; w < FEW_WARPS; ++w) z += part[(w * 16 + row) * 16 + tok];
-                if (e < g.E) {
-                    const uint32_t at = (uint32_t)__cvta_generic_to_shared(logits + tok * g.E + e);
-#pragma unroll
-                    for (int r = 0; r < FEW_CLUSTER; ++r) {
-                        uint32_t there;
-                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(r));
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(z) : "memory");
-                    }
-                }
+                if (e < g.E) st_cluster(logits + tok * g.E + e, tok % FEW_CLUSTER, __float_as_uint(z));      // to the CTA that chooses for the token
             }
         }
         if (FP8) {
@@ -294,22 +301,21 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
             }
         }
     }
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (no CTA has more to hand out behind this: one barrier does)
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-
-    // ---- the choice ----
+    cluster_barrier();
+    // ---- the choice, every eighth token here, for the whole cluster ----
+    const int own_tokens = ((int)g.n - (int)rank + FEW_CLUSTER - 1) / FEW_CLUSTER;             // tokens rank, rank + 8
     if (g.keep == g.groups) {
         const int Ew = (g.E + 3) & ~3;
-        float* scores = reinterpret_cast<float*>(rings);                                        // [n][Ew]
-        uint32_t* keys = reinterpret_cast<uint32_t*>(scores + g.n * Ew);                        // [n][Ew]
-        if (warp < g.n) few_scores(logits + warp * g.E, scores + warp * Ew, keys + warp * Ew, lane, g.E, g.scoring, g.correction);
-        if (threadIdx.x < pairs) idx[threadIdx.x] = -1;
+        float* scores = reinterpret_cast<float*>(rings);                                        // [2][Ew]
+        uint32_t* keys = reinterpret_cast<uint32_t*>(scores + 2 * Ew);                          // [2][Ew]
+        int32_t* chosen = reinterpret_cast<int32_t*>(keys + 2 * Ew);                            // [2][top]
+        if (warp < own_tokens) few_scores(logits + (rank + warp * FEW_CLUSTER) * g.E, scores + warp * Ew, keys + warp * Ew, lane, g.E, g.scoring, g.correction);
+        if (threadIdx.x < own_tokens * g.top) chosen[threadIdx.x] = -1;
         __syncthreads();
         if (g.E <= FEW_RANK_EXPERTS) {
-            // a thread per token and expert counts the scores ahead of its own
+            // a thread per token and expert counts the scores ahead of its own (equal ones of lower experts are)
 #pragma unroll 1
-            for (int i = threadIdx.x; i < g.n * Ew; i += FEW_THREADS) {
+            for (int i = threadIdx.x; i < own_tokens * Ew; i += FEW_THREADS) {
                 const int t = i / Ew, e = i - t * Ew;
                 const uint32_t* key = keys + t * Ew;
                 const uint32_t own = key[e];
@@ -317,32 +323,51 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
 #pragma unroll 2
                 for (int o = 0; o < Ew; o += 4) {
                     const uint4 v = *reinterpret_cast<const uint4*>(key + o);
-                    ahead += (v.x > own || (v.x == own && o < e)) + (v.y > own || (v.y == own && o + 1 < e)) + (v.z > own || (v.z == own && o + 2 < e)) +
-                             (v.w > own || (v.w == own && o + 3 < e));
+                    const uint32_t least = own - (o < e ? 1u : 0u);      // (own > 0 where it counts; the four beside e itself: below)
+                    ahead += (v.x > least) + (v.y > least) + (v.z > least) + (v.w > least);
                 }
-                if (own != 0 && ahead < g.top) idx[t * g.top + ahead] = e;
+                // the group of four around e was compared as if all of it stood before e: itself, and equals behind it, are taken back
+                if (own != 0) {
+                    if ((e & 3) != 0)
+                        for (int o = e; o < (e | 3) + 1; ++o) ahead -= key[o] == own;
+                    if (ahead < g.top) chosen[t * g.top + ahead] = e;
+                }
             }
-        } else if (warp < g.n) {
-            few_search(keys + warp * Ew, lane, g.E, g.top, idx + warp * g.top);
+        } else if (warp < own_tokens) {
+            few_search(keys + warp * Ew, lane, g.E, g.top, chosen + warp * g.top);
         }
         __syncthreads();
-        if (warp < g.n) {
+        if (warp < own_tokens) {
             // the weights, summed in the order of the choice; fewer to choose from than `top`: the rest is expert 0 without a weight
-            const int e = lane < g.top ? idx[warp * g.top + lane] : -1;
+            const int e = lane < g.top ? chosen[warp * g.top + lane] : -1;
             const float w = e >= 0 ? scores[warp * Ew + e] : 0.0f;
             float total = 0.0f;
 #pragma unroll 2
             for (int k = 0; k < g.top; ++k) total += __shfl_sync(0xffffffffu, w, k);
             if (lane < g.top) {
-                idx[warp * g.top + lane] = max(e, 0);
-                wts[warp * g.top + lane] = g.renorm || g.wscale != 1.0f ? w / (g.renorm ? total + 1e-20f : 1.0f) * g.wscale : w;
+                const int at = (rank + warp * FEW_CLUSTER) * g.top + lane;
+                const float weight = g.renorm || g.wscale != 1.0f ? w / (g.renorm ? total + 1e-20f : 1.0f) * g.wscale : w;
+#pragma unroll 1
+                for (int c = 0; c < FEW_CLUSTER; ++c) {
+                    st_cluster(idx + at, c, (uint32_t)max(e, 0));
+                    st_cluster(wts + at, c, __float_as_uint(weight));
+                }
             }
         }
-    } else if (warp < g.n) {
-        moe_route_warp(logits + warp * g.E, reinterpret_cast<float*>(rings) + (size_t)warp * 2 * (g.E + g.groups), lane, g.E, g.top, g.groups, g.keep, idx, wts,
-                       (size_t)warp, g.scoring, g.correction, g.pair_sum, g.renorm, g.wscale);
+    } else if (warp < own_tokens) {
+        const int t = rank + warp * FEW_CLUSTER;
+        int32_t* chosen = places + t * g.top;                   // (not in use yet)
+        float* weight = reinterpret_cast<float*>(entries) + t * g.top;
+        moe_route_warp(logits + t * g.E, reinterpret_cast<float*>(rings) + (size_t)warp * 2 * (g.E + g.groups), lane, g.E, g.top, g.groups, g.keep, places,
+                       reinterpret_cast<float*>(entries), (size_t)t, g.scoring, g.correction, g.pair_sum, g.renorm, g.wscale);
+        __syncwarp();
+        if (lane < g.top)
+            for (int c = 0; c < FEW_CLUSTER; ++c) {
+                st_cluster(idx + t * g.top + lane, c, (uint32_t)chosen[lane]);
+                st_cluster(wts + t * g.top + lane, c, __float_as_uint(weight[lane]));
+            }
     }
-    __syncthreads();
+    cluster_barrier();       // (nobody reaches into another CTA behind this)
     // ---- the experts that someone chose, in order, with their pairs (token * top + choice): a thread per expert counts, a thread per pair finds its place ----
     {
         const int e = threadIdx.x, mine = threadIdx.x < pairs ? idx[threadIdx.x] : -1;
@@ -381,7 +406,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
             entry += sums[FEW_WARPS + w];
         }
         if (threadIdx.x == FEW_THREADS - 1) sums[2 * FEW_WARPS] = entry + parts;
-        int32_t* firsts = reinterpret_cast<int32_t*>(rings) + 2 * FEW_TOKENS * FEW_MAX_EXPERTS;      // [E], behind the scores
+        int32_t* firsts = reinterpret_cast<int32_t*>(rings) + 4 * (FEW_MAX_EXPERTS + FEW_MAX_TOP);      // [E], behind the scores
         if (e < g.E) firsts[e] = first;
         for (int i = 0; i < parts; ++i) {
             entries[3 * (entry + i)] = e;
@@ -906,9 +931,6 @@ MM_EXPORT int mm_moe_few(const void* x, long long ldx, int n, int D, const void*
     MM_REQUIRE(groups > 0 && E % groups == 0 && keep > 0 && keep <= groups && top <= keep * (E / groups),
                "moe few: experts must split into equal runs, 0 < keep <= runs, and top fits into the kept runs");
     MM_REQUIRE(scoring == 0 || scoring == 1, "moe few: the scoring is 0 (softmax) or 1 (sigmoid)");
-    // (the choice's scratch is what the rings and the sums take up later)
-    static_assert(4 * (2 * FEW_TOKENS * FEW_MAX_EXPERTS + FEW_MAX_EXPERTS) <= FEW_WARPS * FEW_RING * FEW_SLOT, "scores, their order and the experts' first places");
-    MM_REQUIRE((size_t)n * 8 * (E + groups) <= (size_t)FEW_WARPS * FEW_RING * FEW_SLOT + 4 * FEW_WARPS * 16 * 16, "moe few: too many experts and runs of them");
     MM_REQUIRE(act >= 0 && act <= MM_GLU_GELU_TANH, "moe few: unknown activation");
     const bool fp8 = s_in != nullptr;
     MM_REQUIRE(fp8 == (s_out != nullptr) && !(fp8 && interleaved), "moe few: both matrices are in bf16 or both in 8 bits");
