@@ -51,6 +51,17 @@ __global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const T* __restrict
     }
 }
 
+// Quantised rows copied to other places: out row r is row source[r], numbers and scales.  A warp per row, 16 bytes a lane.
+__global__ void __launch_bounds__(256) fp8_gather_rows_kernel(const uint4* __restrict__ q, const float* __restrict__ s, const int32_t* __restrict__ source, uint4* __restrict__ oq,
+                                                              float* __restrict__ os, int rows, int pieces, int blocks) {
+    const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const size_t from = source[row];
+#pragma unroll 4
+    for (int i = lane; i < pieces; i += 32) oq[(size_t)row * pieces + i] = q[from * pieces + i];
+    for (int i = lane; i < blocks; i += 32) os[(size_t)row * blocks + i] = s[from * blocks + i];
+}
+
 // One CTA per block of 128 x 128: its largest number first, then the quotients (the block comes from L1 the second time).
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_quant_weight_kernel(const T* __restrict__ w, uint8_t* __restrict__ q, int ldq, float* __restrict__ scales,
@@ -107,6 +118,16 @@ int fp8_quant_rows(const void* x, int x_dtype, long long ldx, const int32_t* sou
 // source [rows] int32 or null: row r is made from row source[r] of x.
 MM_EXPORT int mm_fp8_quant_rows(const void* x, int x_dtype, long long ldx, const void* source, void* q, int ldq, void* scales, int rows, int K, void* stream) {
     return fp8_quant_rows(x, x_dtype, ldx, (const int32_t*)source, q, ldq, (float*)scales, rows, K, (cudaStream_t)stream);
+}
+
+// q [., ldq] e4m3 (ldq a multiple of 16) with scales fp32 [., blocks]: row r of the result is row source[r]
+MM_EXPORT int mm_fp8_gather_rows(const void* q, const void* scales, const void* source, void* out_q, void* out_scales, int rows, int ldq, int blocks, void* stream) {
+    MM_REQUIRE(rows >= 0 && ldq > 0 && ldq % 16 == 0 && blocks > 0 && (((uintptr_t)q | (uintptr_t)out_q) & 15) == 0, "fp8 rows: bad sizes");
+    if (rows == 0) return MM_OK;
+    mm_launch(fp8_gather_rows_kernel, dim3(ceil_div(rows, 8)), dim3(256), 0, (cudaStream_t)stream, (const uint4*)q, (const float*)scales, (const int32_t*)source,
+              (uint4*)out_q, (float*)out_scales, rows, ldq / 16, blocks);
+    MM_CHECK_LAUNCH();
+    return MM_OK;
 }
 
 // w [matrices, N, K] -> q [matrices, N, ldq] e4m3, scales fp32 [matrices, N / 128, K / 128] (both rounded up)

@@ -2240,7 +2240,11 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, wts: torch.Tensor, w_in:
     if n == 0:
         return torch.empty((0, d), dtype=torch.bfloat16, device=x.device)
     rows = moe_sort(idx, E, with_tiles=True)
-    sorted_x = quantize_fp8_rows(x, rows.row_token)
+    # every row quantised once, then copied to its experts' places
+    q = quantize_fp8_rows(x)
+    sorted_x = Fp8Rows(_fp8_buffer(n * top, d, device=x.device), torch.empty((n * top, _blocks(d)), dtype=torch.float32, device=x.device))
+    check(_lib.load().mm_fp8_gather_rows(q.values.data_ptr(), q.scales.data_ptr(), rows.row_token.data_ptr(), sorted_x.values.data_ptr(), sorted_x.scales.data_ptr(),
+                                         n * top, -(-d // 16) * 16, _blocks(d), _stream()), "gather_fp8_rows")
     on_input = weight_on == "input"
     hidden = Fp8Rows(_fp8_buffer(n * top, f, device=x.device), torch.empty((n * top, _blocks(f)), dtype=torch.float32, device=x.device))
     _fp8_grouped(sorted_x, w_in, rows, hidden.values, hidden.scales, act, limit, wts if on_input else None)

@@ -241,3 +241,21 @@ def test_refusals():
         with pytest.raises(KernelError):
             call()
             print("not refused:", i)
+
+
+@pytest.mark.parametrize("rows,top,experts", [(4095, 1, 64), (4096, 2, 64), (5001, 3, 7), (20000, 8, 300), (90000, 6, 128), (9000, 4, 1), (70000, 8, 600)])
+def test_rows_sorted_by_expert_over_a_cluster(rows, top, experts):
+    """many rows: the lists that torch's stable sort gives"""
+    from mimirmind_b200.kernels import ops
+    n = rows // top
+    gen = _gen(rows, top)
+    idx = (torch.randint(0, experts, (n, top), generator=gen, device=DEV) * torch.randint(0, 2, (n, top), generator=gen, device=DEV)).to(torch.int32)      # half on expert 0
+    got = ops.moe_sort(idx, experts, with_tiles=True)
+    flat = idx.flatten().long()
+    order = torch.sort(flat, stable=True).indices
+    counts = torch.bincount(flat, minlength=experts)
+    starts = torch.cumsum(counts, 0) - counts
+    assert torch.equal(got.order[:n * top].long(), order) and torch.equal(got.offsets[:-1].long(), starts) and int(got.offsets[-1]) == n * top
+    assert torch.equal(got.row_token.long(), order // top) and torch.equal(got.place.long()[order], torch.arange(n * top, device=DEV))
+    want = [(s + i, min(s + i + 128, s + c), e) for e, (s, c) in enumerate(zip(starts.tolist(), counts.tolist())) for i in range(0, c, 128)]
+    assert int(got.n_tiles) == len(want) and [tuple(t) for t in got.tiles[:len(want)].tolist()] == want
