@@ -60,7 +60,7 @@ struct Layout {
     static constexpr int STAGE_BYTES = HALF_BYTES * (1 + BN / 128);
     static constexpr int STAGES = BN == 256 ? 4 : 6;
     static constexpr int PIPE_BYTES = STAGES * STAGE_BYTES;
-    static constexpr int STAGING = 2048;           // per warp: 32 rows of 64 bytes
+    static constexpr int STAGING = 4096;           // per warp: 32 rows of 64 bytes, twice
     static constexpr int PART_LD = BN + 4;         // floats of a row of a split tile's sums
 };
 
@@ -100,6 +100,13 @@ __device__ __forceinline__ void tmem_wait32(uint32_t* r) {
                    "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
                    "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
                  :: "memory");
+}
+// the same as a wait, without the instruction: for a second load that the wait before covers
+__device__ __forceinline__ void tmem_arrived32(uint32_t* r) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
 }
 // two sums in one instruction: (a, b) += s (x, y), s = (s, s)
 __device__ __forceinline__ void fma_pair(uint64_t& ab, uint64_t s, uint32_t x, uint32_t y) {
@@ -152,7 +159,16 @@ __device__ __forceinline__ Tile tile_of(const Fp8Args& g, int t, int m_tiles) {
     return x;
 }
 
-// 64 bytes of 32 rows on their way to memory: 16-byte unit u of row r at u ^ (r / 2 & 3), so that neither side meets bank conflicts
+// acc[i] = act(acc[i], acc[N + i]): one kind of activation a loop, so that its exponentials and quotients overlap (with the choice inside, a tile's
+// end took 10,000 cycles)
+template <int ACT, int N>
+__device__ __forceinline__ void gated_half(float* acc, float rs, float limit) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = fp8_glu_as<ACT>(acc[i], acc[N + i], limit, rs);
+}
+
+// 64 bytes of 32 rows on their way to memory: 16-byte unit u of row r at u ^ (r / 2 & 3), so that neither side meets bank conflicts.  Two such
+// areas in turn: the wait of one round (in store_staged) tells that the round before has been read
 __device__ __forceinline__ unsigned char* staged(unsigned char* base, int r, int u) { return base + r * 64 + ((u ^ ((r >> 1) & 3)) << 4); }
 
 template <typename T>
@@ -172,7 +188,6 @@ __device__ __forceinline__ void store_staged(unsigned char* base, int lane, T* o
             if (row0 + r < hi && col0 + c < N) out[(size_t)(row0 + r) * ldo + col0 + c] = reinterpret_cast<const T*>(staged(base, r, c / UNIT))[c % UNIT];
         }
     }
-    __syncwarp();
 }
 
 template <int BN, bool GLU, bool SPLIT>
@@ -268,7 +283,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const int q = warp & 3, part = warp >> 2;
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
         unsigned char* wstage = staging + warp * L::STAGING;
-        uint32_t it = 0, local = 0;
+        uint32_t it = 0, local = 0, round = 0;
         bool ok = true;
         for (int t = first; t < total; t += step, ++local) {
             const Tile x = tile_of<BN, GLU>(g, t, m_tiles);
@@ -292,21 +307,27 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 if (!ok) break;
                 tc_fence_after();
                 if (threadIdx.x == 0) mbar_arrive(smem_u32(&ctl->empty[it % L::STAGES]));      // the block's products are through: so are its copies
-                // a piece is multiplied while the next is on its way; the accumulator is free once the last has arrived
+                // Two pieces are on their way at a time, and the wait is for both: what bounds the loop is how often a warp waits for tensor memory (one
+                // piece at a time: 960 cycles a block).  A piece's registers take the next one as soon as they are multiplied; the accumulator is free once the
+                // last two have arrived.
                 uint32_t r[2][PIECE];
                 tmem_ld32_issue(taddr + ph * BN + column(0, part), r[0]);
+                tmem_ld32_issue(taddr + ph * BN + column(1, part), r[1]);
 #pragma unroll
-                for (int c = 0; c < PIECES; ++c) {
-                    tmem_wait32(r[c & 1]);
-                    if (c + 1 < PIECES) {
-                        tmem_ld32_issue(taddr + ph * BN + column(c + 1, part), r[(c + 1) & 1]);
-                    } else {
+                for (int c = 0; c < PIECES; c += 2) {
+                    tmem_wait32(r[0]);
+                    tmem_arrived32(r[1]);
+                    if (c + 2 == PIECES) {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(smem_u32(&ctl->sum_empty[ph]));
                     }
 #pragma unroll
-                    for (int i = 0; i < PIECE; i += 2) fma_pair(sums[(c * PIECE + i) / 2], GLU && c >= PIECES / 2 ? s1 : s0, r[c & 1][i], r[c & 1][i + 1]);
+                    for (int d = 0; d < 2; ++d) {
+#pragma unroll
+                        for (int i = 0; i < PIECE; i += 2) fma_pair(sums[((c + d) * PIECE + i) / 2], GLU && c + d >= PIECES / 2 ? s1 : s0, r[d][i], r[d][i + 1]);
+                        if (c + 2 < PIECES) tmem_ld32_issue(taddr + ph * BN + column(c + 2 + d, part), r[d]);
+                    }
                 }
             }
             float acc[COLS];
@@ -330,11 +351,13 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             } else if (GLU) {
                 const float rs = g.row_scale && row < x.hi ? g.row_scale[g.order ? g.order[row] : row] : 1.0f;
                 const int n0 = x.n0 + part * (COLS / 2);
+                if (g.act == MM_GLU_SILU) gated_half<MM_GLU_SILU, COLS / 2>(acc, rs, g.limit);
+                else if (g.act == MM_GLU_CLAMPED) gated_half<MM_GLU_CLAMPED, COLS / 2>(acc, rs, g.limit);
+                else gated_half<MM_GLU_GELU_TANH, COLS / 2>(acc, rs, g.limit);
                 uint32_t largest = 0;
 #pragma unroll
                 for (int i = 0; i < COLS / 2; ++i) {
-                    const float h = fp8_glu(acc[i], acc[COLS / 2 + i], g.act, g.limit, rs);
-                    acc[i] = n0 + i < g.N ? h : 0.0f;
+                    if (n0 + i >= g.N) acc[i] = 0.0f;
                     largest = max(largest, fp8_size_bits(acc[i]));
                 }
                 // the other parts of the row's block are the warps' with the same rows
@@ -364,15 +387,15 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 }
                 if (g.out_kind == OUT_F32) {
 #pragma unroll
-                    for (int c = 0; c < COLS; c += 16) {
+                    for (int c = 0; c < COLS; c += 16, ++round) {
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
-                            *reinterpret_cast<float4*>(staged(wstage, lane, u)) = make_float4(acc[c + u * 4], acc[c + u * 4 + 1], acc[c + u * 4 + 2], acc[c + u * 4 + 3]);
-                        store_staged<float>(wstage, lane, (float*)g.out, g.ldo, x.m0 + q * 32, x.hi, x.n0 + part * COLS + c, g.N);
+                            *reinterpret_cast<float4*>(staged(wstage + (round & 1) * 2048, lane, u)) = make_float4(acc[c + u * 4], acc[c + u * 4 + 1], acc[c + u * 4 + 2], acc[c + u * 4 + 3]);
+                        store_staged<float>(wstage + (round & 1) * 2048, lane, (float*)g.out, g.ldo, x.m0 + q * 32, x.hi, x.n0 + part * COLS + c, g.N);
                     }
                 } else {
 #pragma unroll
-                    for (int c = 0; c < COLS; c += 32) {
+                    for (int c = 0; c < COLS; c += 32, ++round) {
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
                             uint32_t p[4];
@@ -381,9 +404,9 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                                 const __nv_bfloat162 v = __floats2bfloat162_rn(acc[c + u * 8 + 2 * j], acc[c + u * 8 + 2 * j + 1]);
                                 p[j] = *reinterpret_cast<const uint32_t*>(&v);
                             }
-                            *reinterpret_cast<uint4*>(staged(wstage, lane, u)) = make_uint4(p[0], p[1], p[2], p[3]);
+                            *reinterpret_cast<uint4*>(staged(wstage + (round & 1) * 2048, lane, u)) = make_uint4(p[0], p[1], p[2], p[3]);
                         }
-                        store_staged<__nv_bfloat16>(wstage, lane, (__nv_bfloat16*)g.out, g.ldo, x.m0 + q * 32, x.hi, x.n0 + part * COLS + c, g.N);
+                        store_staged<__nv_bfloat16>(wstage + (round & 1) * 2048, lane, (__nv_bfloat16*)g.out, g.ldo, x.m0 + q * 32, x.hi, x.n0 + part * COLS + c, g.N);
                     }
                 }
             }
