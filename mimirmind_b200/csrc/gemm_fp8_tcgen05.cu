@@ -8,7 +8,9 @@
 // per block of a 128 x 256 tile the products take 512 cycles and the sums 256 of each scheduler's, so the sums ride along.
 //
 // Roles: warps 0..7 sums and results, warps 8 and 11 TMA, warps 9 and 10 products, each of the two for every other block: one thread's waits and
-// issues take 960 cycles a block, a block's products 540.  A CTA walks over tiles, row tiles first, so that CTAs at work at
+// issues take 960 cycles a block, a block's products 540.  What bounds the loop now is the round of an accumulator: products 600 cycles, the wait for
+// them 200, reading 470, the next products' issue 350, for two blocks.  Pairs of CTAs (cta_group::2, 256 rows a tile, a third less traffic in shared memory) have
+// the same round, with or without the tile in halves, and were not faster (4,096 x 18,944 x 3,584: 281 and 295 us against 272).  A CTA walks over tiles, row tiles first, so that CTAs at work at
 // the same time share weight tiles in L2.  Few tiles: a cluster of S CTAs splits a tile's blocks; every CTA puts its sums into its own shared
 // memory, and after a cluster barrier each finishes every S-th row from all S in rank order (the same order on every run).
 //
@@ -56,10 +58,10 @@ struct Fp8Args {
     int M, N, K, KB, NB, ldo, S;
 };
 
-template <int BN, bool PAIR = false>
+template <int BN>
 struct Layout {
-    static constexpr int STAGE_BYTES = HALF_BYTES * (PAIR ? 2 : 1 + BN / 128);
-    static constexpr int STAGES = BN == 256 && !PAIR ? 4 : 6;
+    static constexpr int STAGE_BYTES = HALF_BYTES * (1 + BN / 128);
+    static constexpr int STAGES = BN == 256 ? 4 : 6;
     static constexpr int PIPE_BYTES = STAGES * STAGE_BYTES;
     static constexpr int STAGING = 4096;           // per warp: 32 rows of 64 bytes, twice
     static constexpr int PART_LD = BN + 4;         // floats of a row of a split tile's sums
@@ -74,8 +76,8 @@ struct Ctl {
 };
 static_assert(128 * Layout<256>::PART_LD * 4 <= Layout<256>::PIPE_BYTES && 128 * Layout<128>::PART_LD * 4 <= Layout<128>::PIPE_BYTES, "split sums");
 
-// fp32 accumulate, e4m3 x e4m3, both K-major
-__host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+// fp32 accumulate, e4m3 x e4m3, both K-major, M = 128
+__host__ __device__ constexpr uint32_t idesc_e4m3(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(T_ROWS >> 4) << 24); }
 
 __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -115,21 +117,6 @@ __device__ __forceinline__ void fma_pair(uint64_t& ab, uint64_t s, uint32_t x, u
 }
 __device__ __forceinline__ uint64_t twice(float s) { return ((uint64_t)__float_as_uint(s) << 32) | __float_as_uint(s); }
 
-// the same over both CTAs of a pair: each multiplies its own 128 rows of A with the 2 x 128 rows of W that the two hold
-__device__ __forceinline__ void umma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
-}
-
-// an arrival on another CTA's barrier that orders no memory: what it tells is that tensor memory has been read (wait::ld and the fence in front see to
-// that).  With .release it takes 1,100 cycles.
-__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar) {
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
 __device__ __forceinline__ float bias_at(const Fp8Args& g, int n) {
     return g.bias_dtype == MM_F32 ? ((const float*)g.bias)[n] : __bfloat162float(((const __nv_bfloat16*)g.bias)[n]);
 }
@@ -145,17 +132,17 @@ struct Tile {
     int m0, hi, n0, w0, w1;
     const float *s0, *s1;
 };
-template <int BN, bool GLU, bool PAIR>
-__device__ __forceinline__ Tile tile_of(const Fp8Args& g, int t, int m_tiles, int rank) {
+template <int BN, bool GLU>
+__device__ __forceinline__ Tile tile_of(const Fp8Args& g, int t, int m_tiles) {
     Tile x;
     const int mt = t % m_tiles, nt = t / m_tiles;
     int e = 0;
     if (g.tiles != nullptr) {
-        x.m0 = g.tiles[3 * mt] + (PAIR ? rank * T_ROWS : 0);
+        x.m0 = g.tiles[3 * mt];
         x.hi = g.tiles[3 * mt + 1];
         e = g.tiles[3 * mt + 2];
     } else {
-        x.m0 = (PAIR ? 2 * mt + rank : mt) * T_ROWS;
+        x.m0 = mt * T_ROWS;
         x.hi = g.M;
     }
     if (GLU) {
@@ -206,12 +193,11 @@ __device__ __forceinline__ void store_staged(unsigned char* base, int lane, T* o
     }
 }
 
-template <int BN, bool GLU, bool SPLIT, bool PAIR>
+template <int BN, bool GLU, bool SPLIT>
 __global__ void __launch_bounds__(T_THREADS, 1)
 gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Fp8Args g) {
     static_assert(!GLU || BN == 256, "a gated tile holds 128 columns of both matrices");
-    static_assert(!PAIR || (BN == 256 && !SPLIT), "a pair's tile has 256 columns");
-    typedef Layout<BN, PAIR> L;
+    typedef Layout<BN> L;
     constexpr int COLS = BN / 2, PIECES = COLS / PIECE;      // columns a thread sums
     extern __shared__ unsigned char smem_raw[];
     unsigned char* pipe = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -219,7 +205,6 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     Ctl* ctl = reinterpret_cast<Ctl*>(staging + SUM_WARPS * L::STAGING);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &ctl->abort_flag;
-    const uint32_t peer_abort = PAIR ? map_to_rank(smem_u32(&ctl->abort_flag), cluster_ctarank() ^ 1u) : 0u;
     // the tile's column of a thread's piece.  GLU: the first half of its sums is of the gate's columns, the second of the up projection's
     auto column = [](int c, int part) { return GLU ? (c < PIECES / 2 ? part * (COLS / 2) + c * PIECE : 128 + part * (COLS / 2) + (c - PIECES / 2) * PIECE) : part * COLS + c * PIECE; };
 
@@ -232,30 +217,26 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(smem_u32(&ctl->sum_full[a]), 1);
-            mbar_init(smem_u32(&ctl->sum_empty[a]), PAIR ? 2 * SUM_WARPS : SUM_WARPS);       // (a pair: the leader's, both CTAs' warps)
+            mbar_init(smem_u32(&ctl->sum_empty[a]), SUM_WARPS);
         }
         for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&ctl->row_known[q]), 2);
         ctl->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == SUM_WARPS + 1 && PAIR) {          // one warp of each CTA; both get the same columns
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)), "r"(2 * BN) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    } else if (warp == SUM_WARPS + 1) {
+    if (warp == SUM_WARPS + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)), "r"(2 * BN) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
-    if (PAIR) pair_sync();         // the peer's barriers exist before anything of this CTA signals them
     tc_fence_after();
     const uint32_t tmem_base = ctl->tmem_base;
 
-    const int m_tiles = g.tiles ? *g.n_tiles : (g.M + (PAIR ? 2 : 1) * T_ROWS - 1) / ((PAIR ? 2 : 1) * T_ROWS), n_tiles = (g.N + (GLU ? 128 : BN) - 1) / (GLU ? 128 : BN);
+    const int m_tiles = g.tiles ? *g.n_tiles : (g.M + T_ROWS - 1) / T_ROWS, n_tiles = (g.N + (GLU ? 128 : BN) - 1) / (GLU ? 128 : BN);
     const int total = m_tiles * n_tiles;
-    const int S = SPLIT ? g.S : 1, rank = SPLIT || PAIR ? (int)cluster_ctarank() : 0;
-    const int first = SPLIT ? blockIdx.x / S : PAIR ? blockIdx.x / 2 : blockIdx.x, step = SPLIT ? 0x40000000 : PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;      // a split tile has its cluster for itself
+    const int S = SPLIT ? g.S : 1, rank = SPLIT ? (int)cluster_ctarank() : 0;
+    const int first = SPLIT ? blockIdx.x / S : blockIdx.x, step = SPLIT ? 0x40000000 : (int)gridDim.x;      // a split tile has its cluster for itself
     const int b_lo = SPLIT ? (int)((long long)g.KB * rank / S) : 0, b_hi = SPLIT ? (int)((long long)g.KB * (rank + 1) / S) : g.KB;
 
     if (warp >= SUM_WARPS) {
@@ -266,49 +247,37 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 uint32_t it = 0;
                 bool ok = true;
                 for (int t = first; t < total && ok; t += step) {
-                    const Tile x = tile_of<BN, GLU, PAIR>(g, t, m_tiles, rank);
+                    const Tile x = tile_of<BN, GLU>(g, t, m_tiles);
                     for (int b = b_lo; b < b_hi; ++b, ++it) {
                         const int s = it % L::STAGES;
                         if ((it & 1) != turn) continue;
                         if (!mbar_wait(smem_u32(&ctl->empty[s]), ((it / L::STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
                         const uint32_t full = smem_u32(&ctl->full[s]), dst = smem_u32(pipe + s * L::STAGE_BYTES);
-                        if (PAIR) {          // this CTA's rows and its half of the weights' rows; all bytes are counted on the leader's barrier
-                            if (rank == 0) mbar_expect_tx(full, 2 * L::STAGE_BYTES);
-                            const uint32_t lead = map_to_rank(full, 0);
-                            tma_load_2d_pair(dst, &tmA, b * FP8_BLOCK, x.m0, lead);
-                            tma_load_2d_pair(dst + HALF_BYTES, &tmW, b * FP8_BLOCK, rank ? x.w1 : x.w0, lead);
-                            continue;
-                        }
                         mbar_expect_tx(full, L::STAGE_BYTES);
                         tma_load_2d(dst, &tmA, b * FP8_BLOCK, x.m0, full);
                         tma_load_2d(dst + HALF_BYTES, &tmW, b * FP8_BLOCK, x.w0, full);
                         if (BN == 256) tma_load_2d(dst + 2 * HALF_BYTES, &tmW, b * FP8_BLOCK, x.w1, full);
                     }
                 }
-                if (PAIR && !ok) st_cluster_u32(peer_abort, 1u);
             }
         } else {
-            if (lane == 0 && (!PAIR || rank == 0)) {
+            if (lane == 0) {
                 uint32_t it = 0;
                 bool ok = true;
                 for (int t = first; t < total && ok; t += step)
                     for (int b = b_lo; b < b_hi; ++b, ++it) {
                         const int s = it % L::STAGES, acc = it & 1;
                         if (acc != turn) continue;
-                        if (!mbar_wait(smem_u32(&ctl->sum_empty[acc]), ((it >> 1) & 1) ^ 1, abort_flag) ||
-                            !mbar_wait(smem_u32(&ctl->full[s]), (it / L::STAGES) & 1, abort_flag)) { ok = false; break; }
-                        tc_fence_after();
                         const uint32_t a_addr = smem_u32(pipe + s * L::STAGE_BYTES);
                         const uint64_t a_desc = smem_desc_sw128(a_addr, 16, 1024), b_desc = smem_desc_sw128(a_addr + HALF_BYTES, 16, 1024);
+                        if (!mbar_wait(smem_u32(&ctl->full[s]), (it / L::STAGES) & 1, abort_flag) ||
+                            !mbar_wait(smem_u32(&ctl->sum_empty[acc]), ((it >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {        // 32 numbers a product: 32 bytes on along the swizzled rows
-                            if (PAIR) umma_e4m3_pair(tmem_base + acc * BN, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc_e4m3(2 * T_ROWS, BN), k ? 1u : 0u);
-                            else umma_e4m3(tmem_base + acc * BN, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc_e4m3(T_ROWS, BN), k ? 1u : 0u);
-                        }
-                        if (PAIR) umma_commit_pair(smem_u32(&ctl->sum_full[acc]), 3);
-                        else umma_commit(smem_u32(&ctl->sum_full[acc]));
+                        for (int k = 0; k < 4; ++k)          // 32 numbers a product: 32 bytes on along the swizzled rows
+                            umma_e4m3(tmem_base + acc * BN, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc_e4m3(BN), k ? 1u : 0u);
+                        umma_commit(smem_u32(&ctl->sum_full[acc]));
                     }
-                if (PAIR && !ok) st_cluster_u32(peer_abort, 1u);
             }
         }
         if (SPLIT) {
@@ -323,7 +292,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         uint32_t it = 0, local = 0, round = 0;
         bool ok = true;
         for (int t = first; t < total; t += step, ++local) {
-            const Tile x = tile_of<BN, GLU, PAIR>(g, t, m_tiles, rank);
+            const Tile x = tile_of<BN, GLU>(g, t, m_tiles);
             const int row = x.m0 + q * 32 + lane;
             const float* sa = g.sa + (size_t)min(row, x.hi - 1) * g.KB;
             const float* sw = GLU || BN == 128 || part == 0 ? x.s0 : x.s1;
@@ -357,10 +326,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                     if (c + 2 == PIECES) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) {
-                            if (PAIR) mbar_arrive_relaxed(map_to_rank(smem_u32(&ctl->sum_empty[ph]), 0));
-                            else mbar_arrive(smem_u32(&ctl->sum_empty[ph]));
-                        }
+                        if (lane == 0) mbar_arrive(smem_u32(&ctl->sum_empty[ph]));
                     }
 #pragma unroll
                     for (int d = 0; d < 2; ++d) {
@@ -377,7 +343,6 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 acc[2 * i + 1] = __uint_as_float((uint32_t)(sums[i] >> 32));
             }
             if (!ok) {
-                if (PAIR && lane == 0) st_cluster_u32(peer_abort, 1u);
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) acc[i] = __uint_as_float(0x7fffffffu);
             }
@@ -456,7 +421,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             __syncwarp();
             pair_sync();               // every CTA's sums stand in its shared memory
             if (first < total) {
-                const Tile x = tile_of<BN, GLU, PAIR>(g, first, m_tiles, rank);
+                const Tile x = tile_of<BN, GLU>(g, first, m_tiles);
                 const uint32_t base = smem_u32(pipe);
                 const int rows = min(T_ROWS, x.hi - x.m0);
                 for (int r = rank + S * warp; r < rows; r += S * SUM_WARPS) {
@@ -513,22 +478,20 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     }
     tc_fence_before();
     __syncthreads();
-    if (SPLIT || PAIR) pair_sync();        // nobody leaves, or gives its tensor memory back, while another may read its shared memory or signal it
+    if (SPLIT) pair_sync();        // nobody leaves while another may read its shared memory
     tc_fence_after();
     if (threadIdx.x == 0 && ctl->abort_flag && g.err != nullptr) atomicExch(g.err, 1);
-    if (warp == SUM_WARPS + 1 && PAIR) {
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN) : "memory");
-    } else if (warp == SUM_WARPS + 1) {
+    if (warp == SUM_WARPS + 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN) : "memory");
     }
 }
 
-template <int BN, bool GLU, bool SPLIT, bool PAIR = false>
+template <int BN, bool GLU, bool SPLIT>
 int launch(const CUtensorMap& a, const CUtensorMap& w, const Fp8Args& g, int grid, cudaStream_t s) {
-    typedef Layout<BN, PAIR> L;
+    typedef Layout<BN> L;
     constexpr size_t smem = (size_t)L::PIPE_BYTES + SUM_WARPS * L::STAGING + 1024 + sizeof(Ctl);
     static_assert(smem <= 227 * 1024, "shared memory");
-    if (!mm_allow_smem<gemm_fp8_tcgen05_kernel<BN, GLU, SPLIT, PAIR>>(smem)) {
+    if (!mm_allow_smem<gemm_fp8_tcgen05_kernel<BN, GLU, SPLIT>>(smem)) {
         mm_set_last_error("gemm_fp8: cannot reserve shared memory");
         return MM_ERR_LAUNCH;
     }
@@ -536,7 +499,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& w, const Fp8Args& g, int gri
         static std::atomic<int> regs{0};          // a register split above what the block starts with would never be granted
         if (regs.load(std::memory_order_relaxed) == 0) {
             cudaFuncAttributes at;
-            if (cudaFuncGetAttributes(&at, gemm_fp8_tcgen05_kernel<BN, GLU, SPLIT, PAIR>) != cudaSuccess) {
+            if (cudaFuncGetAttributes(&at, gemm_fp8_tcgen05_kernel<BN, GLU, SPLIT>) != cudaSuccess) {
                 mm_set_last_error("gemm_fp8: cannot read the kernel's attributes");
                 return MM_ERR_LAUNCH;
             }
@@ -551,11 +514,11 @@ int launch(const CUtensorMap& a, const CUtensorMap& w, const Fp8Args& g, int gri
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = SPLIT ? g.S : 2;
+    attr[0].val.clusterDim.x = SPLIT ? g.S : 1;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = SPLIT || PAIR ? 1 : 0;
-    cudaLaunchKernelEx(&cfg, gemm_fp8_tcgen05_kernel<BN, GLU, SPLIT, PAIR>, a, w, g);
+    cfg.numAttrs = SPLIT ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, gemm_fp8_tcgen05_kernel<BN, GLU, SPLIT>, a, w, g);
     MM_CHECK_LAUNCH();
     return MM_OK;
 }
@@ -576,7 +539,7 @@ bool make_map_bytes(CUtensorMap* map, const void* base, long long rows, int cols
 
 // A e4m3 [M, lda], sa fp32 [M, KB]; W e4m3 [matrices * N, ldw], sw fp32 [matrices, NB, KB] (GLU: pairs of matrices, gate and up).
 // glu 0: out [M, ldo] bf16 or fp32 (+ bias [N]); glu 1: out e4m3 [M, ldo] (ldo = N rounded up to 16) and out_scales fp32 [M, NB].
-// tiles, n_tiles, max_tiles: the grouped form's row tiles.  wide: 256 columns a tile instead of 128 (GLU: always), 2: and 256 rows, a pair of CTAs.  splits: CTAs that share a tile's
+// tiles, n_tiles, max_tiles: the grouped form's row tiles.  wide: 256 columns a tile instead of 128 (GLU: always).  splits: CTAs that share a tile's
 // blocks (1, 2, 4 or 8; only without a list).
 MM_EXPORT int mm_gemm_fp8_tcgen05(const void* A, long long lda, const void* sa, const void* W, long long ldw, const void* sw, int matrices, void* out,
                                   int out_dtype, void* out_scales, int ldo, const void* bias, int bias_dtype, int M, int N, int K, int glu, int act, float limit,
@@ -620,16 +583,10 @@ MM_EXPORT int mm_gemm_fp8_tcgen05(const void* A, long long lda, const void* sa, 
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const bool pair = wide == 2;
-    MM_REQUIRE(!pair || splits == 1, "gemm_fp8: a pair of CTAs does not split a tile's blocks");
     const int bn = glu ? 128 : (wide ? 256 : 128);
-    const long long total = (long long)(tiles ? max_tiles : ceil_div(M, pair ? 2 * T_ROWS : T_ROWS)) * ceil_div(N, bn);
-    MM_REQUIRE(total < 0x3fffffffLL, "gemm_fp8: too many tiles");
+    const long long total = (long long)(tiles ? max_tiles : ceil_div(M, T_ROWS)) * ceil_div(N, bn);
+    MM_REQUIRE(total < 0x40000000LL, "gemm_fp8: too many tiles");
     cudaStream_t s = (cudaStream_t)stream;
-    if (pair) {
-        const int grid = 2 * (int)(total < sms / 2 ? total : sms / 2);
-        return glu ? launch<256, true, false, true>(ta, tw, g, grid, s) : launch<256, false, false, true>(ta, tw, g, grid, s);
-    }
     const int grid = splits > 1 ? (int)total * splits : (int)(total < sms ? total : sms);
     if (glu) return splits > 1 ? launch<256, true, true>(ta, tw, g, grid, s) : launch<256, true, false>(ta, tw, g, grid, s);
     if (wide) return splits > 1 ? launch<256, false, true>(ta, tw, g, grid, s) : launch<256, false, false>(ta, tw, g, grid, s);
@@ -658,8 +615,8 @@ int resident_clusters(int S) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int found = 0;
-    if (mm_allow_smem<gemm_fp8_tcgen05_kernel<BN, GLU, true, false>>(smem) &&
-        cudaOccupancyMaxActiveClusters(&found, gemm_fp8_tcgen05_kernel<BN, GLU, true, false>, &cfg) == cudaSuccess && found > 0) n = found;
+    if (mm_allow_smem<gemm_fp8_tcgen05_kernel<BN, GLU, true>>(smem) &&
+        cudaOccupancyMaxActiveClusters(&found, gemm_fp8_tcgen05_kernel<BN, GLU, true>, &cfg) == cudaSuccess && found > 0) n = found;
     else (void)cudaGetLastError();
     known[S].store(n, std::memory_order_relaxed);
     return n;
@@ -667,7 +624,7 @@ int resident_clusters(int S) {
 
 }  // namespace
 
-// The tile's width and the number of CTAs to a tile with the least estimated time: rounds of tiles x (a start and an end + blocks x 0.5 us, 0.58 of
+// The tile's width and the number of CTAs to a tile with the least estimated time: rounds of tiles x (a start and an end + blocks x 0.4 us, 0.58 of
 // 256 columns), as measured with 4 to 100 rows.  Us estimated and measured: 16 x 3,584 x 18,944 in 128 columns and 4 CTAs 22 and 23, in 2 CTAs 40
 // and 39, in 8 (two rounds) 26 and 29; 16 x 18,944 x 3,584 in 256 columns and 2 CTAs 12 and 19 (the weights' way from memory is 10), in 128 columns and one 16 and 22.
 int fp8_gemm(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, int* err, cudaStream_t s) {
@@ -679,19 +636,13 @@ int fp8_gemm(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, int* 
         for (int splits = 1; splits <= 8 && splits <= blocks; splits *= 2) {
             const long long tiles = m_tiles * ceil_div(w.N, glu || !wide ? 128 : 256);
             const int fit = splits == 1 ? FP8_SM_COUNT : glu ? resident_clusters<256, true>(splits) : wide ? resident_clusters<256, false>(splits) : resident_clusters<128, false>(splits);
-            const float us = (float)((tiles + fit - 1) / fit) * ((splits > 1 ? (wide ? 4.0f + 4.0f * rows : 3.0f + 2.0f * rows) : 2.0f) + (float)((blocks + splits - 1) / splits) * (wide ? 0.58f : 0.5f));
+            const float us = (float)((tiles + fit - 1) / fit) * ((splits > 1 ? (wide ? 4.0f + 4.0f * rows : 3.0f + 2.0f * rows) : 2.0f) + (float)((blocks + splits - 1) / splits) * (wide ? 0.58f : 0.4f));
             if (us < best) {
                 best = us;
                 best_wide = wide;
                 best_splits = splits;
             }
         }
-    // a pair of CTAs on 256 rows: each fetches half of the weights' rows, and its blocks take 0.33 us
-    const long long pairs = (long long)ceil_div(x.rows, 2 * T_ROWS) * ceil_div(w.N, glu ? 128 : 256);
-    if ((float)((pairs + FP8_SM_COUNT / 2 - 1) / (FP8_SM_COUNT / 2)) * (2.5f + (float)blocks * 0.33f) < best) {
-        best_wide = 2;
-        best_splits = 1;
-    }
     return mm_gemm_fp8_tcgen05(x.data, x.ld, x.scales, w.values, w.ld, w.scales, w.matrices, out.data, out.dtype, out.scales, out.ld, out.bias, out.bias_dtype,
                                x.rows, w.N, w.K, glu, out.act, out.limit, nullptr, nullptr, nullptr, nullptr, 0, best_wide, best_splits, err, s);
 }

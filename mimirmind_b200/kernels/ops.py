@@ -1326,19 +1326,19 @@ class ExpertRows:
     place: Optional[torch.Tensor] = None
 
 
-def moe_sort(idx: torch.Tensor, experts: int, with_tiles: bool = False, tile_rows: int = MOE_TILE_ROWS) -> ExpertRows:
-    """Rows (token * top + choice) put side by side by expert, in their order within an expert.  ``tile_rows``: of a tile, at the most."""
+def moe_sort(idx: torch.Tensor, experts: int, with_tiles: bool = False) -> ExpertRows:
+    """Rows (token * top + choice) put side by side by expert, in their order within an expert."""
     _need(idx, "expert choice", torch.int32)
     rows, top = idx.numel(), idx.shape[-1]
     dev = idx.device
     out = ExpertRows(torch.empty((experts + 1,), dtype=torch.int32, device=dev), torch.empty((max(rows, 1),), dtype=torch.int32, device=dev))
     if with_tiles:
-        out.max_tiles = -(-rows // tile_rows) + experts
+        out.max_tiles = -(-rows // MOE_TILE_ROWS) + experts
         out.tiles = torch.empty((out.max_tiles, 3), dtype=torch.int32, device=dev)
         out.n_tiles = torch.empty((1,), dtype=torch.int32, device=dev)
         out.row_token = torch.empty((max(rows, 1),), dtype=torch.int32, device=dev)
         out.place = torch.empty((max(rows, 1),), dtype=torch.int32, device=dev)
-    check(_lib.load().mm_moe_sort(idx.data_ptr(), rows, int(experts), out.offsets.data_ptr(), out.order.data_ptr(), int(top), int(tile_rows),
+    check(_lib.load().mm_moe_sort(idx.data_ptr(), rows, int(experts), out.offsets.data_ptr(), out.order.data_ptr(), int(top), MOE_TILE_ROWS,
                                   _ptr(out.tiles), _ptr(out.n_tiles), _ptr(out.row_token), _ptr(out.place), _stream()), "moe_sort")
     return out
 
@@ -2002,7 +2002,6 @@ def qk_prep(rows: torch.Tensor, q_off: int, k_off: int, v_off: int, q_norm: Opti
 
 
 # ---- layer weights in 8 bits (csrc/fp8.cuh has the formulas) ---------------------------------------------------------------
-FP8_PAIR_ROWS = 200       # (token, choice) rows an expert from which the grouped products run on pairs of CTAs, 256 rows a tile
 FP8_BLOCK = 128           # numbers of a row, and rows and columns of a weight, that share a scale
 _E4M3 = torch.float8_e4m3fn
 
@@ -2174,13 +2173,13 @@ def gemm_fp8(x, w: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: to
 
 
 def _fp8_grouped(x: Fp8Rows, w: Fp8Weight, rows: "ExpertRows", out: torch.Tensor, out_scales: Optional[torch.Tensor], act: int = 0, limit: float = 0.0,
-                 row_scale: Optional[torch.Tensor] = None, pair: bool = False) -> None:
-    """Row tiles of ``rows.tiles`` (``pair``: of up to 256 rows) times their expert's matrix; with ``out_scales`` its pair of matrices, act(gate, up) quantised."""
+                 row_scale: Optional[torch.Tensor] = None) -> None:
+    """Row tiles of ``rows.tiles`` times their expert's matrix; with ``out_scales`` its pair of matrices, act(gate, up) quantised."""
     n, k = w.shape[-2:]
     check(_lib.load().mm_gemm_fp8_tcgen05(x.values.data_ptr(), x.ld, x.scales.data_ptr(), w.values.data_ptr(), w.ld, w.scales.data_ptr(), w.matrices,
                                           out.data_ptr(), F32 if out.dtype == torch.float32 else BF16, _ptr(out_scales), out.stride(0), None, F32, x.shape[0], n, k,
                                           int(out_scales is not None), act, float(limit), _ptr(row_scale), rows.order.data_ptr(), rows.tiles.data_ptr(),
-                                          rows.n_tiles.data_ptr(), rows.max_tiles, 2 if pair else 1, 1, tcgen05_error_flag(w.values.device).data_ptr(), _stream()), "gemm_fp8")
+                                          rows.n_tiles.data_ptr(), rows.max_tiles, 1, 1, tcgen05_error_flag(w.values.device).data_ptr(), _stream()), "gemm_fp8")
 
 
 def _glu_code(activation: str, limit: float, what: str) -> int:
@@ -2240,8 +2239,7 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, wts: torch.Tensor, w_in:
     top = idx.shape[1]
     if n == 0:
         return torch.empty((0, d), dtype=torch.bfloat16, device=x.device)
-    pair = n * top >= FP8_PAIR_ROWS * E
-    rows = moe_sort(idx, E, with_tiles=True, tile_rows=256 if pair else 128)
+    rows = moe_sort(idx, E, with_tiles=True)
     # every row quantised once, then copied to its experts' places
     q = quantize_fp8_rows(x)
     sorted_x = Fp8Rows(_fp8_buffer(n * top, d, device=x.device), torch.empty((n * top, _blocks(d)), dtype=torch.float32, device=x.device))
@@ -2249,9 +2247,9 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, wts: torch.Tensor, w_in:
                                          n * top, -(-d // 16) * 16, _blocks(d), _stream()), "gather_fp8_rows")
     on_input = weight_on == "input"
     hidden = Fp8Rows(_fp8_buffer(n * top, f, device=x.device), torch.empty((n * top, _blocks(f)), dtype=torch.float32, device=x.device))
-    _fp8_grouped(sorted_x, w_in, rows, hidden.values, hidden.scales, act, limit, wts if on_input else None, pair)
+    _fp8_grouped(sorted_x, w_in, rows, hidden.values, hidden.scales, act, limit, wts if on_input else None)
     y = torch.empty((n * top, d), dtype=torch.float32, device=x.device)
-    _fp8_grouped(hidden, w_out, rows, y, None, pair=pair)
+    _fp8_grouped(hidden, w_out, rows, y, None)
     return moe_combine(y, None if on_input else wts, torch.bfloat16, place=rows.place, top=top)
 
 
