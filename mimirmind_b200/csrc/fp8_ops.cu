@@ -16,6 +16,10 @@ long long scratch_bytes(int m, int K) { return m * row_bytes(K) + (4LL * m * cei
 // x as e4m3 rows, in `scratch` if it has to be quantised by a launch; `dependent`: whether that launch was made
 int quantised(Fp8In& x, int K, bool glu, unsigned char* scratch, bool& dependent, cudaStream_t s) {
     if (x.dtype == FP8_QUANTISED || ((long long)x.rows * K <= INSIDE_NUMBERS && fp8_gemv_takes(x.rows, K, glu, true))) return MM_OK;
+    if (scratch == nullptr) {
+        mm_set_last_error("fp8 product: rows of this size need scratch to be quantised in");
+        return MM_ERR_BAD_ARG;
+    }
     float* scales = (float*)(scratch + x.rows * row_bytes(K));
     const int rc = fp8_quant_rows(x.data, x.dtype, x.ld, nullptr, scratch, (int)row_bytes(K), scales, x.rows, K, s);
     x = {scratch, scales, row_bytes(K), FP8_QUANTISED, x.rows};
@@ -30,7 +34,8 @@ int product(const Fp8In& x, const Fp8Mat& w, const Fp8Out& o, bool glu, bool dep
 }  // namespace
 
 // x [m, ldx] bf16 or fp32, or e4m3 with x_scales (dtype 2); W e4m3 [N, ldw], w_scales; bias [N] or null; out [m, N] bf16 or fp32.
-// scratch: m * (K rounded up to 16) + 4 m (K / 128 rounded up) bytes, rounded up to 16 (not read for e4m3 rows).
+// scratch: m * (K rounded up to 16) + 4 m (K / 128 rounded up) bytes, rounded up to 16 (may be null for e4m3
+// rows and for up to 16 rows of 4,096 numbers together).
 MM_EXPORT int mm_fp8_linear(const void* x, int x_dtype, long long ldx, const void* x_scales, int m, const void* W, long long ldw, const void* w_scales, int N, int K,
                             const void* bias, int bias_dtype, void* out, int out_dtype, void* scratch, void* err, void* stream) {
     MM_REQUIRE(m >= 0 && N > 0 && K > 0, "fp8 product: bad sizes");

@@ -2142,6 +2142,7 @@ def _fp8_input(x, k: int, what: str):
 
 
 _FP8_QUANTISED = 2
+FP8_INSIDE = 4096         # numbers of up to 16 rows that the weight-streaming product quantises itself (csrc/fp8_ops.cu has the same)
 
 
 def _fp8_scratch(m: int, k: int) -> int:
@@ -2164,8 +2165,9 @@ def gemm_fp8(x, w: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: to
     ptr, code, ld, scales, m = _fp8_input(x, k, "gemm_fp8")
     dev = w.values.device
     out_code = dtype_code(out_dtype)
-    out = torch.empty((m, n), dtype=out_dtype, device=dev)
-    scratch = None if code == _FP8_QUANTISED else torch.empty(_fp8_scratch(m, k), dtype=torch.uint8, device=dev)
+    # (a tensor's own new_empty is the cheaper call, and a few numbers are quantised without scratch: small products wait for the host)
+    out = x.new_empty((m, n)) if code == out_code and code != _FP8_QUANTISED else torch.empty((m, n), dtype=out_dtype, device=dev)
+    scratch = None if code == _FP8_QUANTISED or (m <= 16 and m * k <= FP8_INSIDE) else torch.empty(_fp8_scratch(m, k), dtype=torch.uint8, device=dev)
     check(_lib.load().mm_fp8_linear(ptr, code, ld, scales, m, w.values.data_ptr(), w.ld, w.scales.data_ptr(), n, k, _ptr(bias),
                                     F32 if bias is None else dtype_code(bias.dtype), out.data_ptr(), out_code, _ptr(scratch),
                                     tcgen05_error_flag(dev).data_ptr(), _stream()), "gemm_fp8")
@@ -2201,7 +2203,7 @@ def glu_mlp_fp8(x, w_in: Fp8Weight, w_out: Fp8Weight, activation: str = "silu", 
     _here("glu_mlp_fp8", w_in.values, w_out.values)
     ptr, code, ld, scales, m = _fp8_input(x, k, "glu_mlp_fp8")
     d, dev = w_out.shape[0], w_in.values.device
-    out = torch.empty((m, d), dtype=torch.bfloat16, device=dev)
+    out = x.new_empty((m, d)) if code == BF16 else torch.empty((m, d), dtype=torch.bfloat16, device=dev)
     scratch = torch.empty(_fp8_scratch(m, k) + _fp8_scratch(m, f), dtype=torch.uint8, device=dev)
     check(_lib.load().mm_fp8_glu_mlp(ptr, code, ld, scales, m, w_in.values.data_ptr(), w_in.ld, w_in.scales.data_ptr(), f, k, w_out.values.data_ptr(), w_out.ld,
                                      w_out.scales.data_ptr(), d, act, float(limit), out.data_ptr(), scratch.data_ptr(),
@@ -2304,7 +2306,7 @@ def moe_few(x: torch.Tensor, w_router: torch.Tensor, w_in, w_out, top: int, grou
             raise KernelError("moe_few: one correction per expert is needed")
     act = _glu_code(activation, limit, "moe_few")
     _here("moe_few", x, w_router, correction, *tensors)
-    out = torch.empty((n, d), dtype=torch.bfloat16, device=x.device)
+    out = x.new_empty((n, d))
     scratch = torch.empty(n * top * (4 * f + f // 2 + 24) + 32 + 36 * n * (d + 160), dtype=torch.uint8, device=x.device)
     check(_lib.load().mm_moe_few(x.data_ptr(), x.stride(0), n, d, w_router.data_ptr(), E, int(top), int(groups), int(keep), ROUTER_SCORINGS[scoring], _ptr(correction),
                                  GROUP_SCORES[group_score], int(scoring == "softmax" if renorm is None else renorm), float(scale), tensors[0].data_ptr(), _ptr(tensors[1]),
