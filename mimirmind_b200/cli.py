@@ -5,6 +5,7 @@ Option names, meanings and defaults are the reference's where it has them
 (default ./config.json, a hard error if the file is missing), ``--model PATH`` (overrides the
 default model's path), ``--prompt``, ``--max-new N`` (20), ``--temperature F`` (0 = greedy),
 ``--top-k N`` (0 off), ``--top-p F`` (1.0 off), ``--seed N`` (0 = random), ``--log-level``, ``--dump-dir``.
+``--weights fp8`` holds the gated feed-forwards' and experts' matrices in 8 bits.
 This engine has no tokenizer (it takes token ids), so ``--prompt`` is a list of ids
 ("5 17 3" or "5,17,3"), as the reference's parity tool takes ``--tokens id,id,…``
 (tools/llama-parity-dump.cpp:111-124); ``--prompt-len N`` makes N seeded random ids instead.
@@ -64,6 +65,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--top-p", type=float, default=1.0, help="top-P cutoff, 1.0 = disabled (default 1.0)")
     ap.add_argument("--seed", type=int, default=0, help="RNG seed, 0 = random (default 0)")
     ap.add_argument("--dtype", default="", choices=["", "bfloat16", "float32"], help="overrides runtime.dtype")
+    ap.add_argument("--weights", default="stored", choices=["stored", "fp8"], help="fp8: feed-forward and expert matrices in 8 bits (with bfloat16)")
     ap.add_argument("--log-level", default="info", choices=["trace", "debug", "info", "warn", "error", "off"])
     ap.add_argument("--dump-dir", default="", help="directory for per-stage dumps of the prefill (sets diagnostics.parityDump to DIR/engine)")
     # replay mode
@@ -120,7 +122,13 @@ def main(argv: Optional[List[str]] = None) -> int:
 
     log = (lambda m: print(m, file=sys.stderr, flush=True)) if args.log_level in ("trace", "debug", "info") else (lambda m: None)
     log(f"loading model '{cfg.model().id}' ({cfg.runtime.dtype})")
-    engine = Engine.from_config(cfg)
+    try:
+        engine = Engine.from_config(cfg, weights=args.weights)
+    except ValueError as e:
+        if args.weights == "stored":
+            raise
+        print(f"error: {e}", file=sys.stderr)
+        return 2
     vocab = engine.model.spec.vocab_size
     if args.prompt_len > 0:
         prompt = np.random.RandomState(args.seed or 1234).randint(0, vocab, size=args.prompt_len).tolist()

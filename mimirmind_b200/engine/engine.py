@@ -76,11 +76,14 @@ class Engine:
         (the weights are loaded), less what a step of ``token_budget`` tokens needs, at most
         ``max_context x max_active`` tokens."""
         from ..cache import sizing
+        from ..parts.moe import fp8_step_bytes
         from ..weights.store import layer_scratch_bytes, layer_tensor_shapes
         esz = 4 if model.rt.dtype == torch.float32 else 2
         shapes = layer_tensor_shapes(model.spec)
         free, _total = torch.cuda.mem_get_info(model.rt.device)
         scratch = layer_scratch_bytes(model.spec, token_budget + max_active, max_active, esz)
+        if model.rt.weights == "fp8":
+            scratch += fp8_step_bytes(model.spec, token_budget + max_active)
         return sizing.pool_tokens(free, fraction, sizing.step_reserve_bytes(model.spec, shapes, esz, token_budget, max_active, scratch),
                                   sizing.cache_bytes_per_token(model.cache_groups(), esz), page_size, max_context, max_active)
 
@@ -94,22 +97,23 @@ class Engine:
 
     # ---- construction ----------------------------------------------------------------
     @classmethod
-    def from_folder(cls, model_dir: str, dtype: str = "bfloat16", **kw) -> "Engine":
-        model, _ = load_model(model_dir, dtype)
+    def from_folder(cls, model_dir: str, dtype: str = "bfloat16", weights: str = "stored", **kw) -> "Engine":
+        """``weights`` ``fp8`` (with bfloat16): the gated feed-forwards' and gated experts' matrices in 8 bits, quantised as they are loaded."""
+        model, _ = load_model(model_dir, dtype, weights=weights)
         return cls(model, **kw)
 
     @classmethod
-    def from_config(cls, cfg, model_id: Optional[str] = None) -> "Engine":
-        """From an :class:`EngineConfig` (the JSON file of the command line)."""
+    def from_config(cls, cfg, model_id: Optional[str] = None, weights: str = "stored") -> "Engine":
+        """From an :class:`EngineConfig` (the JSON file of the command line); ``weights`` as for :meth:`from_folder`."""
         from ..registry import get_architecture
         entry = cfg.model(model_id)
         if entry.random:
             from ..registry import architecture_name
             arch = get_architecture(architecture_name(entry.random["config"]))
             spec = arch.build_spec(arch.parse_config(entry.random["config"], f"models[{entry.id}].random.config"))
-            model = random_model(spec, int(entry.random.get("seed", 0)), cfg.runtime.dtype)
+            model = random_model(spec, int(entry.random.get("seed", 0)), cfg.runtime.dtype, weights=weights)
         else:
-            model, _ = load_model(entry.path, cfg.runtime.dtype)
+            model, _ = load_model(entry.path, cfg.runtime.dtype, weights=weights)
         eng = cls(model, page_size=cfg.serving.blockSize, cache_tokens=cfg.runtime.cacheTokens,
                   max_context=cfg.runtime.maxContextTokens, token_budget=cfg.serving.tokenBudget,
                   max_active=cfg.serving.maxActiveRequests, prefill_chunk=cfg.serving.prefillChunk,

@@ -18,29 +18,37 @@ def require_cuda() -> torch.device:
     return torch.device("cuda", torch.cuda.current_device())
 
 
-def make_runtime(dtype, device=None, matmul: str = "auto") -> Runtime:
+WEIGHT_FORMS = ("stored", "fp8")
+
+
+def make_runtime(dtype, device=None, matmul: str = "auto", weights: str = "stored") -> Runtime:
     if isinstance(dtype, str):
         dtype = parse_dtype(dtype)
     if dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("dtype must be bfloat16 or float32")
+    if weights not in WEIGHT_FORMS:
+        raise ValueError(f"weights must be one of {', '.join(WEIGHT_FORMS)}")
+    if weights == "fp8" and (dtype != torch.bfloat16 or matmul == "simt"):
+        raise ValueError("weights in 8 bits go with dtype bfloat16 and the tensor-core kernels")
     # The 32-bit path must stay true fp32 everywhere, also inside library calls.
     torch.backends.cuda.matmul.allow_tf32 = False
     torch.backends.cudnn.allow_tf32 = False
-    return Runtime(dtype=dtype, device=device or require_cuda(), matmul=matmul)
+    return Runtime(dtype=dtype, device=device or require_cuda(), matmul=matmul, weights=weights)
 
 
-def load_model(model_dir: str, dtype="bfloat16", device=None, matmul: str = "auto") -> Tuple[Model, object]:
-    """Reads config.json (which chooses the model class) and the safetensors weights."""
+def load_model(model_dir: str, dtype="bfloat16", device=None, matmul: str = "auto", weights: str = "stored") -> Tuple[Model, object]:
+    """Reads config.json (which chooses the model class) and the safetensors weights.  ``weights`` ``fp8``: the gated feed-forwards' and gated
+    experts' matrices are quantised to 8 bits as they are loaded."""
     _ensure_builtin()
-    rt = make_runtime(dtype, device, matmul)
+    rt = make_runtime(dtype, device, matmul, weights)
     cfg, spec = load_spec(model_dir)
     tensors = load_tensors(model_dir, spec, rt.dtype, rt.device)
     return Model(spec, tensors, rt), cfg
 
 
-def random_model(spec: ModelSpec, seed: int, dtype="bfloat16", device=None, matmul: str = "auto") -> Model:
+def random_model(spec: ModelSpec, seed: int, dtype="bfloat16", device=None, matmul: str = "auto", weights: str = "stored") -> Model:
     """A model with seeded random weights made directly on the device (no folder written)."""
     _ensure_builtin()
-    rt = make_runtime(dtype, device, matmul)
+    rt = make_runtime(dtype, device, matmul, weights)
     tensors = random_tensors(spec, seed, rt.dtype, rt.device)
     return Model(spec, tensors, rt)

@@ -2108,16 +2108,29 @@ def quantize_fp8_rows(x: torch.Tensor, source: Optional[torch.Tensor] = None) ->
     return out
 
 
-def quantize_fp8_weight(w: torch.Tensor) -> Fp8Weight:
+def fp8_weight_like(*shape: int, device) -> Fp8Weight:
+    """An empty weight [..., N, K] in 8 bits, to be filled matrix by matrix (:func:`quantize_fp8_weight`)."""
+    if len(shape) < 2 or min(shape) < 1:
+        raise KernelError("fp8 weight: expected a matrix or stacked matrices")
+    n, k = shape[-2:]
+    return Fp8Weight(_fp8_buffer(*shape, device=device), torch.empty(tuple(shape[:-2]) + (_blocks(n), _blocks(k)), dtype=torch.float32, device=device))
+
+
+def quantize_fp8_weight(w: torch.Tensor, out: Optional[Fp8Weight] = None, at: int = 0) -> Fp8Weight:
     """A weight [..., N, K] (bf16 or fp32) in 8 bits with a scale per block of 128 x 128 of every matrix: ``s = max(max|w| / 448, 2^-126)``,
-    ``q = e4m3(w / s)``."""
+    ``q = e4m3(w / s)``.  ``out`` (of :func:`fp8_weight_like`, one leading axis more): its entry ``at`` is filled instead of a new weight."""
     _need(w, "fp8 weight")
     if w.dim() < 2 or w.numel() == 0:
         raise KernelError("fp8 weight: expected a matrix or stacked matrices")
-    _here("fp8 weight", w)
-    lead, (n, k) = tuple(w.shape[:-2]), w.shape[-2:]
-    out = Fp8Weight(_fp8_buffer(*lead, n, k, device=w.device), torch.empty(lead + (_blocks(n), _blocks(k)), dtype=torch.float32, device=w.device))
-    check(_lib.load().mm_fp8_quant_weight(w.data_ptr(), dtype_code(w.dtype), out.values.data_ptr(), -(-k // 16) * 16, out.scales.data_ptr(),
+    n, k = w.shape[-2:]
+    if out is None:
+        out = target = fp8_weight_like(*w.shape, device=w.device)
+    elif not isinstance(out, Fp8Weight) or tuple(out.shape[1:]) != tuple(w.shape) or not 0 <= at < out.shape[0] or out.ld != -(-k // 16) * 16:
+        raise KernelError("fp8 weight: the matrices do not fit into the weight that they are to fill")
+    else:
+        target = Fp8Weight(out.values[at], out.scales[at])
+    _here("fp8 weight", w, target.values)
+    check(_lib.load().mm_fp8_quant_weight(w.data_ptr(), dtype_code(w.dtype), target.values.data_ptr(), -(-k // 16) * 16, target.scales.data_ptr(),
                                           w.numel() // (n * k), n, k, _stream()), "quantize_fp8_weight")
     return out
 

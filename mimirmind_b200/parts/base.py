@@ -25,6 +25,7 @@ class Runtime:
     dtype: torch.dtype               # activation / cache dtype: torch.float32 or torch.bfloat16
     device: torch.device
     matmul: str = "auto"             # "auto": tensor-core kernels for bf16; "simt": fp32-FMA kernel everywhere
+    weights: str = "stored"          # "fp8": the gated feed-forwards' and gated experts' matrices in 8 bits, a scale per block of 128 x 128
 
 
 class WeightView:

@@ -20,7 +20,7 @@ from .linear import linear, linear_into
 @FEED_FORWARDS.register("swiglu")
 class SwiGLU(FeedForward):
     """spec params: hidden, intermediate, gate, up, down (tensor names under the prefix), activation (``silu``, the default, or
-    ``gelu_tanh``)."""
+    ``gelu_tanh``).  With a runtime whose weights are ``fp8`` the matrices are in 8 bits and the rows that meet them are quantised."""
 
     @classmethod
     def tensor_specs(cls, spec: PartSpec, prefix: str) -> List[TensorSpec]:
@@ -43,6 +43,12 @@ class SwiGLU(FeedForward):
         if gate.dtype != up.dtype:
             gate, up = gate.float(), up.float()
         f, d = gate.shape
+        self.fp8 = rt.weights == "fp8"
+        if self.fp8:            # two matrices in 8 bits, one after the other, and one: a scale per block of 128 x 128 of each
+            self.w_in = ops.quantize_fp8_weight(torch.stack([gate, up]))
+            del gate, up
+            self.w_out = ops.quantize_fp8_weight(weights.take(spec["down"]).contiguous())
+            return
         # Interleave gate and up rows in blocks of 8 (rows 16j..16j+7 = gate[8j..], 16j+8..16j+15 = up[8j..]):
         # a tensor-core tile then holds a gate value and its up value together, so the activation can be
         # an epilogue of the product.  Plain concatenation when the width is not a multiple of 8.
@@ -55,7 +61,7 @@ class SwiGLU(FeedForward):
         self.w_down = weights.take(spec["down"]).contiguous()       # [d, F]
 
     def native(self):
-        if type(self) is not SwiGLU or self.activation != "silu":
+        if type(self) is not SwiGLU or self.activation != "silu" or self.fp8:
             return None
         return NativeDesc("swiglu", {"hidden": self.hidden, "intermediate": self.intermediate, "interleave": self.interleave},
                           {"w_gate_up": self.w_gate_up, "w_down": self.w_down})
@@ -65,7 +71,7 @@ class SwiGLU(FeedForward):
             and self.w_down.dtype == torch.bfloat16 and self.rt.matmul != "simt"
 
     def fuses(self, n_tokens: int) -> bool:
-        return self.activation == "silu" and self._small(n_tokens)
+        return not self.fp8 and self.activation == "silu" and self._small(n_tokens)
 
     def _small(self, n_tokens: int) -> bool:
         return (self._tensor_cores() and ops.small_batch_supported(n_tokens, 2 * self.intermediate, self.hidden)
@@ -73,6 +79,8 @@ class SwiGLU(FeedForward):
 
     def forward(self, x, ctx: StepContext, sink: Optional[ResidualSink] = None):
         m = x.shape[0]
+        if self.fp8:
+            return ops.glu_mlp_fp8(x, self.w_in, self.w_out, self.activation)
         if self.activation != "silu":
             return linear(self._hidden(x), self.w_down, None, self.rt)
         if self.fuses(m):

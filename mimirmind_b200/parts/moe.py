@@ -18,7 +18,8 @@ added to its score for the choice only (of runs and of experts), the weights are
 The experts' matrices are stacked at load (``[E, 2F, D]`` gate and up rows, ``[E, D, F]``).  A step routes on the
 device, puts the rows of every expert side by side, and runs two grouped products over them: for prompt-sized steps, and smaller ones
 of large experts, in bfloat16 the tcgen05 product over row tiles laid out on the device (``csrc/gemm_tcgen05.cu``, SwiGLU in its epilogue),
-otherwise the ``mma.sync`` or fp32 kernels of ``csrc/moe.cu``.  Nothing waits for the host, so a decode step with this
+otherwise the ``mma.sync`` or fp32 kernels of ``csrc/moe.cu``.  With a runtime whose weights are ``fp8`` gated experts are held in 8 bits: up
+to 16 tokens go through the whole layer in two launches (``csrc/moe_few.cu``), more through the grouped 8-bit products (``csrc/gemm_fp8_tcgen05.cu``).  Nothing waits for the host, so a decode step with this
 feed-forward can be captured.
 """
 from __future__ import annotations
@@ -27,7 +28,7 @@ from typing import List
 
 import torch
 
-from ..config.spec import PartSpec, TensorSpec
+from ..config.spec import ModelSpec, PartSpec, TensorSpec
 from ..kernels import ops
 from ..registry import FEED_FORWARDS
 from .base import FeedForward, Runtime, SplitBranch, StepContext, WeightView
@@ -41,6 +42,20 @@ GROUPED_MIN_ROWS = 1024      # (token, choice) rows from which a step's expert p
 # 443 and 250 to 262, 16 tokens 236 and 250; 128 of 2048 x 768, 32 tokens 375 and 250; 16 of 2048 x 1408 156 and 131; 32 of 1024 x 512
 # (16.8 million numbers) 67 and 85, the two more launches.  A weight on the expert's input would be rounded with it, so that stays.
 GROUPED_MIN_WEIGHTS = 1 << 25
+
+
+def fp8_step_bytes(spec: ModelSpec, n_tokens: int) -> int:
+    """What a step's feed-forwards keep beside their rows when their matrices are in 8 bits, at the most: quantised rows with their scales, and the chosen
+    experts' fp32 results."""
+    most = 0
+    for layer in spec.layers:
+        p = layer.feed_forward
+        if p.kind == "routed_experts":
+            rows, d, f = n_tokens * int(p["top"]), int(p["hidden"]), int(p["ff"])
+            most = max(most, rows * (6 * d + 2 * f) + 36 * ops.MOE_FEW_TOKENS * (d + 160) + ops.MOE_FEW_TOKENS * int(p["top"]) * 5 * f)
+        elif p.kind in ("swiglu", "gated_mlp"):
+            most = max(most, n_tokens * 2 * (int(p["hidden"]) + int(p["intermediate"])))
+    return most
 
 
 def ctx_plain(ctx) -> bool:
@@ -97,6 +112,14 @@ class RoutedExperts(FeedForward):
             self.w_router = torch.cat([self.w_router, weights.take(spec["shared_gate"]).float().reshape(1, -1)], dim=0).contiguous()
         stacked_in, stacked_out = [], []
         f, d = self.ff, self.hidden
+        self.fp8 = rt.weights == "fp8" and self.gated
+        if self.fp8:            # [E, 2, F, D] and [E, D, F] in 8 bits, quantised expert by expert
+            self.w_in, self.w_out = ops.fp8_weight_like(self.experts, 2, f, d, device=rt.device), ops.fp8_weight_like(self.experts, d, f, device=rt.device)
+            for e in range(self.experts):
+                stem = spec["expert"].format(e)
+                ops.quantize_fp8_weight(torch.stack([weights.take(stem + ".gate"), weights.take(stem + ".up")]), out=self.w_in, at=e)
+                ops.quantize_fp8_weight(weights.take(stem + ".down").contiguous(), out=self.w_out, at=e)
+            return
         # bfloat16 with sizes the tensor-memory product takes: gate and up rows alternate in blocks of 8, so that a tile of
         # the product holds a gate value beside its up value and the activation is the product's epilogue
         self.tensor_memory = (rt.dtype == torch.bfloat16 and rt.matmul != "simt" and f % 8 == 0 and d % 8 == 0)
@@ -128,16 +151,31 @@ class RoutedExperts(FeedForward):
 
     def splits_weighed(self) -> bool:
         """True if the result in pieces (``forward_split``) is the chosen rows with their weights and nothing else."""
-        return self.shared is None and self.weight_on == "output"
+        return self.shared is None and self.weight_on == "output" and not self.fp8
 
     def forward_split(self, x: torch.Tensor, ctx: StepContext) -> SplitBranch:
         """The result in pieces: every token's chosen rows with their weights, and the shared expert's with its gate."""
+        if self.fp8:
+            y, gate = self._combined(x, ctx)
+            return SplitBranch(y, None, None, self.shared.forward(x, ctx) if self.shared is not None else None, gate)
         y, wts, place, gate = self._routed(x, ctx)
         if wts is None:
             y, place = ops.moe_combine(y, None, self.rt.dtype, place=place, top=self.top), None
         return SplitBranch(y, wts, place, self.shared.forward(x, ctx) if self.shared is not None else None, gate)
 
+    def _experts_fp8(self, x: torch.Tensor):
+        """(the routed experts' weighted sum, the shared expert's gate per token or None) with experts in 8 bits."""
+        if not self.shared_gated and ops.moe_few_supported(x.shape[0], self.experts, self.top, self.hidden, self.ff):
+            return ops.moe_few(x, self.w_router, self.w_in, self.w_out, self.top, self.groups, self.keep, scoring=self.scoring, renorm=self.renorm,
+                               scale=self.weight_scale, correction=self.correction, group_score=self.group_score, activation=self.activation, limit=self.limit,
+                               weight_on=self.weight_on), None
+        idx, wts, gate = (ops.moe_router(x, self.w_router, self.top, self.groups, self.keep, scoring=self.scoring, correction=self.correction,
+                                         group_score=self.group_score, gate=self.shared_gated, renorm=self.renorm, scale=self.weight_scale) + (None,))[:3]
+        return ops.moe_experts_fp8(x, idx, wts, self.w_in, self.w_out, self.activation, self.limit, self.weight_on), gate
+
     def _combined(self, x: torch.Tensor, ctx: StepContext):
+        if self.fp8:
+            return self._experts_fp8(x)
         y, wts, place, gate = self._routed(x, ctx)
         return ops.moe_combine(y, wts, self.rt.dtype, place=place, top=self.top), gate
 
@@ -196,10 +234,18 @@ class GatedMLP(FeedForward):
         gate, up = weights.take(spec["gate"]), weights.take(spec["up"])
         if gate.dtype != up.dtype:
             gate, up = gate.float(), up.float()
+        self.fp8 = rt.weights == "fp8"
+        if self.fp8:
+            self.w_in = ops.quantize_fp8_weight(torch.stack([gate, up]))
+            del gate, up
+            self.w_out = ops.quantize_fp8_weight(weights.take(spec["down"]).contiguous())
+            return
         self.w_gate_up = torch.cat([gate, up], dim=0).contiguous()          # [2F, D]
         del gate, up
         self.w_down = weights.take(spec["down"]).contiguous()               # [D, F]
 
     def forward(self, x: torch.Tensor, ctx: StepContext) -> torch.Tensor:
+        if self.fp8:
+            return ops.glu_mlp_fp8(x, self.w_in, self.w_out, self.activation, self.limit)
         gu = linear(x, self.w_gate_up, None, self.rt, out_dtype=torch.float32)
         return linear(ops.glu_rows(gu, self.rt.dtype, self.activation, self.limit), self.w_down, None, self.rt)
