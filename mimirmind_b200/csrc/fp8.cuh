@@ -11,6 +11,7 @@
 #include "common.cuh"
 
 constexpr int FP8_BLOCK = 128;
+constexpr int FP8_MAX = 1 << 30;      // rows, columns and depths stay below: places behind their ends are still ints
 
 // |v| as bits: they order as the numbers do, with NaN above infinity, so that a maximum keeps a NaN
 __device__ __forceinline__ uint32_t fp8_size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }

@@ -38,7 +38,7 @@ int product(const Fp8In& x, const Fp8Mat& w, const Fp8Out& o, bool glu, bool dep
 // rows and for up to 16 rows of 4,096 numbers together).
 MM_EXPORT int mm_fp8_linear(const void* x, int x_dtype, long long ldx, const void* x_scales, int m, const void* W, long long ldw, const void* w_scales, int N, int K,
                             const void* bias, int bias_dtype, void* out, int out_dtype, void* scratch, void* err, void* stream) {
-    MM_REQUIRE(m >= 0 && N > 0 && K > 0, "fp8 product: bad sizes");
+    MM_REQUIRE(m >= 0 && m < FP8_MAX && N > 0 && N < FP8_MAX && K > 0 && K < FP8_MAX, "fp8 product: bad sizes");
     if (m == 0) return MM_OK;
     cudaStream_t s = (cudaStream_t)stream;
     Fp8In in = {x, (const float*)x_scales, ldx, x_dtype, m};
@@ -55,7 +55,7 @@ MM_EXPORT int mm_fp8_linear(const void* x, int x_dtype, long long ldx, const voi
 MM_EXPORT int mm_fp8_glu_mlp(const void* x, int x_dtype, long long ldx, const void* x_scales, int m, const void* w_in, long long ld_in, const void* in_scales, int F,
                              int K, const void* w_out, long long ld_out, const void* out_scales, int D, int act, float limit, void* out, void* scratch, void* err,
                              void* stream) {
-    MM_REQUIRE(m >= 0 && F > 0 && K > 0 && D > 0 && act >= 0 && act <= MM_GLU_GELU_TANH, "fp8 feed-forward: bad sizes or activation");
+    MM_REQUIRE(m >= 0 && m < FP8_MAX && F > 0 && F < FP8_MAX && K > 0 && K < FP8_MAX && D > 0 && D < FP8_MAX && act >= 0 && act <= MM_GLU_GELU_TANH, "fp8 feed-forward: bad sizes or activation");
     if (m == 0) return MM_OK;
     cudaStream_t s = (cudaStream_t)stream;
     Fp8In in = {x, (const float*)x_scales, ldx, x_dtype, m};

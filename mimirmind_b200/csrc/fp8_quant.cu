@@ -4,58 +4,44 @@
 
 namespace {
 
-constexpr int UNITS = 1;
-
-// Two blocks of a row per warp and unit, eight numbers a lane, three units' loads on their way at once; where rows start on 16-byte boundaries the loads are wide ones.
-// Bound by memory (3 bytes a number): 4,096 rows of 3,584 bf16 (44 MB) with a division a number 19.7 us, with fp8_quotient PLACEHOLDER us.
+// Two blocks of a row per warp (a unit), eight numbers a lane; where rows start on 16-byte boundaries the loads are wide ones.  Many short warps hide the
+// loads: three units a warp, their loads together on their way, were no faster.
+// Bound by memory (3 bytes a number) and by the work a number: 4,096 rows of 3,584 bf16 (44 MB) with a division a number 19.7 us, with fp8_quotients 13.4 us (3.3 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const T* __restrict__ x, long long ldx, const int32_t* __restrict__ source,
                                                              uint8_t* __restrict__ q, int ldq, float* __restrict__ scales, uint32_t units, int K,
                                                              uint32_t pairs, int blocks, int wide) {
     const int lane = threadIdx.x & 31;
     pdl_trigger();        // a product launched behind this may fetch its first weights meanwhile
-    const uint32_t step = gridDim.x * 8;
-    for (uint32_t u0 = blockIdx.x * 8 + (threadIdx.x >> 5); u0 < units; u0 += UNITS * step) {
-        float v[UNITS][8];
+    const uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (u >= units) return;
+    const uint32_t row = u / pairs;
+    const int b = (int)(u - row * pairs) * 2 + (lane >> 4), k = b * FP8_BLOCK + (lane & 15) * 8;
+    const T* src = x + (source ? source[row] : (int)row) * ldx + k;
+    float v[8];
+    if (wide && k + 8 <= K) {
+        fp8_load8<T>(src, v);
+    } else {
 #pragma unroll
-        for (int n = 0; n < UNITS; ++n) {
-            const uint32_t u = u0 + n * step;
-            if (u >= units) break;
-            const uint32_t row = u / pairs;
-            const int k = ((int)(u - row * pairs) * 2 + (lane >> 4)) * FP8_BLOCK + (lane & 15) * 8;
-            const T* src = x + (source ? source[row] : (int)row) * ldx + k;
-            if (wide && k + 8 <= K) {
-                fp8_load8<T>(src, v[n]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[n][i] = k + i < K ? to_f32<T>(src[i]) : 0.0f;
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < UNITS; ++n) {
-            const uint32_t u = u0 + n * step;
-            if (u >= units) break;
-            const uint32_t row = u / pairs;
-            const int b = (int)(u - row * pairs) * 2 + (lane >> 4), k = b * FP8_BLOCK + (lane & 15) * 8;
-            uint32_t largest = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) largest = max(largest, fp8_size_bits(v[n][i]));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-            const float s = fp8_scale_of(largest);
-            if ((lane & 15) == 0 && b < blocks) scales[(size_t)row * blocks + b] = s;
-            fp8_quotients<8>(v[n], s);
-            if (k + 8 <= ldq)      // ldq is a multiple of 16: the row's padding gets noughts
-                *reinterpret_cast<uint2*>(q + (size_t)row * ldq + k) = make_uint2(fp8_pack4(v[n][0], v[n][1], v[n][2], v[n][3]), fp8_pack4(v[n][4], v[n][5], v[n][6], v[n][7]));
-        }
+        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f32<T>(src[i]) : 0.0f;
     }
+    uint32_t largest = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) largest = max(largest, fp8_size_bits(v[i]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    const float s = fp8_scale_of(largest);
+    if ((lane & 15) == 0 && b < blocks) scales[(size_t)row * blocks + b] = s;
+    fp8_quotients<8>(v, s);
+    if (k + 8 <= ldq)      // ldq is a multiple of 16: the row's padding gets noughts
+        *reinterpret_cast<uint2*>(q + (size_t)row * ldq + k) = make_uint2(fp8_pack4(v[0], v[1], v[2], v[3]), fp8_pack4(v[4], v[5], v[6], v[7]));
 }
 
-// Quantised rows copied to other places: out row r is row source[r], numbers and scales.  A warp per row, 16 bytes a lane.
-__global__ void __launch_bounds__(256) fp8_gather_rows_kernel(const uint4* __restrict__ q, const float* __restrict__ s, const int32_t* __restrict__ source, uint4* __restrict__ oq,
-                                                              float* __restrict__ os, int rows, int pieces, int blocks) {
+// Quantised rows copied to other places: out row r is row source[r], numbers and scales, for the first *count rows.  A warp per row, 16 bytes a lane.
+__global__ void __launch_bounds__(256) fp8_gather_rows_kernel(const uint4* __restrict__ q, const float* __restrict__ s, const int32_t* __restrict__ source, const int32_t* __restrict__ count,
+                                                              uint4* __restrict__ oq, float* __restrict__ os, int rows, int pieces, int blocks) {
     const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= rows) return;
+    if (row >= rows || row >= *count) return;
     const size_t from = source[row];
 #pragma unroll 4
     for (int i = lane; i < pieces; i += 32) oq[(size_t)row * pieces + i] = q[from * pieces + i];
@@ -93,7 +79,7 @@ __global__ void __launch_bounds__(256) fp8_quant_weight_kernel(const T* __restri
 }  // namespace
 
 int fp8_quant_rows(const void* x, int x_dtype, long long ldx, const int32_t* source, void* q, int ldq, float* scales, int rows, int K, cudaStream_t s) {
-    MM_REQUIRE(rows >= 0 && K > 0 && ldx >= 0 && ldq >= K && ldq % 16 == 0 && ldq < K + 16, "fp8 rows: bad sizes");
+    MM_REQUIRE(rows >= 0 && rows < FP8_MAX && K > 0 && K < FP8_MAX && ldx >= 0 && ldq >= K && ldq % 16 == 0 && ldq < K + 16, "fp8 rows: bad sizes");
     MM_REQUIRE(((uintptr_t)q & 15) == 0, "fp8 rows: the numbers must start on a 16-byte boundary");
     if (rows == 0) return MM_OK;
     const int blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
@@ -120,19 +106,19 @@ MM_EXPORT int mm_fp8_quant_rows(const void* x, int x_dtype, long long ldx, const
     return fp8_quant_rows(x, x_dtype, ldx, (const int32_t*)source, q, ldq, (float*)scales, rows, K, (cudaStream_t)stream);
 }
 
-// q [., ldq] e4m3 (ldq a multiple of 16) with scales fp32 [., blocks]: row r of the result is row source[r]
-MM_EXPORT int mm_fp8_gather_rows(const void* q, const void* scales, const void* source, void* out_q, void* out_scales, int rows, int ldq, int blocks, void* stream) {
+// q [., ldq] e4m3 (ldq a multiple of 16) with scales fp32 [., blocks]: row r of the result is row source[r], for the first *count of `rows` rows
+MM_EXPORT int mm_fp8_gather_rows(const void* q, const void* scales, const void* source, const void* count, void* out_q, void* out_scales, int rows, int ldq, int blocks, void* stream) {
     MM_REQUIRE(rows >= 0 && ldq > 0 && ldq % 16 == 0 && blocks > 0 && (((uintptr_t)q | (uintptr_t)out_q) & 15) == 0, "fp8 rows: bad sizes");
     if (rows == 0) return MM_OK;
     mm_launch(fp8_gather_rows_kernel, dim3(ceil_div(rows, 8)), dim3(256), 0, (cudaStream_t)stream, (const uint4*)q, (const float*)scales, (const int32_t*)source,
-              (uint4*)out_q, (float*)out_scales, rows, ldq / 16, blocks);
+              (const int32_t*)count, (uint4*)out_q, (float*)out_scales, rows, ldq / 16, blocks);
     MM_CHECK_LAUNCH();
     return MM_OK;
 }
 
 // w [matrices, N, K] -> q [matrices, N, ldq] e4m3, scales fp32 [matrices, N / 128, K / 128] (both rounded up)
 MM_EXPORT int mm_fp8_quant_weight(const void* w, int w_dtype, void* q, int ldq, void* scales, int matrices, int N, int K, void* stream) {
-    MM_REQUIRE(matrices > 0 && matrices <= 65535 && N > 0 && K > 0 && ldq >= K && ldq % 16 == 0 && ldq < K + 16, "fp8 weight: bad sizes");
+    MM_REQUIRE(matrices > 0 && matrices <= 65535 && N > 0 && N < FP8_MAX && K > 0 && K < FP8_MAX && ldq >= K && ldq % 16 == 0 && ldq < K + 16, "fp8 weight: bad sizes");
     const long long tiles = (long long)((N + FP8_BLOCK - 1) / FP8_BLOCK) * ((K + FP8_BLOCK - 1) / FP8_BLOCK);
     MM_REQUIRE(tiles < 0x7fffffffLL, "fp8 weight: the matrix is too large");
     const dim3 grid((unsigned)tiles, matrices);

@@ -545,7 +545,7 @@ MM_EXPORT int mm_gemm_fp8_tcgen05(const void* A, long long lda, const void* sa, 
                                   int out_dtype, void* out_scales, int ldo, const void* bias, int bias_dtype, int M, int N, int K, int glu, int act, float limit,
                                   const void* row_scale, const void* order, const void* tiles, const void* n_tiles, int max_tiles, int wide, int splits,
                                   void* err, void* stream) {
-    MM_REQUIRE(M > 0 && N > 0 && K > 0 && matrices > 0 && lda >= K && ldw >= K && ldo >= N, "gemm_fp8: bad sizes");
+    MM_REQUIRE(M > 0 && M < FP8_MAX && N > 0 && N < FP8_MAX && K > 0 && K < FP8_MAX && matrices > 0 && lda >= K && ldw >= K && ldo >= N, "gemm_fp8: bad sizes");
     MM_REQUIRE(lda % 16 == 0 && ldw % 16 == 0 && (((uintptr_t)A | (uintptr_t)W) & 15) == 0, "gemm_fp8: rows must start on 16-byte boundaries");
     MM_REQUIRE((long long)matrices * N + 256 < 0x7fffffffLL, "gemm_fp8: too many weight rows");
     MM_REQUIRE(out_dtype == MM_F32 || out_dtype == MM_BF16, "gemm_fp8: the result is bf16 or fp32");

@@ -4,8 +4,8 @@
 // block of 128 is free as long as both operands agree, so a lane takes 16 consecutive bytes of a weight row straight from memory and the same of
 // x.  A block's four products start from nought; their results are multiplied by the block's scales and added up in fp32.
 //
-// A CTA's eight warps are RT tiles of 16 rows times KS runs of blocks.  Every warp keeps four blocks on their way (asynchronous copies, over
-// tile borders too: 128 KB of weights an SM); a lane copies just the bytes that it reads itself, so no lane waits for another.  The runs' sums
+// A CTA's eight warps are RT tiles of 16 rows times KS runs of blocks.  Every warp keeps three blocks on their way (asynchronous copies, over
+// tile borders too: 96 KB of weights an SM); a lane copies just the bytes that it reads itself, so no lane waits for another.  The runs' sums
 // meet in shared memory and are added in order, so a result does not depend on what runs beside it.
 //
 // GLU: a tile is 8 rows of the gate's matrix and the same 8 of the up projection's.  A cluster of S CTAs makes the 128 columns of
@@ -13,7 +13,9 @@
 //
 // Few rows are quantised here (every warp its own run of blocks, into shared memory) instead of by a launch of their own in front of this one.
 //
-// Bound by memory: PLACEHOLDER
+// Bound by memory where the matrix is large: 1 x 152,064 x 3,584 89 us (6.1 TB/s of 6.55).  Smaller ones by the launch, the first block's way from memory and the
+// ends of the runs: 8 x 18,944 x 3,584 12.4 to 16 us (68 MB, floor 10.4), 8 x 4,608 x 3,584 5.9 to 7 us (16.5 MB, floor 2.5).  Four blocks on their way
+// instead of three were no faster; a ring in registers instead of shared memory spilled.
 #include "fp8.cuh"
 #include "fp8_launch.h"
 

@@ -115,7 +115,7 @@ _PROTOTYPES = {
     "mm_fp8_quant_rows": [P, I, c_longlong, P, P, I, P, I, I, P],
     "mm_fp8_quant_weight": [P, I, P, I, P, I, I, I, P],
     "mm_moe_few": [P, c_longlong, I, I, P, I, I, I, I, I, P, I, I, F, P, P, c_longlong, P, P, c_longlong, I, I, F, I, I, P, P, P],
-    "mm_fp8_gather_rows": [P, P, P, P, P, I, I, I, P],
+    "mm_fp8_gather_rows": [P, P, P, P, P, P, I, I, I, P],
     "mm_fp8_linear": [P, I, c_longlong, P, I, P, c_longlong, P, I, I, P, I, P, I, P, P, P],
     "mm_fp8_glu_mlp": [P, I, c_longlong, P, I, P, c_longlong, P, I, I, P, c_longlong, P, I, I, F, P, P, P, P],
     "mm_gemm_fp8_tcgen05": [P, c_longlong, P, P, c_longlong, P, I, P, I, P, I, P, I, I, I, I, I, I, F, P, P, P, P, I, I, I, P, P],

@@ -1327,7 +1327,8 @@ class ExpertRows:
 
 
 def moe_sort(idx: torch.Tensor, experts: int, with_tiles: bool = False) -> ExpertRows:
-    """Rows (token * top + choice) put side by side by expert, in their order within an expert."""
+    """Rows (token * top + choice) put side by side by expert, in their order within an expert.  A row whose number is no expert's stands in no
+    list; its place (``with_tiles``) is -1, and the lists end at ``offsets[experts]``."""
     _need(idx, "expert choice", torch.int32)
     rows, top = idx.numel(), idx.shape[-1]
     dev = idx.device
@@ -2236,7 +2237,7 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, wts: torch.Tensor, w_in:
                     limit: float = 0.0, weight_on: str = "output") -> torch.Tensor:
     """The chosen experts in 8 bits over a step's rows: ``out[t] = sum_c wts[t, c] Wd_e act(Wg_e x_t, Wu_e x_t)``, ``e = idx[t, c]``, as bf16
     [n, D].  ``x`` bf16 or fp32 [n, D] and the hidden rows (from their fp32 values) are quantised per row and block of 128.  ``idx`` int32 and
-    ``wts`` fp32 [n, top] as :func:`moe_router` gives them (every expert's number below E); ``w_in`` [E, 2, F, D] the gates' and up projections' matrices,
+    ``wts`` fp32 [n, top] as :func:`moe_router` gives them (a number that is not 0 to E - 1, a padded row's, adds nothing); ``w_in`` [E, 2, F, D] the gates' and up projections' matrices,
     ``w_out`` [E, D, F].  ``weight_on`` ``input``: the weight multiplies the first products instead of the result."""
     _need(x, "moe rows")
     _need(idx, "expert choice", torch.int32)
@@ -2258,7 +2259,7 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, wts: torch.Tensor, w_in:
     # every row quantised once, then copied to its experts' places
     q = quantize_fp8_rows(x)
     sorted_x = Fp8Rows(_fp8_buffer(n * top, d, device=x.device), torch.empty((n * top, _blocks(d)), dtype=torch.float32, device=x.device))
-    check(_lib.load().mm_fp8_gather_rows(q.values.data_ptr(), q.scales.data_ptr(), rows.row_token.data_ptr(), sorted_x.values.data_ptr(), sorted_x.scales.data_ptr(),
+    check(_lib.load().mm_fp8_gather_rows(q.values.data_ptr(), q.scales.data_ptr(), rows.row_token.data_ptr(), rows.offsets[E:].data_ptr(), sorted_x.values.data_ptr(), sorted_x.scales.data_ptr(),
                                          n * top, -(-d // 16) * 16, _blocks(d), _stream()), "gather_fp8_rows")
     on_input = weight_on == "input"
     hidden = Fp8Rows(_fp8_buffer(n * top, f, device=x.device), torch.empty((n * top, _blocks(f)), dtype=torch.float32, device=x.device))
@@ -2307,7 +2308,8 @@ def moe_few(x: torch.Tensor, w_router: torch.Tensor, w_in, w_out, top: int, grou
         raise KernelError("moe_few: the router's matrix must be [E, D]")
     if not moe_few_supported(n, E, top, d, f):
         raise KernelError(f"moe_few: {n} rows, {E} experts, {top} choices, widths {d} and {f} are not supported")
-    if n and (x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < 0 or x.data_ptr() % 16):
+    ldx = x.stride(0) if n > 1 else d
+    if n and (x.stride(1) != 1 or ldx % 8 or x.data_ptr() % 16):
         raise KernelError("moe_few: rows must be contiguous and start on 16-byte boundaries")
     if scoring not in ROUTER_SCORINGS or group_score not in GROUP_SCORES or weight_on not in ("output", "input"):
         raise KernelError("moe_few: scoring is 'softmax' or 'sigmoid', group_score 'max' or 'top2_sum', weight_on 'output' or 'input'")
@@ -2321,7 +2323,7 @@ def moe_few(x: torch.Tensor, w_router: torch.Tensor, w_in, w_out, top: int, grou
     _here("moe_few", x, w_router, correction, *tensors)
     out = x.new_empty((n, d))
     scratch = torch.empty(n * top * (4 * f + f // 2 + 24) + 32 + 36 * n * (d + 160), dtype=torch.uint8, device=x.device)
-    check(_lib.load().mm_moe_few(x.data_ptr(), x.stride(0), n, d, w_router.data_ptr(), E, int(top), int(groups), int(keep), ROUTER_SCORINGS[scoring], _ptr(correction),
+    check(_lib.load().mm_moe_few(x.data_ptr(), ldx, n, d, w_router.data_ptr(), E, int(top), int(groups), int(keep), ROUTER_SCORINGS[scoring], _ptr(correction),
                                  GROUP_SCORES[group_score], int(scoring == "softmax" if renorm is None else renorm), float(scale), tensors[0].data_ptr(), _ptr(tensors[1]),
                                  ld_in, tensors[2].data_ptr(), _ptr(tensors[3]), ld_out, f, act, float(limit), int(weight_on == "input"), int(bool(interleaved)),
                                  out.data_ptr(), scratch.data_ptr(), _stream()), "moe_few")

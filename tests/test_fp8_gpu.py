@@ -248,6 +248,28 @@ def test_experts_over_a_prompt(m, d, f, experts, top, how):
     ops.check_tcgen05_errors(torch.device(DEV))
 
 
+@pytest.mark.parametrize("m,d,f,experts,top", [(9, 64, 48, 4, 2), (300, 136, 64, 5, 3), (2500, 128, 64, 7, 2), (40, 100, 33, 6, 4)])
+def test_a_choice_that_is_no_expert_adds_nothing(m, d, f, experts, top):
+    from mimirmind_b200.kernels import ops
+    gen = _gen(m, d, f)
+    x, w_in, w_out = _rows(m, d, gen), _weight(experts, 2, f, d, gen=gen), _weight(experts, d, f, gen=gen)
+    idx = torch.randn((m, experts), generator=gen, device=DEV).topk(top, dim=1).indices.to(torch.int32).contiguous()
+    wts = torch.rand((m, top), generator=gen, device=DEV) + 0.1
+    none = torch.rand((m, top), generator=gen, device=DEV) < 0.3
+    none[m // 3] = True
+    none[-2:] = True
+    strange = torch.tensor([-1, experts, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device=DEV)
+    bad = torch.where(none, strange[torch.randint(4, (m, top), generator=gen, device=DEV)], idx).contiguous()
+    x[-1] = float("nan")                    # a padded row may hold anything
+    got = ops.moe_experts_fp8(x, bad, torch.where(none, torch.full_like(wts, float("nan")), wts), w_in, w_out)
+    assert not bool(got[none.all(dim=1)].any())
+    want, err = _experts64(x[:-1], idx[:-1].long(), wts[:-1].masked_fill(none[:-1], 0.0), w_in, w_out, "silu", 0.0, False)
+    _close(got[:-1], want, err)
+    nobody = torch.full_like(idx, experts)
+    assert not bool(ops.moe_experts_fp8(x, nobody, wts, w_in, w_out).any())
+    ops.check_tcgen05_errors(torch.device(DEV))
+
+
 # ---- streams, graphs, refusals ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("m", [1, 12, 60, 300])
 def test_captured_and_on_a_stream_of_its_own(m):

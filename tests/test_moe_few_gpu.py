@@ -213,6 +213,24 @@ def test_no_rows_and_strided_rows():
     assert torch.equal(ops.moe_few(wide[:, 8:264], router, w_in, w_out, 2), ops.moe_few(x, router, w_in, w_out, 2))
 
 
+def test_one_row_of_any_stride_and_two_streams_at_once():
+    from mimirmind_b200.kernels import ops
+    x, router, w_in, w_out = _layer(3, 256, 64, 8, _gen(8), True)
+    want = ops.moe_few(x, router, w_in, w_out, 2)
+    row = x[1].clone().as_strided((1, 256), (7, 1))              # a single row's stride is nobody's business
+    assert torch.equal(ops.moe_few(row, router, w_in, w_out, 2)[0], want[1])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(ops.moe_few(x, router, w_in, w_out, 2))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
 def test_refusals():
     from mimirmind_b200.kernels import ops
     from mimirmind_b200.kernels.lib import KernelError
