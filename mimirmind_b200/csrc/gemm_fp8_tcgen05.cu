@@ -63,7 +63,7 @@ struct Layout {
     static constexpr int STAGE_BYTES = HALF_BYTES * (1 + BN / 128);
     static constexpr int STAGES = BN == 256 ? 4 : 6;
     static constexpr int PIPE_BYTES = STAGES * STAGE_BYTES;
-    static constexpr int STAGING = 4096;           // per warp: 32 rows of 64 bytes, twice
+    static constexpr int STAGING = 4096;           // per warp: 32 rows of 128 bytes
     static constexpr int PART_LD = BN + 4;         // floats of a row of a split tile's sums
 };
 
@@ -170,20 +170,19 @@ __device__ __forceinline__ void gated_half(float* acc, float rs, float limit) {
     for (int i = 0; i < N; ++i) acc[i] = fp8_glu_as<ACT>(acc[i], acc[N + i], limit, rs);
 }
 
-// 64 bytes of 32 rows on their way to memory: 16-byte unit u of row r at u ^ (r / 2 & 3), so that neither side meets bank conflicts.  Two such
-// areas in turn: the wait of one round (in store_staged) tells that the round before has been read
-__device__ __forceinline__ unsigned char* staged(unsigned char* base, int r, int u) { return base + r * 64 + ((u ^ ((r >> 1) & 3)) << 4); }
+// 128 bytes of 32 rows on their way to memory: 16-byte unit u of row r at u ^ (r & 7), so that neither side meets bank conflicts
+__device__ __forceinline__ unsigned char* staged(unsigned char* base, int r, int u) { return base + r * 128 + ((u ^ (r & 7)) << 4); }
 
 template <typename T>
-__device__ __forceinline__ void store_staged(unsigned char* base, int lane, T* out, int ldo, int row0, int hi, int col0, int N) {
-    constexpr int PER = 64 / sizeof(T), UNIT = 16 / sizeof(T);
+__device__ __forceinline__ void store_staged(unsigned char* base, int lane, T* out, int ldo, int row0, int hi, int col0, int N, bool wide) {
+    constexpr int PER = 128 / sizeof(T), UNIT = 16 / sizeof(T);
     __syncwarp();
-    if ((((uintptr_t)out | ((size_t)ldo * sizeof(T))) & 15) == 0 && col0 + PER <= N) {
+    if (wide && col0 + PER <= N) {
+        const int r0 = lane >> 3, u = lane & 7;
+        T* to = out + (size_t)(row0 + r0) * ldo + col0 + u * UNIT;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2), u = lane & 3;
-            if (row0 + r < hi) *reinterpret_cast<uint4*>(out + (size_t)(row0 + r) * ldo + col0 + u * UNIT) = *reinterpret_cast<const uint4*>(staged(base, r, u));
-        }
+        for (int i = 0; i < 8; ++i)
+            if (row0 + r0 + i * 4 < hi) *reinterpret_cast<uint4*>(to + (size_t)(i * 4) * ldo) = *reinterpret_cast<const uint4*>(staged(base, r0 + i * 4, u));
     } else {          // rows that start anywhere, or columns that end here: number by number, neighbours side by side
 #pragma unroll 4
         for (int i = lane; i < 32 * PER; i += 32) {
@@ -191,6 +190,7 @@ __device__ __forceinline__ void store_staged(unsigned char* base, int lane, T* o
             if (row0 + r < hi && col0 + c < N) out[(size_t)(row0 + r) * ldo + col0 + c] = reinterpret_cast<const T*>(staged(base, r, c / UNIT))[c % UNIT];
         }
     }
+    __syncwarp();          // the area may be written again
 }
 
 template <int BN, bool GLU, bool SPLIT>
@@ -289,9 +289,9 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const int q = warp & 3, part = warp >> 2;
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
         unsigned char* wstage = staging + warp * L::STAGING;
-        uint32_t it = 0, local = 0, round = 0;
+        uint32_t it = 0, known = 0;
         bool ok = true;
-        for (int t = first; t < total; t += step, ++local) {
+        for (int t = first; t < total; t += step) {
             const Tile x = tile_of<BN, GLU>(g, t, m_tiles);
             const int row = x.m0 + q * 32 + lane;
             const float* sa = g.sa + (size_t)min(row, x.hi - 1) * g.KB;
@@ -354,6 +354,8 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                     for (int i = 0; i < COLS; i += 4)
                         *reinterpret_cast<float4*>(mine + column(i / PIECE, part) + i % PIECE) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
                 }
+            } else if (GLU && x.m0 + q * 32 >= x.hi) {
+                // none of the tile's rows are this warp's
             } else if (GLU) {
                 const float rs = g.row_scale && row < x.hi ? g.row_scale[g.order ? g.order[row] : row] : 1.0f;
                 const int n0 = x.n0 + part * (COLS / 2);
@@ -367,11 +369,12 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                     largest = max(largest, fp8_size_bits(acc[i]));
                 }
                 // the other parts of the row's block are the warps' with the same rows
-                volatile uint32_t* sizes = reinterpret_cast<volatile uint32_t*>(staging) + ((local & 1) * 4 + q) * 64 + lane;      // [tile parity][rows' quarter][part][row]
+                volatile uint32_t* sizes = reinterpret_cast<volatile uint32_t*>(staging) + ((known & 1) * 4 + q) * 64 + lane;      // [tile parity][rows' quarter][part][row]
                 sizes[part * 32] = largest;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&ctl->row_known[q]));
-                ok = __all_sync(0xffffffffu, ok && mbar_wait(smem_u32(&ctl->row_known[q]), local & 1, abort_flag));
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(smem_u32(&ctl->row_known[q]), known & 1, abort_flag));
+                ++known;
                 const float s = ok ? fp8_scale_of(max(sizes[0], sizes[32])) : __uint_as_float(0x7fffffffu);
                 const float inv = __fdiv_rn(1.0f, s);      // the sums are no closer to their exact values than a product with this to the quotient
                 if (row < x.hi) {
@@ -391,28 +394,29 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                     for (int i = 0; i < COLS; ++i)
                         if (x.n0 + part * COLS + i < g.N) acc[i] += bias_at(g, x.n0 + part * COLS + i);
                 }
+                const bool wide = (((uintptr_t)g.out | ((size_t)g.ldo * (g.out_kind == OUT_F32 ? 4 : 2))) & 15) == 0;
                 if (g.out_kind == OUT_F32) {
 #pragma unroll
-                    for (int c = 0; c < COLS; c += 16, ++round) {
+                    for (int c = 0; c < COLS; c += 32) {
 #pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            *reinterpret_cast<float4*>(staged(wstage + (round & 1) * 2048, lane, u)) = make_float4(acc[c + u * 4], acc[c + u * 4 + 1], acc[c + u * 4 + 2], acc[c + u * 4 + 3]);
-                        store_staged<float>(wstage + (round & 1) * 2048, lane, (float*)g.out, g.ldo, x.m0 + q * 32, x.hi, x.n0 + part * COLS + c, g.N);
+                        for (int u = 0; u < 8; ++u)
+                            *reinterpret_cast<float4*>(staged(wstage, lane, u)) = make_float4(acc[c + u * 4], acc[c + u * 4 + 1], acc[c + u * 4 + 2], acc[c + u * 4 + 3]);
+                        store_staged<float>(wstage, lane, (float*)g.out, g.ldo, x.m0 + q * 32, x.hi, x.n0 + part * COLS + c, g.N, wide);
                     }
                 } else {
 #pragma unroll
-                    for (int c = 0; c < COLS; c += 32, ++round) {
+                    for (int c = 0; c < COLS; c += 64) {
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
+                        for (int u = 0; u < 8; ++u) {
                             uint32_t p[4];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const __nv_bfloat162 v = __floats2bfloat162_rn(acc[c + u * 8 + 2 * j], acc[c + u * 8 + 2 * j + 1]);
                                 p[j] = *reinterpret_cast<const uint32_t*>(&v);
                             }
-                            *reinterpret_cast<uint4*>(staged(wstage + (round & 1) * 2048, lane, u)) = make_uint4(p[0], p[1], p[2], p[3]);
+                            *reinterpret_cast<uint4*>(staged(wstage, lane, u)) = make_uint4(p[0], p[1], p[2], p[3]);
                         }
-                        store_staged<__nv_bfloat16>(wstage + (round & 1) * 2048, lane, (__nv_bfloat16*)g.out, g.ldo, x.m0 + q * 32, x.hi, x.n0 + part * COLS + c, g.N);
+                        store_staged<__nv_bfloat16>(wstage, lane, (__nv_bfloat16*)g.out, g.ldo, x.m0 + q * 32, x.hi, x.n0 + part * COLS + c, g.N, wide);
                     }
                 }
             }
