@@ -521,9 +521,15 @@ EPI_BF16, EPI_SWIGLU, EPI_F32 = 0, 1, 2
 TCGEN05_SWIGLU_MIN_ROWS = 256
 
 
+def _device_number(device) -> int:
+    """A device's number: "cuda" is the current one, whatever its number."""
+    index = torch.device(device).index
+    return torch._C._cuda_getDevice() if index is None else index
+
+
 def tcgen05_error_flag(device) -> torch.Tensor:
     """Device int that the tcgen05 kernels set to 1 when one of their bounded waits ran out."""
-    key = str(device)
+    key = _device_number(device)
     if key not in _TC_ERR:
         _TC_ERR[key] = torch.zeros(1, dtype=torch.int32, device=device)
     return _TC_ERR[key]
@@ -531,7 +537,7 @@ def tcgen05_error_flag(device) -> torch.Tensor:
 
 def check_tcgen05_errors(device) -> None:
     """Raises if a tcgen05 kernel gave up a wait since the last check (synchronises)."""
-    flag = _TC_ERR.get(str(device))
+    flag = _TC_ERR.get(_device_number(device))
     if flag is not None and int(flag.item()) != 0:
         flag.zero_()
         raise KernelError("a tcgen05 kernel gave up waiting on its pipeline; its output is not valid")
@@ -2015,15 +2021,26 @@ def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """All tensors are on the current CUDA device: the launch goes to its current stream."""
     dev = torch._C._cuda_getDevice()
     for t in tensors:
-        if t is not None and t.device.index != dev:
+        if t is not None and t.get_device() != dev:
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
+
+
+_FP8_ERR = {}
+
+
+def _fp8_error(t: torch.Tensor) -> int:
+    """Address of the error flag (:func:`tcgen05_error_flag`) on the tensor's device: small products wait for the host, and finding it by the device's name takes a microsecond."""
+    at = _FP8_ERR.get(t.get_device())
+    if at is None:
+        at = _FP8_ERR[t.get_device()] = tcgen05_error_flag(t.device).data_ptr()
+    return at
 
 
 def _fp8_layout(values, scales, what: str) -> int:
     """The row stride of e4m3 numbers [..., rows, K] in numbers, once the tensors are what a kernel reads."""
     if not isinstance(values, torch.Tensor) or not isinstance(scales, torch.Tensor) or values.dtype is not _E4M3 or not values.is_cuda:
         raise KernelError(f"{what}: expected float8_e4m3fn numbers on a CUDA device")
-    if scales.dtype is not torch.float32 or scales.device != values.device or not scales.is_contiguous():
+    if scales.dtype is not torch.float32 or scales.get_device() != values.get_device() or not scales.is_contiguous():
         raise KernelError(f"{what} scales: expected contiguous float32 on the numbers' device")
     shape, stride = values.shape, values.stride()
     if len(shape) < 2 or shape[-1] < 1:
@@ -2177,14 +2194,13 @@ def gemm_fp8(x, w: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: to
         if bias.shape != (n,):
             raise KernelError("gemm_fp8: bias shape mismatch")
     ptr, code, ld, scales, m = _fp8_input(x, k, "gemm_fp8")
-    dev = w.values.device
     out_code = dtype_code(out_dtype)
     # (a tensor's own new_empty is the cheaper call, and a few numbers are quantised without scratch: small products wait for the host)
-    out = x.new_empty((m, n)) if code == out_code and code != _FP8_QUANTISED else torch.empty((m, n), dtype=out_dtype, device=dev)
-    scratch = None if code == _FP8_QUANTISED or (m <= 16 and m * k <= FP8_INSIDE) else torch.empty(_fp8_scratch(m, k), dtype=torch.uint8, device=dev)
+    out = x.new_empty((m, n)) if code == out_code and code != _FP8_QUANTISED else torch.empty((m, n), dtype=out_dtype, device=w.values.device)
+    scratch = None if code == _FP8_QUANTISED or (m <= 16 and m * k <= FP8_INSIDE) else w.values.new_empty(_fp8_scratch(m, k))
     check(_lib.load().mm_fp8_linear(ptr, code, ld, scales, m, w.values.data_ptr(), w.ld, w.scales.data_ptr(), n, k, _ptr(bias),
                                     F32 if bias is None else dtype_code(bias.dtype), out.data_ptr(), out_code, _ptr(scratch),
-                                    tcgen05_error_flag(dev).data_ptr(), _stream()), "gemm_fp8")
+                                    _fp8_error(w.values), _stream()), "gemm_fp8")
     return out
 
 
@@ -2195,7 +2211,7 @@ def _fp8_grouped(x: Fp8Rows, w: Fp8Weight, rows: "ExpertRows", out: torch.Tensor
     check(_lib.load().mm_gemm_fp8_tcgen05(x.values.data_ptr(), x.ld, x.scales.data_ptr(), w.values.data_ptr(), w.ld, w.scales.data_ptr(), w.matrices,
                                           out.data_ptr(), F32 if out.dtype == torch.float32 else BF16, _ptr(out_scales), out.stride(0), None, F32, x.shape[0], n, k,
                                           int(out_scales is not None), act, float(limit), _ptr(row_scale), rows.order.data_ptr(), rows.tiles.data_ptr(),
-                                          rows.n_tiles.data_ptr(), rows.max_tiles, 1, 1, tcgen05_error_flag(w.values.device).data_ptr(), _stream()), "gemm_fp8")
+                                          rows.n_tiles.data_ptr(), rows.max_tiles, 1, 1, _fp8_error(w.values), _stream()), "gemm_fp8")
 
 
 def _glu_code(activation: str, limit: float, what: str) -> int:
@@ -2216,12 +2232,12 @@ def glu_mlp_fp8(x, w_in: Fp8Weight, w_out: Fp8Weight, activation: str = "silu", 
     act = _glu_code(activation, limit, "glu_mlp_fp8")
     _here("glu_mlp_fp8", w_in.values, w_out.values)
     ptr, code, ld, scales, m = _fp8_input(x, k, "glu_mlp_fp8")
-    d, dev = w_out.shape[0], w_in.values.device
-    out = x.new_empty((m, d)) if code == BF16 else torch.empty((m, d), dtype=torch.bfloat16, device=dev)
-    scratch = torch.empty(_fp8_scratch(m, k) + _fp8_scratch(m, f), dtype=torch.uint8, device=dev)
+    d = w_out.shape[0]
+    out = x.new_empty((m, d)) if code == BF16 else torch.empty((m, d), dtype=torch.bfloat16, device=w_in.values.device)
+    scratch = w_in.values.new_empty(_fp8_scratch(m, k) + _fp8_scratch(m, f))
     check(_lib.load().mm_fp8_glu_mlp(ptr, code, ld, scales, m, w_in.values.data_ptr(), w_in.ld, w_in.scales.data_ptr(), f, k, w_out.values.data_ptr(), w_out.ld,
                                      w_out.scales.data_ptr(), d, act, float(limit), out.data_ptr(), scratch.data_ptr(),
-                                     tcgen05_error_flag(dev).data_ptr(), _stream()), "glu_mlp_fp8")
+                                     _fp8_error(w_in.values), _stream()), "glu_mlp_fp8")
     return out
 
 
@@ -2322,7 +2338,7 @@ def moe_few(x: torch.Tensor, w_router: torch.Tensor, w_in, w_out, top: int, grou
     act = _glu_code(activation, limit, "moe_few")
     _here("moe_few", x, w_router, correction, *tensors)
     out = x.new_empty((n, d))
-    scratch = torch.empty(n * top * (4 * f + f // 2 + 24) + 32 + 36 * n * (d + 160), dtype=torch.uint8, device=x.device)
+    scratch = x.new_empty((n * top * (4 * f + f // 2 + 24) + 32 + 36 * n * (d + 160)) // 2)      # (in numbers of two bytes)
     check(_lib.load().mm_moe_few(x.data_ptr(), ldx, n, d, w_router.data_ptr(), E, int(top), int(groups), int(keep), ROUTER_SCORINGS[scoring], _ptr(correction),
                                  GROUP_SCORES[group_score], int(scoring == "softmax" if renorm is None else renorm), float(scale), tensors[0].data_ptr(), _ptr(tensors[1]),
                                  ld_in, tensors[2].data_ptr(), _ptr(tensors[3]), ld_out, f, act, float(limit), int(weight_on == "input"), int(bool(interleaved)),

@@ -21,9 +21,9 @@ def test_a_tensor_of_another_device_is_refused(monkeypatch):
     from mimirmind_b200.kernels import ops
     from mimirmind_b200.kernels.lib import KernelError
     monkeypatch.setattr(ops.torch._C, "_cuda_getDevice", lambda: 1, raising=False)
-    ops._here("op", None, SimpleNamespace(device=torch.device("cuda", 1)))
+    ops._here("op", None, SimpleNamespace(device=torch.device("cuda", 1), get_device=lambda: 1))
     with pytest.raises(KernelError, match="current device is cuda:1"):
-        ops._here("op", SimpleNamespace(device=torch.device("cuda", 0)))
+        ops._here("op", SimpleNamespace(device=torch.device("cuda", 0), get_device=lambda: 0))
 
 
 def test_sizes_whose_places_would_leave_an_int_are_refused():
