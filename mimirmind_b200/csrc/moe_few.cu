@@ -79,8 +79,14 @@ __device__ __forceinline__ uint32_t pair_f16(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
 __device__ __forceinline__ float low_of(uint32_t bf16_pair) { return __uint_as_float(bf16_pair << 16); }
 __device__ __forceinline__ float high_of(uint32_t bf16_pair) { return __uint_as_float(bf16_pair & 0xffff0000u); }
+__device__ __forceinline__ float2 times(float x, float y, float s) {       // two products in one instruction
+    uint64_t v = ((uint64_t)__float_as_uint(y) << 32) | __float_as_uint(x);
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(((uint64_t)__float_as_uint(s) << 32) | __float_as_uint(s)));
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
 __device__ __forceinline__ void mma_e4m3_f32(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -216,41 +222,42 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
             float acc[2][4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[0][c] = acc[1][c] = 0.0f;
+auto load = [&](int s, int i) {
+                const int k = s * 16 + t4 * 4, on = s < hi && k < g.D ? 1 : 0;       // (D is a multiple of 8)
+                const uint32_t dst = stage + i * STEP_BYTES;
+                const float *pa = wa + (on ? k : 0), *pb = wb + (on ? k : 0);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(pa), "r"(on * 16) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 512), "l"(pb), "r"(on * 16) : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + 1024), "l"(xa + (on ? k : 0)), "r"(on * 8) : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + 1032), "l"(xb + (on ? k : 0)), "r"(on * 8) : "memory");
+                few_commit();
+            };
 #pragma unroll 1
-            for (int s0 = lo; s0 < hi; s0 += BATCH) {
+            for (int i = 0; i < BATCH; ++i) load(lo + i, i);
+#pragma unroll 1
+            for (int s = lo, i = 0; s < hi; ++s, i = i + 1 == BATCH ? 0 : i + 1) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(BATCH - 1) : "memory");
+                const unsigned char* at = mine_at + i * STEP_BYTES;
+                const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + 512);
+                const uint4 xv = *reinterpret_cast<const uint4*>(at + 1024);
+                load(s + BATCH, i);
+                float r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-                for (int i = 0; i < BATCH; ++i) {
-                    const int k = (s0 + i) * 16 + t4 * 4, on = s0 + i < hi && k < g.D ? 1 : 0;       // (D is a multiple of 8)
-                    const uint32_t dst = stage + i * STEP_BYTES;
-                    const float *pa = wa + (on ? k : 0), *pb = wb + (on ? k : 0);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(pa), "r"(on * 16) : "memory");
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 512), "l"(pb), "r"(on * 16) : "memory");
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + 1024), "l"(xa + (on ? k : 0)), "r"(on * 8) : "memory");
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + 1032), "l"(xb + (on ? k : 0)), "r"(on * 8) : "memory");
+                for (int p = 0; p < 3; ++p) {       // hi, mid, lo: eight bits each, cut off, so that nothing is lost
+                    const uint32_t a0 = upper_halves(r[0], r[1]), a2 = upper_halves(r[2], r[3]), a1 = upper_halves(r[4], r[5]), a3 = upper_halves(r[6], r[7]);
+                    if (p < 2) {
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) r[c] -= high_of(__float_as_uint(r[c]));      // exact
+                    }
+                    mma_bf16_f32(acc[0], a0, a1, a2, a3, xv.x, xv.y);
+                    if (g.n > 8) mma_bf16_f32(acc[1], a0, a1, a2, a3, xv.z, xv.w);
                 }
-                asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-#pragma unroll 1
-                for (int i = 0; i < BATCH; ++i) {
-                    const unsigned char* at = mine_at + i * STEP_BYTES;
-                    const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + 512);
-                    const uint4 xv = *reinterpret_cast<const uint4*>(at + 1024);
-                    float r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) {       // hi, mid, lo
-                        const uint32_t a0 = pair_bf16(r[0], r[1]), a2 = pair_bf16(r[2], r[3]), a1 = pair_bf16(r[4], r[5]), a3 = pair_bf16(r[6], r[7]);
-                        if (p < 2) {
-                            r[0] -= low_of(a0); r[1] -= high_of(a0); r[2] -= low_of(a2); r[3] -= high_of(a2);
-                            r[4] -= low_of(a1); r[5] -= high_of(a1); r[6] -= low_of(a3); r[7] -= high_of(a3);
-                        }
-                        mma_bf16_f32(acc[0], a0, a1, a2, a3, xv.x, xv.y);
-                        if (g.n > 8) mma_bf16_f32(acc[1], a0, a1, a2, a3, xv.z, xv.w);
-                    }
-                    if (FP8) {
-                        big0 = max(big0, max(max((xv.x & 0x7fffu) << 16, xv.x & 0x7fff0000u), max((xv.y & 0x7fffu) << 16, xv.y & 0x7fff0000u)));
-                        big1 = max(big1, max(max((xv.z & 0x7fffu) << 16, xv.z & 0x7fff0000u), max((xv.w & 0x7fffu) << 16, xv.w & 0x7fff0000u)));
-                    }
+                if (FP8) {
+                    big0 = max(big0, max(max((xv.x & 0x7fffu) << 16, xv.x & 0x7fff0000u), max((xv.y & 0x7fffu) << 16, xv.y & 0x7fff0000u)));
+                    big1 = max(big1, max(max((xv.z & 0x7fffu) << 16, xv.z & 0x7fff0000u), max((xv.w & 0x7fffu) << 16, xv.w & 0x7fff0000u)));
                 }
             }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");       // (nothing lands behind this: the bytes are used for other things)
             float* mine = part + (warp * 16 + gr) * 16 + t4 * 2;
             __syncthreads();        // the tile before has been read
 #pragma unroll
@@ -316,21 +323,24 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_in_kernel(const __grid_con
         if (threadIdx.x < own_tokens * g.top) chosen[threadIdx.x] = -1;
         __syncthreads();
         if (g.E <= FEW_RANK_EXPERTS) {
-            // a thread per token and expert counts the scores ahead of its own (equal ones of lower experts are)
+            // four threads per token and expert count the scores ahead of its own (equal ones of lower experts are); own_tokens * Ew is a multiple of 4, and
+            // a warp's eight are in the loop together up to the last: the others count for the last one
 #pragma unroll 1
-            for (int i = threadIdx.x; i < own_tokens * Ew; i += FEW_THREADS) {
-                const int t = i / Ew, e = i - t * Ew;
+            for (int i0 = warp * 8; i0 < own_tokens * Ew; i0 += FEW_WARPS * 8) {
+                const int i = min(i0 + (lane >> 2), own_tokens * Ew - 1), t = i / Ew, e = i - t * Ew;
                 const uint32_t* key = keys + t * Ew;
                 const uint32_t own = key[e];
                 int ahead = 0;
 #pragma unroll 2
-                for (int o = 0; o < Ew; o += 4) {
+                for (int o = (lane & 3) * 4; o < Ew; o += 16) {
                     const uint4 v = *reinterpret_cast<const uint4*>(key + o);
                     const uint32_t least = own - (o < e ? 1u : 0u);      // (own > 0 where it counts; the four beside e itself: below)
                     ahead += (v.x > least) + (v.y > least) + (v.z > least) + (v.w > least);
                 }
+                ahead += __shfl_xor_sync(0xffffffffu, ahead, 1);
+                ahead += __shfl_xor_sync(0xffffffffu, ahead, 2);
                 // the group of four around e was compared as if all of it stood before e: itself, and equals behind it, are taken back
-                if (own != 0) {
+                if (own != 0 && (lane & 3) == 0) {
                     if ((e & 3) != 0)
                         for (int o = e; o < (e | 3) + 1; ++o) ahead -= key[o] == own;
                     if (ahead < g.top) chosen[t * g.top + ahead] = e;
@@ -749,7 +759,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
     }
     // an item under way; the hidden numbers of its next block, or of the next item's first, are fetched a block ahead
     struct Item {
-        const float* row;        // of the lane's column, null without one
+        const float* row;        // of the lane's column (one without a row: another's numbers, not stored)
         const float* sw;
         float scale;
         int first, count, split, b, hi;
@@ -763,21 +773,29 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
         it.b = blocks * it.split / g.splits;
         it.hi = blocks * (it.split + 1) / g.splits;
         const int pair = places[it.first + min(gr, it.count - 1)];
-        it.row = gr < it.count ? g.hidden + (size_t)pair * g.F + t4 * (PER / 8) : nullptr;
+        it.row = g.hidden + (size_t)pair * g.F + t4 * (PER / 8) + it.b * PER;
         it.scale = FP8 ? few_scale(largest[pair], HIDDEN_TO) : 1.0f;
         it.sw = FP8 ? g.s_out + ((size_t)entries[3 * entry] * db + min(n0, g.D - 1) / 128) * fb : nullptr;
         return it;
     };
     float4 next[2][HW];
     float s_next = 1.0f;
-    auto fetch = [&](const Item& it, int b) {
+    auto fetch = [&](Item& it, int b) {
+        if (whole) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < HW; ++i) {
-                const int k = b * PER + h * (PER / 2) + i * 4;
-                next[h][i] = it.row != nullptr && (whole || k + t4 * (PER / 8) < g.F) ? *reinterpret_cast<const float4*>(it.row + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);      // (F is a multiple of 8)
-            }
+                for (int i = 0; i < HW; ++i) next[h][i] = *reinterpret_cast<const float4*>(it.row + h * (PER / 2) + i * 4);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < HW; ++i) {
+                    const int k = h * (PER / 2) + i * 4;
+                    next[h][i] = b * PER + t4 * (PER / 8) + k < g.F ? *reinterpret_cast<const float4*>(it.row + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);      // (F is a multiple of 8)
+                }
+        }
+        it.row += PER;
         if (FP8) s_next = it.sw[b];
     };
     int item = warp, slot = 0;
@@ -797,7 +815,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
             for (int i = 0; i < HW; ++i) {
                 const float4 v = next[h][i];
                 if (FP8) {
-                    high[h][i] = make_uint2(pair_f16(v.x * here.scale, v.y * here.scale), pair_f16(v.z * here.scale, v.w * here.scale));
+                    const float2 a = times(v.x, v.y, here.scale), b = times(v.z, v.w, here.scale);
+                    high[h][i] = make_uint2(pair_f16(a.x, a.y), pair_f16(b.x, b.y));
                 } else {
                     const uint2 p = make_uint2(pair_bf16(v.x, v.y), pair_bf16(v.z, v.w));
                     high[h][i] = p;
