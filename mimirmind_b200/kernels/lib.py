@@ -115,7 +115,8 @@ _PROTOTYPES = {
     "mm_fp8_quant_rows": [P, I, c_longlong, P, P, I, P, I, I, P],
     "mm_fp8_quant_weight": [P, I, P, I, P, I, I, I, P],
     "mm_moe_few": [P, c_longlong, I, I, P, I, I, I, I, I, P, I, I, F, P, P, c_longlong, P, P, c_longlong, I, I, F, I, I, P, P, P],
-    "mm_fp8_gather_rows": [P, P, P, P, P, P, I, I, I, P],
+    "mm_fp8_moe_experts": [P, I, I, I, P, P, I, I, P, c_longlong, P, I, P, c_longlong, P, I, F, I, P, P, P, P],
+    "mm_fp8_moe_experts_scratch": [I, I, I, I, I],
     "mm_fp8_linear": [P, I, c_longlong, P, I, P, c_longlong, P, I, I, P, I, P, I, P, P, P],
     "mm_fp8_glu_mlp": [P, I, c_longlong, P, I, P, c_longlong, P, I, I, P, c_longlong, P, I, I, F, P, P, P, P],
     "mm_gemm_fp8_tcgen05": [P, c_longlong, P, P, c_longlong, P, I, P, I, P, I, P, I, I, I, I, I, I, F, P, P, P, P, I, I, I, P, P],
@@ -149,6 +150,7 @@ def load(verbose: bool = True) -> ctypes.CDLL:
                 continue  # optional kernels are declared by the module that binds them
             fn.restype = c_int
             fn.argtypes = args
+        lib.mm_fp8_moe_experts_scratch.restype = c_longlong
         _lib = lib
         return lib
 

@@ -2204,16 +2204,6 @@ def gemm_fp8(x, w: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: to
     return out
 
 
-def _fp8_grouped(x: Fp8Rows, w: Fp8Weight, rows: "ExpertRows", out: torch.Tensor, out_scales: Optional[torch.Tensor], act: int = 0, limit: float = 0.0,
-                 row_scale: Optional[torch.Tensor] = None) -> None:
-    """Row tiles of ``rows.tiles`` times their expert's matrix; with ``out_scales`` its pair of matrices, act(gate, up) quantised."""
-    n, k = w.shape[-2:]
-    check(_lib.load().mm_gemm_fp8_tcgen05(x.values.data_ptr(), x.ld, x.scales.data_ptr(), w.values.data_ptr(), w.ld, w.scales.data_ptr(), w.matrices,
-                                          out.data_ptr(), F32 if out.dtype == torch.float32 else BF16, _ptr(out_scales), out.stride(0), None, F32, x.shape[0], n, k,
-                                          int(out_scales is not None), act, float(limit), _ptr(row_scale), rows.order.data_ptr(), rows.tiles.data_ptr(),
-                                          rows.n_tiles.data_ptr(), rows.max_tiles, 1, 1, _fp8_error(w.values), _stream()), "gemm_fp8")
-
-
 def _glu_code(activation: str, limit: float, what: str) -> int:
     if activation not in GLU_ACTIVATIONS:
         raise KernelError(f"{what}: activation '{activation}' is not one of {', '.join(sorted(GLU_ACTIVATIONS))}")
@@ -2263,26 +2253,20 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, wts: torch.Tensor, w_in:
         raise KernelError("moe_experts_fp8: choice and weights must be [n, top]")
     if weight_on not in ("output", "input"):
         raise KernelError("moe_experts_fp8: weight_on is 'output' or 'input'")
-    act = _glu_code(activation, limit, "moe_experts_fp8")
-    dtype_code(x.dtype)
+    act, code = _glu_code(activation, limit, "moe_experts_fp8"), dtype_code(x.dtype)
     _here("moe_experts_fp8", x, idx, wts, w_in.values, w_in.scales, w_out.values, w_out.scales)
     n, d = x.shape
     E, _, f, _ = w_in.shape
     top = idx.shape[1]
+    out = torch.empty((n, d), dtype=torch.bfloat16, device=x.device)
     if n == 0:
-        return torch.empty((0, d), dtype=torch.bfloat16, device=x.device)
-    rows = moe_sort(idx, E, with_tiles=True)
-    # every row quantised once, then copied to its experts' places
-    q = quantize_fp8_rows(x)
-    sorted_x = Fp8Rows(_fp8_buffer(n * top, d, device=x.device), torch.empty((n * top, _blocks(d)), dtype=torch.float32, device=x.device))
-    check(_lib.load().mm_fp8_gather_rows(q.values.data_ptr(), q.scales.data_ptr(), rows.row_token.data_ptr(), rows.offsets[E:].data_ptr(), sorted_x.values.data_ptr(), sorted_x.scales.data_ptr(),
-                                         n * top, -(-d // 16) * 16, _blocks(d), _stream()), "gather_fp8_rows")
-    on_input = weight_on == "input"
-    hidden = Fp8Rows(_fp8_buffer(n * top, f, device=x.device), torch.empty((n * top, _blocks(f)), dtype=torch.float32, device=x.device))
-    _fp8_grouped(sorted_x, w_in, rows, hidden.values, hidden.scales, act, limit, wts if on_input else None)
-    y = torch.empty((n * top, d), dtype=torch.float32, device=x.device)
-    _fp8_grouped(hidden, w_out, rows, y, None)
-    return moe_combine(y, None if on_input else wts, torch.bfloat16, place=rows.place, top=top)
+        return out
+    lib = _lib.load()
+    scratch = w_in.values.new_empty(lib.mm_fp8_moe_experts_scratch(n, d, f, E, top))
+    check(lib.mm_fp8_moe_experts(x.data_ptr(), code, n, d, idx.data_ptr(), wts.data_ptr(), top, E, w_in.values.data_ptr(), w_in.ld, w_in.scales.data_ptr(), f,
+                                 w_out.values.data_ptr(), w_out.ld, w_out.scales.data_ptr(), act, float(limit), int(weight_on == "input"), out.data_ptr(),
+                                 scratch.data_ptr(), _fp8_error(w_in.values), _stream()), "moe_experts_fp8")
+    return out
 
 
 MOE_FEW_TOKENS = 16         # rows of a step that a routed-experts layer takes in two launches
