@@ -1,6 +1,6 @@
 // Entry points that chain the launches of one 8-bit operator (fp8.cuh has the formulas).
 //
-// Up to 16 rows go to the weight-streaming kernel, more to tcgen05 tiles.  Rows that come in bf16 or fp32 are quantised by a launch in front, or, where they
+// Up to 8 rows, and up to 16 of matrices that are not large, go to the weight-streaming kernel, more to tcgen05 tiles.  Rows that come in bf16 or fp32 are quantised by a launch in front, or, where they
 // are few numbers (every CTA of the streaming kernel then does it for itself), inside it.
 #include "fp8.cuh"
 #include "fp8_launch.h"
@@ -36,8 +36,13 @@ int quantised(Fp8In& x, int K, bool glu, unsigned char* scratch, bool& dependent
     return rc;
 }
 
+// Nine to sixteen rows take a second group of columns through the streaming kernel, and large matrices are then faster over tcgen05 tiles.  Us of the two for 12
+// rows: 4,608 x 3,584 8.6 and 10.6, 8,192 x 2,048 9.5 and 9.3, 32,768 x 1,024 13.9 and 11.7, 18,944 x 3,584 19.4 and 18.0, 5,120 x 13,824 25.3 and 21.6 (8 rows: 19.9 and 21.8).
+constexpr long long TILED_BYTES = 24 << 20;
+
 int product(const Fp8In& x, const Fp8Mat& w, const Fp8Out& o, bool glu, bool dependent, int* err, cudaStream_t s) {
-    return fp8_gemv_takes(x.rows, w.K, glu, x.dtype != FP8_QUANTISED) ? fp8_gemv(x, w, o, glu, dependent, s) : fp8_gemm(x, w, o, glu, err, s);
+    const bool tiled = x.dtype == FP8_QUANTISED && x.rows > 8 && (long long)w.matrices * w.N * w.K > TILED_BYTES;
+    return !tiled && fp8_gemv_takes(x.rows, w.K, glu, x.dtype != FP8_QUANTISED) ? fp8_gemv(x, w, o, glu, dependent, s) : fp8_gemm(x, w, o, glu, err, s);
 }
 
 }  // namespace

@@ -10,7 +10,9 @@
 // Roles: warps 0..7 sums and results, warps 8 and 11 TMA, warps 9 and 10 products, each of the two for every other block: one thread's waits and
 // issues take 960 cycles a block, a block's products 540.  What bounds the loop now is the round of an accumulator: products 600 cycles, the wait for
 // them 200, reading 470, the next products' issue 350, for two blocks.  Pairs of CTAs (cta_group::2, 256 rows a tile, a third less traffic in shared memory) have
-// the same round, with or without the tile in halves, and were not faster (4,096 x 18,944 x 3,584: 281 and 295 us against 272).  A CTA walks over tiles, row tiles first, so that CTAs at work at
+// the same round, with or without the tile in halves, and were not faster (4,096 x 18,944 x 3,584: 281 and 295 us against 272); halves of one CTA's tile, each
+// 128 columns with barriers of its own, took 410; weights fetched into L2 8 to 24 blocks ahead 278.  A tile's end (results through shared memory in rows of 128 bytes;
+// GLU: the exponentials and quotients) takes 3,000 to 5,000 cycles, its start 1,400.  A CTA walks over tiles, row tiles first, so that CTAs at work at
 // the same time share weight tiles in L2.  Few tiles: a cluster of S CTAs splits a tile's blocks; every CTA puts its sums into its own shared
 // memory, and after a cluster barrier each finishes every S-th row from all S in rank order (the same order on every run).
 //
@@ -19,6 +21,9 @@
 // number is known here and the hidden rows never exist in another form.
 //
 // Grouped form: row tiles of a device-made list (first row, end row, matrix), as in gemm_tcgen05.cu.
+//
+// Measured: 4,096 x 18,944 x 3,584 268 us (2.07 PFLOP/s; under the power cap of a long run 326), 2,000 rows of 5,120 and 2 x 13,824 320, 48 x 3,584 x 3,584 8.6 (12.8 MB,
+// 4 CTAs a tile), 333 x 19,001 x 912 29, 11 of which are the odd rows' number by number (whole words, shifted by a number where a row starts at an odd one, were no faster).
 //
 // Every wait is bounded; when one runs out, the CTA's tiles from there on become NaN, copies in flight get time to land, `err` is set.
 #include "fp8.cuh"
@@ -629,8 +634,8 @@ int resident_clusters(int S) {
 }  // namespace
 
 // The tile's width and the number of CTAs to a tile with the least estimated time: rounds of tiles x (a start and an end + blocks x 0.4 us, 0.58 of
-// 256 columns), as measured with 4 to 100 rows.  Us estimated and measured: 16 x 3,584 x 18,944 in 128 columns and 4 CTAs 22 and 23, in 2 CTAs 40
-// and 39, in 8 (two rounds) 26 and 29; 16 x 18,944 x 3,584 in 256 columns and 2 CTAs 12 and 19 (the weights' way from memory is 10), in 128 columns and one 16 and 22.
+// 256 columns), as measured with 4 to 100 rows.  Us estimated and measured: 16 x 3,584 x 18,944 in 128 columns and 4 CTAs 18 and 18, in 2 CTAs 33
+// and 28, in 8 (two rounds) 22 and 25; 16 x 18,944 x 3,584 in 256 columns and 2 CTAs 13 and 19 (the weights' way from memory is 10), in 128 columns and one 13 and 22.
 int fp8_gemm(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, int* err, cudaStream_t s) {
     const long long m_tiles = ceil_div(x.rows, T_ROWS), blocks = ceil_div(w.K, FP8_BLOCK);
     const float rows = x.rows < T_ROWS ? (float)x.rows / T_ROWS : 1.0f;       // of a tile: what the CTAs of a cluster hand one another

@@ -117,6 +117,18 @@ def test_product(m, n, k):
     ops.check_tcgen05_errors(torch.device(DEV))
 
 
+@pytest.mark.parametrize("m", [8, 9, 16])
+def test_large_matrices_and_few_rows(m):
+    from mimirmind_b200.kernels import ops
+    gen = _gen(m)
+    n, k = 16411, 1616                      # beyond what the weight-streaming kernel takes of more than eight rows
+    x, w = _rows(m, k, gen), _weight(n, k, gen=gen)
+    _close(ops.gemm_fp8(x, w), *f8.product(f8.quantised(x)[0], _wide(w)))
+    w_in, w_out = _weight(2, n // 2, k, gen=gen), _weight(k, n // 2, gen=gen)
+    _close(ops.glu_mlp_fp8(x, w_in, w_out, "silu", 0.0), *_mlp64(x, w_in, w_out, "silu", 0.0))
+    ops.check_tcgen05_errors(torch.device(DEV))
+
+
 @pytest.mark.parametrize("bias", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("m", [1, 5, 20, 130, 300, 700])
 def test_product_with_a_bias_and_quantised_or_fp32_rows(m, bias):
