@@ -2091,6 +2091,7 @@ class Fp8Weight:
                 self.matrices *= self.shape[i]
             if self.matrices < 1:
                 raise KernelError("fp8 weight: there is no matrix")
+        _fp8_error(values)      # made here, not by a first product that is being captured: its noughts would only be written when the graph runs
 
     def float(self) -> torch.Tensor:
         """The numbers that the weight stands for, in fp32."""

@@ -325,6 +325,40 @@ def test_captured_and_on_a_stream_of_its_own(m):
     ops.check_tcgen05_errors(torch.device(DEV))
 
 
+FIRST_CALLS = """
+import torch
+from mimirmind_b200.kernels import ops
+def w(*s):
+    return ops.quantize_fp8_weight((0.02 * torch.randn(s, device="cuda")).bfloat16())
+a, w_in, w_out, e_in, e_out = w(512, 1024), w(2, 256, 1024), w(1024, 256), w(4, 2, 64, 1024), w(4, 1024, 64)
+x, router = torch.randn((40, 1024), device="cuda").bfloat16(), torch.randn((4, 1024), device="cuda")
+idx, wts = torch.arange(80, device="cuda", dtype=torch.int32).view(40, 2) % 4, torch.rand((40, 2), device="cuda")
+def run():
+    return (ops.gemm_fp8(x, a), ops.gemm_fp8(x[:3], a), ops.glu_mlp_fp8(x, w_in, w_out), ops.glu_mlp_fp8(x[:5], w_in, w_out),
+            ops.moe_experts_fp8(x, idx, wts, e_in, e_out), ops.moe_few(x[:7], router, e_in, e_out, 2))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = run()
+eager = run()
+ops.check_tcgen05_errors("cuda")
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) for p, q in zip(got, eager))
+ops.check_tcgen05_errors("cuda")
+print("the same")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=300, cwd=root, env={**os.environ, "PYTHONPATH": root})
+    assert run.returncode == 0 and "the same" in run.stdout, run.stderr[-2000:]
+
+
 def test_refusals():
     from mimirmind_b200.kernels import ops
     from mimirmind_b200.kernels.lib import KernelError
