@@ -61,6 +61,7 @@ struct Fp8Args {
     int out_kind, bias_dtype, act;
     float limit;
     int M, N, K, KB, NB, ldo, S;
+    int t0, t1;                 // the tiles that this launch makes (grouped: up to the list's end)
 };
 
 template <int BN>
@@ -239,9 +240,9 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     const uint32_t tmem_base = ctl->tmem_base;
 
     const int m_tiles = g.tiles ? *g.n_tiles : (g.M + T_ROWS - 1) / T_ROWS, n_tiles = (g.N + (GLU ? 128 : BN) - 1) / (GLU ? 128 : BN);
-    const int total = m_tiles * n_tiles;
+    const int total = g.tiles ? m_tiles * n_tiles : g.t1;
     const int S = SPLIT ? g.S : 1, rank = SPLIT ? (int)cluster_ctarank() : 0;
-    const int first = SPLIT ? blockIdx.x / S : blockIdx.x, step = SPLIT ? 0x40000000 : (int)gridDim.x;      // a split tile has its cluster for itself
+    const int first = g.t0 + (SPLIT ? blockIdx.x / S : blockIdx.x), step = SPLIT ? 0x40000000 : (int)gridDim.x;      // a split tile has its cluster for itself
     const int b_lo = SPLIT ? (int)((long long)g.KB * rank / S) : 0, b_hi = SPLIT ? (int)((long long)g.KB * (rank + 1) / S) : g.KB;
 
     if (warp >= SUM_WARPS) {
@@ -546,14 +547,10 @@ bool make_map_bytes(CUtensorMap* map, const void* base, long long rows, int cols
 
 }  // namespace
 
-// A e4m3 [M, lda], sa fp32 [M, KB]; W e4m3 [matrices * N, ldw], sw fp32 [matrices, NB, KB] (GLU: pairs of matrices, gate and up).
-// glu 0: out [M, ldo] bf16 or fp32 (+ bias [N]); glu 1: out e4m3 [M, ldo] (ldo = N rounded up to 16) and out_scales fp32 [M, NB].
-// tiles, n_tiles, max_tiles: the grouped form's row tiles.  wide: 256 columns a tile instead of 128 (GLU: always).  splits: CTAs that share a tile's
-// blocks (1, 2, 4 or 8; only without a list).
-MM_EXPORT int mm_gemm_fp8_tcgen05(const void* A, long long lda, const void* sa, const void* W, long long ldw, const void* sw, int matrices, void* out,
-                                  int out_dtype, void* out_scales, int ldo, const void* bias, int bias_dtype, int M, int N, int K, int glu, int act, float limit,
-                                  const void* row_scale, const void* order, const void* tiles, const void* n_tiles, int max_tiles, int wide, int splits,
-                                  void* err, void* stream) {
+// tiles t0 .. t1 - 1 (t1 < 0: all of them)
+static int gemm_range(const void* A, long long lda, const void* sa, const void* W, long long ldw, const void* sw, int matrices, void* out, int out_dtype, void* out_scales,
+                      int ldo, const void* bias, int bias_dtype, int M, int N, int K, int glu, int act, float limit, const void* row_scale, const void* order,
+                      const void* tiles, const void* n_tiles, int max_tiles, int wide, int splits, void* err, void* stream, long long t0, long long t1) {
     MM_REQUIRE(M > 0 && M < FP8_MAX && N > 0 && N < FP8_MAX && K > 0 && K < FP8_MAX && matrices > 0 && lda >= K && ldw >= K && ldo >= N, "gemm_fp8: bad sizes");
     MM_REQUIRE(lda % 16 == 0 && ldw % 16 == 0 && (((uintptr_t)A | (uintptr_t)W) & 15) == 0, "gemm_fp8: rows must start on 16-byte boundaries");
     MM_REQUIRE((long long)matrices * N + 256 < 0x7fffffffLL, "gemm_fp8: too many weight rows");
@@ -595,11 +592,25 @@ MM_EXPORT int mm_gemm_fp8_tcgen05(const void* A, long long lda, const void* sa, 
     const int bn = glu ? 128 : (wide ? 256 : 128);
     const long long total = (long long)(tiles ? max_tiles : ceil_div(M, T_ROWS)) * ceil_div(N, bn);
     MM_REQUIRE(total < 0x40000000LL, "gemm_fp8: too many tiles");
+    g.t0 = (int)t0;
+    g.t1 = (int)(t1 < 0 ? total : t1);
     cudaStream_t s = (cudaStream_t)stream;
-    const int grid = splits > 1 ? (int)total * splits : (int)(total < sms ? total : sms);
+    const int count = g.t1 - g.t0, grid = splits > 1 ? count * splits : (count < sms ? count : sms);
     if (glu) return splits > 1 ? launch<256, true, true>(ta, tw, g, grid, s) : launch<256, true, false>(ta, tw, g, grid, s);
     if (wide) return splits > 1 ? launch<256, false, true>(ta, tw, g, grid, s) : launch<256, false, false>(ta, tw, g, grid, s);
     return splits > 1 ? launch<128, false, true>(ta, tw, g, grid, s) : launch<128, false, false>(ta, tw, g, grid, s);
+}
+
+// A e4m3 [M, lda], sa fp32 [M, KB]; W e4m3 [matrices * N, ldw], sw fp32 [matrices, NB, KB] (GLU: pairs of matrices, gate and up).
+// glu 0: out [M, ldo] bf16 or fp32 (+ bias [N]); glu 1: out e4m3 [M, ldo] (ldo = N rounded up to 16) and out_scales fp32 [M, NB].
+// tiles, n_tiles, max_tiles: the grouped form's row tiles.  wide: 256 columns a tile instead of 128 (GLU: always).  splits: CTAs that share a tile's
+// blocks (1, 2, 4 or 8; only without a list).
+MM_EXPORT int mm_gemm_fp8_tcgen05(const void* A, long long lda, const void* sa, const void* W, long long ldw, const void* sw, int matrices, void* out,
+                                  int out_dtype, void* out_scales, int ldo, const void* bias, int bias_dtype, int M, int N, int K, int glu, int act, float limit,
+                                  const void* row_scale, const void* order, const void* tiles, const void* n_tiles, int max_tiles, int wide, int splits,
+                                  void* err, void* stream) {
+    return gemm_range(A, lda, sa, W, ldw, sw, matrices, out, out_dtype, out_scales, ldo, bias, bias_dtype, M, N, K, glu, act, limit, row_scale, order, tiles, n_tiles,
+                      max_tiles, wide, splits, err, stream, 0, -1);
 }
 
 namespace {
@@ -633,25 +644,44 @@ int resident_clusters(int S) {
 
 }  // namespace
 
-// The tile's width and the number of CTAs to a tile with the least estimated time: rounds of tiles x (a start and an end + blocks x 0.4 us, 0.58 of
-// 256 columns), as measured with 4 to 100 rows.  Us estimated and measured: 16 x 3,584 x 18,944 in 128 columns and 4 CTAs 18 and 18, in 2 CTAs 33
+// The tile's width and the number of CTAs to a tile with the least estimated time: rounds of tiles x (a start and an end + blocks x 0.58 us, of 128 columns 0.4, or
+// 0.31 where several row tiles share the weights on their way), as measured with 4 to 100, and 300 to 4,096 rows.  Us estimated and measured: 16 x 3,584 x 18,944 in 128 columns and 4 CTAs 18 and 18, in 2 CTAs 33
 // and 28, in 8 (two rounds) 22 and 25; 16 x 18,944 x 3,584 in 256 columns and 2 CTAs 13 and 19 (the weights' way from memory is 10), in 128 columns and one 13 and 22.
+// Beyond whole rounds, what is left may be split: 2,000 x 5,120 x 13,824 (two rounds and 24 tiles) 166 us in one launch, 145 with the 24 over clusters of 4 behind it;
+// 1,400 x 3,584 x 3,584 (one round and 6 tiles, or 308 of 128 columns) 37 and 34, narrow 32.
 int fp8_gemm(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, int* err, cudaStream_t s) {
     const long long m_tiles = ceil_div(x.rows, T_ROWS), blocks = ceil_div(w.K, FP8_BLOCK);
     const float rows = x.rows < T_ROWS ? (float)x.rows / T_ROWS : 1.0f;       // of a tile: what the CTAs of a cluster hand one another
     int best_wide = 1, best_splits = 1;
+    long long best_whole = 0, best_tiles = 0;
     float best = 1e30f;
-    for (int wide = glu ? 1 : 0; wide < 2; ++wide)
+    for (int wide = glu ? 1 : 0; wide < 2; ++wide) {
+        const long long tiles = m_tiles * ceil_div(w.N, glu || !wide ? 128 : 256), rounds = tiles / FP8_SM_COUNT, rest = tiles % FP8_SM_COUNT;
+        const float block = wide ? 0.58f : m_tiles > 1 ? 0.31f : 0.4f, whole = 2.0f + (float)blocks * block;
         for (int splits = 1; splits <= 8 && splits <= blocks; splits *= 2) {
-            const long long tiles = m_tiles * ceil_div(w.N, glu || !wide ? 128 : 256);
             const int fit = splits == 1 ? FP8_SM_COUNT : glu ? resident_clusters<256, true>(splits) : wide ? resident_clusters<256, false>(splits) : resident_clusters<128, false>(splits);
-            const float us = (float)((tiles + fit - 1) / fit) * ((splits > 1 ? (wide ? 4.0f + 4.0f * rows : 3.0f + 2.0f * rows) : 2.0f) + (float)((blocks + splits - 1) / splits) * (wide ? 0.58f : 0.4f));
-            if (us < best) {
-                best = us;
-                best_wide = wide;
-                best_splits = splits;
+            const float part = splits == 1 ? whole : (wide ? 4.0f + 4.0f * rows : 3.0f + 2.0f * rows) + (float)((blocks + splits - 1) / splits) * block;
+            // every tile so, or whole rounds of tiles first and what is left of them split
+            for (int tail = 0; tail < (splits > 1 && rounds > 0 && rest > 0 ? 2 : 1); ++tail) {
+                const long long here = tail ? rest : tiles;
+                const float us = (tail ? (float)rounds * whole + 3.0f : 0.0f) + (float)((here + fit - 1) / fit) * part;
+                if (us < best) {
+                    best = us;
+                    best_wide = wide;
+                    best_splits = splits;
+                    best_whole = tail ? tiles - rest : 0;
+                    best_tiles = tiles;
+                }
             }
         }
-    return mm_gemm_fp8_tcgen05(x.data, x.ld, x.scales, w.values, w.ld, w.scales, w.matrices, out.data, out.dtype, out.scales, out.ld, out.bias, out.bias_dtype,
-                               x.rows, w.N, w.K, glu, out.act, out.limit, nullptr, nullptr, nullptr, nullptr, 0, best_wide, best_splits, err, s);
+    }
+    auto range = [&](int splits, long long t0, long long t1) {
+        return gemm_range(x.data, x.ld, x.scales, w.values, w.ld, w.scales, w.matrices, out.data, out.dtype, out.scales, out.ld, out.bias, out.bias_dtype, x.rows, w.N, w.K, glu,
+                          out.act, out.limit, nullptr, nullptr, nullptr, nullptr, 0, best_wide, splits, err, s, t0, t1);
+    };
+    if (best_whole > 0) {
+        const int rc = range(1, 0, best_whole);
+        if (rc != MM_OK) return rc;
+    }
+    return range(best_splits, best_whole, best_tiles);
 }

@@ -117,6 +117,20 @@ def test_product(m, n, k):
     ops.check_tcgen05_errors(torch.device(DEV))
 
 
+def test_whole_rounds_of_tiles_and_a_split_rest():
+    from mimirmind_b200.kernels import ops
+    gen = _gen(2000)
+    m, n, k = 2000, 5115, 4080              # 320 tiles of 128 x 256: two rounds of 148 and 24 more
+    x, w, bias = _rows(m, k, gen), _weight(n, k, gen=gen), torch.randn(n, generator=gen, device=DEV)
+    y, err = f8.product(f8.quantised(x)[0], _wide(w))
+    y = y + bias.double()
+    _close(ops.gemm_fp8(x, w, bias), y, err + y.abs() * 2.0 ** -24)
+    _close(ops.gemm_fp8(x, w, bias, torch.float32), y, err + y.abs() * 2.0 ** -24)
+    w_in, w_out = _weight(2, n // 2, k, gen=gen), _weight(200, n // 2, gen=gen)
+    _close(ops.glu_mlp_fp8(x, w_in, w_out, "silu", 0.0), *_mlp64(x, w_in, w_out, "silu", 0.0))
+    ops.check_tcgen05_errors(torch.device(DEV))
+
+
 @pytest.mark.parametrize("m", [8, 9, 16])
 def test_large_matrices_and_few_rows(m):
     from mimirmind_b200.kernels import ops
