@@ -22,7 +22,7 @@
 //
 // Grouped form: row tiles of a device-made list (first row, end row, matrix), as in gemm_tcgen05.cu.
 //
-// Measured: 4,096 x 18,944 x 3,584 268 us (2.07 PFLOP/s; under the power cap of a long run 326), 2,000 rows of 5,120 and 2 x 13,824 320, 48 x 3,584 x 3,584 8.6 (12.8 MB,
+// Measured: 4,096 x 18,944 x 3,584 259 us (2.15 PFLOP/s; under the power cap of a long run 320 to 326), 2,000 rows of 5,120 and 2 x 13,824 299, 48 x 3,584 x 3,584 8.6 (12.8 MB,
 // 4 CTAs a tile), 333 x 19,001 x 912 29, 11 of which are the odd rows' number by number (whole words, shifted by a number where a row starts at an odd one, were no faster).
 //
 // Every wait is bounded; when one runs out, the CTA's tiles from there on become NaN, copies in flight get time to land, `err` is set.
@@ -260,9 +260,9 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                         if (!mbar_wait(smem_u32(&ctl->empty[s]), ((it / L::STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
                         const uint32_t full = smem_u32(&ctl->full[s]), dst = smem_u32(pipe + s * L::STAGE_BYTES);
                         mbar_expect_tx(full, L::STAGE_BYTES);
-                        tma_load_2d(dst, &tmA, b * FP8_BLOCK, x.m0, full);
                         tma_load_2d(dst + HALF_BYTES, &tmW, b * FP8_BLOCK, x.w0, full);
                         if (BN == 256) tma_load_2d(dst + 2 * HALF_BYTES, &tmW, b * FP8_BLOCK, x.w1, full);
+                        tma_load_2d(dst, &tmA, b * FP8_BLOCK, x.m0, full);
                     }
                 }
             }
@@ -282,6 +282,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
 #pragma unroll
                         for (int k = 0; k < 4; ++k)          // 32 numbers a product: 32 bytes on along the swizzled rows
                             umma_e4m3(tmem_base + acc * BN, a_desc + (uint64_t)(k * 2), b_desc + (uint64_t)(k * 2), idesc_e4m3(BN), k ? 1u : 0u);
+                        umma_commit(smem_u32(&ctl->empty[s]));          // (a commit, not a summing thread's arrival: 263 us against 258)
                         umma_commit(smem_u32(&ctl->sum_full[acc]));
                     }
             }
@@ -318,7 +319,6 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->sum_full[ph]), (it >> 1) & 1, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
-                if (threadIdx.x == 0) mbar_arrive(smem_u32(&ctl->empty[it % L::STAGES]));      // the block's products are through: so are its copies
                 // Two pieces are on their way at a time, and the wait is for both: what bounds the loop is how often a warp waits for tensor memory (one
                 // piece at a time: 960 cycles a block).  A piece's registers take the next one as soon as they are multiplied; the accumulator is free once the
                 // last two have arrived.
