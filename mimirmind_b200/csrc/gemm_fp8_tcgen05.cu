@@ -22,7 +22,7 @@
 //
 // Grouped form: row tiles of a device-made list (first row, end row, matrix), as in gemm_tcgen05.cu.
 //
-// Measured: 4,096 x 18,944 x 3,584 259 us (2.15 PFLOP/s; under the power cap of a long run 320 to 326), 2,000 rows of 5,120 and 2 x 13,824 299, 48 x 3,584 x 3,584 8.6 (12.8 MB,
+// Measured: 4,096 x 18,944 x 3,584 259 us (2.15 PFLOP/s; under the power cap of a long run 310), 2,000 rows of 5,120 and 2 x 13,824 299, 48 x 3,584 x 3,584 8.6 (12.8 MB,
 // 4 CTAs a tile), 333 x 19,001 x 912 29, 11 of which are the odd rows' number by number (whole words, shifted by a number where a row starts at an odd one, were no faster).
 //
 // Every wait is bounded; when one runs out, the CTA's tiles from there on become NaN, copies in flight get time to land, `err` is set.
@@ -122,6 +122,23 @@ __device__ __forceinline__ void fma_pair(uint64_t& ab, uint64_t s, uint32_t x, u
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(ab) : "l"(((uint64_t)y << 32) | x), "l"(s));
 }
 __device__ __forceinline__ uint64_t twice(float s) { return ((uint64_t)__float_as_uint(s) << 32) | __float_as_uint(s); }
+
+// mbar_wait for the warps that copy and issue: they sleep on the barrier, a microsecond at the most, instead of asking it time and again beside the summing
+// warps (4,096 x 18,944 x 3,584 under the power cap 300 us, so 295; the summing warps themselves lose by it, 306).  Bounded all the same: under 3 s.
+__device__ __forceinline__ bool mbar_sleep(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    for (uint32_t it = 0; it < (1u << 21); ++it) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+        if (ok) return true;
+        if ((it & 255u) == 255u && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    return false;
+}
 
 __device__ __forceinline__ float bias_at(const Fp8Args& g, int n) {
     return g.bias_dtype == MM_F32 ? ((const float*)g.bias)[n] : __bfloat162float(((const __nv_bfloat16*)g.bias)[n]);
@@ -257,7 +274,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                     for (int b = b_lo; b < b_hi; ++b, ++it) {
                         const int s = it % L::STAGES;
                         if ((it & 1) != turn) continue;
-                        if (!mbar_wait(smem_u32(&ctl->empty[s]), ((it / L::STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                        if (!mbar_sleep(smem_u32(&ctl->empty[s]), ((it / L::STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
                         const uint32_t full = smem_u32(&ctl->full[s]), dst = smem_u32(pipe + s * L::STAGE_BYTES);
                         mbar_expect_tx(full, L::STAGE_BYTES);
                         tma_load_2d(dst + HALF_BYTES, &tmW, b * FP8_BLOCK, x.w0, full);
@@ -276,8 +293,8 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                         if (acc != turn) continue;
                         const uint32_t a_addr = smem_u32(pipe + s * L::STAGE_BYTES);
                         const uint64_t a_desc = smem_desc_sw128(a_addr, 16, 1024), b_desc = smem_desc_sw128(a_addr + HALF_BYTES, 16, 1024);
-                        if (!mbar_wait(smem_u32(&ctl->full[s]), (it / L::STAGES) & 1, abort_flag) ||
-                            !mbar_wait(smem_u32(&ctl->sum_empty[acc]), ((it >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                        if (!mbar_sleep(smem_u32(&ctl->full[s]), (it / L::STAGES) & 1, abort_flag) ||
+                            !mbar_sleep(smem_u32(&ctl->sum_empty[acc]), ((it >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
                         tc_fence_after();
 #pragma unroll
                         for (int k = 0; k < 4; ++k)          // 32 numbers a product: 32 bytes on along the swizzled rows
