@@ -13,7 +13,7 @@
 //
 // Few rows are quantised here (every warp its own run of blocks, into shared memory) instead of by a launch of their own in front of this one.
 //
-// Bound by memory where the matrix is large: 1 x 152,064 x 3,584 89 us (6.1 TB/s of 6.55).  Smaller ones by the launch, the first block's way from memory and the
+// Bound by memory where the matrix is large: 1 x 152,064 x 3,584 87 us (6.2 TB/s of 6.55).  Smaller ones by the launch, the first block's way from memory and the
 // ends of the runs: 8 x 18,944 x 3,584 12.4 to 16 us (68 MB, floor 10.4), 8 x 4,608 x 3,584 5.9 to 7 us (16.5 MB, floor 2.5).  Four blocks on their way
 // instead of three were no faster; a ring in registers instead of shared memory spilled.
 #include "fp8.cuh"
@@ -385,8 +385,9 @@ int fp8_gemv(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, bool 
     g.KB = ceil_div(w.K, FP8_BLOCK);
     g.NB = ceil_div(w.N, FP8_BLOCK);
     g.tiles = ceil_div(w.N, 16);
-    // Tiles side by side in a CTA (8, 4, 2, 1) as long as there are one and a half CTAs an SM: the runs of blocks are longer and the
-    // warps meet less often.  No more runs than blocks.
+    // Tiles side by side in a CTA (8, 4, 2, 1) and runs of blocks (no more than blocks): the least number of blocks that a warp goes through one after the other, a meeting
+    // of the warps counted as one, and less than one and a half CTAs an SM as that much less bandwidth.  Us of 8, 4, 2 and 1 tiles: one row of 27,648 x 5,120 28.8, 31.2,
+    // 26.5, 27.1; 65,536 x 3,584 44.2, 43.9, 40.1, 43.7; 32,768 x 1,024 9.8, 10.5, 11.4, 12.1; 18,944 x 3,584 17.2, 14.8, 14.6, 15.5; eight rows of 152,064 x 3,584 99, 94, 92, 96.
     int grid;
     if (glu) {
         g.S = 1;
@@ -398,9 +399,15 @@ int fp8_gemv(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, bool 
         }
         grid = g.NB * g.S;
     } else {
-        g.RT = GV_WARPS;
-        while (g.RT > 1 && ceil_div(g.tiles, g.RT) < FP8_SM_COUNT * 3 / 2) g.RT /= 2;
-        while (GV_WARPS / g.RT > g.KB) g.RT *= 2;
+        float best = 1e30f;
+        for (int rt = GV_WARPS; rt >= 1 && GV_WARPS / rt <= g.KB; rt /= 2) {
+            const int n = ceil_div(g.tiles, rt);
+            const float cost = (float)ceil_div(n, 2 * FP8_SM_COUNT) * ((float)g.KB * rt / GV_WARPS + 1.0f) * (n < FP8_SM_COUNT * 3 / 2 ? FP8_SM_COUNT * 1.5f / n : 1.0f);
+            if (cost < best) {
+                best = cost;
+                g.RT = rt;
+            }
+        }
         const int groups = ceil_div(g.tiles, g.RT);
         grid = groups < 2 * FP8_SM_COUNT ? groups : 2 * FP8_SM_COUNT;
     }
