@@ -24,18 +24,21 @@ __device__ __forceinline__ float fp8_scale_of(uint32_t largest_bits) {
 // v[i] = fl(v[i] / s).  The quotient by Markstein's division theorem (P. Markstein, Computation of elementary functions on the IBM RISC
 // System/6000 processor, 1990): with r = fl(1 / s) and q = fl(v r), fl(q + r (v - q s)) is v / s rounded, as long as the remainder is no
 // subnormal that lost bits: s of 2^-80 and more, where numbers so small that it is (below 2^-100) come out as nought in e4m3 either way.
+// Smaller and very large scales are brought there first, with their numbers, by a power of two: what a large one's numbers lose that way (below 2^-62 of them)
+// is nought in e4m3 too.  An infinite s gives nought for a finite number and NaN for an infinite one, as the division does.
 template <int N>
 __device__ __forceinline__ void fp8_quotients(float* v, float s) {
-    if (s >= 8.27180613e-25f && s < 1e30f) {
-        const float r = __fdiv_rn(1.0f, s);
+    if (!(s >= 8.27180613e-25f && s < 1e30f)) {
+        const float k = s < 1.0f ? 18446744073709551616.0f : 5.42101086e-20f;      // 2^64, 2^-64
+        s *= k;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float q = v[i] * r;
-            v[i] = fmaf(fmaf(-q, s, v[i]), r, q);
-        }
-    } else {
+        for (int i = 0; i < N; ++i) v[i] *= k;
+    }
+    const float r = __fdiv_rn(1.0f, s), d = r == 0.0f ? 0.0f : s;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = __fdiv_rn(v[i], s);
+    for (int i = 0; i < N; ++i) {
+        const float q = v[i] * r;
+        v[i] = fmaf(fmaf(-q, d, v[i]), r, q);
     }
 }
 

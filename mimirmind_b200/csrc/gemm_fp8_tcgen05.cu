@@ -399,7 +399,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 ok = __all_sync(0xffffffffu, ok && mbar_wait(smem_u32(&ctl->row_known[q]), known & 1, abort_flag));
                 ++known;
                 const float s = ok ? fp8_scale_of(max(sizes[0], sizes[32])) : __uint_as_float(0x7fffffffu);
-                const float inv = __fdiv_rn(1.0f, s);      // the sums are no closer to their exact values than a product with this to the quotient
+                fp8_quotients<COLS / 2>(acc, s);
                 if (row < x.hi) {
                     if (part == 0) g.out_scales[(size_t)row * g.NB + x.n0 / 128] = s;
                     uint8_t* dst = (uint8_t*)g.out + (size_t)row * g.ldo + n0;
@@ -407,7 +407,7 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                     for (int i = 0; i < COLS / 2; i += 16) {
                         uint32_t p[4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) p[j] = fp8_pack4(acc[i + 4 * j] * inv, acc[i + 4 * j + 1] * inv, acc[i + 4 * j + 2] * inv, acc[i + 4 * j + 3] * inv);
+                        for (int j = 0; j < 4; ++j) p[j] = fp8_pack4(acc[i + 4 * j], acc[i + 4 * j + 1], acc[i + 4 * j + 2], acc[i + 4 * j + 3]);
                         if (n0 + i < g.ldo) *reinterpret_cast<uint4*>(dst + i) = make_uint4(p[0], p[1], p[2], p[3]);
                     }
                 }
@@ -475,11 +475,11 @@ gemm_fp8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                             if (n + i >= g.N) h[i] = 0.0f;
                             largest = max(largest, fp8_size_bits(h[i]));
                         }
-                        const float s = fp8_scale_of(__reduce_max_sync(0xffffffffu, largest)), inv = __fdiv_rn(1.0f, s);
+                        const float s = fp8_scale_of(__reduce_max_sync(0xffffffffu, largest));
+                        fp8_quotients<4>(h, s);
                         if (lane == 0) g.out_scales[(size_t)row * g.NB + x.n0 / 128] = s;
                         if (n < g.ldo)
-                            *reinterpret_cast<uint32_t*>((uint8_t*)g.out + (size_t)row * g.ldo + n) =
-                                fp8_pack4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+                            *reinterpret_cast<uint32_t*>((uint8_t*)g.out + (size_t)row * g.ldo + n) = fp8_pack4(h[0], h[1], h[2], h[3]);
                     } else {
 #pragma unroll
                         for (int j = 0; j < BN / 128; ++j) {

@@ -302,12 +302,14 @@ __global__ void __launch_bounds__(GV_THREADS, 2) gemv_fp8_kernel(const __grid_co
                 asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
                 big = max(big, v);
             }
-            const float s = fp8_scale_of(big), inv = __fdiv_rn(1.0f, s);
+            const float s = fp8_scale_of(big);
             if (rank == 0 && lane == 0) g.out_scales[(size_t)tok * g.NB + first] = s;
             const int c = lane * 4, f = first * 128 + rank * cols + c;
             if (c < cols && f < g.ldo) {
-                const float* h = hidden + tok * cols + c;
-                *reinterpret_cast<uint32_t*>((uint8_t*)g.out + (size_t)tok * g.ldo + f) = fp8_pack4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+                const float* from = hidden + tok * cols + c;
+                float h[4] = {from[0], from[1], from[2], from[3]};
+                fp8_quotients<4>(h, s);
+                *reinterpret_cast<uint32_t*>((uint8_t*)g.out + (size_t)tok * g.ldo + f) = fp8_pack4(h[0], h[1], h[2], h[3]);
             }
         }
         __syncwarp();
