@@ -16,8 +16,9 @@
 // Experts in bf16: x as it is, the fp32 hidden rows as two bf16 parts (2^-17 of a number is lost).
 // Experts in e4m3 with a scale per block of 128 x 128: a row of x, after a power of two that brings its largest number to 2^7 .. 2^8, is two e4m3 parts, hi and
 // 16 lo: together bf16's eight bits (a number below 2^-13 of the row's largest loses what is below 2^-21 of it).  Four tokens' parts are the eight
-// columns, so the weights are multiplied as they lie.  The hidden rows become fp16 (11 bits; rounding them to bf16 would cost as much again as rounding
-// the result) after a power of two that brings their largest number to 2^14 .. 2^15, and the weights beside them fp16, exactly.
+// columns, so the weights are multiplied as they lie.  The hidden rows become two fp16 parts (22 bits) after a power of two that brings their largest number
+// to 2^14 .. 2^15, beside the weights in fp16, exactly.  (One part, 11 bits, moved one result in ten to the neighbouring bf16 number; the second takes 1 token
+// from 25.8 to 26.0 us, 8 tokens from 71.4 to 74.8, 16 tokens from 97.7 to 103.5.)
 //
 // Bound by memory for the experts' matrices (one token, 128 experts of 768 and 2,048 wide, 8 of them, in 8 bits: 38 MB, 5.9 us), but the fixed parts weigh as much:
 // the router about 5 us (830 cycles a step and warp, of loads in a ring or not, of conversions or not), the choice 3, cluster barriers and set-up 3, the second
@@ -79,6 +80,12 @@ __device__ __forceinline__ uint32_t pair_bf16(float lo, float hi) {
 __device__ __forceinline__ uint32_t pair_f16(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+// how far a pair of fp16 numbers is above (x, y), as a pair
+__device__ __forceinline__ uint32_t f16_excess(uint32_t pair, float x, float y) {
+    float a, b;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\tsub.rn.f32.f16 %1, h, %4;\n\t}" : "=f"(a), "=f"(b) : "r"(pair), "f"(x), "f"(y));
+    return pair_f16(a, b);
 }
 __device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
 __device__ __forceinline__ float low_of(uint32_t bf16_pair) { return __uint_as_float(bf16_pair << 16); }
@@ -808,8 +815,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
     while (item < items) {
-        // the operand's pairs: fp16, or two bf16 parts
-        uint2 high[2][HW], low[2][FP8 ? 1 : HW];
+        // the operand's pairs: two fp16 (the second with its sign turned) or bf16 parts
+        uint2 high[2][HW], low[2][HW];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -817,11 +824,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
                 const float4 v = next[h][i];
                 if (FP8) {
                     const float2 a = times(v.x, v.y, here.scale), b = times(v.z, v.w, here.scale);
-                    high[h][i] = make_uint2(pair_f16(a.x, a.y), pair_f16(b.x, b.y));
+                    const uint2 p = make_uint2(pair_f16(a.x, a.y), pair_f16(b.x, b.y));
+                    high[h][i] = p;
+                    low[h][i] = make_uint2(f16_excess(p.x, a.x, a.y), f16_excess(p.y, b.x, b.y));
                 } else {
                     const uint2 p = make_uint2(pair_bf16(v.x, v.y), pair_bf16(v.z, v.w));
                     high[h][i] = p;
-                    low[h][FP8 ? 0 : i] = make_uint2(pair_bf16(v.x - low_of(p.x), v.y - high_of(p.x)), pair_bf16(v.z - low_of(p.y), v.w - high_of(p.y)));
+                    low[h][i] = make_uint2(pair_bf16(v.x - low_of(p.x), v.y - high_of(p.x)), pair_bf16(v.z - low_of(p.y), v.w - high_of(p.y)));
                 }
             }
         const float s0 = s_next;
@@ -845,15 +854,16 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_out_kernel(const __grid_co
                     uint32_t a0, a1, a2, a3;
                     f16_of(lw[i], a0, a2);
                     f16_of(hw[i], a1, a3);
-                    mma_f16_f32(c[h], a0, a1, a2, a3, high[h][i].x, high[h][i].y);
+                    mma_f16_f32(c[0], a0, a1, a2, a3, high[h][i].x, high[h][i].y);
+                    mma_f16_f32(c[1], a0, a1, a2, a3, low[h][i].x, low[h][i].y);
                 } else {
                     mma_bf16_f32(c[0], lw[2 * i], hw[2 * i], lw[2 * i + 1], hw[2 * i + 1], high[h][i].x, high[h][i].y);
-                    mma_bf16_f32(c[1], lw[2 * i], hw[2 * i], lw[2 * i + 1], hw[2 * i + 1], low[h][FP8 ? 0 : i].x, low[h][FP8 ? 0 : i].y);
+                    mma_bf16_f32(c[1], lw[2 * i], hw[2 * i], lw[2 * i + 1], hw[2 * i + 1], low[h][i].x, low[h][i].y);
                 }
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = FP8 ? fmaf(s0, c[0][i] + c[1][i], acc[i]) : acc[i] + (c[0][i] + c[1][i]);
+        for (int i = 0; i < 4; ++i) acc[i] = FP8 ? fmaf(s0, c[0][i] - c[1][i], acc[i]) : acc[i] + (c[0][i] + c[1][i]);
         load(slot);
         few_commit();
         slot = slot + 1 == FEW_RING ? 0 : slot + 1;

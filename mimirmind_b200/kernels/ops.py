@@ -2285,7 +2285,7 @@ def moe_few(x: torch.Tensor, w_router: torch.Tensor, w_in, w_out, top: int, grou
     :func:`moe_router`: ``top``, ``groups``, ``keep``, ``scoring``, ``renorm``, ``scale``, ``correction``, ``group_score``; ``w_router`` fp32 [E, D]) and
     ``out[t] = sum_c wts[t, c] Wd_e act(Wg_e x_t, Wu_e x_t)``, ``e`` the token's c-th choice, as bf16 [n, D].  Experts in bf16: ``w_in`` [E, 2F, D], the gate's rows then the
     up rows of every expert (``interleaved``: alternating in blocks of 8), ``w_out`` [E, D, F]; or in 8 bits: :class:`Fp8Weight` [E, 2, F, D] and [E, D, F]
-    (the rows keep bf16's bits, as two e4m3 parts; the hidden rows become fp16 after a power of two).  ``activation``, ``limit``: as for :func:`moe_gemm`; ``weight_on`` ``input``: the weight
+    (the rows keep bf16's bits, as two e4m3 parts; the hidden rows become two fp16 parts after a power of two).  ``activation``, ``limit``: as for :func:`moe_gemm`; ``weight_on`` ``input``: the weight
     multiplies the first products.  D and F are multiples of 8; a row of x starts on a 16-byte boundary."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() != 2:
         raise KernelError("moe_few: expected bfloat16 rows on a CUDA device")
