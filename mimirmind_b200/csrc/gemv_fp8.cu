@@ -33,8 +33,8 @@ struct GemvArgs {
     const void* bias;
     void* out;                  // [m, ldo] bf16 or fp32; GLU: e4m3
     float* out_scales;          // GLU: [m, NB]
-    long long ldx, ldw;
-    int x_dtype, ldq, bias_dtype, out_dtype, act;
+    long long ldx, ldq, ldw;
+    int x_dtype, bias_dtype, out_dtype, act;
     float limit;
     int m, N, K, KB, NB, ldo, RT, KS, S, tiles;
 };
@@ -368,7 +368,7 @@ int fp8_gemv(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, bool 
     g.q = (const uint8_t*)x.data;
     g.sa = x.scales;
     g.ldx = x.ld;
-    g.ldq = (int)x.ld;
+    g.ldq = x.ld;
     g.x_dtype = x.dtype;
     g.W = (const uint8_t*)w.values;
     g.sw = w.scales;
