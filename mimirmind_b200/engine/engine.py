@@ -73,13 +73,14 @@ class Engine:
     def cache_tokens_that_fit(model: Model, page_size: int, max_context: int, token_budget: int, max_active: int,
                               fraction: float) -> int:
         """The pool size when none is configured: what fits in ``fraction`` of the device memory that is free now
-        (the weights are loaded), less what a step of ``token_budget`` tokens needs, at most
-        ``max_context x max_active`` tokens."""
+        (the weights are loaded; what loading and quantising them took and gave back is handed to the device first), less what a step of
+        ``token_budget`` tokens needs, at most ``max_context x max_active`` tokens."""
         from ..cache import sizing
         from ..parts.moe import fp8_step_bytes
         from ..weights.store import layer_scratch_bytes, layer_tensor_shapes
         esz = 4 if model.rt.dtype == torch.float32 else 2
         shapes = layer_tensor_shapes(model.spec)
+        torch.cuda.empty_cache()
         free, _total = torch.cuda.mem_get_info(model.rt.device)
         scratch = layer_scratch_bytes(model.spec, token_budget + max_active, max_active, esz)
         if model.rt.weights == "fp8":
