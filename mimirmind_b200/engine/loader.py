@@ -8,7 +8,7 @@ import torch
 from ..config.spec import ModelSpec
 from ..parts.base import Runtime
 from ..registry import _ensure_builtin
-from ..weights.store import load_spec, load_tensors, parse_dtype, random_tensors
+from ..weights.store import load_spec, parse_dtype, random_tensors_on_demand, tensors_on_demand
 from .model import Model
 
 
@@ -42,13 +42,12 @@ def load_model(model_dir: str, dtype="bfloat16", device=None, matmul: str = "aut
     _ensure_builtin()
     rt = make_runtime(dtype, device, matmul, weights)
     cfg, spec = load_spec(model_dir)
-    tensors = load_tensors(model_dir, spec, rt.dtype, rt.device)
-    return Model(spec, tensors, rt), cfg
+    with tensors_on_demand(model_dir, spec, rt.dtype, rt.device) as tensors:
+        return Model(spec, tensors, rt), cfg
 
 
 def random_model(spec: ModelSpec, seed: int, dtype="bfloat16", device=None, matmul: str = "auto", weights: str = "stored") -> Model:
     """A model with seeded random weights made directly on the device (no folder written)."""
     _ensure_builtin()
     rt = make_runtime(dtype, device, matmul, weights)
-    tensors = random_tensors(spec, seed, rt.dtype, rt.device)
-    return Model(spec, tensors, rt)
+    return Model(spec, random_tensors_on_demand(spec, seed, rt.dtype, rt.device), rt)

@@ -12,10 +12,11 @@ fp32 (exact).
 """
 from __future__ import annotations
 
+import contextlib
 import hashlib
 import json
 import os
-from typing import Dict, Iterable, Optional, Tuple
+from typing import Callable, Dict, Iterable, Iterator, Optional, Tuple
 
 import torch
 
@@ -95,19 +96,60 @@ def load_spec(model_dir: str):
     return cfg, entry.build_spec(cfg)
 
 
+class TensorsOnDemand:
+    """Name → tensor like a dict, but a tensor is made when a part asks for it: a part that keeps another form of its tensors (in 8
+    bits) gives the stored form up before the next part's is made.  What ``pop`` hands out is not kept here."""
+
+    def __init__(self, names: Iterable[str], make: Callable[[str], torch.Tensor]):
+        self._names = set(names)
+        self._make = make
+        self._made: Dict[str, torch.Tensor] = {}
+
+    def __contains__(self, name: str) -> bool:
+        return name in self._names
+
+    def __getitem__(self, name: str) -> torch.Tensor:
+        if name not in self._names:
+            raise KeyError(name)
+        if name not in self._made:
+            self._made[name] = self._make(name)
+        return self._made[name]
+
+    def pop(self, name: str) -> torch.Tensor:
+        t = self[name]
+        self._names.discard(name)
+        del self._made[name]
+        return t
+
+
+def _open_folder(model_dir: str, spec: ModelSpec) -> SafetensorsFolder:
+    """The folder's tensors, validated against the spec."""
+    want = expected_tensors(spec)
+    folder = SafetensorsFolder(model_dir)
+    # the comparison and its one message are the container library's (csrc/host/safetensors.cpp)
+    message = folder.mismatch({n: (tuple(ts.shape), ts.optional) for n, ts in want.items()}, model_dir)
+    if message is not None:
+        folder.close()
+        raise WeightsError(message)
+    return folder
+
+
+def _read(folder: SafetensorsFolder, name: str, run_dtype: torch.dtype, device) -> torch.Tensor:
+    t = folder.tensor(name)
+    return t.to(device=device, dtype=_storage_dtype(t, run_dtype))
+
+
 def load_tensors(model_dir: str, spec: ModelSpec, run_dtype: torch.dtype, device) -> Dict[str, torch.Tensor]:
     """All tensors of the folder, validated against the spec, converted and moved to ``device``."""
-    want = expected_tensors(spec)
-    with SafetensorsFolder(model_dir) as folder:
-        # the comparison and its one message are the container library's (csrc/host/safetensors.cpp)
-        message = folder.mismatch({n: (tuple(ts.shape), ts.optional) for n, ts in want.items()}, model_dir)
-        if message is not None:
-            raise WeightsError(message)
-        out: Dict[str, torch.Tensor] = {}
-        for name in folder.names():
-            t = folder.tensor(name)
-            out[name] = t.to(device=device, dtype=_storage_dtype(t, run_dtype))
-    return out
+    with _open_folder(model_dir, spec) as folder:
+        return {name: _read(folder, name, run_dtype, device) for name in folder.names()}
+
+
+@contextlib.contextmanager
+def tensors_on_demand(model_dir: str, spec: ModelSpec, run_dtype: torch.dtype, device) -> Iterator[TensorsOnDemand]:
+    """The same, each tensor read when it is asked for (while the context is open)."""
+    with _open_folder(model_dir, spec) as folder:
+        yield TensorsOnDemand(folder.names(), lambda name: _read(folder, name, run_dtype, device))
 
 
 # ---- random weights ---------------------------------------------------------
@@ -123,44 +165,50 @@ def _tensor_seed(seed: int, name: str) -> int:
     return int.from_bytes(h[:8], "little") & 0x7FFFFFFFFFFFFFFF
 
 
-def random_tensors(spec: ModelSpec, seed: int, dtype: torch.dtype, device="cpu") -> Dict[str, torch.Tensor]:
-    """Seeded random weights for every declared tensor: matrices, tables and biases ~ N(0, 0.02),
+def _random_tensor(name: str, ts: TensorSpec, seed: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    gen = torch.Generator(device=device)
+    gen.manual_seed(_tensor_seed(seed, name))
+    x = torch.randn(ts.shape, generator=gen, device=device, dtype=torch.float32)
+    if ts.role == "norm":
+        x = 1.0 + NORM_STD * x
+    elif ts.role == "norm0":          # a norm weight stored around zero
+        x = NORM_STD * x
+    elif ts.role == "taps":           # a short convolution: a few taps per channel
+        x = 0.5 * x
+    elif ts.role == "router":         # spread enough that the choice of experts is not a near tie
+        x = 0.2 * x
+    elif ts.role == "bias":
+        x = BIAS_STD * x
+    elif ts.role == "stream_read":    # how a sublayer reads several residual streams: near their mean
+        x = 1.0 / ts.shape[0] + 0.05 * x
+    elif ts.role == "stream_mix":     # how the streams are carried on: near the identity
+        x = torch.eye(ts.shape[0], device=device) + 0.05 * x
+    elif ts.role == "mix":
+        x = (0.5 + MIX_STD * x).clamp(0.05, 0.95)
+    elif ts.role == "lower_bound":    # the floor of a forget gate: inside (0, 1)
+        x = torch.sigmoid(x)
+    elif ts.role == "head_mix":       # how the heads' scores are mixed: near the identity
+        x = torch.eye(ts.shape[0], device=device) + 0.3 * x
+    else:
+        x = MATRIX_STD * x
+    return x.to(dtype)
+
+
+def random_tensors_on_demand(spec: ModelSpec, seed: int, dtype: torch.dtype, device="cpu") -> TensorsOnDemand:
+    """Seeded random weights for every declared tensor, each made when it is asked for: matrices, tables and biases ~ N(0, 0.02),
     norm weights ~ 1 + N(0, 0.1).  Each tensor has its own stream keyed by (seed, name)."""
     device = torch.device(device)
-    out: Dict[str, torch.Tensor] = {}
-    for name, ts in expected_tensors(spec).items():
-        if ts.optional:
-            continue
+    want = {name: ts for name, ts in expected_tensors(spec).items() if not ts.optional}
+    for name, ts in want.items():
         if any(int(x) < 0 for x in ts.shape):
             raise WeightsError(f"tensor '{name}' has an extent that only a checkpoint gives; the configuration must name it for random weights")
-        gen = torch.Generator(device=device)
-        gen.manual_seed(_tensor_seed(seed, name))
-        x = torch.randn(ts.shape, generator=gen, device=device, dtype=torch.float32)
-        if ts.role == "norm":
-            x = 1.0 + NORM_STD * x
-        elif ts.role == "norm0":          # a norm weight stored around zero
-            x = NORM_STD * x
-        elif ts.role == "taps":           # a short convolution: a few taps per channel
-            x = 0.5 * x
-        elif ts.role == "router":         # spread enough that the choice of experts is not a near tie
-            x = 0.2 * x
-        elif ts.role == "bias":
-            x = BIAS_STD * x
-        elif ts.role == "stream_read":    # how a sublayer reads several residual streams: near their mean
-            x = 1.0 / ts.shape[0] + 0.05 * x
-        elif ts.role == "stream_mix":     # how the streams are carried on: near the identity
-            x = torch.eye(ts.shape[0], device=device) + 0.05 * x
-        elif ts.role == "mix":
-            x = (0.5 + MIX_STD * x).clamp(0.05, 0.95)
-        elif ts.role == "lower_bound":    # the floor of a forget gate: inside (0, 1)
-            x = torch.sigmoid(x)
-        elif ts.role == "head_mix":       # how the heads' scores are mixed: near the identity
-            x = torch.eye(ts.shape[0], device=device) + 0.3 * x
-        else:
-            x = MATRIX_STD * x
-        out[name] = x.to(dtype)
-        del x
-    return out
+    return TensorsOnDemand(want, lambda name: _random_tensor(name, want[name], seed, dtype, device))
+
+
+def random_tensors(spec: ModelSpec, seed: int, dtype: torch.dtype, device="cpu") -> Dict[str, torch.Tensor]:
+    """The same, all of them at once."""
+    made = random_tensors_on_demand(spec, seed, dtype, device)
+    return {name: made.pop(name) for name, ts in expected_tensors(spec).items() if not ts.optional}
 
 
 _DTYPE_NAMES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "fp32": torch.float32, "bf16": torch.bfloat16}

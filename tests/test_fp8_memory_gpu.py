@@ -35,3 +35,22 @@ def test_the_cache_is_sized_with_what_quantising_gave_back():
     torch.cuda.empty_cache()
     assert torch.cuda.memory_reserved() - torch.cuda.memory_allocated() < 128 * MIB
     assert abs(found - _fits(model)) < 64 * MIB
+
+
+def test_a_model_is_quantised_as_it_is_loaded(tmp_path):
+    """16 layers of 48 MiB of feed-forwards in bf16: at no time are all of them on the device"""
+    from mimirmind_b200.engine.loader import load_model, random_model
+    from mimirmind_b200.registry import _ensure_builtin, get_architecture
+    from mimirmind_b200.weights import write_random_model
+    _ensure_builtin()
+    config = dict(CONFIG, intermediate_size=8192, num_hidden_layers=16)
+    arch = get_architecture("Qwen2ForCausalLM")
+    spec = arch.build_spec(arch.parse_config(config, "test"))
+    write_random_model(str(tmp_path), config, 1, "bfloat16")
+    for load in (lambda: random_model(spec, 1, "bfloat16", weights="fp8"), lambda: load_model(str(tmp_path), "bfloat16", weights="fp8")[0]):
+        torch.cuda.empty_cache()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        model = load()
+        assert torch.cuda.max_memory_allocated() - before < 16 * 48 * MIB
+        del model
