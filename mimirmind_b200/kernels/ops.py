@@ -2182,6 +2182,16 @@ def _fp8_scratch(m: int, k: int) -> int:
     return m * ((k + 15) // 16 * 16) + (4 * m * _blocks(k) + 15) // 16 * 16
 
 
+def glu_mlp_fp8_scratch(m: int, k: int, f: int) -> int:
+    """Bytes of scratch that :func:`glu_mlp_fp8` takes."""
+    return _fp8_scratch(m, k) + _fp8_scratch(m, f)
+
+
+def moe_experts_fp8_scratch(n: int, d: int, f: int, experts: int, top: int) -> int:
+    """Bytes of scratch that :func:`moe_experts_fp8` takes (0: sizes that it refuses, and no rows)."""
+    return _lib.load().mm_fp8_moe_experts_scratch(n, d, f, experts, top)
+
+
 def gemm_fp8(x, w: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """x [m, K] times a weight [N, K] in 8 bits (+ bias [N]): ``sum_b sx[m, b] sw[n / 128, b] sum_{k in b} qx[m, k] qw[n, k]``, sums in
     fp32, rounded once to ``out_dtype`` (bf16 or fp32).  ``x``: :class:`Fp8Rows`, or bf16 or fp32 rows, which are quantised first
@@ -2225,7 +2235,7 @@ def glu_mlp_fp8(x, w_in: Fp8Weight, w_out: Fp8Weight, activation: str = "silu", 
     ptr, code, ld, scales, m = _fp8_input(x, k, "glu_mlp_fp8")
     d = w_out.shape[0]
     out = x.new_empty((m, d)) if code == BF16 else torch.empty((m, d), dtype=torch.bfloat16, device=w_in.values.device)
-    scratch = w_in.values.new_empty(_fp8_scratch(m, k) + _fp8_scratch(m, f))
+    scratch = w_in.values.new_empty(glu_mlp_fp8_scratch(m, k, f))
     check(_lib.load().mm_fp8_glu_mlp(ptr, code, ld, scales, m, w_in.values.data_ptr(), w_in.ld, w_in.scales.data_ptr(), f, k, w_out.values.data_ptr(), w_out.ld,
                                      w_out.scales.data_ptr(), d, act, float(limit), out.data_ptr(), scratch.data_ptr(),
                                      _fp8_error(w_in.values), _stream()), "glu_mlp_fp8")
@@ -2263,7 +2273,7 @@ def moe_experts_fp8(x: torch.Tensor, idx: torch.Tensor, wts: torch.Tensor, w_in:
     if n == 0:
         return out
     lib = _lib.load()
-    scratch = w_in.values.new_empty(lib.mm_fp8_moe_experts_scratch(n, d, f, E, top))
+    scratch = w_in.values.new_empty(moe_experts_fp8_scratch(n, d, f, E, top))
     check(lib.mm_fp8_moe_experts(x.data_ptr(), code, n, d, idx.data_ptr(), wts.data_ptr(), top, E, w_in.values.data_ptr(), w_in.ld, w_in.scales.data_ptr(), f,
                                  w_out.values.data_ptr(), w_out.ld, w_out.scales.data_ptr(), act, float(limit), int(weight_on == "input"), out.data_ptr(),
                                  scratch.data_ptr(), _fp8_error(w_in.values), _stream()), "moe_experts_fp8")
@@ -2276,6 +2286,11 @@ MOE_FEW_TOKENS = 16         # rows of a step that a routed-experts layer takes i
 def moe_few_supported(n: int, experts: int, top: int, d: int, f: int) -> bool:
     """True if :func:`moe_few` takes a layer of these sizes."""
     return 0 <= n <= MOE_FEW_TOKENS and 1 <= experts <= 512 and 1 <= top <= min(32, experts) and d % 8 == 0 and f % 8 == 0 and d > 0 and f > 0
+
+
+def moe_few_scratch(n: int, top: int, d: int, f: int) -> int:
+    """Bytes of scratch that :func:`moe_few` takes."""
+    return n * top * (4 * f + f // 2 + 24) + 32 + 36 * n * (d + 160)
 
 
 def moe_few(x: torch.Tensor, w_router: torch.Tensor, w_in, w_out, top: int, groups: int = 1, keep: int = 1, *, scoring: str = "softmax",
@@ -2323,7 +2338,7 @@ def moe_few(x: torch.Tensor, w_router: torch.Tensor, w_in, w_out, top: int, grou
     act = _glu_code(activation, limit, "moe_few")
     _here("moe_few", x, w_router, correction, *tensors)
     out = x.new_empty((n, d))
-    scratch = x.new_empty((n * top * (4 * f + f // 2 + 24) + 32 + 36 * n * (d + 160)) // 2)      # (in numbers of two bytes)
+    scratch = x.new_empty(moe_few_scratch(n, top, d, f) // 2)      # (in numbers of two bytes)
     check(_lib.load().mm_moe_few(x.data_ptr(), ldx, n, d, w_router.data_ptr(), E, int(top), int(groups), int(keep), ROUTER_SCORINGS[scoring], _ptr(correction),
                                  GROUP_SCORES[group_score], int(scoring == "softmax" if renorm is None else renorm), float(scale), tensors[0].data_ptr(), _ptr(tensors[1]),
                                  ld_in, tensors[2].data_ptr(), _ptr(tensors[3]), ld_out, f, act, float(limit), int(weight_on == "input"), int(bool(interleaved)),

@@ -44,18 +44,22 @@ GROUPED_MIN_ROWS = 1024      # (token, choice) rows from which a step's expert p
 GROUPED_MIN_WEIGHTS = 1 << 25
 
 
+def _fp8_part_bytes(p: PartSpec, n_tokens: int) -> int:
+    if p.kind == "routed_experts":
+        total = _fp8_part_bytes(p["shared"], n_tokens) if p.get("shared") is not None else 0       # (beside the routed experts' result)
+        if p.get("gated", True):
+            d, f, experts, top, few = int(p["hidden"]), int(p["ff"]), int(p["experts"]), int(p["top"]), min(n_tokens, ops.MOE_FEW_TOKENS)
+            total += max(ops.moe_experts_fp8_scratch(n_tokens, d, f, experts, top), ops.moe_few_scratch(few, top, d, f)) + 8 * n_tokens * top + 4 * n_tokens * (experts + 1)
+        return total
+    if p.kind in ("swiglu", "gated_mlp"):
+        return ops.glu_mlp_fp8_scratch(n_tokens, int(p["hidden"]), int(p["intermediate"]))
+    return 0
+
+
 def fp8_step_bytes(spec: ModelSpec, n_tokens: int) -> int:
-    """What a step's feed-forwards keep beside their rows when their matrices are in 8 bits, at the most: quantised rows with their scales, and the chosen
-    experts' fp32 results."""
-    most = 0
-    for layer in spec.layers:
-        p = layer.feed_forward
-        if p.kind == "routed_experts":
-            rows, d, f = n_tokens * int(p["top"]), int(p["hidden"]), int(p["ff"])
-            most = max(most, rows * (6 * d + 2 * f) + 36 * ops.MOE_FEW_TOKENS * (d + 160) + ops.MOE_FEW_TOKENS * int(p["top"]) * 5 * f)
-        elif p.kind in ("swiglu", "gated_mlp"):
-            most = max(most, n_tokens * 2 * (int(p["hidden"]) + int(p["intermediate"])))
-    return most
+    """What a step's feed-forwards keep beside their rows when their matrices are in 8 bits, at the most: the operators' scratch, and the router's choice with its
+    logits."""
+    return max((_fp8_part_bytes(p, n_tokens) for layer in spec.layers for p in (layer.feed_forward, *layer.extras.values())), default=0)
 
 
 def ctx_plain(ctx) -> bool:
