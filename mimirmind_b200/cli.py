@@ -5,7 +5,7 @@ Option names, meanings and defaults are the reference's where it has them
 (default ./config.json, a hard error if the file is missing), ``--model PATH`` (overrides the
 default model's path), ``--prompt``, ``--max-new N`` (20), ``--temperature F`` (0 = greedy),
 ``--top-k N`` (0 off), ``--top-p F`` (1.0 off), ``--seed N`` (0 = random), ``--log-level``, ``--dump-dir``.
-``--weights fp8`` holds the gated feed-forwards' and experts' matrices in 8 bits.
+``--weights fp8`` holds the gated feed-forwards' and experts' matrices in 8 bits (steps of more than 16 tokens quantise the experts' rows as well).
 This engine has no tokenizer (it takes token ids), so ``--prompt`` is a list of ids
 ("5 17 3" or "5,17,3"), as the reference's parity tool takes ``--tokens id,id,…``
 (tools/llama-parity-dump.cpp:111-124); ``--prompt-len N`` makes N seeded random ids instead.

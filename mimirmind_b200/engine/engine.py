@@ -99,7 +99,9 @@ class Engine:
     # ---- construction ----------------------------------------------------------------
     @classmethod
     def from_folder(cls, model_dir: str, dtype: str = "bfloat16", weights: str = "stored", **kw) -> "Engine":
-        """``weights`` ``fp8`` (with bfloat16): the gated feed-forwards' and gated experts' matrices in 8 bits, quantised as they are loaded."""
+        """``weights`` ``fp8`` (with bfloat16): the gated feed-forwards' and gated experts' matrices in 8 bits, quantised as they are loaded.
+        The rows that meet them are quantised too, those of experts only in steps of more than 16 tokens: there a token's result of such a layer changes by up to e4m3's
+        rounding of its rows (a few percent) with the size of the step that it is part of."""
         model, _ = load_model(model_dir, dtype, weights=weights)
         return cls(model, **kw)
 

@@ -19,7 +19,8 @@ The experts' matrices are stacked at load (``[E, 2F, D]`` gate and up rows, ``[E
 device, puts the rows of every expert side by side, and runs two grouped products over them: for prompt-sized steps, and smaller ones
 of large experts, in bfloat16 the tcgen05 product over row tiles laid out on the device (``csrc/gemm_tcgen05.cu``, SwiGLU in its epilogue),
 otherwise the ``mma.sync`` or fp32 kernels of ``csrc/moe.cu``.  With a runtime whose weights are ``fp8`` gated experts are held in 8 bits: up
-to 16 tokens go through the whole layer in two launches (``csrc/moe_few.cu``), more through the grouped 8-bit products (``csrc/gemm_fp8_tcgen05.cu``).  Nothing waits for the host, so a decode step with this
+to 16 tokens go through the whole layer in two launches (``csrc/moe_few.cu``), more through the grouped 8-bit products (``csrc/gemm_fp8_tcgen05.cu``).  The first keep the rows' bits, the second quantise rows and hidden rows to
+e4m3, so the same token's result differs by those roundings (half a step is 2^-4 of a number) between a step of 16 tokens and one of 17.  Nothing waits for the host, so a decode step with this
 feed-forward can be captured.
 """
 from __future__ import annotations
