@@ -27,7 +27,7 @@ struct Fp8Out {                           // rows [., ld] bf16 or fp32; gated pr
     float limit;
 };
 
-int fp8_quant_rows(const void* x, int x_dtype, long long ldx, const int32_t* source, void* q, int ldq, float* scales, int rows, int K, cudaStream_t s);
+int fp8_quant_rows(const void* x, int x_dtype, long long ldx, int x_rows, const int32_t* source, void* q, int ldq, float* scales, int rows, int K, cudaStream_t s);
 // up to 16 rows; `dependent`: launched behind a kernel of this library in the same stream, whose end it waits for itself.  Rows that are not quantised
 // yet are quantised in the kernel (few numbers: it has them in shared memory).
 int fp8_gemv(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, bool dependent, cudaStream_t s);

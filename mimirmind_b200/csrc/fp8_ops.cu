@@ -30,7 +30,7 @@ int quantised(Fp8In& x, int K, bool glu, unsigned char* scratch, bool& dependent
         return MM_ERR_BAD_ARG;
     }
     float* scales = (float*)(scratch + x.rows * row_bytes(K));
-    const int rc = fp8_quant_rows(x.data, x.dtype, x.ld, nullptr, scratch, (int)row_bytes(K), scales, x.rows, K, s);
+    const int rc = fp8_quant_rows(x.data, x.dtype, x.ld, x.rows, nullptr, scratch, (int)row_bytes(K), scales, x.rows, K, s);
     x = {scratch, scales, row_bytes(K), FP8_QUANTISED, x.rows};
     dependent = true;
     return rc;
@@ -141,7 +141,7 @@ MM_EXPORT int mm_fp8_moe_experts(const void* x, int x_dtype, int n, int D, const
     const int rows = n * top, max_tiles = ceil_div(rows, TILE_ROWS) + E, db = ceil_div(D, FP8_BLOCK);
     int32_t* offsets = (int32_t*)(base + at.offsets);
     int rc = mm_moe_sort(idx, rows, E, offsets, base + at.order, top, TILE_ROWS, base + at.tiles, base + at.n_tiles, base + at.row_token, base + at.place, stream);
-    if (rc == MM_OK) rc = fp8_quant_rows(x, x_dtype, D, nullptr, base + at.q, (int)row_bytes(D), (float*)(base + at.q_scales), n, D, (cudaStream_t)stream);
+    if (rc == MM_OK) rc = fp8_quant_rows(x, x_dtype, D, n, nullptr, base + at.q, (int)row_bytes(D), (float*)(base + at.q_scales), n, D, (cudaStream_t)stream);
     if (rc == MM_OK)
         rc = mm_fp8_gather_rows(base + at.q, base + at.q_scales, base + at.row_token, offsets + E, base + at.sorted, base + at.sorted_scales, rows, (int)row_bytes(D), db, stream);
     if (rc == MM_OK)

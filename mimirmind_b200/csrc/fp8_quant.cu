@@ -8,7 +8,7 @@ namespace {
 // loads: three units a warp, their loads together on their way, were no faster.
 // Bound by memory (3 bytes a number) and by the work a number: 4,096 rows of 3,584 bf16 (44 MB) with a division a number 19.7 us, with fp8_quotients 12.1 us (3.6 TB/s).
 template <typename T>
-__global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const T* __restrict__ x, long long ldx, const int32_t* __restrict__ source,
+__global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const T* __restrict__ x, long long ldx, int x_rows, const int32_t* __restrict__ source,
                                                              uint8_t* __restrict__ q, int ldq, float* __restrict__ scales, uint32_t units, int K,
                                                              uint32_t pairs, int blocks, int wide) {
     const int lane = threadIdx.x & 31;
@@ -17,13 +17,14 @@ __global__ void __launch_bounds__(256) fp8_quant_rows_kernel(const T* __restrict
     if (u >= units) return;
     const uint32_t row = u / pairs;
     const int b = (int)(u - row * pairs) * 2 + (lane >> 4), k = b * FP8_BLOCK + (lane & 15) * 8;
-    const T* src = x + (source ? source[row] : (int)row) * ldx + k;
+    const int from = source ? source[row] : (int)row, end = (unsigned)from < (unsigned)x_rows ? K : 0;      // (a number that is no row's, as of padding: noughts)
+    const T* src = x + from * ldx + k;
     float v[8];
-    if (wide && k + 8 <= K) {
+    if (wide && k + 8 <= end) {
         fp8_load8<T>(src, v);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f32<T>(src[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) v[i] = k + i < end ? to_f32<T>(src[i]) : 0.0f;
     }
     uint32_t largest = 0;
 #pragma unroll
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(256) fp8_quant_weight_kernel(const T* __restri
 
 }  // namespace
 
-int fp8_quant_rows(const void* x, int x_dtype, long long ldx, const int32_t* source, void* q, int ldq, float* scales, int rows, int K, cudaStream_t s) {
+int fp8_quant_rows(const void* x, int x_dtype, long long ldx, int x_rows, const int32_t* source, void* q, int ldq, float* scales, int rows, int K, cudaStream_t s) {
     MM_REQUIRE(rows >= 0 && rows < FP8_MAX && K > 0 && K < FP8_MAX && ldx >= 0 && ldq >= K && ldq % 16 == 0 && ldq < K + 16, "fp8 rows: bad sizes");
     MM_REQUIRE(((uintptr_t)q & 15) == 0, "fp8 rows: the numbers must start on a 16-byte boundary");
     if (rows == 0) return MM_OK;
@@ -89,10 +90,10 @@ int fp8_quant_rows(const void* x, int x_dtype, long long ldx, const int32_t* sou
     const int grid = (int)((units + 7) / 8);
     const int wide = ldx % (x_dtype == MM_BF16 ? 8 : 4) == 0 && ((uintptr_t)x & 15) == 0;
     if (x_dtype == MM_BF16)
-        mm_launch(fp8_quant_rows_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, (const __nv_bfloat16*)x, ldx, source, (uint8_t*)q, ldq,
+        mm_launch(fp8_quant_rows_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, (const __nv_bfloat16*)x, ldx, x_rows, source, (uint8_t*)q, ldq,
                   scales, (uint32_t)units, K, (uint32_t)pairs, blocks, wide);
     else if (x_dtype == MM_F32)
-        mm_launch(fp8_quant_rows_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)x, ldx, source, (uint8_t*)q, ldq, scales,
+        mm_launch(fp8_quant_rows_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)x, ldx, x_rows, source, (uint8_t*)q, ldq, scales,
                   (uint32_t)units, K, (uint32_t)pairs, blocks, wide);
     else
         MM_REQUIRE(false, "fp8 rows: dtype must be float32 or bfloat16");
@@ -100,10 +101,17 @@ int fp8_quant_rows(const void* x, int x_dtype, long long ldx, const int32_t* sou
     return MM_OK;
 }
 
-// x [rows, ldx] (K leading columns) -> q [rows, ldq] e4m3 (ldq = K rounded up to 16, the rest noughts), scales fp32 [rows, K / 128 rounded up].
-// source [rows] int32 or null: row r is made from row source[r] of x.
+// x [rows, ldx] (K leading columns) -> q [rows, ldq] e4m3 (ldq = K rounded up to 16, the rest noughts), scales fp32 [rows, K / 128 rounded up]; `source` null.
 MM_EXPORT int mm_fp8_quant_rows(const void* x, int x_dtype, long long ldx, const void* source, void* q, int ldq, void* scales, int rows, int K, void* stream) {
-    return fp8_quant_rows(x, x_dtype, ldx, (const int32_t*)source, q, ldq, (float*)scales, rows, K, (cudaStream_t)stream);
+    MM_REQUIRE(source == nullptr, "fp8 rows: rows made from others want x's number of rows (mm_fp8_quant_rows_from)");
+    return fp8_quant_rows(x, x_dtype, ldx, rows, nullptr, q, ldq, (float*)scales, rows, K, (cudaStream_t)stream);
+}
+
+// The same with source [rows] int32: row r is made from row source[r] of x's x_rows rows, or of noughts where there is no such row.
+MM_EXPORT int mm_fp8_quant_rows_from(const void* x, int x_dtype, long long ldx, int x_rows, const void* source, void* q, int ldq, void* scales, int rows, int K,
+                                     void* stream) {
+    MM_REQUIRE(source != nullptr && x_rows >= 0, "fp8 rows: bad source");
+    return fp8_quant_rows(x, x_dtype, ldx, x_rows, (const int32_t*)source, q, ldq, (float*)scales, rows, K, (cudaStream_t)stream);
 }
 
 // q [., ldq] e4m3 (ldq a multiple of 16) with scales fp32 [., blocks]: row r of the result is row source[r], for the first *count of `rows` rows

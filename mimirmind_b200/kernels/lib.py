@@ -113,6 +113,7 @@ _PROTOTYPES = {
     "mm_scaled_sum2": [P, P, P, I, c_longlong, F, F, P, I, P],
     "mm_gemm_tcgen05_grouped": [P, P, P, I, I, I, I, I, I, I, P, P, I, P, P],
     "mm_fp8_quant_rows": [P, I, c_longlong, P, P, I, P, I, I, P],
+    "mm_fp8_quant_rows_from": [P, I, c_longlong, I, P, P, I, P, I, I, P],
     "mm_fp8_quant_weight": [P, I, P, I, P, I, I, I, P],
     "mm_moe_few": [P, c_longlong, I, I, P, I, I, I, I, I, P, I, I, F, P, P, c_longlong, P, P, c_longlong, I, I, F, I, I, P, P, P],
     "mm_fp8_moe_experts": [P, I, I, I, P, P, I, I, P, c_longlong, P, I, P, c_longlong, P, I, F, I, P, P, P, P],

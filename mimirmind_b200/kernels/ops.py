@@ -2108,7 +2108,7 @@ def _fp8_buffer(*shape, device) -> torch.Tensor:
 
 def quantize_fp8_rows(x: torch.Tensor, source: Optional[torch.Tensor] = None) -> Fp8Rows:
     """Rows [m, K] (bf16 or fp32, contiguous along K) in 8 bits, per row and block of 128: ``s = max(max|x| / 448, 2^-126)``,
-    ``q = e4m3(x / s)``, quotients in fp32.  ``source`` int32 [rows]: row r is made from row ``source[r]`` (each within x).
+    ``q = e4m3(x / s)``, quotients in fp32.  ``source`` int32 [rows]: row r is made from row ``source[r]``, or is noughts where x has no such row.
     A NaN or an infinity in a row makes every product with it NaN; other rows do not see it."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 2:
         raise KernelError("fp8 rows: expected a CUDA matrix")
@@ -2122,8 +2122,11 @@ def quantize_fp8_rows(x: torch.Tensor, source: Optional[torch.Tensor] = None) ->
         m = source.numel()
     _here("fp8 rows", x, source)
     out = Fp8Rows(_fp8_buffer(m, k, device=x.device), torch.empty((m, _blocks(k)), dtype=torch.float32, device=x.device))
-    check(_lib.load().mm_fp8_quant_rows(x.data_ptr(), dtype_code(x.dtype), x.stride(0), _ptr(source), out.values.data_ptr(), -(-k // 16) * 16,
-                                        out.scales.data_ptr(), m, k, _stream()), "quantize_fp8_rows")
+    to = (out.values.data_ptr(), -(-k // 16) * 16, out.scales.data_ptr(), m, k, _stream())
+    if source is None or m == 0:
+        check(_lib.load().mm_fp8_quant_rows(x.data_ptr(), dtype_code(x.dtype), x.stride(0), None, *to), "quantize_fp8_rows")
+    else:
+        check(_lib.load().mm_fp8_quant_rows_from(x.data_ptr(), dtype_code(x.dtype), x.stride(0), min(x.shape[0], 2 ** 31 - 1), source.data_ptr(), *to), "quantize_fp8_rows")
     return out
 
 
