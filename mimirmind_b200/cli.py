@@ -65,7 +65,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--top-p", type=float, default=1.0, help="top-P cutoff, 1.0 = disabled (default 1.0)")
     ap.add_argument("--seed", type=int, default=0, help="RNG seed, 0 = random (default 0)")
     ap.add_argument("--dtype", default="", choices=["", "bfloat16", "float32"], help="overrides runtime.dtype")
-    ap.add_argument("--weights", default="stored", choices=["stored", "fp8"], help="fp8: feed-forward and expert matrices in 8 bits (with bfloat16)")
+    ap.add_argument("--weights", default="stored", choices=["stored", "fp8"], help="(smoke) fp8: feed-forward and expert matrices in 8 bits (with bfloat16)")
     ap.add_argument("--log-level", default="info", choices=["trace", "debug", "info", "warn", "error", "off"])
     ap.add_argument("--dump-dir", default="", help="directory for per-stage dumps of the prefill (sets diagnostics.parityDump to DIR/engine)")
     # replay mode
@@ -78,6 +78,8 @@ def build_parser() -> argparse.ArgumentParser:
 
 def main(argv: Optional[List[str]] = None) -> int:
     args = build_parser().parse_args(argv)
+    if args.mode != "smoke" and args.weights != "stored":
+        raise SystemExit(f"{args.mode} runs with the weights as they are stored: --weights belongs to smoke")
     if args.mode == "replay":
         from .replay import main as replay_main
         if not (args.model and args.out and args.max_tokens):
