@@ -56,3 +56,17 @@ def test_hidden_rows_are_quotients(m, d):
         assert torch.equal(got, (q * s).to(torch.bfloat16).expand(m, 128))
     assert differ > 50                                        # (the middles do tell the two apart)
     ops.check_tcgen05_errors(torch.device(DEV))
+
+
+@pytest.mark.parametrize("exponent", [-149, -140, -127, -126, -120, -100, -90, -81, -80, -79, -64, 0, 63, 90, 98, 99, 100, 101, 110, 119])
+def test_rows_of_any_size_are_quotients(exponent):
+    """rows whose largest numbers are a few hundred 2^exponent (as far as fp32 has them), the others down to nought: the numbers of torch's own division"""
+    from mimirmind_b200.kernels import ops
+    gen = torch.Generator(device=DEV).manual_seed(exponent + 200)
+    x = torch.randn((64, 640), generator=gen, device=DEV, dtype=torch.float64) * torch.exp2(-12.0 * torch.rand((64, 640), generator=gen, device=DEV, dtype=torch.float64))
+    x = (100.0 * x * 2.0 ** exponent).float()
+    assert bool(x.isfinite().all()) and bool((x != 0).any())
+    s = (x.view(64, 5, 128).abs().amax(dim=2) / torch.full((64, 5), 448.0, device=DEV)).clamp_min(2.0 ** -126)
+    q = (x.view(64, 5, 128) / s.unsqueeze(2)).to(torch.float8_e4m3fn).view(64, 640)
+    got = ops.quantize_fp8_rows(x)
+    assert torch.equal(got.scales, s) and torch.equal(got.values.float(), q.float())
