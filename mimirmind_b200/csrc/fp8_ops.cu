@@ -16,6 +16,9 @@ MM_EXPORT int mm_gemm_fp8_tcgen05(const void* A, long long lda, const void* sa, 
 
 namespace {
 
+// Numbers up to which the streaming kernel's CTAs quantise the rows, each for itself.  Us inside and with a launch in front: 1 x 4,608 x 3,584 5.7 and 6.1, 4 x 1,024 x 896
+// 4.0 and 4.3, a feed-forward of 1 row (896, 4,864) 11.5 and 12.1; 8 x 1,024 x 896 5.1 and 4.5, 2 x 4,608 x 3,584 7.1 and 6.1, 16 x 2,048 x 1,024 7.5 and 4.8.  (One row alone stays a little
+// faster inside up to 8,192 numbers, 12.8 and 13.2; at 16,384 it is 53 and 50.)
 constexpr int INSIDE_NUMBERS = 4096;
 
 long long row_bytes(int K) { return (long long)(K + 15) / 16 * 16; }

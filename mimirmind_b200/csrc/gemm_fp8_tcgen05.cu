@@ -4,12 +4,12 @@
 //
 // tcgen05.mma kind::f8f6f4 (128 x BN x 32, fp32 in tensor memory) makes one block's inner sums from operands that TMA brought into shared
 // memory (rows of 128 bytes, 128-byte swizzle); while it makes the next block's, eight warps read these back, multiply them by the block's
-// scales and add them to sums in registers, BN / 2 columns of one row a thread.  Two accumulators in tensor memory keep both sides busy:
-// per block of a 128 x 256 tile the products take 512 cycles and the sums 256 of each scheduler's, so the sums ride along.
+// scales and add them to sums in registers, BN / 2 columns of one row a thread, with two accumulators in tensor memory, one per block in turn.
 //
-// Roles: warps 0..7 sums and results, warps 8 and 11 TMA, warps 9 and 10 products, each of the two for every other block: one thread's waits and
-// issues take 960 cycles a block, a block's products 540.  What bounds the loop now is the round of an accumulator: products 600 cycles, the wait for
-// them 200, reading 470, the next products' issue 350, for two blocks.  Pairs of CTAs (cta_group::2, 256 rows a tile, a third less traffic in shared memory) have
+// Roles: warps 0..7 sums and results, warps 8 and 11 TMA, warps 9 and 10 products, each of the two for every other block (one thread that issued for all
+// took 960 cycles a block).  A block of a 128 x 256 tile is 512 cycles of the tensor pipe.  What bounds the loop is the round of an accumulator, 1,620 cycles, in which
+// every one of the two makes a block, 810 a block: from issue to the end of its products 600, the wait for
+// them 200, reading 470, the next products' issue 350.  Pairs of CTAs (cta_group::2, 256 rows a tile, a third less traffic in shared memory) have
 // the same round, with or without the tile in halves, and were not faster (4,096 x 18,944 x 3,584: 281 and 295 us against 272); halves of one CTA's tile, each
 // 128 columns with barriers of its own, took 410; weights fetched into L2 8 to 24 blocks ahead 278.  A tile's end (results through shared memory in rows of 128 bytes;
 // GLU: the exponentials and quotients) takes 3,000 to 5,000 cycles, its start 1,400.  A CTA walks over tiles, row tiles first, so that CTAs at work at
@@ -22,7 +22,7 @@
 //
 // Grouped form: row tiles of a device-made list (first row, end row, matrix), as in gemm_tcgen05.cu.
 //
-// Measured: 4,096 x 18,944 x 3,584 259 us (2.15 PFLOP/s; under the power cap of a long run 310), 2,000 rows of 5,120 and 2 x 13,824 299, 48 x 3,584 x 3,584 8.6 (12.8 MB,
+// Measured, rows quantised before: 4,096 x 18,944 x 3,584 257 us (2.16 PFLOP/s; under the power cap of a long run 296), 2,000 rows of 5,120 and 2 x 13,824 302, 48 x 3,584 x 3,584 8.5 (12.8 MB,
 // 4 CTAs a tile), 333 x 19,001 x 912 29, 11 of which are the odd rows' number by number (whole words, shifted by a number where a row starts at an odd one, were no faster).
 //
 // Every wait is bounded; when one runs out, the CTA's tiles from there on become NaN, copies in flight get time to land, `err` is set.
@@ -124,7 +124,7 @@ __device__ __forceinline__ void fma_pair(uint64_t& ab, uint64_t s, uint32_t x, u
 __device__ __forceinline__ uint64_t twice(float s) { return ((uint64_t)__float_as_uint(s) << 32) | __float_as_uint(s); }
 
 // mbar_wait for the warps that copy and issue: they sleep on the barrier, a microsecond at the most, instead of asking it time and again beside the summing
-// warps (4,096 x 18,944 x 3,584 under the power cap 300 us, so 295; the summing warps themselves lose by it, 306).  Bounded all the same: under 3 s.
+// warps (4,096 x 18,944 x 3,584 under the power cap 301 us, so 296; the summing warps themselves lose by it, 306).  Bounded all the same: under 3 s.
 __device__ __forceinline__ bool mbar_sleep(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
     for (uint32_t it = 0; it < (1u << 21); ++it) {
         uint32_t ok;
@@ -664,6 +664,8 @@ int resident_clusters(int S) {
 // The tile's width and the number of CTAs to a tile with the least estimated time: rounds of tiles x (a start and an end + blocks x 0.58 us, of 128 columns 0.4, or
 // 0.31 where several row tiles share the weights on their way), as measured with 4 to 100, and 300 to 4,096 rows.  Us estimated and measured: 16 x 3,584 x 18,944 in 128 columns and 4 CTAs 18 and 18, in 2 CTAs 33
 // and 28, in 8 (two rounds) 22 and 25; 16 x 18,944 x 3,584 in 256 columns and 2 CTAs 13 and 19 (the weights' way from memory is 10), in 128 columns and one 13 and 22.
+// An end is longer than that where a tile's rows of results start at odd places: 333 x 19,001 x 912 is estimated at 13 us and takes 29 (19,008
+// columns: 18), whatever the width.
 // Beyond whole rounds, what is left may be split: 2,000 x 5,120 x 13,824 (two rounds and 24 tiles) 166 us in one launch, 145 with the 24 over clusters of 4 behind it;
 // 1,400 x 3,584 x 3,584 (one round and 6 tiles, or 308 of 128 columns) 37 and 34, narrow 32.
 int fp8_gemm(const Fp8In& x, const Fp8Mat& w, const Fp8Out& out, bool glu, int* err, cudaStream_t s) {

@@ -13,8 +13,8 @@
 //
 // Few rows are quantised here (every warp its own run of blocks, into shared memory) instead of by a launch of their own in front of this one.
 //
-// Bound by memory where the matrix is large: 1 x 152,064 x 3,584 87 us (6.2 TB/s of 6.55).  Smaller ones by the launch, the first block's way from memory and the
-// ends of the runs: 8 x 18,944 x 3,584 12.4 to 16 us (68 MB, floor 10.4), 8 x 4,608 x 3,584 5.9 to 7 us (16.5 MB, floor 2.5).  Four blocks on their way
+// Bound by memory where the matrix is large: 1 x 152,064 x 3,584 84 to 87 us (6.2 TB/s of 6.55).  Smaller ones by the launch, the first block's way from memory and the
+// ends of the runs: 8 x 18,944 x 3,584 12.7 us (68 MB, floor 10.4), 8 x 4,608 x 3,584 5.9 us (16.5 MB, floor 2.5).  Four blocks on their way
 // instead of three were no faster; a ring in registers instead of shared memory spilled.
 #include "fp8.cuh"
 #include "fp8_launch.h"

@@ -23,7 +23,8 @@
 // Bound by memory for the experts' matrices (one token, 128 experts of 768 and 2,048 wide, 8 of them, in 8 bits: 38 MB, 5.9 us), but the fixed parts weigh as much:
 // the router about 5 us (830 cycles a step and warp, of loads in a ring or not, of conversions or not), the choice 3, cluster barriers and set-up 3, the second
 // launch's set-up 3; then 700 to 1,000 cycles a warp for 2 KB, the latency of a block's own instructions (a ring of six slots takes the same, half a depth a warp
-// no less).  As captured: 1 token 27.5 us, 8 tokens 70, 16 tokens 104 (floor 59.6); 8 tokens on 16 experts of 1,408 in bf16, 4 each, 60 (38.1).
+// no less).  As captured, one input again and again: 1 token 26 us (27.5 with other inputs in turn), 8 tokens 72 to 79, 16 tokens 103 to 112 on 76 to 83 experts (floor 59.6); 8 tokens
+// on 16 experts of 1,408 in bf16, 4 each, 60 (38.1).
 #include <cuda_fp16.h>
 
 #include "fp8.cuh"
